@@ -57,7 +57,8 @@ typedef enum {
   TMH_S32 = 6,
   TMH_S64 = 7,
   TMH_F16 = 10,
-  TMH_BF16 = 16
+  TMH_BF16 = 16,
+  TMH_F8E4M3 = 17 /* FLOAT8E4M3FN: 4 exponent and 3 mantissa bits, no infinities, at most 448 */
 } tmh_dtype;
 
 /* Zero points of a MatMulNBits weight (quantized.ex:306-325): none (2^(bits-1)), packed
@@ -368,6 +369,127 @@ int tmh_qmoe(tmh_ctx* ctx, const void* d_x, int x_dtype, int64_t T, int64_t H, c
              const tmh_weight* fc2, const void* d_fc2_bias, const tmh_weight* fc3, const void* d_fc3_bias,
              int bias_dtype, int activation, int swiglu_fusion, float alpha, float beta, float limit,
              void* d_y, void* stream);
+
+/* ------------------------------------------------------------------ decoder layers in 8-bit floating point */
+
+/*
+ * The operators that a decoder layer with F8E4M3 weights calls between and around its products, in the
+ * order of their calls: tmh_rms_norm, tmh_matmul_fp8 (q/k/v merged), tmh_paged_append,
+ * tmh_paged_attention, tmh_quantize_rows, tmh_matmul_fp8 (output), tmh_rms_norm, tmh_matmul_fp8
+ * (gate/up merged), tmh_quantize_rows (gated), tmh_matmul_fp8 (down). No reference counterpart: the
+ * reference keeps norms and attention on the Nx backend and has no 8-bit floats.
+ *
+ * Rows in 8 bits: q [T, N] F8E4M3 with one f32 scale for each block of 128 columns (the last block of a
+ * row may be shorter), and scales [ceil(N/128), T], the rows of one block of columns side by side, as
+ * the product reads them: value (t, n) is q[t, n] * scales[n / 128, t]. A block's scale is its largest
+ * magnitude / 448, at least 2^-126, and 1 for a block of zeros; its values divided by the scale (as
+ * f32 multiplied by the scale's f32 reciprocal) round to nearest even. A NaN in a block makes its scale
+ * NaN, an infinity makes it infinite (finite values of the block become 0, infinite ones NaN).
+ * Sums and statistics are f32; leading dimensions (ld*) are in elements and at least the row's width.
+ */
+
+/*
+ * y = h * rsqrt(mean(h^2) + eps) * gamma over rows h = x + residual (h = x without a residual).
+ *  d_x, d_residual (or NULL) [T, N] of dtype (F32, F16, BF16); d_gamma [N] of gamma_dtype
+ *  d_sum  NULL or [T, N] of dtype: h, rounded once (y is computed from h before that rounding); it may be
+ *         d_x or d_residual itself, with the same leading dimension
+ *  d_y    NULL or [T, N] of dtype: y, rounded once; it may be d_x or d_residual if d_sum is not
+ *  d_q, d_q_scales  both NULL, or y in 8 bits (above), rounded once from f32; rows ldq bytes apart
+ * At least one of d_y and d_q is given. T = 0 does nothing.
+ */
+int tmh_rms_norm(tmh_ctx* ctx, const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, int dtype,
+                 int64_t T, int64_t N, const void* d_gamma, int gamma_dtype, float eps, void* d_sum, int64_t lds,
+                 void* d_y, int64_t ldy, void* d_q, int64_t ldq, float* d_q_scales, void* stream);
+
+/*
+ * Rows in 8 bits (above) of x, or with d_gate of gate * sigmoid(gate) * x (SwiGLU: the halves of a merged
+ * gate/up product are d_gate and d_x, both with its leading dimension). x and gate [T, N] of dtype.
+ */
+int tmh_quantize_rows(tmh_ctx* ctx, const void* d_x, int64_t ldx, const void* d_gate, int64_t ldg, int dtype,
+                      int64_t T, int64_t N, void* d_q, int64_t ldq, float* d_q_scales, void* stream);
+
+/*
+ * A weight [N, K] of F8E4M3 (row-major, on the device) with f32 scales [ceil(N/128), ceil(K/128)], one for
+ * each 128 x 128 block, laid out once in the product's tiles, with zeros to whole tiles of 16 x 128;
+ * asynchronous on `stream`, whose later work may use the weight at once (d_b and d_scales must stay until
+ * then). K and N at most 2^22. Free with tmh_fp8_weight_free after that work is done.
+ */
+typedef struct tmh_fp8_weight tmh_fp8_weight;
+int tmh_fp8_weight_prepare(tmh_ctx* ctx, const void* d_b, const float* d_scales, int64_t K, int64_t N,
+                           void* stream, tmh_fp8_weight** out);
+void tmh_fp8_weight_free(tmh_fp8_weight* w);
+int tmh_fp8_weight_info(const tmh_fp8_weight* w, int64_t* K, int64_t* N, size_t* device_bytes);
+
+/*
+ * Y = A . W^T (+ bias): y[m, n] = sum over blocks b of a_scales[b, m] * w_scales[n / 128, b] *
+ * sum over k in b of a[m, k] * w[n, k], summed in f32 and rounded once to y_dtype. With y_dtype F16 or BF16 the
+ * 8-bit matrix unit sums a block: it cuts each product to a multiple of 2^-13 of the largest of the eight that
+ * it adds first (1.5e-5 to 5e-5 of Y in the 2-norm, below the rounding of Y). With F32 products are exact.
+ *  d_a [M, K] F8E4M3, rows lda bytes apart; d_a_scales [ceil(K/128), M]; d_bias NULL or [N] of bias_dtype
+ *  d_y [M, N] of y_dtype (F32, F16, BF16), rows ldy elements apart
+ * Rows of A that do not start at multiples of 16 bytes, or whose K is no multiple of 16, are copied to the
+ * context's workspace first, and products that are split over K keep their partial sums there: inside a
+ * capture that finds it too small the call fails with TMH_ERR_UNSUPPORTED. M at most 2^22.
+ */
+int tmh_matmul_fp8(tmh_ctx* ctx, const tmh_fp8_weight* w, const void* d_a, int64_t M, int64_t lda,
+                   const float* d_a_scales, const void* d_bias, int bias_dtype, void* d_y, int y_dtype,
+                   int64_t ldy, void* stream);
+
+/*
+ * A cache of keys and values in pages: token `at` of page p, kv head h has its head_dim values, contiguous,
+ * at element p * page_stride + at * token_stride + h * head_stride of k and of v, so a page may hold its
+ * tokens' heads side by side ([page_size, kv_heads, head_dim]) or each head's tokens ([kv_heads, page_size,
+ * head_dim]). dtype F32, F16 or BF16; head_dim a multiple of 8 up to 256; k, v and the strides multiples of 16
+ * bytes; pages * page_size below 2^31. Slot s of the cache is token s % page_size of page s / page_size.
+ * Device pointers in a struct of plain values: the call copies it.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  int dtype;
+  int kv_heads;
+  int head_dim;
+  int page_size;
+  int64_t pages;
+  int64_t page_stride, token_stride, head_stride;
+} tmh_paged_cache;
+
+/*
+ * Rotary positions of a step's queries and keys, and its keys and values into their slots of the cache.
+ *  d_q [T, heads, head_dim] (NULL with heads 0), d_k, d_v [T, kv_heads, head_dim] of the cache's dtype; a
+ *    token's heads are contiguous, its rows ldq, ldk, ldv elements apart (the parts of a merged q/k/v product
+ *    have its leading dimension)
+ *  d_positions [T] S64 (NULL with rotary_dim 0); d_cos, d_sin [max_positions, rotary_dim / 2] of table_dtype;
+ *    positions clamp to [0, max_positions - 1], as the gather clamps its ids
+ *  rotary_dim  0, or even and at most head_dim: those first dimensions turn, pair i being dimensions
+ *    (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved is not 0: (a cos - b sin, a sin + b cos) in
+ *    f32, rounded once
+ *  d_slots [T] S64: the token's slot; a token whose slot is outside [0, pages * page_size) is not stored
+ *    (padded rows take -1). No two tokens of a call may name the same slot.
+ *  d_q_out [T, heads, head_dim], rows ldqo apart; it may be d_q itself where rotary_dim is 0
+ */
+int tmh_paged_append(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v,
+                     int64_t ldv, int64_t T, int heads, const int64_t* d_positions, const void* d_cos,
+                     const void* d_sin, int table_dtype, int64_t max_positions, int rotary_dim, int interleaved,
+                     const int64_t* d_slots, const tmh_paged_cache* cache, void* d_q_out, int64_t ldqo, void* stream);
+
+/*
+ * Attention of one new token a sequence over the pages of its cache: for each sequence b and query head h,
+ * y = sum_t softmax_t(scale * q . k_t) v_t over the tokens t in [max(0, length - window), length) (all of
+ * them with window 0), in f32, rounded once. Query heads are grouped: head h reads kv head
+ * h / (heads / kv_heads).
+ *  d_q [B, heads, head_dim] of the cache's dtype, 16-byte aligned rows ldq elements apart (ldq a multiple of
+ *    16 bytes); d_y likewise, ldy
+ *  d_page_table [B, max_pages] S32: token t of sequence b is token t % page_size of page
+ *    d_page_table[b, t / page_size]; an entry outside [0, pages) holds no tokens (its positions are masked)
+ *  d_lengths [B] S32, the tokens in the cache (the new one among them), clamped to [0, max_pages * page_size]
+ * A sequence without tokens answers zeros, and so does a row whose every score is -infinity. What lies in
+ * masked places of the cache, infinities and NaN too, has no effect. max_pages * page_size below 2^31. The
+ * context's workspace keeps the parts of long sequences (its size depends on B, heads and head_dim only).
+ */
+int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, int heads,
+                        const tmh_paged_cache* cache, const int32_t* d_page_table, int64_t max_pages,
+                        const int32_t* d_lengths, float scale, int64_t window, void* d_y, int64_t ldy, void* stream);
 
 /* ------------------------------------------------------------------ measurement floors */
 

@@ -17,7 +17,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "transmuter_hip.h")
 # tmh_status
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_DEVICE, ERR_OOM, ERR_NO_DEVICE = 0, 1, 2, 3, 4, 5
 # tmh_dtype: ONNX TensorProto.DataType codes
-F32, U8, S8, U16, S16, S32, S64, F16, BF16 = 1, 2, 3, 4, 5, 6, 7, 10, 16
+F32, U8, S8, U16, S16, S32, S64, F16, BF16, F8E4M3 = 1, 2, 3, 4, 5, 6, 7, 10, 16, 17
 # tmh_zp_kind
 ZP_NONE, ZP_PACKED, ZP_FLOAT = 0, 1, 2
 # tmh_qparam_mode
@@ -33,6 +33,17 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
+
+
+
+class PagedCacheDesc(ctypes.Structure):
+    """tmh_paged_cache: where a paged cache's keys and values lie on the device."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("dtype", _i), ("kv_heads", _i), ("head_dim", _i), ("page_size", _i),
+                ("pages", _i64), ("page_stride", _i64), ("token_stride", _i64), ("head_stride", _i64)]
+
+
+_cache = ctypes.POINTER(PagedCacheDesc)
 
 # name -> (restype, argtypes); the declarations of include/transmuter_hip.h.
 SIGNATURES = {
@@ -92,6 +103,17 @@ SIGNATURES = {
                                     ctypes.POINTER(_vp)]),
     "tmh_qmoe": (_i, [_vp, _vp, _i, _i64, _i64, _vp, _i, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i,
                       ctypes.c_float, ctypes.c_float, ctypes.c_float, _vp, _vp]),
+    "tmh_rms_norm": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _i64, _i64, _vp, _i, ctypes.c_float, _vp, _i64, _vp, _i64,
+                          _vp, _i64, _vp, _vp]),
+    "tmh_quantize_rows": (_i, [_vp, _vp, _i64, _vp, _i64, _i, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "tmh_fp8_weight_prepare": (_i, [_vp, _vp, _vp, _i64, _i64, _vp, ctypes.POINTER(_vp)]),
+    "tmh_fp8_weight_free": (None, [_vp]),
+    "tmh_fp8_weight_info": (_i, [_vp, ctypes.POINTER(_i64), ctypes.POINTER(_i64), ctypes.POINTER(_sz)]),
+    "tmh_matmul_fp8": (_i, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i, _vp, _i, _i64, _vp]),
+    "tmh_paged_append": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _vp, _vp, _vp, _i, _i64, _i, _i, _vp,
+                              _cache, _vp, _i64, _vp]),
+    "tmh_paged_attention": (_i, [_vp, _vp, _i64, _i64, _i, _cache, _vp, _i64, _vp, ctypes.c_float, _i64, _vp, _i64,
+                                 _vp]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,122 @@
+// F8E4M3 rows with a scale for each block of 128 columns: what the norm and the quantizer write and
+// the 8-bit product reads.
+#pragma once
+
+#include "tmh_device.h"
+#include "tmh_paged_plan.h"
+
+namespace tmh {
+
+constexpr int kF8Block = 128;
+constexpr float kF8Max = 448.f;
+
+// The largest of a value over the 16 lanes of a row of lanes, in all of them: exchanges within pairs, quads,
+// halves and the row (DPP moves, no LDS). The values are magnitudes' bit patterns, which order as unsigned
+// integers with NaNs above infinity, so a NaN among them stays the largest.
+__device__ __forceinline__ uint32_t row_max_bits(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true)));   // lane ^ 1
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4E, 0xF, 0xF, true)));   // lane ^ 2
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x141, 0xF, 0xF, true)));  // 7 - lane
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x140, 0xF, 0xF, true)));  // 15 - lane
+  return v;
+}
+
+__device__ __forceinline__ float row_sum(float v) {
+  auto add = [](float x, int y) { return x + __builtin_bit_cast(float, y); };
+  v = add(v, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+  v = add(v, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
+  v = add(v, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true));
+  v = add(v, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true));
+  return v;
+}
+
+// Eight f32 values of a lane, 16 lanes holding a block: the block's scale (largest magnitude / 448, at least
+// the smallest normal number so that its reciprocal is finite, 1 for zeros), and the values divided by it in
+// e4m3. The quotients are at most 448 but for the last bits of the two roundings, which e4m3's rounding takes
+// back, so they need no clamp (which would turn a NaN into a number).
+__device__ __forceinline__ float f8_block(const float (&v)[8], uint2& q) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu);
+  top = row_max_bits(top);
+  float scale = __builtin_bit_cast(float, top) / kF8Max;
+  if (top == 0) scale = 1.f;
+  else if (scale < 1.17549435e-38f) scale = 1.17549435e-38f;  // (false for a NaN)
+  const float inv = 1.f / scale;
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inv, v[5] * inv, hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inv, v[7] * inv, hi, true);
+  q = make_uint2(static_cast<uint32_t>(lo), static_cast<uint32_t>(hi));
+  return scale;
+}
+
+// Eight consecutive elements of type DT: one or two 16-byte accesses (VEC), or one at a time, `n` of them
+// (past which loads give zeros and stores leave memory alone).
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void* p, int64_t at, int n, float (&v)[8]) {
+  if constexpr (VEC) {
+    if (n <= 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    } else if constexpr (DT == DT_F32) {
+      const float4_t* f = reinterpret_cast<const float4_t*>(static_cast<const float*>(p) + at);
+      const float4_t a = f[0], b = f[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
+      }
+    } else {
+      const uint4_t w = *reinterpret_cast<const uint4_t*>(static_cast<const uint16_t*>(p) + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = DT == DT_F16 ? f16_bits_to_f32(static_cast<uint16_t>(w[i])) : __builtin_bit_cast(float, w[i] << 16);
+        v[2 * i + 1] = DT == DT_F16 ? f16_bits_to_f32(static_cast<uint16_t>(w[i] >> 16))
+                                    : __builtin_bit_cast(float, w[i] & 0xFFFF0000u);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? load_as_f32<DT>(p, at + i) : 0.f;
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == DT_BF16) return pack_bf16_rne(a, b);
+  else return static_cast<uint32_t>(f32_to_f16_bits(a)) | static_cast<uint32_t>(f32_to_f16_bits(b)) << 16;
+}
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void store8(void* p, int64_t at, int n, const float (&v)[8]) {
+  if constexpr (VEC) {
+    if (n <= 0) return;
+    if constexpr (DT == DT_F32) {
+      float4_t* f = reinterpret_cast<float4_t*>(static_cast<float*>(p) + at);
+      f[0] = float4_t{v[0], v[1], v[2], v[3]};
+      f[1] = float4_t{v[4], v[5], v[6], v[7]};
+    } else {
+      *reinterpret_cast<uint4_t*>(static_cast<uint16_t*>(p) + at) =
+          uint4_t{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) store_as<DT>(p, at + i, v[i]);
+  }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store8_f8(uint8_t* p, int64_t at, int n, uint2 q) {
+  if constexpr (VEC) {
+    if (n > 0) *reinterpret_cast<uint2*>(p + at) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[at + i] = static_cast<uint8_t>((i < 4 ? q.x >> (8 * i) : q.y >> (8 * (i - 4))) & 0xFFu);
+  }
+}
+
+}  // namespace tmh

@@ -1,0 +1,289 @@
+// The root-mean-square norm with the residual's addition, and rows in 8 bits (tmh_rms_norm,
+// tmh_quantize_rows). Both are bound by memory: each input is read once and each output written once.
+#include <algorithm>
+
+#include "tmh_f8.h"
+#include "tmh_internal.h"
+
+namespace tmh {
+namespace {
+
+struct NormArgs {
+  const void* x;
+  const void* residual;
+  const void* gamma;
+  void* sum;
+  void* y;
+  uint8_t* q;
+  float* scales;
+  int64_t ldx, ldr, lds, ldy, ldq, rows;
+  int cols, gamma_dtype;
+  float eps;
+};
+
+// Consecutive rows on one XCD (workgroups go to the eight XCDs in turn): their scales of one block lie side by
+// side, and lines that one XCD's L2 holds whole are written to memory whole.
+__device__ __forceinline__ int64_t xcd_row_group(uint32_t block, uint32_t blocks) {
+  const uint32_t per = blocks / 8;
+  return block < 8 * per ? (block & 7) * per + (block >> 3) : block;
+}
+
+__device__ __forceinline__ void load_gamma(const NormArgs& p, int col, int n, float (&g)[8], bool vec) {
+  if (vec && p.gamma_dtype == DT_F16) load8<DT_F16, true>(p.gamma, col, n, g);
+  else if (vec && p.gamma_dtype == DT_BF16) load8<DT_BF16, true>(p.gamma, col, n, g);
+  else if (vec) load8<DT_F32, true>(p.gamma, col, n, g);
+  else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = i < n ? load_float_rt(p.gamma, p.gamma_dtype, col + i) : 0.f;
+  }
+}
+
+// The sum of a value over the TPR threads of a row, in all of them.
+template <int TPR>
+__device__ __forceinline__ float row_total(float v) {
+  v = row_sum(v);
+  v += __shfl_xor(v, 16);
+  v += __shfl_xor(v, 32);
+  if constexpr (TPR > 64) {
+    __shared__ float part[TPR / 64];
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int i = 1; i < TPR / 64; ++i) v += part[i];
+  }
+  return v;
+}
+
+// 1 / sqrt(mean(h^2) + eps) of a row, given a thread's own sum of (f h)^2 for a factor f. Squares of values of 2^64
+// and more overflow f32, though their root would not: such a row (its total is infinite, for all its threads) is
+// summed again with f = 2^-80, which leaves room for 2^30 of the largest numbers; eps is far below its last bits then.
+template <int TPR, typename Sum>
+__device__ __forceinline__ float row_rstd(const NormArgs& p, Sum sum) {
+  float total = row_total<TPR>(sum(1.f));
+  if (total != __builtin_inff()) return 1.f / sqrtf(total / static_cast<float>(p.cols) + p.eps);
+  if constexpr (TPR > 64) __syncthreads();  // every thread has read the wavefronts' sums
+  total = row_total<TPR>(sum(0x1p-80f));
+  return 0x1p-80f / sqrtf(total / static_cast<float>(p.cols));
+}
+
+template <int DT, bool VEC>
+__device__ __forceinline__ void norm_outputs(const NormArgs& p, int64_t row, int col, int n, const float (&h)[8],
+                                             const float (&g)[8], float rstd) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = h[i] * rstd * g[i];
+  if (p.y) store8<DT, VEC>(p.y, row * p.ldy + col, n, v);
+  if (p.q) {
+    uint2 q;
+    const float scale = f8_block(v, q);
+    store8_f8<VEC>(p.q, row * p.ldq + col, n, q);
+    if (n > 0 && (threadIdx.x & 15) == 0) p.scales[static_cast<int64_t>(col / kF8Block) * p.rows + row] = scale;
+  }
+}
+
+// A row to TPR threads, each with NCH pieces of eight columns in registers, so that a row is read once; the
+// sum of squares is f32, taken in a tree. Sixteen lanes hold a block of 128 columns, whose largest magnitude
+// they find among themselves. Rows of up to 512 columns go to a wavefront each (no barrier), of up to 8192 to
+// 256 threads, of up to 32768 to 1024.
+template <int DT, int TPR, int NCH>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_rms_norm(NormArgs p) {
+  constexpr int RPW = TPR < 256 ? 256 / TPR : 1;
+  const int t = threadIdx.x % TPR;
+  const int64_t row = xcd_row_group(blockIdx.x, gridDim.x) * RPW + threadIdx.x / TPR;
+  if (row >= p.rows) return;  // (with a barrier, RPW is 1 and every row exists)
+  float h[NCH][8], g[NCH][8];
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int col = (c * TPR + t) * 8;
+    load8<DT, true>(p.x, row * p.ldx + col, p.cols - col, h[c]);
+    load_gamma(p, col, p.cols - col, g[c], true);
+    if (p.residual) {
+      float r[8];
+      load8<DT, true>(p.residual, row * p.ldr + col, p.cols - col, r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[c][i] += r[i];
+    }
+  }
+  auto squares = [&](float f) {
+    float s = 0.f;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fmaf(f * h[c][i], f * h[c][i], s);
+    return s;
+  };
+  if (p.sum) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = (c * TPR + t) * 8;
+      store8<DT, true>(p.sum, row * p.lds + col, p.cols - col, h[c]);
+    }
+  }
+  const float rstd = row_rstd<TPR>(p, squares);
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int col = (c * TPR + t) * 8;
+    norm_outputs<DT, true>(p, row, col, p.cols - col, h[c], g[c], rstd);
+  }
+}
+
+// Rows of any width, alignment and pitch: the inputs are read twice, the second time from the caches. An
+// output may be an input's memory: a row is read whole ahead of the barrier, and its outputs are written by the
+// thread that has just read the same elements again.
+template <int DT>
+__global__ __launch_bounds__(256) void k_rms_norm_any(NormArgs p) {
+  const int64_t row = xcd_row_group(blockIdx.x, gridDim.x);
+  auto load = [&](int col, float (&h)[8]) {
+    load8<DT, false>(p.x, row * p.ldx + col, p.cols - col, h);
+    if (p.residual) {
+      float r[8];
+      load8<DT, false>(p.residual, row * p.ldr + col, p.cols - col, r);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] += r[i];
+    }
+  };
+  const float rstd = row_rstd<256>(p, [&](float f) {
+    float s = 0.f;
+    for (int col = threadIdx.x * 8; col < p.cols; col += 2048) {
+      float h[8];
+      load(col, h);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s = fmaf(f * h[i], f * h[i], s);
+    }
+    return s;
+  });
+  // Whole blocks of 16 lanes stay together: lanes past the row hold zeros.
+  for (int col = threadIdx.x * 8; col - 8 * static_cast<int>(threadIdx.x & 15) < p.cols; col += 2048) {
+    float h[8], g[8];
+    load(col, h);
+    load_gamma(p, col, p.cols - col, g, false);
+    if (p.sum) store8<DT, false>(p.sum, row * p.lds + col, p.cols - col, h);
+    norm_outputs<DT, false>(p, row, col, p.cols - col, h, g, rstd);
+  }
+}
+
+struct QuantizeArgs {
+  const void* x;
+  const void* gate;
+  uint8_t* q;
+  float* scales;
+  int64_t ldx, ldg, ldq, rows;
+  int cols;
+  uint32_t blocks;  // of 128 columns in a row
+  FastDiv by_blocks;
+};
+
+// Sixteen lanes to a block of 128 columns, the blocks of the rows one after another.
+template <int DT, bool VEC, bool GATE>
+__global__ __launch_bounds__(256) void k_quantize_rows(QuantizeArgs p, int64_t first) {
+  const int64_t all = p.rows * p.blocks;
+  const uint32_t local = blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int64_t block = first * p.blocks + local;
+  if (block >= all) return;  // whole rows of lanes
+  const uint32_t r = p.by_blocks.div(local);
+  const int64_t row = first + r;
+  const uint32_t b = local - r * p.blocks;
+  const int col = static_cast<int>(b) * kF8Block + (threadIdx.x & 15) * 8, n = p.cols - col;
+  float v[8];
+  load8<DT, VEC>(p.x, row * p.ldx + col, n, v);
+  if constexpr (GATE) {
+    float g[8];
+    load8<DT, VEC>(p.gate, row * p.ldg + col, n, g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = g[i] / (1.f + __expf(-g[i])) * v[i];
+  }
+  uint2 q;
+  const float scale = f8_block(v, q);
+  store8_f8<VEC>(p.q, row * p.ldq + col, n, q);
+  if ((threadIdx.x & 15) == 0) p.scales[static_cast<int64_t>(b) * p.rows + row] = scale;
+}
+
+bool aligned(const void* p, int64_t ld, int dtype, int64_t bytes = 16) {
+  return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld * (dtype == TMH_F8E4M3 ? 1 : dtype_size(dtype)) % bytes == 0);
+}
+
+template <int DT>
+void launch_norm(const NormArgs& p, bool vec, hipStream_t s) {
+  const unsigned rows = static_cast<unsigned>(p.rows), fours = static_cast<unsigned>((p.rows + 3) / 4);
+  if (!vec || p.cols > 32768) k_rms_norm_any<DT><<<rows, 256, 0, s>>>(p);
+  else if (p.cols <= 512) k_rms_norm<DT, 64, 1><<<fours, 256, 0, s>>>(p);
+  else if (p.cols <= 2048) k_rms_norm<DT, 256, 1><<<rows, 256, 0, s>>>(p);
+  else if (p.cols <= 4096) k_rms_norm<DT, 256, 2><<<rows, 256, 0, s>>>(p);
+  else if (p.cols <= 8192) k_rms_norm<DT, 256, 4><<<rows, 256, 0, s>>>(p);
+  else if (p.cols <= 16384) k_rms_norm<DT, 1024, 2><<<rows, 1024, 0, s>>>(p);
+  else k_rms_norm<DT, 1024, 4><<<rows, 1024, 0, s>>>(p);
+}
+
+template <int DT>
+void launch_quantize(const QuantizeArgs& p, bool vec, hipStream_t s) {
+  // Launches of whole rows, each below 2^31 blocks (the division's range).
+  const int64_t most = ((int64_t{1} << 31) - 16) / p.blocks;
+  for (int64_t first = 0; first < p.rows; first += most) {
+    const int64_t blocks = std::min(most, p.rows - first) * p.blocks;
+    const unsigned grid = static_cast<unsigned>((blocks + 15) / 16);
+    if (p.gate) {
+      if (vec) k_quantize_rows<DT, true, true><<<grid, 256, 0, s>>>(p, first);
+      else k_quantize_rows<DT, false, true><<<grid, 256, 0, s>>>(p, first);
+    } else {
+      if (vec) k_quantize_rows<DT, true, false><<<grid, 256, 0, s>>>(p, first);
+      else k_quantize_rows<DT, false, false><<<grid, 256, 0, s>>>(p, first);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace tmh
+
+using namespace tmh;
+
+extern "C" {
+
+int tmh_rms_norm(tmh_ctx* ctx, const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, int dtype,
+                 int64_t T, int64_t N, const void* d_gamma, int gamma_dtype, float eps, void* d_sum, int64_t lds,
+                 void* d_y, int64_t ldy, void* d_q, int64_t ldq, float* d_q_scales, void* stream) {
+  if (!is_float_dtype(dtype)) return fail(ctx, TMH_ERR_INVALID, "the norm takes f32, f16 or bf16 rows, got %s", dtype_name(dtype));
+  if (!is_float_dtype(gamma_dtype)) return fail(ctx, TMH_ERR_INVALID, "the norm's gamma must be f32, f16 or bf16, got %s", dtype_name(gamma_dtype));
+  if (T < 0 || N < 1 || T >= (int64_t{1} << 31) || N > (int64_t{1} << 30))
+    return fail(ctx, TMH_ERR_INVALID, "the norm cannot take %lld rows of %lld columns", (long long)T, (long long)N);
+  if (!(eps >= 0.f)) return fail(ctx, TMH_ERR_INVALID, "the norm's eps must not be negative or NaN");
+  if (!d_y && !d_q) return fail(ctx, TMH_ERR_INVALID, "the norm has no output: y and q are NULL");
+  if (!d_q != !d_q_scales) return fail(ctx, TMH_ERR_INVALID, "the norm's q and its scales go together");
+  if (ldx < N || (d_residual && ldr < N) || (d_sum && lds < N) || (d_y && ldy < N) || (d_q && ldq < N))
+    return fail(ctx, TMH_ERR_INVALID, "the norm's leading dimensions must be at least N=%lld", (long long)N);
+  TMH_TRY(use_device(ctx));
+  if (T == 0) return TMH_OK;
+  if (!d_x || !d_gamma) return fail(ctx, TMH_ERR_INVALID, "tmh_rms_norm: NULL pointer");
+  NormArgs p{d_x, d_residual, d_gamma, d_sum, d_y, static_cast<uint8_t*>(d_q), d_q_scales, ldx, ldr, lds, ldy, ldq, T,
+             static_cast<int>(N), gamma_dtype, eps};
+  const bool vec = N % 8 == 0 && aligned(d_x, ldx, dtype) && aligned(d_residual, ldr, dtype) && aligned(d_sum, lds, dtype) &&
+                   aligned(d_y, ldy, dtype) && aligned(d_q, ldq, TMH_F8E4M3, 8) && aligned(d_gamma, 0, gamma_dtype);
+  hipStream_t s = pick_stream(ctx, stream);
+  if (dtype == TMH_F32) launch_norm<DT_F32>(p, vec, s);
+  else if (dtype == TMH_F16) launch_norm<DT_F16>(p, vec, s);
+  else launch_norm<DT_BF16>(p, vec, s);
+  return check_launch(ctx, "k_rms_norm");
+}
+
+int tmh_quantize_rows(tmh_ctx* ctx, const void* d_x, int64_t ldx, const void* d_gate, int64_t ldg, int dtype,
+                      int64_t T, int64_t N, void* d_q, int64_t ldq, float* d_q_scales, void* stream) {
+  if (!is_float_dtype(dtype)) return fail(ctx, TMH_ERR_INVALID, "rows to quantize must be f32, f16 or bf16, got %s", dtype_name(dtype));
+  if (T < 0 || N < 1 || T >= (int64_t{1} << 31) || N > (int64_t{1} << 30))
+    return fail(ctx, TMH_ERR_INVALID, "cannot quantize %lld rows of %lld columns", (long long)T, (long long)N);
+  if (ldx < N || (d_gate && ldg < N) || ldq < N)
+    return fail(ctx, TMH_ERR_INVALID, "the leading dimensions of rows to quantize must be at least N=%lld", (long long)N);
+  TMH_TRY(use_device(ctx));
+  if (T == 0) return TMH_OK;
+  if (!d_x || !d_q || !d_q_scales) return fail(ctx, TMH_ERR_INVALID, "tmh_quantize_rows: NULL pointer");
+  const uint32_t blocks = static_cast<uint32_t>((N + kF8Block - 1) / kF8Block);
+  QuantizeArgs p{d_x, d_gate, static_cast<uint8_t*>(d_q), d_q_scales, ldx, ldg, ldq, T, static_cast<int>(N), blocks,
+                 FastDiv(blocks)};
+  const bool vec = N % 8 == 0 && aligned(d_x, ldx, dtype) && aligned(d_gate, ldg, dtype) && aligned(d_q, ldq, TMH_F8E4M3, 8);
+  hipStream_t s = pick_stream(ctx, stream);
+  if (dtype == TMH_F32) launch_quantize<DT_F32>(p, vec, s);
+  else if (dtype == TMH_F16) launch_quantize<DT_F16>(p, vec, s);
+  else launch_quantize<DT_BF16>(p, vec, s);
+  return check_launch(ctx, "k_quantize_rows");
+}
+
+}  // extern "C"

@@ -1,0 +1,710 @@
+// A paged cache of keys and values: rotary positions and the new tokens into their slots
+// (tmh_paged_append), and attention of one new token a sequence over its pages (tmh_paged_attention).
+#include <algorithm>
+#include <cmath>
+
+#include "tmh_f8.h"
+#include "tmh_internal.h"
+
+namespace tmh {
+namespace {
+
+// ------------------------------------------------------------------ append
+
+struct AppendArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int64_t* positions;
+  const void* cos;
+  const void* sin;
+  const int64_t* slots;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  int64_t ldq, ldk, ldv, ldqo, max_positions;
+  int64_t page_stride, token_stride, head_stride;
+  int64_t num_slots;
+  int table_dtype, rotary, interleaved, heads, kv_heads;
+  uint32_t pieces;  // of eight dimensions in a token's heads, keys and values
+  FastDiv by_pieces, by_head, by_page;
+};
+
+// Eight entries of a rotary table row.
+__device__ __forceinline__ void load_table(const void* p, int dtype, int64_t at, bool vec, float (&v)[8]) {
+  if (vec && dtype == DT_F32) load8<DT_F32, true>(p, at, 8, v);
+  else if (vec && dtype == DT_F16) load8<DT_F16, true>(p, at, 8, v);
+  else if (vec) load8<DT_BF16, true>(p, at, 8, v);
+  else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = load_float_rt(p, dtype, at + i);
+  }
+}
+
+// A thread answers eight dimensions of one head of one token; those that turn by halves read their partners
+// too (the same lines, from the cache). VEC: rows and partners lie on 16 bytes.
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void k_paged_append(AppendArgs p, int64_t first, uint32_t count, bool table_vec) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  const uint32_t tl = p.by_pieces.div(i);
+  const int64_t t = first + tl;
+  const uint32_t piece = i - tl * p.pieces;
+  const int head = static_cast<int>(p.by_head.div(piece));
+  const int dim = static_cast<int>(piece - head * p.by_head.d) * 8, head_dim = static_cast<int>(p.by_head.d) * 8;
+  const bool is_q = head < p.heads, is_k = !is_q && head < p.heads + p.kv_heads;
+  int64_t slot = 0;
+  if (!is_q) {
+    slot = p.slots[t];
+    if (slot < 0 || slot >= p.num_slots) return;
+  }
+  const void* src = is_q ? p.q : is_k ? p.k : p.v;
+  const int h = is_q ? head : is_k ? head - p.heads : head - p.heads - p.kv_heads;
+  const int64_t row = (is_q ? p.ldq : is_k ? p.ldk : p.ldv) * t + static_cast<int64_t>(h) * head_dim;
+  float v[8];
+  load8<DT, VEC>(src, row + dim, 8, v);
+  if ((is_q || is_k) && dim < p.rotary) {
+    const int64_t position = min(max(p.positions[t], int64_t{0}), p.max_positions - 1);
+    const int half = p.rotary / 2;
+    const int64_t table = position * half;
+    if (p.interleaved) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (dim + 2 * j >= p.rotary) continue;
+        const float c = load_float_rt(p.cos, p.table_dtype, table + dim / 2 + j);
+        const float s = load_float_rt(p.sin, p.table_dtype, table + dim / 2 + j);
+        const float a = v[2 * j], b = v[2 * j + 1];
+        v[2 * j] = a * c - b * s;
+        v[2 * j + 1] = fmaf(a, s, b * c);
+      }
+    } else if (VEC) {
+      const bool low = dim < half;
+      const int at = low ? dim : dim - half;
+      float o[8], c[8], s[8];
+      load8<DT, VEC>(src, row + (low ? dim + half : dim - half), 8, o);
+      load_table(p.cos, p.table_dtype, table + at, table_vec, c);
+      load_table(p.sin, p.table_dtype, table + at, table_vec, s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = low ? v[j] * c[j] - o[j] * s[j] : fmaf(o[j], s[j], v[j] * c[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int d = dim + j;
+        if (d >= p.rotary) continue;
+        const bool low = d < half;
+        const int at = low ? d : d - half;
+        const float o = load_as_f32<DT>(src, row + (low ? d + half : d - half));
+        const float c = load_float_rt(p.cos, p.table_dtype, table + at);
+        const float s = load_float_rt(p.sin, p.table_dtype, table + at);
+        v[j] = low ? v[j] * c - o * s : fmaf(o, s, v[j] * c);
+      }
+    }
+  }
+  if (is_q) {
+    store8<DT, VEC>(p.q_out, t * p.ldqo + static_cast<int64_t>(h) * head_dim + dim, 8, v);
+  } else {
+    const uint32_t page = p.by_page.div(static_cast<uint32_t>(slot));
+    const uint32_t at = static_cast<uint32_t>(slot) - page * p.by_page.d;
+    store8<DT, true>(is_k ? p.k_cache : p.v_cache,
+                     page * p.page_stride + at * p.token_stride + h * p.head_stride + dim, 8, v);
+  }
+}
+
+template <int DT>
+void launch_append(const AppendArgs& p, int64_t T, bool vec, bool table_vec, hipStream_t s) {
+  const int64_t most = ((int64_t{1} << 31) - 256) / p.pieces;  // tokens a launch, within the divisions' range
+  for (int64_t first = 0; first < T; first += most) {
+    const uint32_t count = static_cast<uint32_t>(std::min(most, T - first) * p.pieces);
+    const unsigned grid = (count + 255) / 256;
+    if (vec) k_paged_append<DT, true><<<grid, 256, 0, s>>>(p, first, count, table_vec);
+    else k_paged_append<DT, false><<<grid, 256, 0, s>>>(p, first, count, table_vec);
+  }
+}
+
+// ------------------------------------------------------------------ attention
+
+constexpr int kHeads = 16;  // query heads of one kv head that a workgroup answers (the columns of an MFMA tile)
+constexpr float kNone = -__builtin_inff();
+
+struct AttendArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int32_t* table;
+  const int32_t* lengths;
+  void* y;
+  float* part;    // [2 workers][heads of an item][head_dim], then their (maximum, sum) pairs
+  float2* stats;
+  int64_t ldq, ldy, max_pages;
+  PageShape cache;
+  int64_t head_stride;
+  int64_t window, most;  // most: max_pages * page_size
+  int B, group, kv_heads, chunks, head_dim;
+  uint32_t workers;
+  float scale;  // of the scores in base-2 logarithms: scale * log2(e)
+};
+
+template <int UT>
+__device__ __forceinline__ Span span_at(const AttendArgs& p, int b) {
+  return span_of(p.lengths[b], p.most, p.window, UT);
+}
+
+// The units of the sequences before b (all of them for b = B), by one wavefront. (The host has checked that all
+// items' units are below 2^31.)
+template <int UT>
+__device__ __forceinline__ uint32_t units_before(const AttendArgs& p, int b) {
+  uint32_t n = 0;
+  for (int i = threadIdx.x & 63; i < b; i += 64) n += static_cast<uint32_t>(span_at<UT>(p, i).units);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
+  return n;
+}
+
+// The sequence whose units hold `target` (below the total), and the units before it.
+template <int UT>
+__device__ __forceinline__ int find_sequence(const AttendArgs& p, uint32_t target, uint32_t& before) {
+  const int lane = threadIdx.x & 63;
+  uint32_t base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const uint32_t mine = b0 + lane < p.B ? static_cast<uint32_t>(span_at<UT>(p, b0 + lane).units) : 0;
+    uint32_t sum = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t up = __shfl_up(sum, o);
+      if (lane >= o) sum += up;
+    }
+    const uint64_t past = __ballot(base + sum > target);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      before = base + __shfl(sum - mine, at);
+      return b0 + at;
+    }
+    base += __shfl(sum, 63);
+  }
+  before = base;
+  return p.B - 1;  // (not reached: target is below the total)
+}
+
+// (By value: __builtin_bit_cast of a vector's element, an lvalue, reads element 0.)
+__device__ __forceinline__ float as_float(uint32_t v) { return __builtin_bit_cast(float, v); }
+
+template <int DT>
+struct Lane16 {  // 16 bytes of a lane as MFMA operands
+  typedef _Float16 vec __attribute__((ext_vector_type(8)));
+};
+template <>
+struct Lane16<DT_BF16> {
+  typedef __bf16 vec __attribute__((ext_vector_type(8)));
+};
+
+template <int DT>
+__device__ __forceinline__ float4_t mfma16(uint4_t a, uint4_t b, float4_t c) {
+  typedef typename Lane16<DT>::vec vec;
+  if constexpr (DT == DT_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+}
+
+// Two probabilities as the sums of two 16-bit parts each: rounded towards zero, and the rest. Neither part is
+// zero or negative (at least f16's smallest number, of a maximum of 2^15, or bf16's smallest normal one), so that
+// an infinity in V stays what it is in both products.
+template <int DT>
+__device__ __forceinline__ uint2 split2(float a, float b) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  constexpr uint16_t tiny = DT == DT_F16 ? 0x0001 : 0x0080;
+  uint32_t hi;
+  float ra, rb;
+  if constexpr (DT == DT_F16) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    hi = __builtin_bit_cast(uint32_t, h);
+    ra = a - static_cast<float>(h[0]);
+    rb = b - static_cast<float>(h[1]);
+  } else {
+    hi = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+    ra = a - __builtin_bit_cast(float, hi << 16);
+    rb = b - __builtin_bit_cast(float, hi & 0xFFFF0000u);
+  }
+  const u16x2 least = {tiny, tiny};
+  return make_uint2(__builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, hi), least)),
+                    __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, pack2<DT>(ra, rb)), least)));
+}
+
+// The maximum (sum) over the four lanes of one column of an MFMA tile, in all of them.
+__device__ __forceinline__ float column_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// One workgroup's share of the units. Four wavefronts take the tiles of a unit (TILE tokens each), with
+// running maxima, sums and answers of their own, which meet in LDS where an item ends or the share does.
+//
+// A tile: S^T = K Q^T on MFMA, a lane's operand rows being 16 bytes of a token's row as it lies in memory (both
+// operands take the dimensions in the same order, any order). A lane then holds four (two times four, TILE 32)
+// tokens' scores of one head, column l & 15, which are the operand that O^T = V^T P^T wants in the order
+// token(g, j) = 16 (j / 4) + 4 g + j % 4 of its lane row g = l / 16: no score leaves its lane. V's rows come
+// as they lie in memory too, 16 bytes of token(g, j) a lane (a load reads four whole rows of 128 dimensions),
+// and pairs of tokens are put side by side with one v_perm_b32 per two values. The answer's dimension
+// E (4 g + i) + e (of a block of 16 E, E values to 16 bytes) lies in element i of product e: a lane's answers of one i
+// are 16 consecutive bytes.
+// f32: the same with v_mfma_f32_16x16x4_f32, whose operands are single values.
+//
+// Probabilities are split into two 16-bit parts, each multiplied: the sum keeps 16 bits (bf16) or 21 (f16) of
+// each (one part would round each to 8 or 11, as far off as the answer's own type).
+// f16 parts are taken of 2^15 times the probability, so that small ones of long rows do not fall below f16's
+// range; f32 and bf16 ones of 2^-32 times it, so that sums of up to 2^31 values near the type's largest stay
+// finite. The factor is in the running sum too and drops out.
+template <int DT, int NB>  // NB: blocks of 16 E dimensions
+__global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void k_paged_attention(AttendArgs p) {
+  constexpr bool F32 = DT == DT_F32;
+  constexpr int SIZE = F32 ? 4 : 2, E = 16 / SIZE, TILE = F32 ? 16 : 32, UT = 4 * TILE;
+  constexpr int NH = TILE / 16;           // 16-token halves of a tile
+  constexpr int NC = 4 * NB;              // chunks of 4 E dimensions of a row
+  constexpr int VT = F32 ? 4 : 8;         // tokens a lane reads of V
+  constexpr float BIAS = DT == DT_F16 ? 15.f : -32.f;
+  constexpr int ROW = 16 * E * NB + 4;    // floats of a head's answer in LDS (+ 4: off a bank's multiple)
+  __shared__ __align__(16) float lds_o[4][kHeads][ROW];
+  __shared__ float lds_m[4][kHeads], lds_l[4][kHeads];
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t items = static_cast<uint32_t>(p.kv_heads * p.chunks);
+  const uint32_t all = units_before<UT>(p, p.B) * items;
+  const uint32_t per = units_per_worker(all, p.workers);
+  const uint32_t worker = blockIdx.x;
+  uint32_t at = worker * per;
+  if (per == 0 || at >= all) return;
+  const uint32_t stop = min(at + per, all);
+  const uint32_t run = at;
+  uint32_t before;
+  int b = find_sequence<UT>(p, at / items, before);
+  Span sp = span_at<UT>(p, b);
+  uint32_t first = before * items;  // the first unit of the sequence's first item
+  const int chunks_of_row = (p.head_dim + 4 * E - 1) / (4 * E);
+  const bool ragged = p.head_dim % (4 * E) != 0;
+  while (at < stop) {
+    while (at >= first + static_cast<uint32_t>(sp.units) * items) {
+      first += static_cast<uint32_t>(sp.units) * items;
+      sp = span_at<UT>(p, ++b);
+    }
+    const uint32_t item = (at - first) / static_cast<uint32_t>(sp.units);
+    const uint32_t item_first = first + item * sp.units;
+    const uint32_t from = at - item_first, to = min(stop - item_first, static_cast<uint32_t>(sp.units));
+    const int kv_head = static_cast<int>(item) / p.chunks, chunk = static_cast<int>(item) % p.chunks;
+    const int heads = min(kHeads, p.group - chunk * kHeads);
+    const int head0 = kv_head * p.group + chunk * kHeads;
+    const char* kb = static_cast<const char*>(p.k) + static_cast<int64_t>(kv_head) * p.head_stride * SIZE;
+    const char* vb = static_cast<const char*>(p.v) + static_cast<int64_t>(kv_head) * p.head_stride * SIZE;
+    const int32_t* table = p.table + static_cast<int64_t>(b) * p.max_pages;
+
+    uint4_t qf[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      qf[c] = uint4_t{0u, 0u, 0u, 0u};
+      const int dim = 4 * E * c + E * g;
+      if (col < heads && dim < p.head_dim)
+        qf[c] = *reinterpret_cast<const uint4_t*>(static_cast<const char*>(p.q) +
+                                                  (b * p.ldq + static_cast<int64_t>(head0 + col) * p.head_dim + dim) * SIZE);
+    }
+    float m = kNone, l = 0.f;  // of column col, l over this lane's tokens only
+    float4_t acc[NB][E];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[nb][e] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+    for (uint32_t u = from; u < to; ++u) {
+      const int base = (sp.unit + static_cast<int>(u)) * UT + wave * TILE;
+      if (base >= sp.end || base + TILE <= sp.begin) continue;
+      // Lane i looks token base + i % TILE up: its row's offset in bytes, 0 (a row of page 0) where it is masked.
+      const int token = base + lane % TILE;
+      bool ok = token >= sp.begin && token < sp.end;
+      int64_t offset = 0;
+      if (ok) {
+        offset = token_offset(p.cache, table, static_cast<uint32_t>(token)) * SIZE;
+        ok = offset >= 0;
+        if (!ok) offset = 0;
+      }
+      const uint32_t valid = static_cast<uint32_t>(__ballot(ok));  // (TILE 16: the four copies agree)
+      const bool full = TILE == 32 ? valid == 0xFFFFFFFFu : (valid & 0xFFFFu) == 0xFFFFu;
+      auto row_offset = [&](int tk) { return __shfl(offset, tk); };
+      uint4_t kf[NH][NC], vf[VT][NB];
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const char* row = kb + row_offset(16 * h + col);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const int dim = 4 * E * c + E * g;
+          if (c < chunks_of_row) kf[h][c] = *reinterpret_cast<const uint4_t*>(row + (dim < p.head_dim ? dim * SIZE : 0));
+          if (ragged && dim >= p.head_dim) kf[h][c] = uint4_t{0u, 0u, 0u, 0u};
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VT; ++j) {
+        const char* row = vb + row_offset(16 * (j / 4) + 4 * g + j % 4);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          const int dim = 16 * E * nb + E * col;
+          vf[j][nb] = *reinterpret_cast<const uint4_t*>(row + (dim < p.head_dim ? dim * SIZE : 0));
+        }
+      }
+      float4_t s[NH];
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        s[h] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          if (c >= chunks_of_row) continue;
+          if constexpr (F32) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_float(kf[h][c][x]),
+                                                          as_float(qf[c][x]), s[h], 0, 0, 0);
+          } else {
+            s[h] = mfma16<DT>(kf[h][c], qf[c], s[h]);
+          }
+        }
+      }
+      float t[NH][4], top = kNone;
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          t[h][i] = s[h][i] * p.scale;
+          if (!full && !(valid >> (16 * h + 4 * g + i) & 1u)) t[h][i] = kNone;
+          top = fmaxf(top, t[h][i]);
+        }
+      top = column_max(top);
+      if (!full) {
+#pragma unroll
+        for (int j = 0; j < VT; ++j)
+          if (!(valid >> (16 * (j / 4) + 4 * g + j % 4) & 1u))
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) vf[j][nb] = uint4_t{0u, 0u, 0u, 0u};
+      }
+      if (__ballot(top > m)) {
+        const float next = fmaxf(m, top);
+        const float keep = next == m ? 1.f : __builtin_amdgcn_exp2f(m - next);  // (m -inf: 0)
+        m = next;
+        l *= keep;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[nb][e] *= keep;
+      }
+      const float ref = (m == kNone ? 0.f : m) - BIAS;
+      float pr[NH][4];
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pr[h][i] = __builtin_amdgcn_exp2f(t[h][i] - ref);
+          l += pr[h][i];
+        }
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+              acc[nb][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_float(vf[i][nb][e]), pr[0][i],
+                                                                acc[nb][e], 0, 0, 0);
+      } else {
+        uint4_t hi, lo;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint2 parts = split2<DT>(pr[x >> 1][2 * (x & 1)], pr[x >> 1][2 * (x & 1) + 1]);
+          hi[x] = parts.x;
+          lo[x] = parts.y;
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            uint4_t vt;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              vt[x] = __builtin_amdgcn_perm(vf[2 * x + 1][nb][e >> 1], vf[2 * x][nb][e >> 1],
+                                            e & 1 ? 0x07060302u : 0x05040100u);
+            acc[nb][e] = mfma16<DT>(vt, hi, acc[nb][e]);
+            acc[nb][e] = mfma16<DT>(vt, lo, acc[nb][e]);
+          }
+      }
+    }
+
+    // The four wavefronts' parts of the item meet in LDS.
+    l = column_sum(l);
+    if (g == 0) {
+      lds_m[wave][col] = m;
+      lds_l[wave][col] = l;
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<float4_t*>(&lds_o[wave][col][16 * E * nb + E * (4 * g + i) + e]) =
+              float4_t{acc[nb][e][i], acc[nb][e + 1][i], acc[nb][e + 2][i], acc[nb][e + 3][i]};
+    __syncthreads();
+    const bool whole = from == 0 && to == static_cast<uint32_t>(sp.units);
+    const uint32_t slot = part_place(worker, at == run);
+    const int quads = p.head_dim / 4;
+    for (int i = threadIdx.x; i < heads * quads; i += 256) {
+      const int hd = i / quads, dim = (i - hd * quads) * 4;
+      float top = lds_m[0][hd];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) top = fmaxf(top, lds_m[w][hd]);
+      float total = 0.f;
+      float4_t o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = lds_m[w][hd] == top ? 1.f : __builtin_amdgcn_exp2f(lds_m[w][hd] - top);
+        total += f * lds_l[w][hd];
+        o += f * *reinterpret_cast<const float4_t*>(&lds_o[w][hd][dim]);
+      }
+      if (whole) {
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        const int64_t out = b * p.ldy + static_cast<int64_t>(head0 + hd) * p.head_dim + dim;
+        if constexpr (F32)
+          *reinterpret_cast<float4_t*>(static_cast<float*>(p.y) + out) = o * inv;
+        else
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + out) =
+              make_uint2(pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv));
+      } else {
+        const int64_t row = static_cast<int64_t>(slot) * min(kHeads, p.group) + hd;
+        *reinterpret_cast<float4_t*>(p.part + row * p.head_dim + dim) = o;
+        if (dim == 0) p.stats[row] = make_float2(top, total);
+      }
+    }
+    at = item_first + to;
+    __syncthreads();
+  }
+}
+
+// The parts of an item that several workers shared (one workgroup a query head), and zeros for sequences
+// without tokens. Which workers those are follows from the lengths, as in the kernel above.
+template <int DT>
+__global__ __launch_bounds__(256) void k_paged_join(AttendArgs p) {
+  constexpr int UT = DT == DT_F32 ? 64 : 128;
+  const int b = blockIdx.y;
+  const int head = blockIdx.x, kv_head = head / p.group, in_group = head - kv_head * p.group;
+  const int chunk = in_group / kHeads, hd = in_group - chunk * kHeads;
+  const Span sp = span_at<UT>(p, b);
+  const int quads = p.head_dim / 4;  // at most 64
+  auto store = [&](int dim, float4_t o) {
+    const int64_t out = b * p.ldy + static_cast<int64_t>(head) * p.head_dim + dim;
+    if constexpr (DT == DT_F32)
+      *reinterpret_cast<float4_t*>(static_cast<float*>(p.y) + out) = o;
+    else
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + out) = make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
+  };
+  if (sp.units == 0) {
+    if (static_cast<int>(threadIdx.x) < quads) store(4 * threadIdx.x, float4_t{0.f, 0.f, 0.f, 0.f});
+    return;
+  }
+  const uint32_t items = static_cast<uint32_t>(p.kv_heads * p.chunks);
+  const uint32_t all = units_before<UT>(p, p.B) * items;
+  const uint32_t first = units_before<UT>(p, b) * items + static_cast<uint32_t>(kv_head * p.chunks + chunk) * sp.units;
+  const Parts parts = parts_of(first, static_cast<uint32_t>(sp.units), units_per_worker(all, p.workers));
+  if (parts.count == 1) return;
+  auto row_of = [&](uint32_t i) { return static_cast<int64_t>(place_of(parts, i)) * min(kHeads, p.group) + hd; };
+  __shared__ float red[4];
+  __shared__ __align__(16) float4_t sums[256];
+  __shared__ float totals[256];
+  float top = kNone;
+  for (uint32_t i = threadIdx.x; i < parts.count; i += 256) top = fmaxf(top, p.stats[row_of(i)].x);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  // 256 / quads threads to a group of four dimensions, each every so many parts.
+  const int groups = 256 / quads, mine = threadIdx.x / quads, dim = (threadIdx.x - mine * quads) * 4;
+  float total = 0.f;
+  float4_t o{0.f, 0.f, 0.f, 0.f};
+  if (mine < groups) {
+    for (uint32_t i = mine; i < parts.count; i += groups) {
+      const int64_t row = row_of(i);
+      const float2 st = p.stats[row];
+      const float f = st.x == top ? 1.f : __builtin_amdgcn_exp2f(st.x - top);
+      total += f * st.y;
+      o += f * *reinterpret_cast<const float4_t*>(p.part + row * p.head_dim + dim);
+    }
+  }
+  sums[threadIdx.x] = o;
+  totals[threadIdx.x] = total;
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) >= quads) return;
+  for (int i = 1; i < groups; ++i) {
+    total += totals[i * quads + threadIdx.x];
+    o += sums[i * quads + threadIdx.x];
+  }
+  store(dim, total == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / total));
+}
+
+int check_cache(tmh_ctx* ctx, const tmh_paged_cache* c) {
+  if (!c) return fail(ctx, TMH_ERR_INVALID, "the paged cache is NULL");
+  if (!is_float_dtype(c->dtype))
+    return fail(ctx, TMH_ERR_INVALID, "a paged cache holds f32, f16 or bf16 values, got %s", dtype_name(c->dtype));
+  if (c->kv_heads < 1 || c->page_size < 1 || c->pages < 1)
+    return fail(ctx, TMH_ERR_INVALID, "a paged cache needs kv_heads, page_size and pages of at least 1, got %d, %d, %lld",
+                c->kv_heads, c->page_size, (long long)c->pages);
+  if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8 != 0)
+    return fail(ctx, TMH_ERR_UNSUPPORTED, "a paged cache's head_dim must be a multiple of 8 up to 256, got %d", c->head_dim);
+  if (c->pages >= (int64_t{1} << 31) / c->page_size + ((int64_t{1} << 31) % c->page_size != 0))
+    return fail(ctx, TMH_ERR_UNSUPPORTED, "a paged cache needs pages * page_size below 2^31");
+  if (!c->k || !c->v) return fail(ctx, TMH_ERR_INVALID, "a paged cache's k and v must not be NULL");
+  const int64_t e = 16 / dtype_size(c->dtype);
+  if (reinterpret_cast<uintptr_t>(c->k) % 16 != 0 || reinterpret_cast<uintptr_t>(c->v) % 16 != 0 || c->page_stride % e != 0 ||
+      c->token_stride % e != 0 || c->head_stride % e != 0)
+    return fail(ctx, TMH_ERR_UNSUPPORTED, "a paged cache's k, v and strides must be multiples of 16 bytes");
+  if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0)
+    return fail(ctx, TMH_ERR_INVALID, "a paged cache's strides must not be negative");
+  return TMH_OK;
+}
+
+template <int DT>
+void launch_attention(const AttendArgs& p, int heads, hipStream_t s) {
+  constexpr int per_block = DT == DT_F32 ? 64 : 128;
+  const int nb = (p.head_dim + per_block - 1) / per_block;
+  if (nb == 1) k_paged_attention<DT, 1><<<p.workers, 256, 0, s>>>(p);
+  else if (nb == 2) k_paged_attention<DT, 2><<<p.workers, 256, 0, s>>>(p);
+  else if constexpr (DT == DT_F32) k_paged_attention<DT, 4><<<p.workers, 256, 0, s>>>(p);
+  k_paged_join<DT><<<dim3(static_cast<unsigned>(heads), static_cast<unsigned>(p.B)), 256, 0, s>>>(p);
+}
+
+}  // namespace
+}  // namespace tmh
+
+using namespace tmh;
+
+extern "C" {
+
+int tmh_paged_append(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v,
+                     int64_t ldv, int64_t T, int heads, const int64_t* d_positions, const void* d_cos,
+                     const void* d_sin, int table_dtype, int64_t max_positions, int rotary_dim, int interleaved,
+                     const int64_t* d_slots, const tmh_paged_cache* cache, void* d_q_out, int64_t ldqo, void* stream) {
+  TMH_TRY(check_cache(ctx, cache));
+  const int dim = cache->head_dim;
+  if (T < 0 || heads < 0 || T >= (int64_t{1} << 31) || static_cast<int64_t>(heads) + 2 * static_cast<int64_t>(cache->kv_heads) > (1 << 20))
+    return fail(ctx, TMH_ERR_INVALID, "cannot append %lld tokens of %d query heads", (long long)T, heads);
+  if (rotary_dim < 0 || rotary_dim > dim || rotary_dim % 2 != 0)
+    return fail(ctx, TMH_ERR_INVALID, "rotary_dim must be even and from 0 to head_dim=%d, got %d", dim, rotary_dim);
+  if (rotary_dim && !is_float_dtype(table_dtype))
+    return fail(ctx, TMH_ERR_INVALID, "rotary tables must be f32, f16 or bf16, got %s", dtype_name(table_dtype));
+  if (rotary_dim && max_positions < 1) return fail(ctx, TMH_ERR_INVALID, "rotary tables hold no positions");
+  const int64_t kv_width = static_cast<int64_t>(cache->kv_heads) * dim, q_width = static_cast<int64_t>(heads) * dim;
+  if (ldk < kv_width || ldv < kv_width || (heads && (ldq < q_width || ldqo < q_width)))
+    return fail(ctx, TMH_ERR_INVALID, "the leading dimensions of q, k and v must be at least their heads' widths");
+  TMH_TRY(use_device(ctx));
+  if (T == 0) return TMH_OK;
+  if (!d_k || !d_v || !d_slots || (heads && (!d_q || !d_q_out)) || (rotary_dim && (!d_positions || !d_cos || !d_sin)))
+    return fail(ctx, TMH_ERR_INVALID, "tmh_paged_append: NULL pointer");
+  if (heads && rotary_dim && d_q_out == d_q) return fail(ctx, TMH_ERR_INVALID, "rotated queries need a place of their own");
+  AppendArgs p;
+  p.q = d_q;
+  p.k = d_k;
+  p.v = d_v;
+  p.positions = d_positions;
+  p.cos = d_cos;
+  p.sin = d_sin;
+  p.slots = d_slots;
+  p.q_out = d_q_out;
+  p.k_cache = cache->k;
+  p.v_cache = cache->v;
+  p.ldq = ldq;
+  p.ldk = ldk;
+  p.ldv = ldv;
+  p.ldqo = ldqo;
+  p.max_positions = max_positions;
+  p.page_stride = cache->page_stride;
+  p.token_stride = cache->token_stride;
+  p.head_stride = cache->head_stride;
+  p.num_slots = cache->pages * cache->page_size;
+  p.table_dtype = table_dtype;
+  p.rotary = rotary_dim;
+  p.interleaved = interleaved;
+  p.heads = heads;
+  p.kv_heads = cache->kv_heads;
+  p.pieces = static_cast<uint32_t>((heads + 2 * cache->kv_heads) * (dim / 8));
+  p.by_pieces = FastDiv(p.pieces);
+  p.by_head = FastDiv(static_cast<uint32_t>(dim / 8));
+  p.by_page = FastDiv(static_cast<uint32_t>(cache->page_size));
+  const int64_t e = 16 / dtype_size(cache->dtype);
+  auto on16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
+  const bool vec = on16(d_k) && on16(d_v) && ldk % e == 0 && ldv % e == 0 &&
+                   (!heads || (on16(d_q) && on16(d_q_out) && ldq % e == 0 && ldqo % e == 0)) &&
+                   (interleaved ? true : rotary_dim % 16 == 0);
+  const bool table_vec = on16(d_cos) && on16(d_sin) && rotary_dim % 16 == 0;
+  hipStream_t s = pick_stream(ctx, stream);
+  if (cache->dtype == TMH_F32) launch_append<DT_F32>(p, T, vec, table_vec, s);
+  else if (cache->dtype == TMH_F16) launch_append<DT_F16>(p, T, vec, table_vec, s);
+  else launch_append<DT_BF16>(p, T, vec, table_vec, s);
+  return check_launch(ctx, "k_paged_append");
+}
+
+int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, int heads, const tmh_paged_cache* cache,
+                        const int32_t* d_page_table, int64_t max_pages, const int32_t* d_lengths, float scale,
+                        int64_t window, void* d_y, int64_t ldy, void* stream) {
+  TMH_TRY(check_cache(ctx, cache));
+  if (heads < 1 || heads % cache->kv_heads != 0)
+    return fail(ctx, TMH_ERR_INVALID, "%d query heads are no multiple of %d kv heads", heads, cache->kv_heads);
+  if (B < 0 || B > 65535) return fail(ctx, TMH_ERR_INVALID, "attention takes 0 to 65535 sequences, got %lld", (long long)B);
+  if (max_pages < 0 || window < 0) return fail(ctx, TMH_ERR_INVALID, "max_pages and window must not be negative");
+  if (std::isnan(scale)) return fail(ctx, TMH_ERR_INVALID, "the scale is NaN");
+  const int64_t width = static_cast<int64_t>(heads) * cache->head_dim;
+  if (ldq < width || ldy < width)
+    return fail(ctx, TMH_ERR_INVALID, "the leading dimensions of q and y must be at least %lld", (long long)width);
+  if (max_pages >= (int64_t{1} << 31) / cache->page_size)
+    return fail(ctx, TMH_ERR_UNSUPPORTED, "attention needs max_pages * page_size below 2^31");
+  TMH_TRY(use_device(ctx));
+  if (B == 0) return TMH_OK;
+  if (!d_q || !d_y || !d_lengths || (max_pages && !d_page_table)) return fail(ctx, TMH_ERR_INVALID, "tmh_paged_attention: NULL pointer");
+  const int64_t e = 16 / dtype_size(cache->dtype);
+  if (reinterpret_cast<uintptr_t>(d_q) % 16 != 0 || reinterpret_cast<uintptr_t>(d_y) % 16 != 0 || ldq % e != 0 || ldy % e != 0)
+    return fail(ctx, TMH_ERR_UNSUPPORTED, "attention's q and y must be aligned to 16 bytes, their leading dimensions too");
+  const int group = heads / cache->kv_heads, chunks = (group + kHeads - 1) / kHeads;
+  const int64_t unit = cache->dtype == TMH_F32 ? 64 : 128;
+  const int64_t units = (max_pages * cache->page_size + unit - 1) / unit * B * cache->kv_heads * chunks;
+  if (units >= (int64_t{1} << 31)) return fail(ctx, TMH_ERR_UNSUPPORTED, "attention over too many tokens at once");
+  AttendArgs p;
+  p.q = d_q;
+  p.k = cache->k;
+  p.v = cache->v;
+  p.table = d_page_table;
+  p.lengths = d_lengths;
+  p.y = d_y;
+  p.ldq = ldq;
+  p.ldy = ldy;
+  p.max_pages = max_pages;
+  p.cache = PageShape{cache->pages, cache->page_stride, cache->token_stride, FastDiv(static_cast<uint32_t>(cache->page_size))};
+  p.head_stride = cache->head_stride;
+  p.window = window;
+  p.most = max_pages * cache->page_size;
+  p.B = static_cast<int>(B);
+  p.group = group;
+  p.kv_heads = cache->kv_heads;
+  p.chunks = chunks;
+  p.head_dim = cache->head_dim;
+  p.scale = scale * 1.44269504088896340736f;
+  // Two workgroups a compute unit, or one a unit of work where the table has room for fewer.
+  const int64_t workers = std::max<int64_t>(1, std::min<int64_t>(2 * ctx->num_cus, units));
+  p.workers = static_cast<uint32_t>(workers);
+  hipStream_t s = pick_stream(ctx, stream);
+  const size_t rows = 2 * static_cast<size_t>(2 * ctx->num_cus) * std::min(kHeads, group);
+  void* ws = workspace(ctx, rows * (cache->head_dim * 4 + sizeof(float2)), s);
+  if (!ws) return fail(ctx, TMH_ERR_UNSUPPORTED, "attention's workspace cannot grow here: run one call before the capture");
+  p.part = static_cast<float*>(ws);
+  p.stats = reinterpret_cast<float2*>(p.part + rows * cache->head_dim);
+  if (cache->dtype == TMH_F32) launch_attention<DT_F32>(p, heads, s);
+  else if (cache->dtype == TMH_F16) launch_attention<DT_F16>(p, heads, s);
+  else launch_attention<DT_BF16>(p, heads, s);
+  return check_launch(ctx, "k_paged_attention");
+}
+
+}  // extern "C"

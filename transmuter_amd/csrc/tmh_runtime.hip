@@ -27,6 +27,7 @@ const char* dtype_name(int dt) {
     case TMH_S16: return "s16";
     case TMH_S32: return "s32";
     case TMH_S64: return "s64";
+    case TMH_F8E4M3: return "f8_e4m3fn";
     default: return "unknown type";
   }
 }

@@ -1,7 +1,8 @@
 """Device context and device-resident tensors over the C ABI of libtmhip.
 
 Types are named as Nx names them ("f32", "f16", "bf16", "u8", "s8", "s32", "s64", ...). bf16
-host arrays are uint16 bit patterns in a `BF16Host` array, which `nx_type` names "bf16".
+host arrays are uint16 bit patterns in a `BF16Host` array, which `nx_type` names "bf16"; host
+arrays of "f8_e4m3fn" are uint8 bit patterns (`Context.put` is told their type).
 """
 
 from __future__ import annotations
@@ -18,12 +19,12 @@ from ._lib import check, lib
 NX_TO_TMH = {
     "f32": _lib.F32, "f16": _lib.F16, "bf16": _lib.BF16,
     "u8": _lib.U8, "s8": _lib.S8, "u16": _lib.U16, "s16": _lib.S16,
-    "s32": _lib.S32, "s64": _lib.S64,
+    "s32": _lib.S32, "s64": _lib.S64, "f8_e4m3fn": _lib.F8E4M3,
 }
 NX_TO_NUMPY = {
     "f32": np.float32, "f16": np.float16, "bf16": np.uint16,
     "u8": np.uint8, "s8": np.int8, "u16": np.uint16, "s16": np.int16,
-    "s32": np.int32, "s64": np.int64,
+    "s32": np.int32, "s64": np.int64, "f8_e4m3fn": np.uint8,
 }
 NUMPY_TO_NX = {
     np.dtype(np.float32): "f32", np.dtype(np.float16): "f16",

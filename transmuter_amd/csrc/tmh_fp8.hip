@@ -8,6 +8,7 @@
 // to f16, which holds every e4m3 value, and multiplied by v_mfma_f32_16x16x32_f16, whose products are exact and
 // summed in f32 (8e-8 in the 2-norm), at half the rate or less.
 #include <algorithm>
+#include <cmath>
 #include <new>
 
 #include "tmh_f8.h"
@@ -68,6 +69,12 @@ __device__ __forceinline__ float4_t block_product(const Piece<true> (&w)[2], con
   return c;
 }
 
+// Row r of a tile. Tiles t and t + 1 (t even) share 32 rows of W in turns of four, so that a lane's outputs of the
+// pair (rows 4 g .. + 3 of each) are eight consecutive columns of Y.
+__host__ __device__ __forceinline__ int64_t tile_row(int64_t tile, int r) {
+  return (tile >> 1) * 32 + (r >> 2) * 8 + (tile & 1) * 4 + (r & 3);
+}
+
 // W [N][K] into its tiles: a workgroup's four wavefronts take a tile each.
 template <bool VEC>
 __global__ __launch_bounds__(256) void k_f8_tile(const uint8_t* __restrict__ w, int64_t N, int64_t K, int64_t kb, int64_t tiles,
@@ -76,7 +83,7 @@ __global__ __launch_bounds__(256) void k_f8_tile(const uint8_t* __restrict__ w, 
   if (at >= tiles * kb) return;
   const int64_t tile = at / kb, b = at - tile * kb;
   const int lane = threadIdx.x & 63;
-  const int64_t n = tile * 16 + (lane & 15);
+  const int64_t n = tile_row(tile, lane & 15);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int64_t k = b * kF8Block + 64 * h + 16 * (lane >> 4);
@@ -154,91 +161,222 @@ __device__ __forceinline__ void store4(const F8Args& p, int64_t m, int n, float4
   }
 }
 
-// Few rows: a workgroup of KW wavefronts takes one tile of 16 columns of Y for all (up to 16 MT) rows, the
-// wavefronts every KW-th block of K each, and adds their sums in LDS.
-template <int MT, int KW, bool EXACT>
+// 4 bytes per lane from a buffer into LDS at lds + 4 * lane (lds_dma16's form for single values).
+__device__ __forceinline__ void lds_dma4(__amdgpu_buffer_rsrc_t rsrc, uint8_t* lds, uint32_t voffset, uint32_t soffset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds), 4, voffset, soffset, 0, 0);
+#endif
+}
+
+// At most N (below 64) vector-memory operations of this thread outstanding, and no LDS operation.
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | (7 << 4));
+}
+
+// Few rows: a workgroup of KW wavefronts takes NT tiles of 16 columns of Y for 16 MT rows, the
+// wavefronts every KW-th block of K each, and adds their sums in LDS. A wavefront has the next block's loads on
+// their way while it multiplies one: W's tiles to registers, A's rows to a place of its own in LDS (no barrier),
+// eight lanes to a row's line (the fragments' own 16 bytes of 16 rows would be 64 lookups a load, k_f8_gemm).
+template <int MT, int NT, int KW, bool EXACT>
 __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
+  constexpr int STAGE = MT * kTileBytes;
+  extern __shared__ __align__(16) uint8_t lds[];  // [KW][2][STAGE]; then the sums, [KW - 1][MT * NT][64] float4
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = blockIdx.x;
+  const int groups = p.tiles / NT, row_group = blockIdx.x / groups, tile = (blockIdx.x - row_group * groups) * NT;
   const uint8_t* w = p.w + (static_cast<int64_t>(tile) * p.kb) * kTileBytes + lane * 16;
   const float* ws = p.w_scales + static_cast<int64_t>(tile / 8) * p.kb;
-  float4_t acc[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
   const int first = blockIdx.z * p.per, last = min(first + p.per, p.kb);
-  for (int b = first + wave; b < last; b += KW) {
-    Piece<EXACT> wp[2];
+  uint8_t* mine = lds + wave * 2 * STAGE;
+  const int a_row = lane >> 3, a_chunk = (lane & 7) ^ a_row;
+  const int m0 = row_group * 16 * MT;
+  const auto a_rsrc = buffer_rsrc(p.a + m0 * p.lda, static_cast<uint32_t>(min((static_cast<int64_t>(p.M) - m0 - 1) * p.lda + p.K, int64_t{0x7FFFFFF0})));
+  const uint32_t a_off = static_cast<uint32_t>(a_row * p.lda) + 16 * a_chunk, a_rows = static_cast<uint32_t>(8 * p.lda);
+  const uint32_t a_at[2] = {static_cast<uint32_t>(r * 128 + 16 * (g ^ (r & 7))), static_cast<uint32_t>(r * 128 + 16 * ((g + 4) ^ (r & 7)))};
+  uint4_t wr[2][NT][2];
+  float sw[2], sa[2][MT];
+  constexpr int LOADS = 2 * NT + 1 + 3 * MT;
+  auto load = [&](int b, int buf) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) wp[h].set(*reinterpret_cast<const uint4_t*>(w + static_cast<int64_t>(b) * kTileBytes + 1024 * h));
-    const float sw = ws[b];
-    const int k = b * kF8Block + 16 * g;
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        wr[buf][j][h] = *reinterpret_cast<const uint4_t*>(w + (static_cast<int64_t>(j) * p.kb + b) * kTileBytes + 1024 * h);
+    sw[buf] = ws[b];
+    const int k0 = b * kF8Block;
+#pragma unroll
+    for (int q = 0; q < 2 * MT; ++q)
+      lds_dma16(a_rsrc, mine + buf * STAGE + q * 1024, k0 + 16 * a_chunk < p.K ? a_off + q * a_rows : 0x80000000u, static_cast<uint32_t>(k0));
+#pragma unroll
+    for (int t = 0; t < MT; ++t) sa[buf][t] = p.a_scales[static_cast<int64_t>(b) * p.M + min(m0 + 16 * t + r, p.M - 1)];
+  };
+  float4_t acc[MT][NT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[t][j] = float4_t{0.f, 0.f, 0.f, 0.f};
+  auto block = [&](int b, int buf) {
+    if (b + KW < last) {
+      load(b + KW, buf ^ 1);
+      asm volatile("" ::: "memory");
+      wait_vm<LOADS>();  // this block's loads: the next one's are the youngest
+    } else {
+      wait_vm<0>();
+    }
+    asm volatile("" ::: "memory");
+    Piece<EXACT> wp[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) wp[j][h].set(wr[buf][j][h]);
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-      const int m = 16 * t + r;
-      uint4_t a0{0u, 0u, 0u, 0u}, a1{0u, 0u, 0u, 0u};
-      float sa = 0.f;
-      if (m < p.M) {
-        const uint8_t* a = p.a + m * p.lda + k;
-        if (k < p.K) a0 = *reinterpret_cast<const uint4_t*>(a);
-        if (k + 64 < p.K) a1 = *reinterpret_cast<const uint4_t*>(a + 64);
-        sa = p.a_scales[static_cast<int64_t>(b) * p.M + m];
-      }
       Piece<EXACT> ap[2];
-      ap[0].set(a0);
-      ap[1].set(a1);
-      acc[t] += block_product(wp, ap) * (sa * sw);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) ap[h].set(*reinterpret_cast<const uint4_t*>(mine + buf * STAGE + t * kTileBytes + a_at[h]));
+      const float s = sa[buf][t] * sw[buf];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const float4_t c = block_product(wp[j], ap);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t][j][e] = fmaf(c[e], s, acc[t][j][e]);
+      }
     }
+  };
+  int b = first + wave;
+  if (b < last) {
+    load(b, 0);
+    for (; b + KW < last; b += 2 * KW) {
+      block(b, 0);
+      block(b + KW, 1);
+    }
+    if (b < last) block(b, 0);
   }
-  __shared__ __align__(16) float4_t part[KW > 1 ? KW - 1 : 1][MT][64];
+  wait_vm<0>();     // nothing is on its way to LDS
+  __syncthreads();  // where the sums lie now
+  float4_t* part = reinterpret_cast<float4_t*>(lds);
   if (wave > 0) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) part[wave - 1][t][lane] = acc[t];
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) part[((wave - 1) * MT * NT + t * NT + j) * 64 + lane] = acc[t][j];
   }
   __syncthreads();
-  // Wavefront t adds up and stores row tile t (all of them wavefront 0 where there are fewer wavefronts).
-  if (wave > 0) return;
+  // The wavefronts take the tiles of Y in turn: their sums in the wavefronts' order.
+  if (wave == 0) {
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-    for (int i = 0; i < KW - 1; ++i) acc[t] += part[i][t][lane];
-    const int m = 16 * t + r, n = 16 * tile + 4 * g;
-    if (m < p.M && n < p.N) store4(p, m, n, acc[t]);
+      for (int j = 0; j < NT; ++j) part[((KW - 1) * MT * NT + t * NT + j) * 64 + lane] = acc[t][j];
+  }
+  if constexpr (MT * NT > 1) __syncthreads();
+  for (int i = wave; i < MT * NT; i += KW) {
+    float4_t sum = part[((KW - 1) * MT * NT + i) * 64 + lane];
+#pragma unroll
+    for (int k = 0; k < KW - 1; ++k) sum += part[(k * MT * NT + i) * 64 + lane];
+    const int m = m0 + 16 * (i / NT) + r, n = static_cast<int>(tile_row(tile + i % NT, 4 * g));
+    if (m < p.M && n < p.N) store4(p, m, n, sum);
   }
 }
 
-// At most N (below 16) vector-memory operations of this thread outstanding, and no LDS operation.
-template <int N>
-__device__ __forceinline__ void wait_vm() {
-  __builtin_amdgcn_s_waitcnt(N | (7 << 4));
+// A wavefront's outputs. A lane holds eight consecutive columns of a row for each pair of tiles, but its
+// neighbours other rows: the lanes trade (l = 16 g + r's answers go to lane 4 r + g), so that four lanes
+// in a row write a row's 32 columns and a store is 16 lines' work, not 64. Where rows of Y do not lie on 16 bytes they
+// go through LDS (`own`, kOwnBytes of the wavefront's), and half a wavefront writes a row's 32 columns one each.
+constexpr int kOwnPitch = 36, kOwnBytes = 16 * kOwnPitch * 4;
+
+template <int DT, bool PART, int TM, int TN>
+__device__ __forceinline__ void gemm_outputs(const F8Args& p, const float4_t (&acc)[TM][TN], int m_wave, int n_wave, uint8_t* own) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, to_r = lane >> 2, to_g = lane & 3;
+  const int source = 4 * (16 * to_g + to_r);
+  auto trade = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(source, static_cast<int>(v))); };
+  constexpr int SIZE = DT == DT_F32 ? 4 : 2;
+  char* base = PART ? reinterpret_cast<char*>(p.part + static_cast<int64_t>(blockIdx.z) * p.M * p.N) : static_cast<char*>(p.y);
+  const int64_t ld = PART ? p.N : p.ldy;
+  const bool on16 = (reinterpret_cast<uintptr_t>(base) | static_cast<uintptr_t>(ld * SIZE)) % 16 == 0;
+  if (!on16) __syncthreads();  // every wavefront has read the last of A, and no load of A is on its way
+#pragma unroll
+  for (int jp = 0; jp < TN / 2; ++jp) {
+    const int n_pair = n_wave + 32 * jp, from = n_pair + 8 * g, n = n_pair + 8 * to_g;
+    float bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bias[e] = 0.f;
+    if (!PART && p.bias) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (from + e < p.N) bias[e] = load_float_rt(p.bias, p.bias_dtype, from + e);
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = acc[i][2 * jp + (e >> 2)][e & 3] + bias[e];
+      if (!on16) {
+        float* rows = reinterpret_cast<float*>(own);
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          *reinterpret_cast<float4_t*>(rows + r * kOwnPitch + 8 * g + e) = float4_t{v[e], v[e + 1], v[e + 2], v[e + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int m = m_wave + 16 * i + 2 * k + (lane >> 5), col = lane & 31;
+          const float x = rows[(2 * k + (lane >> 5)) * kOwnPitch + col];
+          if (m < p.M && n_pair + col < p.N) store_as<DT>(base, m * ld + n_pair + col, x);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        continue;
+      }
+      uint32_t w[2 * SIZE];
+#pragma unroll
+      for (int e = 0; e < 2 * SIZE; ++e) w[e] = trade(SIZE == 4 ? __builtin_bit_cast(uint32_t, v[e]) : pack2<DT>(v[(2 * e) & 7], v[(2 * e + 1) & 7]));
+      const int m = m_wave + 16 * i + to_r;
+      if (m >= p.M || n >= p.N) continue;
+      char* out = base + (m * ld + n) * SIZE;
+      if (n + 8 <= p.N) {
+#pragma unroll
+        for (int e = 0; e < SIZE / 2; ++e) *reinterpret_cast<uint4_t*>(out + 16 * e) = uint4_t{w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]};
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (n + e >= p.N) continue;
+          if constexpr (SIZE == 4) reinterpret_cast<uint32_t*>(out)[e] = w[e];
+          else reinterpret_cast<uint16_t*>(out)[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+        }
+      }
+    }
+  }
 }
 
 // Many rows: BM rows of A times BN of W a workgroup, WM x WN wavefronts of (BM / WM) x (BN / WN) outputs each.
-// A step is one block of K: both operands' bytes go global -> LDS (buffer_load ... lds) in the order of the MFMA
-// operands, 1 KiB an instruction, a step ahead, and each wavefront reads its fragments back 16 bytes a lane in a
-// row, without conflicts. Offsets are scalar along k; what lies past M, N or K is past the buffers' ranges and
-// arrives as zeros.
+// A step is one block of K. A's bytes go global -> LDS (buffer_load ... lds) in the order of the MFMA operands,
+// 1 KiB an instruction, two steps ahead, with the step's row scales; W's tiles, which are operands as they lie, go
+// to registers a step ahead and past LDS, whose reads would bound the loop otherwise. What lies past M, N or K is
+// past the buffers' ranges and arrives as zeros.
 template <int BM, int BN, int WM, int WN, bool EXACT>
-__global__ __launch_bounds__(64 * WM * WN) void k_f8_gemm(F8Args p) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   constexpr int NW = WM * WN, TM = BM / 16 / WM, TN = BN / 16 / WN;
-  constexpr int A_TILES = BM / 16, W_TILES = BN / 16;
-  constexpr int STAGE = (A_TILES + W_TILES) * kTileBytes;
-  constexpr int A_DMA = 2 * A_TILES / NW, W_DMA = 2 * W_TILES / NW;
-  static_assert(A_DMA * NW == 2 * A_TILES && W_DMA * NW == 2 * W_TILES, "whole instructions a wavefront");
-  extern __shared__ __align__(16) uint8_t lds[];
+  constexpr int A_TILES = BM / 16, A_DMA = 2 * A_TILES / NW;
+  constexpr int STAGE = A_TILES * kTileBytes;
+  static_assert(A_DMA * NW == 2 * A_TILES && BM % 64 == 0 && TN % 2 == 0, "whole instructions a wavefront, pairs of tiles");
+  static_assert(NW * kOwnBytes <= 3 * STAGE, "the outputs' way through LDS");
+  extern __shared__ __align__(16) uint8_t lds[];  // [3][STAGE], then the rows' scales [3][BM]
+  float* lds_s = reinterpret_cast<float*>(lds + 3 * STAGE);
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  // Workgroups go to the eight XCDs in turn: XCD x takes a run of the tiles, in an order that walks groups of four
+  // Workgroups go to the eight XCDs in turn: XCD x takes a run of the tiles, in an order that walks groups of eight
   // row tiles, rows fastest, so that an XCD's tiles share few rows of A and of W (its own L2).
-  uint32_t tile = blockIdx.y * gridDim.x + blockIdx.x;
-  const uint32_t tiles = gridDim.x * gridDim.y;
+  const uint32_t cols = static_cast<uint32_t>((p.N + BN - 1) / BN), rows = static_cast<uint32_t>((p.M + BM - 1) / BM), tiles = cols * rows;
+  uint32_t tile = blockIdx.x;
   if (tiles >= 8) {
     const uint32_t per = tiles / 8;
     if (tile < 8 * per) tile = (tile % 8) * per + tile / 8;
   }
-  const uint32_t group = tile / (4 * gridDim.x), first_m = 4 * group;
-  const uint32_t group_m = min(4u, gridDim.y - first_m), in_group = tile - group * 4 * gridDim.x;
+  const uint32_t group = tile / (8 * cols), first_m = 8 * group;
+  const uint32_t group_m = min(8u, rows - first_m), in_group = tile - group * 8 * cols;
   const int m0 = static_cast<int>(first_m + in_group % group_m) * BM;
   const int n0 = static_cast<int>(in_group / group_m) * BN;
   const int64_t a_bytes = (static_cast<int64_t>(p.M) - m0 - 1) * p.lda + p.K;
@@ -246,119 +384,262 @@ __global__ __launch_bounds__(64 * WM * WN) void k_f8_gemm(F8Args p) {
   const auto a_rsrc = buffer_rsrc(p.a + m0 * p.lda, static_cast<uint32_t>(min(a_bytes, int64_t{0x7FFFFFF0})));
   const auto w_rsrc = buffer_rsrc(p.w + static_cast<int64_t>(n0 / 16) * p.kb * kTileBytes,
                                   static_cast<uint32_t>(min(w_bytes, int64_t{0x7FFFFFF0})));
-  // Instruction j of this wavefront fills half h of tile t, 2 t + h = A_DMA * wave + j.
-  uint32_t a_off[A_DMA], w_off[W_DMA];
+  // Instruction j of this wavefront fetches rows 8 i .. 8 i + 7, i = A_DMA * wave + j: eight lanes to a row's 128
+  // bytes, one line, which the cache then looks up once (16 bytes of 64 rows each would be 64 lookups). Chunk c (16
+  // bytes) of a row lies at place c ^ (row % 8) of its 128 bytes in LDS, so that the fragments' reads below meet no
+  // bank twice.
+  // (A row past M starts past the range by itself.)
+  const int a_row = 8 * A_DMA * wave + (lane >> 3), a_chunk = (lane & 7) ^ (lane >> 3);
+  const uint32_t a_off = static_cast<uint32_t>(a_row * p.lda) + 16 * a_chunk, a_rows = static_cast<uint32_t>(8 * p.lda);
+  // (Tiles past the last are the last again: their columns are not stored.)
+  uint32_t w_off[TN];
 #pragma unroll
-  for (int j = 0; j < A_DMA; ++j) {
-    const int i = A_DMA * wave + j, row = 16 * (i >> 1) + r;
-    // A row past M starts past the range by itself; one before the last may not run on into the next.
-    a_off[j] = m0 + row < p.M ? static_cast<uint32_t>(row * p.lda) + 64 * (i & 1) + 16 * g : 0x80000000u;
-  }
-#pragma unroll
-  for (int j = 0; j < W_DMA; ++j) {
-    const int i = W_DMA * wave + j;
-    w_off[j] = n0 / 16 + (i >> 1) < p.tiles ? static_cast<uint32_t>(i >> 1) * p.kb * kTileBytes + (i & 1) * 1024 + lane * 16 : 0x80000000u;
-  }
+  for (int j = 0; j < TN; ++j)
+    w_off[j] = static_cast<uint32_t>(min(wn * TN + j, p.tiles - 1 - n0 / 16)) * static_cast<uint32_t>(p.kb) * kTileBytes;
   const int first = blockIdx.z * p.per, last = min(first + p.per, p.kb);
-  auto issue = [&](int b) {
-    uint8_t* sa = lds + ((b - first) & 1) * STAGE;
-    uint8_t* sw = sa + A_TILES * kTileBytes;
-    const uint32_t k0 = static_cast<uint32_t>(b) * kF8Block;
-    if (b * kF8Block + kF8Block <= p.K) {
-#pragma unroll
-      for (int j = 0; j < A_DMA; ++j) lds_dma16(a_rsrc, sa + (A_DMA * wave + j) * 1024, a_off[j], k0);
+  const int n_wave = n0 + wn * (BN / WN), m_wave = m0 + wm * (BM / WM);
+  // The wavefront's columns lie in one block of 128 rows of W (n0 and BN / WN divide it).
+  const float* ws = p.w_scales + static_cast<int64_t>(min(n_wave, p.N - 1) / kF8Block) * p.kb;
+  const int s_part = wave % (BM / 64);
+  uint4_t wr[2][TN][2];
+  float sw[2];
+  // The loads of a step, one at a time: W's tiles of block b + 1, then A's rows and scales of block b + 2. (No
+  // branches, which the compiler would move the products' FMAs behind: past the last block the loads of A have no
+  // range and those of W and the scales are the last block's again.)
+  constexpr int LOADS_W = 2 * TN + 1, LOADS_A = A_DMA + 1;
+  auto load_w = [&](int q, int at, int buf) {
+    const int b = min(at, last - 1);
+    if (q < 2 * TN)
+      wr[buf][q >> 1][q & 1] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(
+          w_rsrc, lane * 16 + 1024 * (q & 1), w_off[q >> 1] + static_cast<uint32_t>(b) * kTileBytes, 0));
+    else
+      sw[buf] = ws[b];
+  };
+  auto load_a = [&](int q, int b, int slot) {
+    if (q < A_DMA) {
+      const int k0 = b < last ? b * kF8Block : 0, left = b < last ? p.K - k0 : 0;
+      lds_dma16(a_rsrc, lds + slot * STAGE + (A_DMA * wave + q) * 1024, 16 * a_chunk < left ? a_off + q * a_rows : 0x80000000u, static_cast<uint32_t>(k0));
     } else {
-#pragma unroll
-      for (int j = 0; j < A_DMA; ++j) {
-        const int i = A_DMA * wave + j;
-        const bool in = static_cast<int>(k0) + 64 * (i & 1) + 16 * g < p.K;
-        lds_dma16(a_rsrc, sa + i * 1024, in ? a_off[j] + (a_off[j] < 0x80000000u ? k0 : 0u) : 0x80000000u, 0);
-      }
+      const auto s_rsrc = buffer_rsrc(p.a_scales + static_cast<int64_t>(min(b, last - 1)) * p.M + m0, static_cast<uint32_t>(min(BM, p.M - m0)) * 4);
+      // (Where there are more wavefronts than 64 rows each, several load the same scales.)
+      lds_dma4(s_rsrc, reinterpret_cast<uint8_t*>(lds_s + slot * BM + s_part * 64), (s_part * 64 + lane) * 4, 0);
     }
-#pragma unroll
-    for (int j = 0; j < W_DMA; ++j)
-      lds_dma16(w_rsrc, sw + (W_DMA * wave + j) * 1024, w_off[j], static_cast<uint32_t>(b) * kTileBytes);
   };
-  auto barrier = [&]() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
+  const uint32_t a_at[2] = {static_cast<uint32_t>(r * 128 + 16 * (g ^ (r & 7))), static_cast<uint32_t>(r * 128 + 16 * ((g + 4) ^ (r & 7)))};
   float4_t acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
-  const int m_wave = m0 + wm * (BM / WM), n_wave = n0 + wn * (BN / WN);
-  // The wavefront's columns lie in one block of 128 rows of W (n0 and BN / WN divide it).
-  const float* ws = p.w_scales + static_cast<int64_t>(min(n_wave, p.N - 1) / kF8Block) * p.kb;
-  int sa_row[TM];
+  int slot = 0;
+  auto step = [&](int b, int buf) {
+    // The youngest outstanding loads are those of the next step's A: this step's W, scales and A are there.
+    wait_vm<A_DMA + 1>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // everybody's; and everybody has read the stage that is filled next
+    asm volatile("" ::: "memory");
+    const int free_slot = slot == 0 ? 2 : slot - 1;
+    auto load = [&](int q) {
+      if (q < LOADS_W) load_w(q, b + 1, buf ^ 1);
+      else load_a(q - LOADS_W, b + 2, free_slot);
+    };
+    const uint8_t* la = lds + slot * STAGE + wm * TM * kTileBytes;
+    const float* ls = lds_s + slot * BM + wm * (BM / WM) + r;
+    auto load_af = [&](int i, Piece<EXACT> (&af)[2]) {
 #pragma unroll
-  for (int i = 0; i < TM; ++i) sa_row[i] = min(m_wave + 16 * i + r, p.M - 1);
-  if (first < last) issue(first);
-  for (int b = first; b < last; ++b) {
-    float sa[TM];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) sa[i] = p.a_scales[static_cast<int64_t>(b) * p.M + sa_row[i]];
-    const float sw = ws[b];
-    wait_vm<0>();  // this step's stage, and its scales
-    barrier();     // everybody's; and everybody has read the stage that the next issue overwrites
-    if (b + 1 < last) issue(b + 1);
-    const uint8_t* la = lds + ((b - first) & 1) * STAGE + wm * TM * kTileBytes + lane * 16;
-    const uint8_t* lw = lds + ((b - first) & 1) * STAGE + (A_TILES + wn * TN) * kTileBytes + lane * 16;
+      for (int h = 0; h < 2; ++h) af[h].set(*reinterpret_cast<const uint4_t*>(la + i * kTileBytes + a_at[h]));
+    };
     Piece<EXACT> wf[TN][2];
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) wf[j][h].set(*reinterpret_cast<const uint4_t*>(lw + j * kTileBytes + h * 1024));
+      for (int h = 0; h < 2; ++h) wf[j][h].set(wr[buf][j][h]);
+    if constexpr (EXACT) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      Piece<EXACT> af[2];
+      for (int q = 0; q < LOADS_W + LOADS_A; ++q) load(q);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) af[h].set(*reinterpret_cast<const uint4_t*>(la + i * kTileBytes + h * 1024));
-      const float s = sa[i] * sw;
+      for (int i = 0; i < TM; ++i) {
+        Piece<EXACT> af[2];
+        load_af(i, af);
+        const float s = ls[16 * i] * sw[buf];
+        float4_t c[TN];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const float4_t c = block_product(wf[j], af);
+        for (int j = 0; j < TN; ++j) c[j] = block_product(wf[j], af);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(c[e], s, acc[i][j][e]);
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(c[j][e], s, acc[i][j][e]);
+      }
+    } else {
+      // A product's four FMAs come three products later, when it has left the matrix unit, a fragment is read while
+      // the one before it is multiplied, and the loads are spread over the step (in a row they would hold
+      // the wavefronts up until the address unit has taken them all): in this order, which the compiler would give
+      // up to save registers.
+      constexpr int LAG = 3, ALL = TM * TN, LOADS = LOADS_W + LOADS_A;
+      Piece<EXACT> af[2][2];
+      constexpr int SR = (LAG + TN - 1) / TN + 1;  // rows whose scales the pending FMAs hold
+      float sr[2], s[SR];
+      float4_t c[LAG + 1];
+      load_af(0, af[0]);
+      sr[0] = ls[0];
+#pragma unroll
+      for (int t = 0; t < ALL + LAG; ++t) {
+        const int i = t / TN, j = t % TN;
+        if (t < ALL) {
+          if (j == 0 && i + 1 < TM) {
+            load_af(i + 1, af[(i + 1) & 1]);
+            sr[(i + 1) & 1] = ls[16 * (i + 1)];
+          }
+#pragma unroll
+          for (int q = (t * LOADS + ALL - 1) / ALL; q < ((t + 1) * LOADS + ALL - 1) / ALL; ++q) load(q);
+          c[t % (LAG + 1)] = block_product(wf[j], af[i & 1]);
+          if (j == 0) s[i % SR] = sr[i & 1] * sw[buf];
+        }
+        if (t >= LAG) {
+          const int u = t - LAG;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[u / TN][u % TN][e] = fmaf(c[u % (LAG + 1)][e], s[u / TN % SR], acc[u / TN][u % TN][e]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-  }
+    slot = slot == 2 ? 0 : slot + 1;
+  };
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = m_wave + 16 * i + r;
-    if (m >= p.M) continue;
+  for (int q = 0; q < LOADS_A; ++q) load_a(q, first, 0);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int n = n_wave + 16 * j + 4 * g;
-      if (n < p.N) store4(p, m, n, acc[i][j]);
-    }
+  for (int q = 0; q < LOADS_W; ++q) load_w(q, first, 0);
+#pragma unroll
+  for (int q = 0; q < LOADS_A; ++q) load_a(q, first + 1, 1);
+  int b = first;
+  for (; b + 1 < last; b += 2) {
+    step(b, 0);
+    step(b + 1, 1);
   }
+  if (b < last) step(b, 0);
+  wait_vm<0>();  // nothing is on its way to LDS when the workgroup ends
+  if (p.part) gemm_outputs<DT_F32, true, TM, TN>(p, acc, m_wave, n_wave, lds + wave * kOwnBytes);
+  else if (EXACT) gemm_outputs<DT_F32, false, TM, TN>(p, acc, m_wave, n_wave, lds + wave * kOwnBytes);
+  else if (p.y_dtype == DT_F16) gemm_outputs<DT_F16, false, TM, TN>(p, acc, m_wave, n_wave, lds + wave * kOwnBytes);
+  else gemm_outputs<DT_BF16, false, TM, TN>(p, acc, m_wave, n_wave, lds + wave * kOwnBytes);
 }
 
-// Y = the sum of the parts (+ bias), in order.
+// Y = the sum of the parts (+ bias), in order. A thread takes four columns (their parts lie on 16 bytes where four
+// divides N).
 __global__ __launch_bounds__(256) void k_f8_reduce(F8Args p) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int quads = (p.N + 3) / 4;
+  const int64_t m = i / quads;
+  if (m >= p.M) return;
+  const int n = static_cast<int>(i - m * quads) * 4;
   const int64_t all = static_cast<int64_t>(p.M) * p.N;
-  if (i >= all) return;
-  float v = p.part[i];
-  for (int s = 1; s < p.splits; ++s) v += p.part[s * all + i];
-  const int64_t m = i / p.N;
-  const int n = static_cast<int>(i - m * p.N);
-  if (p.bias) v += load_float_rt(p.bias, p.bias_dtype, n);
-  store_float_rt(p.y, p.y_dtype, m * p.ldy + n, v);
+  const float* part = p.part + m * p.N + n;
+  float4_t v{0.f, 0.f, 0.f, 0.f};
+  if (p.N % 4 == 0) {
+    v = *reinterpret_cast<const float4_t*>(part);
+#pragma unroll 4
+    for (int s = 1; s < p.splits; ++s) v += *reinterpret_cast<const float4_t*>(part + s * all);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      for (int s = 0; s < p.splits && n + e < p.N; ++s) v[e] += part[s * all + e];
+  }
+  F8Args q = p;
+  q.part = nullptr;
+  store4(q, m, n, v);
+}
+
+// The kernels of a product, and how many parts K is cut into.
+enum : int { ROWS16, ROWS16_WIDE, ROWS32, ROWS32_WIDE, ROWS64, GEMM_64x64, GEMM_64x128, GEMM_128x128, GEMM_128x256 };
+struct F8Plan {
+  int kernel, splits;
+};
+
+// One workgroup's step of 128 of K, in us: alone on its CU (the loads' latency), and with the CU full (the matrix
+// and memory units), as measured over K at sizes that fill the chip once and several times.
+struct F8Shape {
+  int kernel, bm, bn;
+  float alone[2], full[2];  // for a 16-bit Y, and for an f32 Y
+};
+constexpr F8Shape kF8Shapes[] = {
+    {GEMM_64x64, 64, 64, {0.26f, 0.50f}, {0.19f, 0.35f}},
+    {GEMM_64x128, 64, 128, {0.36f, 0.94f}, {0.32f, 0.53f}},
+    {GEMM_128x128, 128, 128, {0.60f, 1.40f}, {0.52f, 1.00f}},
+    {GEMM_128x256, 128, 256, {0.95f, 0.f}, {0.87f, 0.f}},  // (its f32 form's registers would not fit)
+};
+
+// The kernel by what it is expected to take: k_f8_rows up to 32 rows; above, the least of its four row tiles and
+// k_f8_gemm's shapes. Parts of K cost their sums' way to memory and back (4.5 TB/s) and the second launch (2.4 us). Measured, us
+// (f16 Y): 64 rows 2048 -> 2048 4.2 by ROWS64, 6.5 by 64x64, 7.8 by 64x128; 2048 -> 22016 10.7 by 64x64, 15.0 by ROWS64
+// with two column tiles; 128 rows 11008 -> 2048 14.1 by 64x64 in 8 parts, 15.7 in 4, 39.6 in one of 64x128; 512 rows 2048
+// -> 2048 6.9 by 64x64, 11.1 by 128x128; 512 rows 2048 -> 22016 27.0 by 128x128, 28.3 by 128x256, 43.9 by 64x64; 4096 rows 11008 -> 2048
+// 81 by 128x256, 87 by 128x128, 119 by a tile of 256 x 256, which no size was best with.
+F8Plan plan_of(int64_t M, int64_t N, int kb, int64_t tiles, bool f32, int num_cus) {
+  // Two column tiles a wavefront read A half as often: with four workgroups a CU to hide the longer steps (2048 -> 22016, one
+  // row 8.3 us, 8.8 with one tile, 24 rows 9.3, 10.8); with fewer one is better (2048 -> 2048, 24 rows 3.7, 3.3 with one).
+  const bool wide = tiles >= 4 * num_cus;
+  if (M <= 32) return {M <= 16 ? (wide ? ROWS16_WIDE : ROWS16) : (wide ? ROWS32_WIDE : ROWS32), 1};
+  F8Plan best{GEMM_128x128, 1};
+  double least = 1e30;
+  auto offer = [&](int kernel, int splits, double us) {
+    if (splits > 1) us += 2.4 + 8.0 * splits * static_cast<double>(M) * static_cast<double>(N) / 4.5e6;
+    if (us < least) {
+      least = us;
+      best = {kernel, splits};
+    }
+  };
+  for (int splits = 1; splits <= 8; splits *= 2) {
+    const int per = (kb + splits - 1) / splits;
+    if (splits > 1 && per < 4) break;
+    const double row_groups = static_cast<double>(tiles * ((M + 63) / 64) * splits) / num_cus;
+    offer(ROWS64, splits, 2.4 + 0.9 * ((per + 7) / 8) * std::max(1.0, std::ceil(row_groups)));
+    for (const F8Shape& f : kF8Shapes) {
+      if (f.full[f32] == 0.f) continue;
+      const double groups = static_cast<double>((M + f.bm - 1) / f.bm * ((N + f.bn - 1) / f.bn) * splits) / num_cus;
+      const double step = std::max<double>(f.alone[f32], f.full[f32] * (groups <= 4 ? std::ceil(groups) : groups + 0.4));
+      offer(f.kernel, splits, 2.6 + step * per);
+    }
+  }
+  return best;
+}
+
+template <int MT, int NT, int KW, bool EXACT>
+void launch_rows(const F8Args& p, hipStream_t s) {
+  // The wavefronts' stages of A, and in their place (or past it) their sums.
+  constexpr int kLds = KW * MT * std::max(2 * kTileBytes, NT * 1024);
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_f8_rows<MT, NT, KW, EXACT>),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  (void)attr;
+  const dim3 grid(static_cast<unsigned>(p.tiles / NT) * static_cast<unsigned>((p.M + 16 * MT - 1) / (16 * MT)), 1, static_cast<unsigned>(p.splits));
+  k_f8_rows<MT, NT, KW, EXACT><<<grid, 64 * KW, kLds, s>>>(p);
 }
 
 template <int BM, int BN, int WM, int WN, bool EXACT>
 void launch_gemm(const F8Args& p, hipStream_t s) {
-  constexpr int kLds = 2 * (BM + BN) / 16 * kTileBytes;
+  constexpr int kLds = 3 * (BM / 16 * kTileBytes + 4 * BM);
   static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_f8_gemm<BM, BN, WM, WN, EXACT>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   (void)attr;
-  const dim3 grid(static_cast<unsigned>((p.N + BN - 1) / BN), static_cast<unsigned>((p.M + BM - 1) / BM),
+  const dim3 grid(static_cast<unsigned>((p.N + BN - 1) / BN) * static_cast<unsigned>((p.M + BM - 1) / BM), 1,
                   static_cast<unsigned>(p.splits));
   k_f8_gemm<BM, BN, WM, WN, EXACT><<<grid, 64 * WM * WN, kLds, s>>>(p);
+}
+
+template <bool F32>
+void launch_plan(const F8Plan& plan, const F8Args& p, hipStream_t s) {
+  switch (plan.kernel) {
+    case ROWS16: launch_rows<1, 1, 8, F32>(p, s); break;
+    case ROWS16_WIDE: launch_rows<1, 2, 8, F32>(p, s); break;
+    case ROWS32: launch_rows<2, 1, 8, F32>(p, s); break;
+    case ROWS32_WIDE: launch_rows<2, 2, 8, F32>(p, s); break;
+    case ROWS64: launch_rows<4, 1, 8, F32>(p, s); break;
+    case GEMM_64x64: launch_gemm<64, 64, 2, 2, F32>(p, s); break;
+    case GEMM_64x128: launch_gemm<64, 128, 1, 4, F32>(p, s); break;
+    case GEMM_128x128: launch_gemm<128, 128, 1, 4, F32>(p, s); break;
+    case GEMM_128x256:
+      if constexpr (!F32) launch_gemm<128, 256, 1, 4, false>(p, s);
+      break;
+  }
 }
 
 }  // namespace
@@ -377,7 +658,7 @@ int tmh_fp8_weight_prepare(tmh_ctx* ctx, const void* d_b, const float* d_scales,
     return fail(ctx, TMH_ERR_UNSUPPORTED, "an 8-bit weight's K and N must be at most 2^22, got %lld, %lld", (long long)K, (long long)N);
   TMH_TRY(use_device(ctx));
   if (!d_b || !d_scales) return fail(ctx, TMH_ERR_INVALID, "tmh_fp8_weight_prepare: NULL pointer");
-  const int64_t kb = (K + kF8Block - 1) / kF8Block, tiles = (N + 15) / 16;
+  const int64_t kb = (K + kF8Block - 1) / kF8Block, tiles = (N + 31) / 32 * 2;
   auto* w = new (std::nothrow) tmh_fp8_weight();
   if (!w) return fail(ctx, TMH_ERR_OOM, "tmh_fp8_weight_prepare: out of host memory");
   w->device = ctx->device;
@@ -461,30 +742,31 @@ int tmh_matmul_fp8(tmh_ctx* ctx, const tmh_fp8_weight* w, const void* d_a, int64
   p.tiles = static_cast<int>(w->tiles);
   p.bias_dtype = bias_dtype;
   p.y_dtype = y_dtype;
-  p.splits = 1;
-  p.per = p.kb;
+  const F8Plan plan = plan_of(M, w->N, p.kb, w->tiles, y_dtype == TMH_F32, ctx->num_cus);
+  p.per = (p.kb + plan.splits - 1) / plan.splits;
+  p.splits = (p.kb + p.per - 1) / p.per;  // (no part is empty)
   const bool pad = w->K % 16 != 0 || lda % 16 != 0 || reinterpret_cast<uintptr_t>(d_a) % 16 != 0;
   const int64_t Kp = (w->K + 15) / 16 * 16;
   const size_t pad_bytes = pad ? static_cast<size_t>(M * Kp + 255) / 256 * 256 : 0;
-  if (pad_bytes) {
-    void* ws = workspace(ctx, pad_bytes, s);
+  const size_t part_bytes = p.splits > 1 ? static_cast<size_t>(p.splits) * M * w->N * sizeof(float) : 0;
+  uint8_t* ws = nullptr;
+  if (pad_bytes + part_bytes) {
+    ws = static_cast<uint8_t*>(workspace(ctx, pad_bytes + part_bytes, s));
     if (!ws) return fail(ctx, TMH_ERR_UNSUPPORTED, "the 8-bit product's workspace cannot grow here: run one call before the capture");
-    k_f8_pad_rows<<<static_cast<unsigned>((M * (Kp / 16) + 255) / 256), 256, 0, s>>>(p.a, lda, M, w->K, Kp, static_cast<uint8_t*>(ws));
+    if (part_bytes) p.part = reinterpret_cast<float*>(ws + pad_bytes);
+  }
+  if (pad) {
+    k_f8_pad_rows<<<static_cast<unsigned>((M * (Kp / 16) + 255) / 256), 256, 0, s>>>(p.a, lda, M, w->K, Kp, ws);
     TMH_TRY(check_launch(ctx, "k_f8_pad_rows"));
-    p.a = static_cast<const uint8_t*>(ws);
+    p.a = ws;
     p.lda = Kp;
     p.K = static_cast<int>(Kp);
   }
-  const unsigned tiles = static_cast<unsigned>(p.tiles);
-  if (y_dtype == TMH_F32) {
-    if (M <= 16) k_f8_rows<1, 8, true><<<tiles, 512, 0, s>>>(p);
-    else if (M <= 32) k_f8_rows<2, 8, true><<<tiles, 512, 0, s>>>(p);
-    else launch_gemm<128, 128, 2, 2, true>(p, s);
-  } else {
-    if (M <= 16) k_f8_rows<1, 8, false><<<tiles, 512, 0, s>>>(p);
-    else if (M <= 32) k_f8_rows<2, 8, false><<<tiles, 512, 0, s>>>(p);
-    else if (M <= 128) launch_gemm<128, 128, 2, 2, false>(p, s);
-    else launch_gemm<256, 256, 2, 4, false>(p, s);
+  if (y_dtype == TMH_F32) launch_plan<true>(plan, p, s);
+  else launch_plan<false>(plan, p, s);
+  if (p.splits > 1) {
+    TMH_TRY(check_launch(ctx, "k_f8_gemm"));
+    k_f8_reduce<<<static_cast<unsigned>((M * ((w->N + 3) / 4) + 255) / 256), 256, 0, s>>>(p);
   }
   return check_launch(ctx, "k_f8_gemm");
 }

@@ -31,6 +31,9 @@ struct tmh_ctx {
   // kernel arguments, so they stay allocated until the context is destroyed.
   std::vector<void*> ws_retired;
   tmh_timeline_state* tl = nullptr;  // while a timeline is recorded
+  // Counters of workgroups that meet within a kernel (2 a compute unit): zero between calls, the last of those that
+  // meet clears theirs.
+  uint32_t* meet = nullptr;
 };
 
 // Tiled device layout of a MatMulNBits weight.

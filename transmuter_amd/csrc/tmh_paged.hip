@@ -2,6 +2,7 @@
 // (tmh_paged_append), and attention of one new token a sequence over its pages (tmh_paged_attention).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "tmh_f8.h"
 #include "tmh_internal.h"
@@ -125,6 +126,9 @@ void launch_append(const AppendArgs& p, int64_t T, bool vec, bool table_vec, hip
 
 constexpr int kHeads = 16;  // query heads of one kv head that a workgroup answers (the columns of an MFMA tile)
 constexpr float kNone = -__builtin_inff();
+constexpr int64_t kJoinBytes = 72 << 10;
+constexpr int kThrough = 16;  // sc1 of a buffer access: past the XCD's L2, to where all XCDs meet
+typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 
 struct AttendArgs {
   const void* q;
@@ -135,6 +139,8 @@ struct AttendArgs {
   void* y;
   float* part;    // [2 workers][heads of an item][head_dim], then their (maximum, sum) pairs
   float2* stats;
+  uint32_t part_bytes, stats_bytes;
+  uint32_t* meet;  // [workers] parts of the item that begins in a worker, kept so far; zero between calls
   int64_t ldq, ldy, max_pages;
   PageShape cache;
   int64_t head_stride;
@@ -160,6 +166,15 @@ __device__ __forceinline__ uint32_t units_before(const AttendArgs& p, int b) {
   return n;
 }
 
+__device__ __forceinline__ uint32_t scan64(uint32_t v) {  // the sum over the lanes up to this one
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t up = __shfl_up(v, o);
+    if ((threadIdx.x & 63) >= o) v += up;
+  }
+  return v;
+}
+
 // The sequence whose units hold `target` (below the total), and the units before it.
 template <int UT>
 __device__ __forceinline__ int find_sequence(const AttendArgs& p, uint32_t target, uint32_t& before) {
@@ -167,12 +182,7 @@ __device__ __forceinline__ int find_sequence(const AttendArgs& p, uint32_t targe
   uint32_t base = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     const uint32_t mine = b0 + lane < p.B ? static_cast<uint32_t>(span_at<UT>(p, b0 + lane).units) : 0;
-    uint32_t sum = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t up = __shfl_up(sum, o);
-      if (lane >= o) sum += up;
-    }
+    const uint32_t sum = scan64(mine);
     const uint64_t past = __ballot(base + sum > target);
     if (past) {
       const int at = __builtin_ctzll(past);
@@ -258,29 +268,79 @@ __device__ __forceinline__ float column_sum(float v) {
 // f16 parts are taken of 2^15 times the probability, so that small ones of long rows do not fall below f16's
 // range; f32 and bf16 ones of 2^-32 times it, so that sums of up to 2^31 values near the type's largest stay
 // finite. The factor is in the running sum too and drops out.
-template <int DT, int NB>  // NB: blocks of 16 E dimensions
-__global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void k_paged_attention(AttendArgs p) {
+//
+// What happens to items that several workers share:
+//  JOIN  they meet here. Each leaves its part in memory (stores that pass the XCD's own L2), then counts itself; the one that
+//        finds all others counted joins the parts in their order, whoever it is, so the answer does not depend on who comes
+//        last.
+//  PARTS k_paged_join joins them.
+//  WHOLE there are none: a workgroup of eight wavefronts takes an item, and looks at its own sequence's length only.
+enum : int { JOIN, PARTS, WHOLE };
+template <int DT, int NB, int HOW>  // NB: blocks of 16 E dimensions
+__global__ __launch_bounds__(HOW == WHOLE ? 512 : 256, NB == 1 || (DT == DT_F32 && NB == 2) ? 2 : 1) void k_paged_attention(AttendArgs p) {
   constexpr bool F32 = DT == DT_F32;
-  constexpr int SIZE = F32 ? 4 : 2, E = 16 / SIZE, TILE = F32 ? 16 : 32, UT = 4 * TILE;
+  constexpr int WAVES = HOW == WHOLE ? 8 : 4, THREADS = 64 * WAVES;
+  constexpr int SIZE = F32 ? 4 : 2, E = 16 / SIZE, TILE = F32 ? 16 : 32, UT = WAVES * TILE;
   constexpr int NH = TILE / 16;           // 16-token halves of a tile
   constexpr int NC = 4 * NB;              // chunks of 4 E dimensions of a row
   constexpr int VT = F32 ? 4 : 8;         // tokens a lane reads of V
   constexpr float BIAS = DT == DT_F16 ? 15.f : -32.f;
   constexpr int ROW = 16 * E * NB + 4;    // floats of a head's answer in LDS (+ 4: off a bank's multiple)
-  __shared__ __align__(16) float lds_o[4][kHeads][ROW];
-  __shared__ float lds_m[4][kHeads], lds_l[4][kHeads];
+  __shared__ __align__(16) float lds_o[WAVES][kHeads][ROW];
+  __shared__ float lds_m[WAVES][kHeads], lds_l[WAVES][kHeads];
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t items = static_cast<uint32_t>(p.kv_heads * p.chunks);
-  const uint32_t all = units_before<UT>(p, p.B) * items;
-  const uint32_t per = units_per_worker(all, p.workers);
   const uint32_t worker = blockIdx.x;
-  uint32_t at = worker * per;
-  if (per == 0 || at >= all) return;
-  const uint32_t stop = min(at + per, all);
-  const uint32_t run = at;
-  uint32_t before;
-  int b = find_sequence<UT>(p, at / items, before);
+  [[maybe_unused]] const auto parts_rsrc = buffer_rsrc(p.part, p.part_bytes), stats_rsrc = buffer_rsrc(p.stats, p.stats_bytes);
+  auto store = [&](int b, int head, int dim, float4_t o) {
+    const int64_t out = b * p.ldy + static_cast<int64_t>(head) * p.head_dim + dim;
+    if constexpr (F32)
+      *reinterpret_cast<float4_t*>(static_cast<float*>(p.y) + out) = o;
+    else
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + out) = make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
+  };
+  if constexpr (HOW == JOIN) {  // zeros for the sequences without tokens
+    const int quads = p.group * p.kv_heads * p.head_dim / 4;
+    for (int b = static_cast<int>(worker); b < p.B; b += static_cast<int>(p.workers))
+      if (span_at<UT>(p, b).units == 0)
+        for (int i = threadIdx.x; i < quads; i += 256) store(b, 0, 4 * i, float4_t{0.f, 0.f, 0.f, 0.f});
+  }
+  uint32_t per = 0, at, stop, before = 0;
+  int b;
+  if constexpr (HOW == WHOLE) {
+    b = static_cast<int>(worker / items);
+    const uint32_t units = static_cast<uint32_t>(span_at<UT>(p, b).units), item = worker - b * items;
+    at = item * units;
+    stop = at + units;
+    if (units == 0) {
+      const int kv_head = static_cast<int>(item) / p.chunks, chunk = static_cast<int>(item) % p.chunks;
+      const int quads = min(kHeads, p.group - chunk * kHeads) * p.head_dim / 4;
+      for (int i = threadIdx.x; i < quads; i += THREADS) store(b, kv_head * p.group + chunk * kHeads, 4 * i, float4_t{0.f, 0.f, 0.f, 0.f});
+      return;
+    }
+  } else {
+    // Up to 64 sequences: one look at their lengths tells the total and where this worker's units are.
+    uint32_t mine = 0, upto = 0, all;
+    if (p.B <= 64) {
+      mine = lane < p.B ? static_cast<uint32_t>(span_at<UT>(p, lane).units) : 0;
+      upto = scan64(mine);
+      all = __shfl(upto, 63) * items;
+    } else {
+      all = units_before<UT>(p, p.B) * items;
+    }
+    per = units_per_worker(all, p.workers);
+    at = worker * per;
+    if (per == 0 || at >= all) return;
+    stop = min(at + per, all);
+    if (p.B <= 64) {
+      b = __builtin_ctzll(__ballot(upto > at / items));
+      before = __shfl(upto - mine, b);
+    } else {
+      b = find_sequence<UT>(p, at / items, before);
+    }
+  }
+  [[maybe_unused]] const uint32_t run = at;
   Span sp = span_at<UT>(p, b);
   uint32_t first = before * items;  // the first unit of the sequence's first item
   const int chunks_of_row = (p.head_dim + 4 * E - 1) / (4 * E);
@@ -316,40 +376,53 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void k_paged_attention(Attend
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[nb][e] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-    for (uint32_t u = from; u < to; ++u) {
-      const int base = (sp.unit + static_cast<int>(u)) * UT + wave * TILE;
-      if (base >= sp.end || base + TILE <= sp.begin) continue;
-      // Lane i looks token base + i % TILE up: its row's offset in bytes, 0 (a row of page 0) where it is masked.
-      const int token = base + lane % TILE;
-      bool ok = token >= sp.begin && token < sp.end;
-      int64_t offset = 0;
-      if (ok) {
-        offset = token_offset(p.cache, table, static_cast<uint32_t>(token)) * SIZE;
-        ok = offset >= 0;
-        if (!ok) offset = 0;
-      }
-      const uint32_t valid = static_cast<uint32_t>(__ballot(ok));  // (TILE 16: the four copies agree)
-      const bool full = TILE == 32 ? valid == 0xFFFFFFFFu : (valid & 0xFFFFu) == 0xFFFFu;
-      auto row_offset = [&](int tk) { return __shfl(offset, tk); };
-      uint4_t kf[NH][NC], vf[VT][NB];
+    // Lane i looks token i % TILE of a unit's tile up, a unit ahead: its row's offset in bytes, -1 where it is masked.
+    auto look = [&](uint32_t u) -> int64_t {
+      const int token = (sp.unit + static_cast<int>(u)) * UT + wave * TILE + lane % TILE;
+      if (u >= to || token < sp.begin || token >= sp.end) return -1;
+      return token_offset(p.cache, table, static_cast<uint32_t>(token)) * SIZE;  // (a page that is none: negative)
+    };
+    // The loads are a unit ahead of the products, without more registers: K's next rows follow when the scores have
+    // read these, V's when the answers have. Rows that are masked are row 0 of page 0, not used.
+    uint4_t kf[NH][NC], vf[VT][NB];
+    auto load_k = [&](int64_t offset) {
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        const char* row = kb + row_offset(16 * h + col);
+        const char* row = kb + __shfl(offset, 16 * h + col);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const int dim = 4 * E * c + E * g;
           if (c < chunks_of_row) kf[h][c] = *reinterpret_cast<const uint4_t*>(row + (dim < p.head_dim ? dim * SIZE : 0));
-          if (ragged && dim >= p.head_dim) kf[h][c] = uint4_t{0u, 0u, 0u, 0u};
         }
       }
+    };
+    auto load_v = [&](int64_t offset) {
 #pragma unroll
       for (int j = 0; j < VT; ++j) {
-        const char* row = vb + row_offset(16 * (j / 4) + 4 * g + j % 4);
+        const char* row = vb + __shfl(offset, 16 * (j / 4) + 4 * g + j % 4);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           const int dim = 16 * E * nb + E * col;
           vf[j][nb] = *reinterpret_cast<const uint4_t*>(row + (dim < p.head_dim ? dim * SIZE : 0));
         }
+      }
+    };
+    int64_t found = look(from), coming = look(from + 1);
+    load_k(found < 0 ? 0 : found);
+    load_v(found < 0 ? 0 : found);
+    for (uint32_t u = from; u < to; ++u) {
+      const uint32_t valid = static_cast<uint32_t>(__ballot(found >= 0));  // (TILE 16: the four copies agree)
+      const int64_t next_row = coming < 0 ? 0 : coming;
+      const bool more = u + 1 < to;
+      found = coming;
+      coming = look(u + 2);
+      const bool full = TILE == 32 ? valid == 0xFFFFFFFFu : (valid & 0xFFFFu) == 0xFFFFu;
+      if (ragged) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            if (4 * E * c + E * g >= p.head_dim) kf[h][c] = uint4_t{0u, 0u, 0u, 0u};
       }
       float4_t s[NH];
 #pragma unroll
@@ -368,6 +441,7 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void k_paged_attention(Attend
           }
         }
       }
+      if (more) load_k(next_row);
       float t[NH][4], top = kNone;
 #pragma unroll
       for (int h = 0; h < NH; ++h)
@@ -434,9 +508,10 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void k_paged_attention(Attend
             acc[nb][e] = mfma16<DT>(vt, lo, acc[nb][e]);
           }
       }
+      if (more) load_v(next_row);
     }
 
-    // The four wavefronts' parts of the item meet in LDS.
+    // The wavefronts' parts of the item meet in LDS.
     l = column_sum(l);
     if (g == 0) {
       lds_m[wave][col] = m;
@@ -451,37 +526,115 @@ __global__ __launch_bounds__(256, NB == 1 ? 2 : 1) void k_paged_attention(Attend
           *reinterpret_cast<float4_t*>(&lds_o[wave][col][16 * E * nb + E * (4 * g + i) + e]) =
               float4_t{acc[nb][e][i], acc[nb][e + 1][i], acc[nb][e + 2][i], acc[nb][e + 3][i]};
     __syncthreads();
-    const bool whole = from == 0 && to == static_cast<uint32_t>(sp.units);
-    const uint32_t slot = part_place(worker, at == run);
-    const int quads = p.head_dim / 4;
-    for (int i = threadIdx.x; i < heads * quads; i += 256) {
-      const int hd = i / quads, dim = (i - hd * quads) * 4;
-      float top = lds_m[0][hd];
+    const bool whole = HOW == WHOLE || (from == 0 && to == static_cast<uint32_t>(sp.units));
+    [[maybe_unused]] const uint32_t slot = part_place(worker, at == run);
+    const int part_heads = min(kHeads, p.group), quads = p.head_dim / 4;
+    auto joined = [&](int hd, int dim, float& top, float& total) {
+      top = lds_m[0][hd];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) top = fmaxf(top, lds_m[w][hd]);
-      float total = 0.f;
+      for (int w = 1; w < WAVES; ++w) top = fmaxf(top, lds_m[w][hd]);
+      total = 0.f;
       float4_t o{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < WAVES; ++w) {
         const float f = lds_m[w][hd] == top ? 1.f : __builtin_amdgcn_exp2f(lds_m[w][hd] - top);
         total += f * lds_l[w][hd];
         o += f * *reinterpret_cast<const float4_t*>(&lds_o[w][hd][dim]);
       }
+      return o;
+    };
+    for (int i = threadIdx.x; i < heads * quads; i += THREADS) {
+      const int hd = i / quads, dim = (i - hd * quads) * 4;
+      float top, total;
+      const float4_t o = joined(hd, dim, top, total);
+      const int64_t row = static_cast<int64_t>(slot) * part_heads + hd;
       if (whole) {
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-        const int64_t out = b * p.ldy + static_cast<int64_t>(head0 + hd) * p.head_dim + dim;
-        if constexpr (F32)
-          *reinterpret_cast<float4_t*>(static_cast<float*>(p.y) + out) = o * inv;
-        else
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + out) =
-              make_uint2(pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv));
+        store(b, head0 + hd, dim, o * (total == 0.f ? 0.f : 1.f / total));
+      } else if constexpr (HOW == JOIN) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4_t, o), parts_rsrc, static_cast<uint32_t>(row * p.head_dim + dim) * 4, 0, kThrough);
+        if (dim == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uint2_t, make_float2(top, total)), stats_rsrc, static_cast<uint32_t>(row) * 8, 0, kThrough);
       } else {
-        const int64_t row = static_cast<int64_t>(slot) * min(kHeads, p.group) + hd;
         *reinterpret_cast<float4_t*>(p.part + row * p.head_dim + dim) = o;
         if (dim == 0) p.stats[row] = make_float2(top, total);
       }
     }
     at = item_first + to;
+    if constexpr (HOW == JOIN) {
+      if (!whole) {
+        const Parts parts = parts_of(item_first, static_cast<uint32_t>(sp.units), per);
+        // The parts are stored and loaded past the XCDs' L2 caches, so that the order is all that is left to see to: this
+        // thread's stores have arrived, then everybody's, then the count. (Fences of that scope would also write the L2
+        // back and empty it: 32 x 8000 tokens took 163 us with them, 58 without.)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        __shared__ uint32_t others;
+        if (threadIdx.x == 0) {
+          others = __hip_atomic_fetch_add(p.meet + parts.from, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          if (others == parts.count - 1) __hip_atomic_store(p.meet + parts.from, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (others == parts.count - 1) {
+          // A thread takes four dimensions of one head and every so many parts, BATCH parts' loads at a time, with a running
+          // maximum; the threads of the same dimensions then meet in LDS.
+          constexpr int BATCH = F32 && NB == 2 ? 8 : 16;  // (what the registers hold)
+          const int all_quads = heads * quads, groups = max(256 / all_quads, 1), mine_group = static_cast<int>(threadIdx.x) / all_quads;
+          float4_t* sums = reinterpret_cast<float4_t*>(&lds_o[0][0][0]);
+          float2* tops = reinterpret_cast<float2*>(sums + 256);
+          for (int i0 = 0; i0 < all_quads; i0 += 256) {
+            const int i = groups > 1 ? static_cast<int>(threadIdx.x) - mine_group * all_quads : i0 + static_cast<int>(threadIdx.x);
+            const int hd = i / quads, dim = (i - hd * quads) * 4;
+            float top = kNone, total = 0.f;
+            float4_t o{0.f, 0.f, 0.f, 0.f};
+            if (mine_group < groups && i < all_quads) {
+              for (uint32_t k0 = mine_group; k0 < parts.count; k0 += BATCH * groups) {
+                float2 st[BATCH];
+                float4_t po[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                  const uint32_t row = place_of(parts, min(k0 + k * groups, parts.count - 1)) * part_heads + hd;
+                  st[k] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(stats_rsrc, row * 8, 0, kThrough));
+                  po[k] = __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(parts_rsrc, (row * p.head_dim + dim) * 4, 0, kThrough));
+                }
+                float next = top;
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) next = fmaxf(next, st[k].x);
+                const float keep = top == next ? 1.f : __builtin_amdgcn_exp2f(top - next);
+                total *= keep;
+                o *= keep;
+                top = next;
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                  if (k0 + k * groups >= parts.count) continue;
+                  const float f = st[k].x == top ? 1.f : __builtin_amdgcn_exp2f(st[k].x - top);
+                  total += f * st[k].y;
+                  o += f * po[k];
+                }
+              }
+            }
+            if (groups > 1) {
+              sums[threadIdx.x] = o;
+              tops[threadIdx.x] = make_float2(top, total);
+              __syncthreads();
+              if (mine_group == 0) {
+                float most = top;
+                for (int k = 1; k < groups; ++k) most = fmaxf(most, tops[k * all_quads + i].x);
+                const float keep = top == most ? 1.f : __builtin_amdgcn_exp2f(top - most);
+                total *= keep;
+                o *= keep;
+                for (int k = 1; k < groups; ++k) {
+                  const float2 t = tops[k * all_quads + i];
+                  const float f = t.x == most ? 1.f : __builtin_amdgcn_exp2f(t.x - most);
+                  total += f * t.y;
+                  o += f * sums[k * all_quads + i];
+                }
+              }
+            }
+            if (mine_group == 0 && i < all_quads) store(b, head0 + hd, dim, total == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / total));
+          }
+        }
+      }
+    }
     __syncthreads();
   }
 }
@@ -568,14 +721,17 @@ int check_cache(tmh_ctx* ctx, const tmh_paged_cache* c) {
   return TMH_OK;
 }
 
-template <int DT>
+template <int DT, int HOW>
 void launch_attention(const AttendArgs& p, int heads, hipStream_t s) {
   constexpr int per_block = DT == DT_F32 ? 64 : 128;
   const int nb = (p.head_dim + per_block - 1) / per_block;
-  if (nb == 1) k_paged_attention<DT, 1><<<p.workers, 256, 0, s>>>(p);
-  else if (nb == 2) k_paged_attention<DT, 2><<<p.workers, 256, 0, s>>>(p);
-  else if constexpr (DT == DT_F32) k_paged_attention<DT, 4><<<p.workers, 256, 0, s>>>(p);
-  k_paged_join<DT><<<dim3(static_cast<unsigned>(heads), static_cast<unsigned>(p.B)), 256, 0, s>>>(p);
+  constexpr int threads = HOW == WHOLE ? 512 : 256;
+  if (nb == 1) k_paged_attention<DT, 1, HOW><<<p.workers, threads, 0, s>>>(p);
+  else if constexpr (HOW != WHOLE || DT == DT_F32) {
+    if (nb == 2) k_paged_attention<DT, 2, HOW><<<p.workers, threads, 0, s>>>(p);
+    else if constexpr (HOW != WHOLE && DT == DT_F32) k_paged_attention<DT, 4, HOW><<<p.workers, threads, 0, s>>>(p);
+  }
+  if constexpr (HOW == PARTS) k_paged_join<DT><<<dim3(static_cast<unsigned>(heads), static_cast<unsigned>(p.B)), 256, 0, s>>>(p);
 }
 
 }  // namespace
@@ -701,9 +857,30 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
   if (!ws) return fail(ctx, TMH_ERR_UNSUPPORTED, "attention's workspace cannot grow here: run one call before the capture");
   p.part = static_cast<float*>(ws);
   p.stats = reinterpret_cast<float2*>(p.part + rows * cache->head_dim);
-  if (cache->dtype == TMH_F32) launch_attention<DT_F32>(p, heads, s);
-  else if (cache->dtype == TMH_F16) launch_attention<DT_F16>(p, heads, s);
-  else launch_attention<DT_BF16>(p, heads, s);
+  p.meet = ctx->meet;
+  p.part_bytes = static_cast<uint32_t>(rows * cache->head_dim * 4);
+  p.stats_bytes = static_cast<uint32_t>(rows * sizeof(float2));
+  // WHOLE where the table has room for few tokens (the lengths are the device's): a workgroup's turn of 256 tokens costs 2.6 us
+  // more, parts that meet 3.3 us, f16 4 kv heads of 128: one sequence of 300 8.4 us (9.2 in parts), of 700 11.3 (9.4); and
+  // with workgroups for half the CUs and more, 32 x 700 12.9 (16.1), 60 x 1..1000 16.7 (20.0), 8 x 1000 15.2 (10.7).
+  const int64_t all_items = B * cache->kv_heads * chunks;
+  const bool whole = cache->head_dim <= 128 && all_items <= ctx->num_cus &&
+                     (p.most <= 512 || (p.most <= 1024 && all_items >= ctx->num_cus / 2));
+  // JOIN where one workgroup has few parts to read (of equal lengths; of others it may be more): one sequence of 4096 (32 parts of 2
+  // KiB) 9.9 us, 11.8 as PARTS; 32 x 4000 56.6 and 58.7; one of 32768 (128 parts) 25.5 and 24.6, 64 x 2000 with 16 heads of one kv
+  // head (8 parts of 8 KiB) 22.6 and 20.6.
+  const int64_t parts = std::min<int64_t>((p.most + unit - 1) / unit, workers / all_items + 2);
+  const bool join = parts * std::min(kHeads, group) * cache->head_dim * 4 <= kJoinBytes;
+  if (whole) p.workers = static_cast<uint32_t>(all_items);
+  auto launch = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (whole) launch_attention<DT, WHOLE>(p, heads, s);
+    else if (join) launch_attention<DT, JOIN>(p, heads, s);
+    else launch_attention<DT, PARTS>(p, heads, s);
+  };
+  if (cache->dtype == TMH_F32) launch(std::integral_constant<int, DT_F32>{});
+  else if (cache->dtype == TMH_F16) launch(std::integral_constant<int, DT_F16>{});
+  else launch(std::integral_constant<int, DT_BF16>{});
   return check_launch(ctx, "k_paged_attention");
 }
 

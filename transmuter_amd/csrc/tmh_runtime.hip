@@ -182,6 +182,16 @@ int tmh_ctx_create(int device, tmh_ctx** out) {
     delete ctx;
     return check_hip(nullptr, err, "hipStreamCreateWithFlags");
   }
+  const size_t meet_bytes = 2 * static_cast<size_t>(ctx->num_cus) * sizeof(uint32_t);
+  err = hipMalloc(reinterpret_cast<void**>(&ctx->meet), meet_bytes);
+  if (err == hipSuccess) err = hipMemsetAsync(ctx->meet, 0, meet_bytes, ctx->stream);
+  if (err == hipSuccess) err = hipStreamSynchronize(ctx->stream);
+  if (err != hipSuccess) {
+    (void)hipFree(ctx->meet);
+    (void)hipStreamDestroy(ctx->stream);
+    delete ctx;
+    return check_hip(nullptr, err, "the context's counters");
+  }
   *out = ctx;
   return TMH_OK;
 }
@@ -194,6 +204,7 @@ void tmh_ctx_destroy(tmh_ctx* ctx) {
     (void)hipStreamDestroy(ctx->stream);
   }
   if (ctx->ws) (void)hipFree(ctx->ws);
+  (void)hipFree(ctx->meet);
   for (void* p : ctx->ws_retired) (void)hipFree(p);
   delete ctx->tl;
   delete ctx;

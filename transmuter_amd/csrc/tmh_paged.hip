@@ -27,8 +27,11 @@ struct AppendArgs {
   int64_t page_stride, token_stride, head_stride;
   int64_t num_slots;
   int table_dtype, rotary, interleaved, heads, kv_heads;
-  uint32_t pieces;  // of eight dimensions in a token's heads, keys and values
-  FastDiv by_pieces, by_head, by_page;
+  // A token's pieces: of each query and key head (`turned` of them pairs of eight dimensions half a rotary row apart), then
+  // of each value head.
+  uint32_t pieces, value_pieces;
+  int turned, head_dim;
+  FastDiv by_pieces, by_head, by_value, by_page;
 };
 
 // Eight entries of a rotary table row.
@@ -42,26 +45,39 @@ __device__ __forceinline__ void load_table(const void* p, int dtype, int64_t at,
   }
 }
 
-// A thread answers eight dimensions of one head of one token; those that turn by halves read their partners
-// too (the same lines, from the cache). VEC: rows and partners lie on 16 bytes.
+// A thread answers eight dimensions of one head of one token, and with VEC of those that turn by halves their partners
+// too. VEC: rows and partners lie on 16 bytes.
 template <int DT, bool VEC>
-__global__ __launch_bounds__(256) void k_paged_append(AppendArgs p, int64_t first, uint32_t count, bool table_vec) {
+__global__ __launch_bounds__(256) void k_paged_append(AppendArgs p, int64_t first, uint32_t count, bool table_vec, bool pairs_vec) {
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;
   if (i >= count) return;
   const uint32_t tl = p.by_pieces.div(i);
   const int64_t t = first + tl;
   const uint32_t piece = i - tl * p.pieces;
-  const int head = static_cast<int>(p.by_head.div(piece));
-  const int dim = static_cast<int>(piece - head * p.by_head.d) * 8, head_dim = static_cast<int>(p.by_head.d) * 8;
-  const bool is_q = head < p.heads, is_k = !is_q && head < p.heads + p.kv_heads;
+  const bool is_v = piece >= p.pieces - p.value_pieces;
+  const uint32_t local = is_v ? piece - (p.pieces - p.value_pieces) : piece;
+  const FastDiv by = is_v ? p.by_value : p.by_head;
+  const int head = static_cast<int>(by.div(local)), at = static_cast<int>(local - head * by.d), head_dim = p.head_dim;
+  const bool is_q = !is_v && head < p.heads, is_k = !is_v && !is_q, pair = !is_v && at < p.turned;
+  const int dim = 8 * (is_v || pair ? at : at + p.turned);
   int64_t slot = 0;
   if (!is_q) {
     slot = p.slots[t];
     if (slot < 0 || slot >= p.num_slots) return;
   }
   const void* src = is_q ? p.q : is_k ? p.k : p.v;
-  const int h = is_q ? head : is_k ? head - p.heads : head - p.heads - p.kv_heads;
+  const int h = is_k ? head - p.heads : head;
   const int64_t row = (is_q ? p.ldq : is_k ? p.ldk : p.ldv) * t + static_cast<int64_t>(h) * head_dim;
+  auto put = [&](int at, const float (&x)[8]) {
+    if (is_q) {
+      store8<DT, VEC>(p.q_out, t * p.ldqo + static_cast<int64_t>(h) * head_dim + at, 8, x);
+    } else {
+      const uint32_t page = p.by_page.div(static_cast<uint32_t>(slot));
+      const uint32_t place = static_cast<uint32_t>(slot) - page * p.by_page.d;
+      store8<DT, true>(is_k ? p.k_cache : p.v_cache,
+                       page * p.page_stride + place * p.token_stride + h * p.head_stride + at, 8, x);
+    }
+  };
   float v[8];
   load8<DT, VEC>(src, row + dim, 8, v);
   if ((is_q || is_k) && dim < p.rotary) {
@@ -69,24 +85,42 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs p, int64_t firs
     const int half = p.rotary / 2;
     const int64_t table = position * half;
     if (p.interleaved) {
+      float c[4], s[4];
+      if (pairs_vec) {
+        const float4_t cv = *reinterpret_cast<const float4_t*>(static_cast<const float*>(p.cos) + table + dim / 2);
+        const float4_t sv = *reinterpret_cast<const float4_t*>(static_cast<const float*>(p.sin) + table + dim / 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          c[j] = cv[j];
+          s[j] = sv[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool in = dim + 2 * j < p.rotary;
+          c[j] = in ? load_float_rt(p.cos, p.table_dtype, table + dim / 2 + j) : 1.f;
+          s[j] = in ? load_float_rt(p.sin, p.table_dtype, table + dim / 2 + j) : 0.f;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (dim + 2 * j >= p.rotary) continue;
-        const float c = load_float_rt(p.cos, p.table_dtype, table + dim / 2 + j);
-        const float s = load_float_rt(p.sin, p.table_dtype, table + dim / 2 + j);
+        if (!pairs_vec && dim + 2 * j >= p.rotary) continue;
         const float a = v[2 * j], b = v[2 * j + 1];
-        v[2 * j] = a * c - b * s;
-        v[2 * j + 1] = fmaf(a, s, b * c);
+        v[2 * j] = a * c[j] - b * s[j];
+        v[2 * j + 1] = fmaf(a, s[j], b * c[j]);
       }
-    } else if (VEC) {
-      const bool low = dim < half;
-      const int at = low ? dim : dim - half;
+    } else if (VEC) {  // a pair
       float o[8], c[8], s[8];
-      load8<DT, VEC>(src, row + (low ? dim + half : dim - half), 8, o);
-      load_table(p.cos, p.table_dtype, table + at, table_vec, c);
-      load_table(p.sin, p.table_dtype, table + at, table_vec, s);
+      load8<DT, VEC>(src, row + dim + half, 8, o);
+      load_table(p.cos, p.table_dtype, table + dim, table_vec, c);
+      load_table(p.sin, p.table_dtype, table + dim, table_vec, s);
+      float high[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = low ? v[j] * c[j] - o[j] * s[j] : fmaf(o[j], s[j], v[j] * c[j]);
+      for (int j = 0; j < 8; ++j) {
+        high[j] = fmaf(v[j], s[j], o[j] * c[j]);
+        v[j] = v[j] * c[j] - o[j] * s[j];
+      }
+      put(dim + half, high);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -101,24 +135,17 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs p, int64_t firs
       }
     }
   }
-  if (is_q) {
-    store8<DT, VEC>(p.q_out, t * p.ldqo + static_cast<int64_t>(h) * head_dim + dim, 8, v);
-  } else {
-    const uint32_t page = p.by_page.div(static_cast<uint32_t>(slot));
-    const uint32_t at = static_cast<uint32_t>(slot) - page * p.by_page.d;
-    store8<DT, true>(is_k ? p.k_cache : p.v_cache,
-                     page * p.page_stride + at * p.token_stride + h * p.head_stride + dim, 8, v);
-  }
+  put(dim, v);
 }
 
 template <int DT>
-void launch_append(const AppendArgs& p, int64_t T, bool vec, bool table_vec, hipStream_t s) {
+void launch_append(const AppendArgs& p, int64_t T, bool vec, bool table_vec, bool pairs_vec, hipStream_t s) {
   const int64_t most = ((int64_t{1} << 31) - 256) / p.pieces;  // tokens a launch, within the divisions' range
   for (int64_t first = 0; first < T; first += most) {
     const uint32_t count = static_cast<uint32_t>(std::min(most, T - first) * p.pieces);
     const unsigned grid = (count + 255) / 256;
-    if (vec) k_paged_append<DT, true><<<grid, 256, 0, s>>>(p, first, count, table_vec);
-    else k_paged_append<DT, false><<<grid, 256, 0, s>>>(p, first, count, table_vec);
+    if (vec) k_paged_append<DT, true><<<grid, 256, 0, s>>>(p, first, count, table_vec, pairs_vec);
+    else k_paged_append<DT, false><<<grid, 256, 0, s>>>(p, first, count, table_vec, pairs_vec);
   }
 }
 
@@ -787,20 +814,26 @@ int tmh_paged_append(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void* d_k
   p.interleaved = interleaved;
   p.heads = heads;
   p.kv_heads = cache->kv_heads;
-  p.pieces = static_cast<uint32_t>((heads + 2 * cache->kv_heads) * (dim / 8));
-  p.by_pieces = FastDiv(p.pieces);
-  p.by_head = FastDiv(static_cast<uint32_t>(dim / 8));
   p.by_page = FastDiv(static_cast<uint32_t>(cache->page_size));
   const int64_t e = 16 / dtype_size(cache->dtype);
   auto on16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
   const bool vec = on16(d_k) && on16(d_v) && ldk % e == 0 && ldv % e == 0 &&
                    (!heads || (on16(d_q) && on16(d_q_out) && ldq % e == 0 && ldqo % e == 0)) &&
                    (interleaved ? true : rotary_dim % 16 == 0);
+  p.head_dim = dim;
+  p.turned = vec && !interleaved ? rotary_dim / 16 : 0;
+  const uint32_t of_head = static_cast<uint32_t>(dim / 8 - p.turned);
+  p.value_pieces = static_cast<uint32_t>(cache->kv_heads * (dim / 8));
+  p.pieces = static_cast<uint32_t>(heads + cache->kv_heads) * of_head + p.value_pieces;
+  p.by_pieces = FastDiv(p.pieces);
+  p.by_head = FastDiv(of_head);
+  p.by_value = FastDiv(static_cast<uint32_t>(dim / 8));
   const bool table_vec = on16(d_cos) && on16(d_sin) && rotary_dim % 16 == 0;
+  const bool pairs_vec = table_dtype == TMH_F32 && on16(d_cos) && on16(d_sin) && rotary_dim % 8 == 0;  // four pairs an access
   hipStream_t s = pick_stream(ctx, stream);
-  if (cache->dtype == TMH_F32) launch_append<DT_F32>(p, T, vec, table_vec, s);
-  else if (cache->dtype == TMH_F16) launch_append<DT_F16>(p, T, vec, table_vec, s);
-  else launch_append<DT_BF16>(p, T, vec, table_vec, s);
+  if (cache->dtype == TMH_F32) launch_append<DT_F32>(p, T, vec, table_vec, pairs_vec, s);
+  else if (cache->dtype == TMH_F16) launch_append<DT_F16>(p, T, vec, table_vec, pairs_vec, s);
+  else launch_append<DT_BF16>(p, T, vec, table_vec, pairs_vec, s);
   return check_launch(ctx, "k_paged_append");
 }
 

@@ -3,8 +3,9 @@ layers in 8-bit floating point"): the residual's addition and the root-mean-squa
 8-bit product, and a paged cache of keys and values with the attention that reads it.
 
 Rows in 8 bits (`Rows8`) are f8_e4m3fn values with one f32 scale for each block of 128 columns. Every call is
-asynchronous on `stream` (None: the context's); its operands must stay until its work is done. No reference
-counterpart: the reference's norms and attention stay on the Nx backend.
+asynchronous on `stream` (None: the context's); its operands must stay until its work is done. A call's answer is new
+device memory, or `out`, of the same shapes and types, which a step that is recorded into a graph has to give
+(nothing can be allocated there). No reference counterpart: the reference's norms and attention stay on the Nx backend.
 """
 
 from __future__ import annotations
@@ -41,6 +42,15 @@ def _at(t: DeviceTensor, elements: int) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.ptr.value + elements * np.dtype(NX_TO_NUMPY[t.dtype]).itemsize)
 
 
+def _out(out: DeviceTensor | None, ctx: Context, shape, dtype: str) -> DeviceTensor:
+    """The answer's memory: `out`, if it has the answer's shape and type, or new."""
+    if out is None:
+        return ctx.empty(shape, dtype)
+    if out.shape != tuple(shape) or out.dtype != dtype:
+        _refuse(f"out must be {dtype} {tuple(shape)}, got {out.dtype} {out.shape}")
+    return out
+
+
 class Rows8(NamedTuple):
     """Rows [..., N] in 8 bits: value (t, n) is q[t, n] * scales[n // 128, t]."""
 
@@ -49,8 +59,13 @@ class Rows8(NamedTuple):
 
     @classmethod
     def empty(cls, ctx: Context, shape) -> "Rows8":
+        return cls._of(ctx, shape, None)
+
+    @classmethod
+    def _of(cls, ctx: Context, shape, out: "Rows8 | None") -> "Rows8":
         rows = math.prod(shape[:-1])
-        return cls(ctx.empty(shape, "f8_e4m3fn"), ctx.empty((-(-shape[-1] // BLOCK), rows), "f32"))
+        return cls(_out(out.q if out is not None else None, ctx, shape, "f8_e4m3fn"),
+                   _out(out.scales if out is not None else None, ctx, (-(-shape[-1] // BLOCK), rows), "f32"))
 
 
 class Norm(NamedTuple):
@@ -62,17 +77,19 @@ class Norm(NamedTuple):
 
 
 def rms_norm(x: DeviceTensor, gamma: DeviceTensor, residual: DeviceTensor | None = None, eps: float = 1e-6, *,
-             y: bool = False, rows: bool = True, stream=None) -> Norm:
+             y: bool = False, rows: bool = True, out: Norm | None = None, stream=None) -> Norm:
     """h * rsqrt(mean(h^2) + eps) * gamma over the rows of h = x + residual, in x's type (`y`), in 8 bits (`rows`),
-    or both; `sum` is h, where there is a residual."""
+    or both; `sum` is h, where there is a residual. Of `out` the parts that are asked for are used; its sum may be x
+    or the residual itself."""
     t, n = _rows(x, "the norm")
     if gamma.shape != (n,):
         _refuse(f"the norm's gamma must be [{n}], got {gamma.shape}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         _refuse(f"the residual must be {x.dtype} {x.shape}, got {residual.dtype} {residual.shape}")
     ctx = x.ctx
-    out = Norm(ctx.empty(x.shape, x.dtype) if y else None, Rows8.empty(ctx, x.shape) if rows else None,
-               ctx.empty(x.shape, x.dtype) if residual is not None else None)
+    out = out or Norm(None, None, None)
+    out = Norm(_out(out.y, ctx, x.shape, x.dtype) if y else None, Rows8._of(ctx, x.shape, out.rows) if rows else None,
+               _out(out.sum, ctx, x.shape, x.dtype) if residual is not None else None)
     ctx.check(lib().tmh_rms_norm(
         ctx.handle, x.ptr, n, residual.ptr if residual is not None else None, n, x.tmh_dtype, t, n, gamma.ptr,
         gamma.tmh_dtype, eps, out.sum.ptr if out.sum else None, n, out.y.ptr if out.y else None, n,
@@ -80,22 +97,22 @@ def rms_norm(x: DeviceTensor, gamma: DeviceTensor, residual: DeviceTensor | None
     return out
 
 
-def quantize_rows(x: DeviceTensor, *, stream=None) -> Rows8:
+def quantize_rows(x: DeviceTensor, *, out: Rows8 | None = None, stream=None) -> Rows8:
     """x's rows in 8 bits."""
     t, n = _rows(x, "quantization")
-    out = Rows8.empty(x.ctx, x.shape)
+    out = Rows8._of(x.ctx, x.shape, out)
     x.ctx.check(lib().tmh_quantize_rows(x.ctx.handle, x.ptr, n, None, 0, x.tmh_dtype, t, n, out.q.ptr, n,
                                         out.scales.ptr, stream))
     return out
 
 
-def quantize_swiglu(gate_up: DeviceTensor, *, stream=None) -> Rows8:
+def quantize_swiglu(gate_up: DeviceTensor, *, out: Rows8 | None = None, stream=None) -> Rows8:
     """gate * sigmoid(gate) * up in 8 bits, of a merged gate/up product [..., 2 N] (the gate's columns first)."""
     t, width = _rows(gate_up, "SwiGLU")
     if width % 2:
         _refuse(f"a merged gate/up product has two equal halves, got {width} columns")
     n = width // 2
-    out = Rows8.empty(gate_up.ctx, (*gate_up.shape[:-1], n))
+    out = Rows8._of(gate_up.ctx, (*gate_up.shape[:-1], n), out)
     gate_up.ctx.check(lib().tmh_quantize_rows(gate_up.ctx.handle, _at(gate_up, n), width, gate_up.ptr, width,
                                               gate_up.tmh_dtype, t, n, out.q.ptr, n, out.scales.ptr, stream))
     return out
@@ -161,7 +178,8 @@ class Fp8Weight:
         return f"Fp8Weight(N={self.n}, K={self.k})"
 
 
-def matmul_fp8(a: Rows8, w: Fp8Weight, bias: DeviceTensor | None = None, *, y_type: str = "f16", stream=None) -> DeviceTensor:
+def matmul_fp8(a: Rows8, w: Fp8Weight, bias: DeviceTensor | None = None, *, y_type: str = "f16",
+               out: DeviceTensor | None = None, stream=None) -> DeviceTensor:
     """Y = A . W^T (+ bias) of rows and a weight in 8 bits, in y_type."""
     ctx = w.ctx
     if a.q.shape[-1] != w.k:
@@ -174,7 +192,7 @@ def matmul_fp8(a: Rows8, w: Fp8Weight, bias: DeviceTensor | None = None, *, y_ty
         _refuse(f"the 8-bit product's bias must be [{w.n}], got {bias.shape}")
     if y_type not in FLOAT_TYPES:
         _refuse(f"the 8-bit product's y must be f32, f16 or bf16, got {y_type}")
-    y = ctx.empty((*a.q.shape[:-1], w.n), y_type)
+    y = _out(out, ctx, (*a.q.shape[:-1], w.n), y_type)
     ctx.check(lib().tmh_matmul_fp8(ctx.handle, w.handle, a.q.ptr, m, w.k, a.scales.ptr, bias.ptr if bias else None,
                                    bias.tmh_dtype if bias else 0, y.ptr, y.tmh_dtype, w.n, stream))
     return y
@@ -204,7 +222,7 @@ class PagedCache:
 
     def append(self, qkv: DeviceTensor, heads: int, slots: DeviceTensor, positions: DeviceTensor | None = None,
                cos: DeviceTensor | None = None, sin: DeviceTensor | None = None, *, interleaved: bool = False,
-               stream=None) -> DeviceTensor:
+               out: DeviceTensor | None = None, stream=None) -> DeviceTensor:
         """The keys and values of a merged q/k/v product [T, (heads + 2 kv_heads) * head_dim] into slots [T] (s64,
         page * page_size + place; outside the cache: not stored), its queries and keys turned by their positions [T]
         (s64) first where tables cos and sin [max_positions, rotary_dim / 2] are given. Returns the queries."""
@@ -221,7 +239,7 @@ class PagedCache:
             if positions.dtype != "s64" or positions.size != t:
                 _refuse(f"a step of {t} tokens takes {t} s64 positions, got {positions.dtype} {positions.shape}")
             most, rotary, table = cos.shape[0], 2 * cos.shape[1], cos.tmh_dtype
-        q = self.ctx.empty((*qkv.shape[:-1], heads * d), self.dtype)
+        q = _out(out, self.ctx, (*qkv.shape[:-1], heads * d), self.dtype)
         self.ctx.check(lib().tmh_paged_append(
             self.ctx.handle, qkv.ptr, width, _at(qkv, heads * d), width, _at(qkv, (heads + g) * d), width, t, heads,
             positions.ptr if rotary else None, cos.ptr if rotary else None, sin.ptr if rotary else None, table, most,
@@ -229,7 +247,7 @@ class PagedCache:
         return q
 
     def attend(self, q: DeviceTensor, page_table: DeviceTensor, lengths: DeviceTensor, *, scale: float | None = None,
-               window: int = 0, stream=None) -> DeviceTensor:
+               window: int = 0, out: DeviceTensor | None = None, stream=None) -> DeviceTensor:
         """Attention of one token a sequence, q [B, heads * head_dim], over the first lengths[b] (s32) tokens of the
         pages page_table[b] (s32, [B, max_pages]), or the last `window` of them. The scale is 1 / sqrt(head_dim) by
         default."""
@@ -240,7 +258,7 @@ class PagedCache:
             _refuse(f"the page table is s32 [{b}, pages], got {page_table.dtype} {page_table.shape}")
         if lengths.dtype != "s32" or lengths.shape != (b,):
             _refuse(f"the lengths are s32 [{b}], got {lengths.dtype} {lengths.shape}")
-        y = self.ctx.empty(q.shape, q.dtype)
+        y = _out(out, self.ctx, q.shape, q.dtype)
         scale = 1 / math.sqrt(self.head_dim) if scale is None else scale
         self.ctx.check(lib().tmh_paged_attention(
             self.ctx.handle, q.ptr, q.shape[1], b, q.shape[1] // self.head_dim, ctypes.byref(self.desc), page_table.ptr,

@@ -175,27 +175,27 @@ __device__ __forceinline__ void wait_vm() {
 }
 
 // Few rows: a workgroup of KW wavefronts takes NT tiles of 16 columns of Y for 16 MT rows, the
-// wavefronts every KW-th block of K each, and adds their sums in LDS. A wavefront has the next block's loads on
+// wavefronts every KW-th block of K each, and adds their sums in LDS. A wavefront has the next DEPTH - 1 blocks' loads on
 // their way while it multiplies one: W's tiles to registers, A's rows to a place of its own in LDS (no barrier),
 // eight lanes to a row's line (the fragments' own 16 bytes of 16 rows would be 64 lookups a load, k_f8_gemm).
-template <int MT, int NT, int KW, bool EXACT>
+template <int MT, int NT, int KW, int DEPTH, bool EXACT>
 __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
   constexpr int STAGE = MT * kTileBytes;
-  extern __shared__ __align__(16) uint8_t lds[];  // [KW][2][STAGE]; then the sums, [KW - 1][MT * NT][64] float4
+  extern __shared__ __align__(16) uint8_t lds[];  // [KW][DEPTH][STAGE]; then the sums, [KW - 1][MT * NT][64] float4
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int groups = p.tiles / NT, row_group = blockIdx.x / groups, tile = (blockIdx.x - row_group * groups) * NT;
   const uint8_t* w = p.w + (static_cast<int64_t>(tile) * p.kb) * kTileBytes + lane * 16;
   const float* ws = p.w_scales + static_cast<int64_t>(tile / 8) * p.kb;
   const int first = blockIdx.z * p.per, last = min(first + p.per, p.kb);
-  uint8_t* mine = lds + wave * 2 * STAGE;
+  uint8_t* mine = lds + wave * DEPTH * STAGE;
   const int a_row = lane >> 3, a_chunk = (lane & 7) ^ a_row;
   const int m0 = row_group * 16 * MT;
   const auto a_rsrc = buffer_rsrc(p.a + m0 * p.lda, static_cast<uint32_t>(min((static_cast<int64_t>(p.M) - m0 - 1) * p.lda + p.K, int64_t{0x7FFFFFF0})));
   const uint32_t a_off = static_cast<uint32_t>(a_row * p.lda) + 16 * a_chunk, a_rows = static_cast<uint32_t>(8 * p.lda);
   const uint32_t a_at[2] = {static_cast<uint32_t>(r * 128 + 16 * (g ^ (r & 7))), static_cast<uint32_t>(r * 128 + 16 * ((g + 4) ^ (r & 7)))};
-  uint4_t wr[2][NT][2];
-  float sw[2], sa[2][MT];
+  uint4_t wr[DEPTH][NT][2];
+  float sw[DEPTH], sa[DEPTH][MT];
   constexpr int LOADS = 2 * NT + 1 + 3 * MT;
   auto load = [&](int b, int buf) {
 #pragma unroll
@@ -217,10 +217,13 @@ __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[t][j] = float4_t{0.f, 0.f, 0.f, 0.f};
   auto block = [&](int b, int buf) {
-    if (b + KW < last) {
-      load(b + KW, buf ^ 1);
+    const int ahead = b + (DEPTH - 1) * KW;
+    if (ahead < last) {
+      load(ahead, (buf + DEPTH - 1) % DEPTH);
       asm volatile("" ::: "memory");
-      wait_vm<LOADS>();  // this block's loads: the next one's are the youngest
+      wait_vm<(DEPTH - 1) * LOADS>();  // this block's loads: the later ones' are the youngest
+    } else if (DEPTH > 2 && ahead - KW < last) {
+      wait_vm<LOADS>();
     } else {
       wait_vm<0>();
     }
@@ -245,13 +248,13 @@ __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
     }
   };
   int b = first + wave;
-  if (b < last) {
-    load(b, 0);
-    for (; b + KW < last; b += 2 * KW) {
-      block(b, 0);
-      block(b + KW, 1);
-    }
-    if (b < last) block(b, 0);
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d)
+    if (b + d * KW < last) load(b + d * KW, d);
+  for (; b < last; b += DEPTH * KW) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+      if (b + d * KW < last) block(b + d * KW, d);
   }
   wait_vm<0>();     // nothing is on its way to LDS
   __syncthreads();  // where the sums lie now
@@ -555,8 +558,8 @@ struct F8Plan {
   int kernel, splits;
 };
 
-// One workgroup's step of 128 of K, in us: alone on its CU (the loads' latency), and with the CU full (the matrix
-// and memory units), as measured over K at sizes that fill the chip once and several times.
+// k_f8_gemm: one workgroup's step of 128 of K, in us: alone on its CU (the loads' latency), and with the CU full (the
+// matrix and memory units), as measured over K at sizes that fill the chip once and several times.
 struct F8Shape {
   int kernel, bm, bn;
   float alone[2], full[2];  // for a 16-bit Y, and for an f32 Y
@@ -567,51 +570,65 @@ constexpr F8Shape kF8Shapes[] = {
     {GEMM_128x128, 128, 128, {0.60f, 1.40f}, {0.52f, 1.00f}},
     {GEMM_128x256, 128, 256, {0.95f, 0.f}, {0.87f, 0.f}},  // (its f32 form's registers would not fit)
 };
+// k_f8_rows by row tiles (of 16), column tiles and wavefronts: a CU takes in 88 KB of weights and rows of A a us, a wavefront
+// a block of K every 0.33 us at most, and a turn of workgroups costs `turn` us beside (ROWS32 and ROWS64 fill a CU's LDS, so
+// that their turns do not overlap).
+struct F8Rows {
+  int kernel, row_tiles, col_tiles, waves;
+  double first, turn;
+};
+constexpr F8Rows kF8Rows[] = {{ROWS16, 1, 1, 8, 2.0, 0.35}, {ROWS16_WIDE, 1, 2, 8, 2.0, 0.35}, {ROWS32, 2, 1, 16, 1.4, 1.0},
+                              {ROWS32_WIDE, 2, 2, 8, 2.0, 0.5}, {ROWS64, 4, 1, 8, 1.4, 1.0}};
 
-// The kernel by what it is expected to take: k_f8_rows up to 32 rows; above, the least of its four row tiles and
-// k_f8_gemm's shapes. Parts of K cost their sums' way to memory and back (4.5 TB/s) and the second launch (2.4 us). Measured, us
-// (f16 Y): 64 rows 2048 -> 2048 4.2 by ROWS64, 6.5 by 64x64, 7.8 by 64x128; 2048 -> 22016 10.7 by 64x64, 15.0 by ROWS64
-// with two column tiles; 128 rows 11008 -> 2048 14.1 by 64x64 in 8 parts, 15.7 in 4, 39.6 in one of 64x128; 512 rows 2048
-// -> 2048 6.9 by 64x64, 11.1 by 128x128; 512 rows 2048 -> 22016 27.0 by 128x128, 28.3 by 128x256, 43.9 by 64x64; 4096 rows 11008 -> 2048
-// 81 by 128x256, 87 by 128x128, 119 by a tile of 256 x 256, which no size was best with.
+// The kernel by what it is expected to take; parts of K cost their sums' way to memory and back (4.5 TB/s, 8 TB/s while the
+// last-level cache holds them) and the second launch (2.4 us). Measured, us (f16 Y): one row 2048 -> 22016 8.5 by ROWS16_WIDE, 8.9
+// by ROWS16; 2048 -> 2048 3.7 by ROWS16, 3.9 by ROWS16_WIDE; 32 rows 11008 -> 2048 6.5 by ROWS16 (twice over W), 7.8 by ROWS32; 64
+// rows 8.0 by ROWS16_WIDE, 8.8 by ROWS32, 10.0 by ROWS16, 12.1 by ROWS64, 10.3 by 64x64 in 8 parts; 64 rows 4096 -> 4096 6.1 by
+// ROWS32_WIDE, 7.1 by ROWS64, 9.7 by 64x64 in 4 parts; 64 rows 2048 -> 22016 11.1 by 64x64, 21.9 by ROWS64; 128 rows 11008 -> 2048 14.1 by
+// 64x64 in 8 parts, 15.7 in 4, 39.6 in one of 64x128; 512 rows 2048 -> 2048 6.9 by 64x64, 11.1 by 128x128; 512 rows 2048 -> 22016
+// 27.0 by 128x128, 28.3 by 128x256, 43.9 by 64x64; 4096 rows 11008 -> 2048 81 by 128x256, 87 by 128x128, 119 by a tile of 256 x
+// 256, which no size was best with.
 F8Plan plan_of(int64_t M, int64_t N, int kb, int64_t tiles, bool f32, int num_cus) {
-  // Two column tiles a wavefront read A half as often: with four workgroups a CU to hide the longer steps (2048 -> 22016, one
-  // row 8.3 us, 8.8 with one tile, 24 rows 9.3, 10.8); with fewer one is better (2048 -> 2048, 24 rows 3.7, 3.3 with one).
-  const bool wide = tiles >= 4 * num_cus;
-  if (M <= 32) return {M <= 16 ? (wide ? ROWS16_WIDE : ROWS16) : (wide ? ROWS32_WIDE : ROWS32), 1};
   F8Plan best{GEMM_128x128, 1};
   double least = 1e30;
   auto offer = [&](int kernel, int splits, double us) {
-    if (splits > 1) us += 2.4 + 8.0 * splits * static_cast<double>(M) * static_cast<double>(N) / 4.5e6;
+    const double sums = 8.0 * splits * static_cast<double>(M) * static_cast<double>(N);
+    if (splits > 1) us += 2.4 + sums / (sums > 128e6 ? 4.5e6 : 8e6);
     if (us < least) {
       least = us;
       best = {kernel, splits};
     }
   };
+  auto turns = [&](double groups) { return groups <= 4 ? std::ceil(groups) : groups + 0.4; };
+  for (const F8Rows& r : kF8Rows) {
+    const int64_t rows = 16 * r.row_tiles;
+    const double groups = static_cast<double>(tiles / r.col_tiles * ((M + rows - 1) / rows)) / num_cus;
+    const double work = std::max(0.33 * ((kb + r.waves - 1) / r.waves), kb * 2.048 * (r.row_tiles + r.col_tiles) / 88);
+    // (An f32 Y: conversions, and twice the answers. 512 rows 2048 -> 2048 17.0 by ROWS64, 11.2 by 64x64.)
+    offer(r.kernel, 1, r.first + turns(groups) * (f32 ? r.turn + 0.6 + 1.2 * work : r.turn + work));
+  }
+  if (M <= 16) return best;
   for (int splits = 1; splits <= 8; splits *= 2) {
     const int per = (kb + splits - 1) / splits;
     if (splits > 1 && per < 4) break;
-    const double row_groups = static_cast<double>(tiles * ((M + 63) / 64) * splits) / num_cus;
-    offer(ROWS64, splits, 2.4 + 0.9 * ((per + 7) / 8) * std::max(1.0, std::ceil(row_groups)));
     for (const F8Shape& f : kF8Shapes) {
       if (f.full[f32] == 0.f) continue;
       const double groups = static_cast<double>((M + f.bm - 1) / f.bm * ((N + f.bn - 1) / f.bn) * splits) / num_cus;
-      const double step = std::max<double>(f.alone[f32], f.full[f32] * (groups <= 4 ? std::ceil(groups) : groups + 0.4));
-      offer(f.kernel, splits, 2.6 + step * per);
+      offer(f.kernel, splits, 2.6 + std::max<double>(f.alone[f32], f.full[f32] * turns(groups)) * per);
     }
   }
   return best;
 }
 
-template <int MT, int NT, int KW, bool EXACT>
+template <int MT, int NT, int KW, int DEPTH, bool EXACT>
 void launch_rows(const F8Args& p, hipStream_t s) {
   // The wavefronts' stages of A, and in their place (or past it) their sums.
-  constexpr int kLds = KW * MT * std::max(2 * kTileBytes, NT * 1024);
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_f8_rows<MT, NT, KW, EXACT>),
+  constexpr int kLds = KW * MT * std::max(DEPTH * kTileBytes, NT * 1024);
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_f8_rows<MT, NT, KW, DEPTH, EXACT>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   (void)attr;
   const dim3 grid(static_cast<unsigned>(p.tiles / NT) * static_cast<unsigned>((p.M + 16 * MT - 1) / (16 * MT)), 1, static_cast<unsigned>(p.splits));
-  k_f8_rows<MT, NT, KW, EXACT><<<grid, 64 * KW, kLds, s>>>(p);
+  k_f8_rows<MT, NT, KW, DEPTH, EXACT><<<grid, 64 * KW, kLds, s>>>(p);
 }
 
 template <int BM, int BN, int WM, int WN, bool EXACT>
@@ -628,11 +645,11 @@ void launch_gemm(const F8Args& p, hipStream_t s) {
 template <bool F32>
 void launch_plan(const F8Plan& plan, const F8Args& p, hipStream_t s) {
   switch (plan.kernel) {
-    case ROWS16: launch_rows<1, 1, 8, F32>(p, s); break;
-    case ROWS16_WIDE: launch_rows<1, 2, 8, F32>(p, s); break;
-    case ROWS32: launch_rows<2, 1, 8, F32>(p, s); break;
-    case ROWS32_WIDE: launch_rows<2, 2, 8, F32>(p, s); break;
-    case ROWS64: launch_rows<4, 1, 8, F32>(p, s); break;
+    case ROWS16: launch_rows<1, 1, 8, 3, F32>(p, s); break;
+    case ROWS16_WIDE: launch_rows<1, 2, 8, 2, F32>(p, s); break;
+    case ROWS32: launch_rows<2, 1, 16, 2, F32>(p, s); break;
+    case ROWS32_WIDE: launch_rows<2, 2, 8, 2, F32>(p, s); break;
+    case ROWS64: launch_rows<4, 1, 8, 2, F32>(p, s); break;
     case GEMM_64x64: launch_gemm<64, 64, 2, 2, F32>(p, s); break;
     case GEMM_64x128: launch_gemm<64, 128, 1, 4, F32>(p, s); break;
     case GEMM_128x128: launch_gemm<128, 128, 1, 4, F32>(p, s); break;

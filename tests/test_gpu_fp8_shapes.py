@@ -19,7 +19,7 @@ pytestmark = pytest.mark.gpu
 # parts of K; K of one block, of an odd and an even number of them, ending inside one.
 SHAPES = [(16, 272, 530), (20, 400, 16401), (32, 2064, 16500), (33, 4112, 100), (64, 1936, 31), (65, 272, 40),
           (100, 400, 333), (190, 528, 70), (130, 128, 1100), (66, 3984, 4000), (300, 5008, 130), (1024, 144, 2048),
-          (1000, 400, 2001), (1000, 8208, 301), (515, 144, 22001), (2050, 144, 12301), (1300, 656, 5003)]
+          (1000, 400, 2001), (1000, 8208, 301), (515, 144, 22001), (2050, 144, 12301), (1300, 656, 5003), (2100, 272, 21001)]
 
 
 @pytest.mark.parametrize("dtype", base.TYPES)

@@ -358,7 +358,7 @@ __device__ __forceinline__ void gemm_outputs(const F8Args& p, const float4_t (&a
 // 1 KiB an instruction, two steps ahead, with the step's row scales; W's tiles, which are operands as they lie, go
 // to registers a step ahead and past LDS, whose reads would bound the loop otherwise. What lies past M, N or K is
 // past the buffers' ranges and arrives as zeros.
-template <int BM, int BN, int WM, int WN, bool EXACT>
+template <int BM, int BN, int WM, int WN, bool EXACT, bool TOUCH>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   constexpr int NW = WM * WN, TM = BM / 16 / WM, TN = BN / 16 / WN;
   constexpr int A_TILES = BM / 16, A_DMA = 2 * A_TILES / NW;
@@ -410,6 +410,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   // branches, which the compiler would move the products' FMAs behind: past the last block the loads of A have no
   // range and those of W and the scales are the last block's again.)
   constexpr int LOADS_W = 2 * TN + 1, LOADS_A = A_DMA + 1;
+  // TOUCH: a look at W's lines four blocks further on, a line a lane, each line by one of the row tiles that walk together,
+  // which brings them from memory to the XCD's L2 (the loads of the next block alone would arrive late).
+  const bool mine = TOUCH && lane < 16 * TN && (lane >> 3) % group_m == in_group % group_m;
+  const uint32_t touch_off = mine ? static_cast<uint32_t>(min(wn * TN + (lane >> 4), p.tiles - 1 - n0 / 16)) * static_cast<uint32_t>(p.kb) * kTileBytes + (lane & 15) * 128
+                                  : 0x80000000u;
+  auto touch = [&](int b) {
+    lds_dma4(w_rsrc, lds + 3 * STAGE + 3 * BM * 4 + wave * 256, touch_off, static_cast<uint32_t>(min(b, last - 1)) * kTileBytes);
+  };
   auto load_w = [&](int q, int at, int buf) {
     const int b = min(at, last - 1);
     if (q < 2 * TN)
@@ -436,15 +444,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
     for (int j = 0; j < TN; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
   int slot = 0;
   auto step = [&](int b, int buf) {
-    // The youngest outstanding loads are those of the next step's A: this step's W, scales and A are there.
-    wait_vm<A_DMA + 1>();
+    // The youngest outstanding loads are those of the next step's A (and a touch): this step's W, scales and A are there.
+    wait_vm<LOADS_A + TOUCH>();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();  // everybody's; and everybody has read the stage that is filled next
     asm volatile("" ::: "memory");
     const int free_slot = slot == 0 ? 2 : slot - 1;
     auto load = [&](int q) {
       if (q < LOADS_W) load_w(q, b + 1, buf ^ 1);
-      else load_a(q - LOADS_W, b + 2, free_slot);
+      else if (q < LOADS_W + LOADS_A) load_a(q - LOADS_W, b + 2, free_slot);
+      else touch(b + 4);
     };
     const uint8_t* la = lds + slot * STAGE + wm * TM * kTileBytes;
     const float* ls = lds_s + slot * BM + wm * (BM / WM) + r;
@@ -459,7 +468,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
       for (int h = 0; h < 2; ++h) wf[j][h].set(wr[buf][j][h]);
     if constexpr (EXACT) {
 #pragma unroll
-      for (int q = 0; q < LOADS_W + LOADS_A; ++q) load(q);
+      for (int q = 0; q < LOADS_W + LOADS_A + TOUCH; ++q) load(q);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         Piece<EXACT> af[2];
@@ -478,7 +487,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
       // the one before it is multiplied, and the loads are spread over the step (in a row they would hold
       // the wavefronts up until the address unit has taken them all): in this order, which the compiler would give
       // up to save registers.
-      constexpr int LAG = 3, ALL = TM * TN, LOADS = LOADS_W + LOADS_A;
+      constexpr int LAG = 3, ALL = TM * TN, LOADS = LOADS_W + LOADS_A + TOUCH;
       Piece<EXACT> af[2][2];
       constexpr int SR = (LAG + TN - 1) / TN + 1;  // rows whose scales the pending FMAs hold
       float sr[2], s[SR];
@@ -514,6 +523,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   for (int q = 0; q < LOADS_W; ++q) load_w(q, first, 0);
 #pragma unroll
   for (int q = 0; q < LOADS_A; ++q) load_a(q, first + 1, 1);
+  if (TOUCH) touch(first + 2);
   int b = first;
   for (; b + 1 < last; b += 2) {
     step(b, 0);
@@ -631,15 +641,15 @@ void launch_rows(const F8Args& p, hipStream_t s) {
   k_f8_rows<MT, NT, KW, DEPTH, EXACT><<<grid, 64 * KW, kLds, s>>>(p);
 }
 
-template <int BM, int BN, int WM, int WN, bool EXACT>
+template <int BM, int BN, int WM, int WN, bool EXACT, bool TOUCH = false>
 void launch_gemm(const F8Args& p, hipStream_t s) {
-  constexpr int kLds = 3 * (BM / 16 * kTileBytes + 4 * BM);
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_f8_gemm<BM, BN, WM, WN, EXACT>),
+  constexpr int kLds = 3 * (BM / 16 * kTileBytes + 4 * BM) + (TOUCH ? 256 * WM * WN : 0);
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_f8_gemm<BM, BN, WM, WN, EXACT, TOUCH>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   (void)attr;
   const dim3 grid(static_cast<unsigned>((p.N + BN - 1) / BN) * static_cast<unsigned>((p.M + BM - 1) / BM), 1,
                   static_cast<unsigned>(p.splits));
-  k_f8_gemm<BM, BN, WM, WN, EXACT><<<grid, 64 * WM * WN, kLds, s>>>(p);
+  k_f8_gemm<BM, BN, WM, WN, EXACT, TOUCH><<<grid, 64 * WM * WN, kLds, s>>>(p);
 }
 
 template <bool F32>
@@ -654,7 +664,14 @@ void launch_plan(const F8Plan& plan, const F8Args& p, hipStream_t s) {
     case GEMM_64x128: launch_gemm<64, 128, 1, 4, F32>(p, s); break;
     case GEMM_128x128: launch_gemm<128, 128, 1, 4, F32>(p, s); break;
     case GEMM_128x256:
-      if constexpr (!F32) launch_gemm<128, 256, 1, 4, false>(p, s);
+      if constexpr (!F32) {
+        // Touches where a call's own operands are a good part of the last-level cache (256 MB), so that W comes from
+        // memory: us, over three sets of them in turn, 4096 rows 2048 -> 22016 (233 MB) 207 (224 without), 1024 rows (92 MB) 57
+        // (62); 4096 rows 11008 -> 2048 (84 MB) 89 (86).
+        const int64_t bytes = static_cast<int64_t>(p.M) * p.K + static_cast<int64_t>(p.tiles) * p.kb * kTileBytes + 2 * static_cast<int64_t>(p.M) * p.N;
+        if (bytes > 90'000'000) launch_gemm<128, 256, 1, 4, false, true>(p, s);
+        else launch_gemm<128, 256, 1, 4, false>(p, s);
+      }
       break;
   }
 }

@@ -462,32 +462,51 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
       for (int h = 0; h < 2; ++h) af[h].set(*reinterpret_cast<const uint4_t*>(la + i * kTileBytes + a_at[h]));
     };
     Piece<EXACT> wf[TN][2];
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) wf[j][h].set(wr[buf][j][h]);
+    constexpr int LOADS = LOADS_W + LOADS_A + TOUCH;
     if constexpr (EXACT) {
+      // A's next fragment is read, and a share of the loads issued, while this one is converted and multiplied.
+      uint4_t raw[2][2];
+      auto read_a = [&](int i) {
 #pragma unroll
-      for (int q = 0; q < LOADS_W + LOADS_A + TOUCH; ++q) load(q);
+        for (int h = 0; h < 2; ++h) raw[i & 1][h] = *reinterpret_cast<const uint4_t*>(la + i * kTileBytes + a_at[h]);
+      };
+      read_a(0);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) wf[j][h].set(wr[buf][j][h]);
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
+        if (i + 1 < TM) read_a(i + 1);
+#pragma unroll
+        for (int q = (i * LOADS + TM - 1) / TM; q < ((i + 1) * LOADS + TM - 1) / TM; ++q) load(q);
         Piece<EXACT> af[2];
-        load_af(i, af);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) af[h].set(raw[i & 1][h]);
         const float s = ls[16 * i] * sw[buf];
         float4_t c[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) c[j] = block_product(wf[j], af);
+        for (int j = 0; j < TN; ++j) c[j] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) c[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[j][x >> 1].h[x & 1], af[x >> 1].h[x & 1], c[j], 0, 0, 0);
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(c[j][e], s, acc[i][j][e]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) wf[j][h].set(wr[buf][j][h]);
       // A product's four FMAs come three products later, when it has left the matrix unit, a fragment is read while
       // the one before it is multiplied, and the loads are spread over the step (in a row they would hold
       // the wavefronts up until the address unit has taken them all): in this order, which the compiler would give
       // up to save registers.
-      constexpr int LAG = 3, ALL = TM * TN, LOADS = LOADS_W + LOADS_A + TOUCH;
+      constexpr int LAG = 3, ALL = TM * TN;
       Piece<EXACT> af[2][2];
       constexpr int SR = (LAG + TN - 1) / TN + 1;  // rows whose scales the pending FMAs hold
       float sr[2], s[SR];

@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cmath>
 #include <new>
+#include <type_traits>
 
 #include "tmh_f8.h"
 #include "tmh_internal.h"
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int groups = p.tiles / NT, row_group = blockIdx.x / groups, tile = (blockIdx.x - row_group * groups) * NT;
   const uint8_t* w = p.w + (static_cast<int64_t>(tile) * p.kb) * kTileBytes + lane * 16;
-  const float* ws = p.w_scales + static_cast<int64_t>(tile / 8) * p.kb;
+  const auto ws_rsrc = buffer_rsrc(p.w_scales + static_cast<int64_t>(tile / 8) * p.kb, static_cast<uint32_t>(p.kb) * 4);
   const int first = blockIdx.z * p.per, last = min(first + p.per, p.kb);
   uint8_t* mine = lds + wave * DEPTH * STAGE;
   const int a_row = lane >> 3, a_chunk = (lane & 7) ^ a_row;
@@ -197,19 +198,23 @@ __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
   uint4_t wr[DEPTH][NT][2];
   float sw[DEPTH], sa[DEPTH][MT];
   constexpr int LOADS = 2 * NT + 1 + 3 * MT;
+  // A block's rows first, then what goes to registers, whose own waits the compiler sees to: so the wait for the rows below
+  // holds with all of them and with fewer. (The scales by vector loads like the others, in this order: they are counted.)
   auto load = [&](int b, int buf) {
+    const int k0 = b * kF8Block;
+#pragma unroll
+    for (int q = 0; q < 2 * MT; ++q)
+      lds_dma16(a_rsrc, mine + buf * STAGE + q * 1024, k0 + 16 * a_chunk < p.K ? a_off + q * a_rows : 0x80000000u, static_cast<uint32_t>(k0));
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         wr[buf][j][h] = *reinterpret_cast<const uint4_t*>(w + (static_cast<int64_t>(j) * p.kb + b) * kTileBytes + 1024 * h);
-    sw[buf] = ws[b];
-    const int k0 = b * kF8Block;
-#pragma unroll
-    for (int q = 0; q < 2 * MT; ++q)
-      lds_dma16(a_rsrc, mine + buf * STAGE + q * 1024, k0 + 16 * a_chunk < p.K ? a_off + q * a_rows : 0x80000000u, static_cast<uint32_t>(k0));
+    sw[buf] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(ws_rsrc, 0, static_cast<uint32_t>(b) * 4, 0));
 #pragma unroll
     for (int t = 0; t < MT; ++t) sa[buf][t] = p.a_scales[static_cast<int64_t>(b) * p.M + min(m0 + 16 * t + r, p.M - 1)];
+    asm volatile("" ::: "memory");
   };
   float4_t acc[MT][NT];
 #pragma unroll
@@ -220,7 +225,6 @@ __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
     const int ahead = b + (DEPTH - 1) * KW;
     if (ahead < last) {
       load(ahead, (buf + DEPTH - 1) % DEPTH);
-      asm volatile("" ::: "memory");
       wait_vm<(DEPTH - 1) * LOADS>();  // this block's loads: the later ones' are the youngest
     } else if (DEPTH > 2 && ahead - KW < last) {
       wait_vm<LOADS>();
@@ -354,19 +358,20 @@ __device__ __forceinline__ void gemm_outputs(const F8Args& p, const float4_t (&a
 }
 
 // Many rows: BM rows of A times BN of W a workgroup, WM x WN wavefronts of (BM / WM) x (BN / WN) outputs each.
-// A step is one block of K. A's bytes go global -> LDS (buffer_load ... lds) in the order of the MFMA operands,
-// 1 KiB an instruction, two steps ahead, with the step's row scales; W's tiles, which are operands as they lie, go
-// to registers a step ahead and past LDS, whose reads would bound the loop otherwise. What lies past M, N or K is
-// past the buffers' ranges and arrives as zeros.
-template <int BM, int BN, int WM, int WN, bool EXACT, bool TOUCH>
+// A step is one block of K. A's bytes go global -> LDS (buffer_load ... lds), 1 KiB an instruction, DA steps ahead, with
+// the step's row scales; W's tiles, which are operands as they lie, go to registers DW steps ahead and past LDS, whose
+// reads would bound the loop otherwise. What lies past M, N or K is past the buffers' ranges and arrives as zeros.
+template <int BM, int BN, int WM, int WN, int DW, int DA, bool EXACT, bool TOUCH>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   constexpr int NW = WM * WN, TM = BM / 16 / WM, TN = BN / 16 / WN;
   constexpr int A_TILES = BM / 16, A_DMA = 2 * A_TILES / NW;
   constexpr int STAGE = A_TILES * kTileBytes;
   static_assert(A_DMA * NW == 2 * A_TILES && BM % 64 == 0 && TN % 2 == 0, "whole instructions a wavefront, pairs of tiles");
-  static_assert(NW * kOwnBytes <= 3 * STAGE, "the outputs' way through LDS");
-  extern __shared__ __align__(16) uint8_t lds[];  // [3][STAGE], then the rows' scales [3][BM]
-  float* lds_s = reinterpret_cast<float*>(lds + 3 * STAGE);
+  static_assert(NW * kOwnBytes <= (DA + 1) * STAGE, "the outputs' way through LDS");
+  constexpr int STAGES = DA + 1;
+  static_assert(DA >= DW, "a block's rows are asked for no later than its weights");
+  extern __shared__ __align__(16) uint8_t lds[];  // [STAGES][STAGE], then the rows' scales [STAGES][BM]
+  float* lds_s = reinterpret_cast<float*>(lds + STAGES * STAGE);
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
@@ -402,11 +407,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   const int first = blockIdx.z * p.per, last = min(first + p.per, p.kb);
   const int n_wave = n0 + wn * (BN / WN), m_wave = m0 + wm * (BM / WM);
   // The wavefront's columns lie in one block of 128 rows of W (n0 and BN / WN divide it).
-  const float* ws = p.w_scales + static_cast<int64_t>(min(n_wave, p.N - 1) / kF8Block) * p.kb;
+  const auto ws_rsrc = buffer_rsrc(p.w_scales + static_cast<int64_t>(min(n_wave, p.N - 1) / kF8Block) * p.kb, static_cast<uint32_t>(p.kb) * 4);
   const int s_part = wave % (BM / 64);
-  uint4_t wr[2][TN][2];
-  float sw[2];
-  // The loads of a step, one at a time: W's tiles of block b + 1, then A's rows and scales of block b + 2. (No
+  uint4_t wr[DW + 1][TN][2];
+  float sw[DW + 1];
+  // The loads of a step, one at a time: W's tiles of block b + DW, then A's rows and scales of block b + DA. (No
   // branches, which the compiler would move the products' FMAs behind: past the last block the loads of A have no
   // range and those of W and the scales are the last block's again.)
   constexpr int LOADS_W = 2 * TN + 1, LOADS_A = A_DMA + 1;
@@ -416,15 +421,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   const uint32_t touch_off = mine ? static_cast<uint32_t>(min(wn * TN + (lane >> 4), p.tiles - 1 - n0 / 16)) * static_cast<uint32_t>(p.kb) * kTileBytes + (lane & 15) * 128
                                   : 0x80000000u;
   auto touch = [&](int b) {
-    lds_dma4(w_rsrc, lds + 3 * STAGE + 3 * BM * 4 + wave * 256, touch_off, static_cast<uint32_t>(min(b, last - 1)) * kTileBytes);
+    lds_dma4(w_rsrc, lds + STAGES * (STAGE + BM * 4) + wave * 256, touch_off, static_cast<uint32_t>(min(b, last - 1)) * kTileBytes);
   };
   auto load_w = [&](int q, int at, int buf) {
     const int b = min(at, last - 1);
     if (q < 2 * TN)
       wr[buf][q >> 1][q & 1] = __builtin_bit_cast(uint4_t, __builtin_amdgcn_raw_buffer_load_b128(
           w_rsrc, lane * 16 + 1024 * (q & 1), w_off[q >> 1] + static_cast<uint32_t>(b) * kTileBytes, 0));
-    else
-      sw[buf] = ws[b];
+    else  // (a vector load like the others: they are counted)
+      sw[buf] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(ws_rsrc, 0, static_cast<uint32_t>(b) * 4, 0));
   };
   auto load_a = [&](int q, int b, int slot) {
     if (q < A_DMA) {
@@ -443,16 +448,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
   int slot = 0;
-  auto step = [&](int b, int buf) {
-    // The youngest outstanding loads are those of the next step's A (and a touch): this step's W, scales and A are there.
-    wait_vm<LOADS_A + TOUCH>();
+  auto barrier = [&]() {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // everybody's; and everybody has read the stage that is filled next
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int free_slot = slot == 0 ? 2 : slot - 1;
+  };
+  // MORE: with the loads of later blocks. (Without, what it reads has been waited for.)
+  auto step = [&](int b, int buf, auto more) {
+    constexpr bool MORE = decltype(more)::value;
+    if constexpr (MORE) {
+      // This step's W, scales and A are there: behind them the steps before have asked for later blocks. The barrier: everybody's are,
+      // and everybody has read the stage that is filled next.
+      constexpr int A_STEP = LOADS_W + LOADS_A + TOUCH;
+      wait_vm<(DW - 1) * A_STEP + (DA > DW ? LOADS_A + TOUCH : TOUCH)>();
+      barrier();
+    }
+    const int free_slot = slot == 0 ? DA : slot - 1;
     auto load = [&](int q) {
-      if (q < LOADS_W) load_w(q, b + 1, buf ^ 1);
-      else if (q < LOADS_W + LOADS_A) load_a(q - LOADS_W, b + 2, free_slot);
+      if (!MORE) return;
+      if (q < LOADS_W) load_w(q, b + DW, (buf + DW) % (DW + 1));
+      else if (q < LOADS_W + LOADS_A) load_a(q - LOADS_W, b + DA, free_slot);
       else touch(b + 4);
     };
     const uint8_t* la = lds + slot * STAGE + wm * TM * kTileBytes;
@@ -534,22 +549,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    slot = slot == 2 ? 0 : slot + 1;
+    slot = slot == DA ? 0 : slot + 1;
   };
 #pragma unroll
-  for (int q = 0; q < LOADS_A; ++q) load_a(q, first, 0);
+  for (int d = 0; d < DA; ++d) {  // what the steps before the first would have asked for, in their order
+    if (d >= DA - DW) {
 #pragma unroll
-  for (int q = 0; q < LOADS_W; ++q) load_w(q, first, 0);
+      for (int q = 0; q < LOADS_W; ++q) load_w(q, first + d - (DA - DW), d - (DA - DW));
+      asm volatile("" ::: "memory");
+    }
 #pragma unroll
-  for (int q = 0; q < LOADS_A; ++q) load_a(q, first + 1, 1);
-  if (TOUCH) touch(first + 2);
-  int b = first;
-  for (; b + 1 < last; b += 2) {
-    step(b, 0);
-    step(b + 1, 1);
+    for (int q = 0; q < LOADS_A; ++q) load_a(q, first + d, d);
+    if (TOUCH && d >= DA - DW) touch(first + 2);
+    asm volatile("" ::: "memory");
   }
-  if (b < last) step(b, 0);
-  wait_vm<0>();  // nothing is on its way to LDS when the workgroup ends
+  int b = first;
+  for (; b + DW < last; b += DW + 1) {
+#pragma unroll
+    for (int d = 0; d < DW + 1; ++d) step(b + d, d, std::true_type{});
+  }
+  // Up to DW steps are left. Their loads have no later ones of a known number behind them (what nobody would read the compiler
+  // leaves out), so they are all waited for.
+  wait_vm<0>();
+  barrier();
+#pragma unroll
+  for (int d = 0; d < DW; ++d)
+    if (b + d < last) step(b + d, d, std::false_type{});
   if (p.part) gemm_outputs<DT_F32, true, TM, TN>(p, acc, m_wave, n_wave, lds + wave * kOwnBytes);
   else if (EXACT) gemm_outputs<DT_F32, false, TM, TN>(p, acc, m_wave, n_wave, lds + wave * kOwnBytes);
   else if (p.y_dtype == DT_F16) gemm_outputs<DT_F16, false, TM, TN>(p, acc, m_wave, n_wave, lds + wave * kOwnBytes);
@@ -588,15 +613,18 @@ struct F8Plan {
 };
 
 // k_f8_gemm: one workgroup's step of 128 of K, in us: alone on its CU (the loads' latency), and with the CU full (the
-// matrix and memory units), as measured over K at sizes that fill the chip once and several times.
+// matrix and memory units), as measured over K at sizes that fill the chip once and several times. How far ahead the loads are
+// (DW, DA) is what the registers leave room for, and three blocks with 64 x 64 against one: us, 512 rows 2048 -> 2048 7.1
+// (9.4 with one), 256 rows 4096 -> 4096 10.5 (15.3); two with 64 x 128: 1024 rows 11008 -> 2048 31.5 (41.6); one with 128 x 128, whose
+// third workgroup on a CU two would cost: 2048 rows 2048 -> 22016 109 (115 with two).
 struct F8Shape {
   int kernel, bm, bn;
   float alone[2], full[2];  // for a 16-bit Y, and for an f32 Y
 };
 constexpr F8Shape kF8Shapes[] = {
-    {GEMM_64x64, 64, 64, {0.26f, 0.50f}, {0.19f, 0.35f}},
-    {GEMM_64x128, 64, 128, {0.36f, 0.94f}, {0.32f, 0.53f}},
-    {GEMM_128x128, 128, 128, {0.60f, 1.40f}, {0.52f, 1.00f}},
+    {GEMM_64x64, 64, 64, {0.25f, 0.48f}, {0.25f, 0.39f}},
+    {GEMM_64x128, 64, 128, {0.34f, 0.75f}, {0.33f, 0.60f}},
+    {GEMM_128x128, 128, 128, {0.60f, 1.40f}, {0.54f, 1.05f}},
     {GEMM_128x256, 128, 256, {0.95f, 0.f}, {0.87f, 0.f}},  // (its f32 form's registers would not fit)
 };
 // k_f8_rows by row tiles (of 16), column tiles and wavefronts: a CU takes in 88 KB of weights and rows of A a us, a wavefront
@@ -660,15 +688,15 @@ void launch_rows(const F8Args& p, hipStream_t s) {
   k_f8_rows<MT, NT, KW, DEPTH, EXACT><<<grid, 64 * KW, kLds, s>>>(p);
 }
 
-template <int BM, int BN, int WM, int WN, bool EXACT, bool TOUCH = false>
+template <int BM, int BN, int WM, int WN, int DW, int DA, bool EXACT, bool TOUCH = false>
 void launch_gemm(const F8Args& p, hipStream_t s) {
-  constexpr int kLds = 3 * (BM / 16 * kTileBytes + 4 * BM) + (TOUCH ? 256 * WM * WN : 0);
-  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_f8_gemm<BM, BN, WM, WN, EXACT, TOUCH>),
+  constexpr int kLds = (DA + 1) * (BM / 16 * kTileBytes + 4 * BM) + (TOUCH ? 256 * WM * WN : 0);
+  static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_f8_gemm<BM, BN, WM, WN, DW, DA, EXACT, TOUCH>),
                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   (void)attr;
   const dim3 grid(static_cast<unsigned>((p.N + BN - 1) / BN) * static_cast<unsigned>((p.M + BM - 1) / BM), 1,
                   static_cast<unsigned>(p.splits));
-  k_f8_gemm<BM, BN, WM, WN, EXACT, TOUCH><<<grid, 64 * WM * WN, kLds, s>>>(p);
+  k_f8_gemm<BM, BN, WM, WN, DW, DA, EXACT, TOUCH><<<grid, 64 * WM * WN, kLds, s>>>(p);
 }
 
 template <bool F32>
@@ -679,17 +707,17 @@ void launch_plan(const F8Plan& plan, const F8Args& p, hipStream_t s) {
     case ROWS32: launch_rows<2, 1, 16, 2, F32>(p, s); break;
     case ROWS32_WIDE: launch_rows<2, 2, 8, 2, F32>(p, s); break;
     case ROWS64: launch_rows<4, 1, 8, 2, F32>(p, s); break;
-    case GEMM_64x64: launch_gemm<64, 64, 2, 2, F32>(p, s); break;
-    case GEMM_64x128: launch_gemm<64, 128, 1, 4, F32>(p, s); break;
-    case GEMM_128x128: launch_gemm<128, 128, 1, 4, F32>(p, s); break;
+    case GEMM_64x64: launch_gemm<64, 64, 2, 2, F32 ? 2 : 3, F32 ? 2 : 3, F32>(p, s); break;
+    case GEMM_64x128: launch_gemm<64, 128, 1, 4, 2, 2, F32>(p, s); break;
+    case GEMM_128x128: launch_gemm<128, 128, 1, 4, 1, 2, F32>(p, s); break;
     case GEMM_128x256:
       if constexpr (!F32) {
         // Touches where a call's own operands are a good part of the last-level cache (256 MB), so that W comes from
         // memory: us, over three sets of them in turn, 4096 rows 2048 -> 22016 (233 MB) 207 (224 without), 1024 rows (92 MB) 57
         // (62); 4096 rows 11008 -> 2048 (84 MB) 89 (86).
         const int64_t bytes = static_cast<int64_t>(p.M) * p.K + static_cast<int64_t>(p.tiles) * p.kb * kTileBytes + 2 * static_cast<int64_t>(p.M) * p.N;
-        if (bytes > 90'000'000) launch_gemm<128, 256, 1, 4, false, true>(p, s);
-        else launch_gemm<128, 256, 1, 4, false>(p, s);
+        if (bytes > 90'000'000) launch_gemm<128, 256, 1, 4, 1, 2, false, true>(p, s);
+        else launch_gemm<128, 256, 1, 4, 1, 2, false>(p, s);
       }
       break;
   }

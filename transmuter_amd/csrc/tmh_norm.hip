@@ -1,6 +1,7 @@
 // The root-mean-square norm with the residual's addition, and rows in 8 bits (tmh_rms_norm,
 // tmh_quantize_rows). Both are bound by memory: each input is read once and each output written once.
 #include <algorithm>
+#include <type_traits>
 
 #include "tmh_f8.h"
 #include "tmh_internal.h"
@@ -86,22 +87,23 @@ __device__ __forceinline__ void norm_outputs(const NormArgs& p, int64_t row, int
 // largest magnitude they find among themselves. Rows of up to 512 columns go to a wavefront each (no barrier), others to as many
 // wavefronts as hold them, with one piece a thread while a workgroup can: 4096 rows of 4096 f16 with a residual 26.4 us, 30.3
 // with two pieces and half the threads, 45.0 with a wavefront to a row.
-template <int DT, bool WIDE, int NCH>
+template <int DT, bool WIDE, int NCH, bool VEC>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void k_rms_norm(NormArgs p) {
   const int tpr = WIDE ? static_cast<int>(blockDim.x) : 64;
   const int t = WIDE ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) % 64;
   const int64_t group = xcd_row_group(blockIdx.x, gridDim.x);
   const int64_t row = WIDE ? group : group * 4 + threadIdx.x / 64;
   if (row >= p.rows) return;  // (a row of a workgroup always exists)
+  auto column = [&](int c) { return c * tpr * 8 + (t >> 4) * kF8Block + lane_columns(VEC); };
   float h[NCH][8], g[NCH][8];
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
-    const int col = (c * tpr + t) * 8;
-    load8<DT, true>(p.x, row * p.ldx + col, p.cols - col, h[c]);
-    load_gamma(p, col, p.cols - col, g[c], true);
+    const int col = column(c);
+    load8<DT, VEC, kLaneStep>(p.x, row * p.ldx + col, p.cols - col, h[c]);
+    load_gamma(p, col, p.cols - col, g[c], VEC);
     if (p.residual) {
       float r[8];
-      load8<DT, true>(p.residual, row * p.ldr + col, p.cols - col, r);
+      load8<DT, VEC, kLaneStep>(p.residual, row * p.ldr + col, p.cols - col, r);
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[c][i] += r[i];
     }
@@ -117,23 +119,23 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void k_rms_norm(NormArgs p) {
   if (p.sum) {
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
-      const int col = (c * tpr + t) * 8;
-      store8<DT, true>(p.sum, row * p.lds + col, p.cols - col, h[c]);
+      const int col = column(c);
+      store8<DT, VEC, kLaneStep>(p.sum, row * p.lds + col, p.cols - col, h[c]);
     }
   }
   const float rstd = row_rstd<WIDE>(p, squares);
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
-    const int col = (c * tpr + t) * 8;
-    norm_outputs<DT, true>(p, row, col, p.cols - col, h[c], g[c], rstd);
+    const int col = column(c);
+    norm_outputs<DT, VEC>(p, row, col, p.cols - col, h[c], g[c], rstd);
   }
 }
 
-// Rows of any width, alignment and pitch: the inputs are read twice, the second time from the caches. An
+// Rows of more than 32768 columns: the inputs are read twice, the second time from the caches. An
 // output may be an input's memory: a row is read whole ahead of the barrier, and its outputs are written by the
 // thread that has just read the same elements again.
 template <int DT>
-__global__ __launch_bounds__(256) void k_rms_norm_any(NormArgs p) {
+__global__ __launch_bounds__(1024) void k_rms_norm_any(NormArgs p) {
   const int64_t row = xcd_row_group(blockIdx.x, gridDim.x);
   const int own = static_cast<int>(threadIdx.x >> 4) * kF8Block + lane_columns(false);
   auto load = [&](int col, float (&h)[8]) {
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(256) void k_rms_norm_any(NormArgs p) {
   };
   const float rstd = row_rstd<true>(p, [&](float f) {
     float s = 0.f;
-    for (int col = own; col < p.cols; col += 2048) {
+    for (int col = own; col < p.cols; col += 8 * static_cast<int>(blockDim.x)) {
       float h[8];
       load(col, h);
 #pragma unroll
@@ -156,7 +158,7 @@ __global__ __launch_bounds__(256) void k_rms_norm_any(NormArgs p) {
     return s;
   });
   // Whole blocks of 16 lanes stay together: lanes past the row hold zeros.
-  for (int col = own; col - static_cast<int>(threadIdx.x & 15) < p.cols; col += 2048) {
+  for (int col = own; col - static_cast<int>(threadIdx.x & 15) < p.cols; col += 8 * static_cast<int>(blockDim.x)) {
     float h[8], g[8];
     load(col, h);
     load_gamma(p, col, p.cols - col, g, false);
@@ -216,11 +218,16 @@ void launch_norm(const NormArgs& p, bool vec, hipStream_t s) {
   const unsigned rows = static_cast<unsigned>(p.rows), fours = static_cast<unsigned>((p.rows + 3) / 4);
   // Whole wavefronts of `pieces` pieces of eight columns a thread.
   auto threads = [&](int pieces) { return static_cast<unsigned>((p.cols + 512 * pieces - 1) / (512 * pieces) * 64); };
-  if (!vec || p.cols > 32768) k_rms_norm_any<DT><<<rows, 256, 0, s>>>(p);
-  else if (p.cols <= 512) k_rms_norm<DT, false, 1><<<fours, 256, 0, s>>>(p);
-  else if (p.cols <= 8192) k_rms_norm<DT, true, 1><<<rows, threads(1), 0, s>>>(p);
-  else if (p.cols <= 16384) k_rms_norm<DT, true, 2><<<rows, threads(2), 0, s>>>(p);
-  else k_rms_norm<DT, true, 4><<<rows, threads(4), 0, s>>>(p);
+  auto launch = [&](auto v) {
+    constexpr bool VEC = decltype(v)::value;
+    if (p.cols > 32768) k_rms_norm_any<DT><<<rows, 1024, 0, s>>>(p);
+    else if (p.cols <= 512) k_rms_norm<DT, false, 1, VEC><<<fours, 256, 0, s>>>(p);
+    else if (p.cols <= 8192) k_rms_norm<DT, true, 1, VEC><<<rows, threads(1), 0, s>>>(p);
+    else if (p.cols <= 16384) k_rms_norm<DT, true, 2, VEC><<<rows, threads(2), 0, s>>>(p);
+    else k_rms_norm<DT, true, 4, VEC><<<rows, threads(4), 0, s>>>(p);
+  };
+  if (vec) launch(std::true_type{});
+  else launch(std::false_type{});
 }
 
 template <int DT>

@@ -20,6 +20,10 @@ CASES = {  # lengths, tokens that the table has room for, heads, kv heads, dim, 
     "whole, half the chip": (RAGGED * 2, 1024, 16, 4, 128, 16, 0),
     "whole, a window": ([700, 0, 5, 1024] * 8, 1024, 8, 4, 64, 32, 100),
     "whole, two chunks of heads": ([400, 0, 77], 448, 40, 2, 80, 7, 0),
+    "whole, one unit": ([1, 0, 128, 77, 5] * 60, 128, 8, 2, 128, 16, 0),
+    "whole, one unit of wide heads": ([1, 0, 45, 33] * 20, 60, 16, 4, 256, 20, 0),
+    "whole, a window in a long table": ([5000, 0, 100, 129, 1], 8192, 8, 2, 128, 16, 100),
+    "whole, a window of wide heads": ([900, 0, 70, 128], 4096, 64, 4, 256, 16, 60),
     "meet, few items": ([1, 4000, 900], 4096, 8, 8, 128, 16, 0),
     "meet, one sequence": ([2111], 2112, 16, 4, 128, 64, 0),
     "meet, many sequences": (RAGGED * 10, 2048, 4, 2, 64, 16, 0),

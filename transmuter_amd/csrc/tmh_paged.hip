@@ -301,12 +301,12 @@ __device__ __forceinline__ float column_sum(float v) {
 //        finds all others counted joins the parts in their order, whoever it is, so the answer does not depend on who comes
 //        last.
 //  PARTS k_paged_join joins them.
-//  WHOLE there are none: a workgroup of eight wavefronts takes an item, and looks at its own sequence's length only.
-enum : int { JOIN, PARTS, WHOLE };
+//  WHOLE there are none: a workgroup (WHOLE8: of eight wavefronts) takes an item, and looks at its own sequence's length only.
+enum : int { JOIN, PARTS, WHOLE, WHOLE8 };
 template <int DT, int NB, int HOW>  // NB: blocks of 16 E dimensions
-__global__ __launch_bounds__(HOW == WHOLE ? 512 : 256, NB == 1 || (DT == DT_F32 && NB == 2) ? 2 : 1) void k_paged_attention(AttendArgs p) {
-  constexpr bool F32 = DT == DT_F32;
-  constexpr int WAVES = HOW == WHOLE ? 8 : 4, THREADS = 64 * WAVES;
+__global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32 && NB == 2) ? 2 : 1) void k_paged_attention(AttendArgs p) {
+  constexpr bool F32 = DT == DT_F32, ALONE = HOW == WHOLE || HOW == WHOLE8;
+  constexpr int WAVES = HOW == WHOLE8 ? 8 : 4, THREADS = 64 * WAVES;
   constexpr int SIZE = F32 ? 4 : 2, E = 16 / SIZE, TILE = F32 ? 16 : 32, UT = WAVES * TILE;
   constexpr int NH = TILE / 16;           // 16-token halves of a tile
   constexpr int NC = 4 * NB;              // chunks of 4 E dimensions of a row
@@ -335,7 +335,7 @@ __global__ __launch_bounds__(HOW == WHOLE ? 512 : 256, NB == 1 || (DT == DT_F32 
   }
   uint32_t per = 0, at, stop, before = 0;
   int b;
-  if constexpr (HOW == WHOLE) {
+  if constexpr (ALONE) {
     b = static_cast<int>(worker / items);
     const uint32_t units = static_cast<uint32_t>(span_at<UT>(p, b).units), item = worker - b * items;
     at = item * units;
@@ -553,7 +553,7 @@ __global__ __launch_bounds__(HOW == WHOLE ? 512 : 256, NB == 1 || (DT == DT_F32 
           *reinterpret_cast<float4_t*>(&lds_o[wave][col][16 * E * nb + E * (4 * g + i) + e]) =
               float4_t{acc[nb][e][i], acc[nb][e + 1][i], acc[nb][e + 2][i], acc[nb][e + 3][i]};
     __syncthreads();
-    const bool whole = HOW == WHOLE || (from == 0 && to == static_cast<uint32_t>(sp.units));
+    const bool whole = ALONE || (from == 0 && to == static_cast<uint32_t>(sp.units));
     [[maybe_unused]] const uint32_t slot = part_place(worker, at == run);
     const int part_heads = min(kHeads, p.group), quads = p.head_dim / 4;
     auto joined = [&](int hd, int dim, float& top, float& total) {
@@ -752,12 +752,13 @@ template <int DT, int HOW>
 void launch_attention(const AttendArgs& p, int heads, hipStream_t s) {
   constexpr int per_block = DT == DT_F32 ? 64 : 128;
   const int nb = (p.head_dim + per_block - 1) / per_block;
-  constexpr int threads = HOW == WHOLE ? 512 : 256;
+  constexpr int threads = HOW == WHOLE8 ? 512 : 256;
+  constexpr int most = HOW != WHOLE8 ? (DT == DT_F32 ? 4 : 2) : (DT == DT_F32 ? 2 : 1);  // (eight wavefronts' registers)
   if (nb == 1) k_paged_attention<DT, 1, HOW><<<p.workers, threads, 0, s>>>(p);
-  else if constexpr (HOW != WHOLE || DT == DT_F32) {
+  if constexpr (most >= 2)
     if (nb == 2) k_paged_attention<DT, 2, HOW><<<p.workers, threads, 0, s>>>(p);
-    else if constexpr (HOW != WHOLE && DT == DT_F32) k_paged_attention<DT, 4, HOW><<<p.workers, threads, 0, s>>>(p);
-  }
+  if constexpr (most >= 4)
+    if (nb > 2) k_paged_attention<DT, 4, HOW><<<p.workers, threads, 0, s>>>(p);
   if constexpr (HOW == PARTS) k_paged_join<DT><<<dim3(static_cast<unsigned>(heads), static_cast<unsigned>(p.B)), 256, 0, s>>>(p);
 }
 
@@ -893,21 +894,28 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
   p.meet = ctx->meet;
   p.part_bytes = static_cast<uint32_t>(rows * cache->head_dim * 4);
   p.stats_bytes = static_cast<uint32_t>(rows * sizeof(float2));
-  // WHOLE where the table has room for few tokens (the lengths are the device's): a workgroup's turn of 256 tokens costs 2.6 us
-  // more, parts that meet 3.3 us, f16 4 kv heads of 128: one sequence of 300 8.4 us (9.2 in parts), of 700 11.3 (9.4); and
-  // with workgroups for half the CUs and more, 32 x 700 12.9 (16.1), 60 x 1..1000 16.7 (20.0), 8 x 1000 15.2 (10.7).
+  // Tokens that a sequence may have as far as the host knows (the lengths are the device's), and the units they lie in.
+  const int64_t tokens = window > 0 ? std::min(p.most, window) : p.most;
+  auto units_of = [&](int64_t u) { return (tokens + u - 1) / u + (tokens < p.most ? 1 : 0); };
   const int64_t all_items = B * cache->kv_heads * chunks;
-  const bool whole = cache->head_dim <= 128 && all_items <= ctx->num_cus &&
-                     (p.most <= 512 || (p.most <= 1024 && all_items >= ctx->num_cus / 2));
+  // WHOLE where an item is one unit, which cannot be cut (116 x 1..45, bf16 4 kv heads of 256, 17.1 us as parts, 13.4 whole; one token of f16 4 kv heads of 128 5.5 and 4.7). Few items
+  // of a few units go WHOLE8, where the registers allow it: a turn of 256 tokens (f32: 128) costs 2.6 us more (3.6), parts that meet
+  // 3.3 us, f16 4 kv heads of 128: one sequence of 300 8.4 us (9.2 in parts), of 700 11.3 (9.4); and with workgroups for half the
+  // CUs and more, 32 x 700 12.9 (16.1), 60 x 1..1000 16.7 (20.0), 8 x 1000 15.2 (10.7).
+  const bool eight = cache->head_dim <= 128 && all_items <= ctx->num_cus &&
+                     (units_of(2 * unit) <= 2 || (units_of(2 * unit) <= 4 && all_items >= ctx->num_cus / 2));
+  const bool whole = units_of(unit) == 1 ||
+                     (!eight && all_items <= ctx->num_cus && (units_of(unit) <= 2 || (units_of(unit) <= 4 && all_items >= ctx->num_cus / 2)));
+  if (whole || eight) p.workers = static_cast<uint32_t>(all_items);
   // JOIN where one workgroup has few parts to read (of equal lengths; of others it may be more): one sequence of 4096 (32 parts of 2
   // KiB) 9.9 us, 11.8 as PARTS; 32 x 4000 56.6 and 58.7; one of 32768 (128 parts) 25.5 and 24.6, 64 x 2000 with 16 heads of one kv
   // head (8 parts of 8 KiB) 22.6 and 20.6.
-  const int64_t parts = std::min<int64_t>((p.most + unit - 1) / unit, workers / all_items + 2);
+  const int64_t parts = std::min<int64_t>(units_of(unit), workers / all_items + 2);
   const bool join = parts * std::min(kHeads, group) * cache->head_dim * 4 <= kJoinBytes;
-  if (whole) p.workers = static_cast<uint32_t>(all_items);
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (whole) launch_attention<DT, WHOLE>(p, heads, s);
+    else if (eight) launch_attention<DT, WHOLE8>(p, heads, s);
     else if (join) launch_attention<DT, JOIN>(p, heads, s);
     else launch_attention<DT, PARTS>(p, heads, s);
   };

@@ -18,7 +18,8 @@
  *  - `stream` is a hipStream_t; NULL means the context's own stream. Calls are asynchronous
  *    on that stream unless stated otherwise.
  *  - Shapes are int64_t element counts; no call reads or writes outside the extents given.
- *  - Prefill MatMulNBits (split K), DynamicQuantizeLinear and QMoE keep
+ *  - Prefill MatMulNBits (split K), DynamicQuantizeLinear, QMoE, the 8-bit product (rows at any
+ *    address, parts of K) and paged attention (parts of sequences, and counters beside) keep
  *    intermediates in one workspace per context, grown outside graph capture. Calls of one
  *    context on two streams must not run at the same time; use a context per concurrent stream.
  *    A call that would have to grow the workspace while its stream is being captured into a
@@ -383,7 +384,7 @@ int tmh_qmoe(tmh_ctx* ctx, const void* d_x, int x_dtype, int64_t T, int64_t H, c
  * row may be shorter), and scales [ceil(N/128), T], the rows of one block of columns side by side, as
  * the product reads them: value (t, n) is q[t, n] * scales[n / 128, t]. A block's scale is its largest
  * magnitude / 448, at least 2^-126, and 1 for a block of zeros; its values divided by the scale (as
- * f32 multiplied by the scale's f32 reciprocal) round to nearest even. A NaN in a block makes its scale
+ * f32 multiplied by the scale's reciprocal, which is within a step of f32) round to nearest even. A NaN in a block makes its scale
  * NaN, an infinity makes it infinite (finite values of the block become 0, infinite ones NaN).
  * Sums and statistics are f32; leading dimensions (ld*) are in elements and at least the row's width.
  */
@@ -410,7 +411,7 @@ int tmh_quantize_rows(tmh_ctx* ctx, const void* d_x, int64_t ldx, const void* d_
 
 /*
  * A weight [N, K] of F8E4M3 (row-major, on the device) with f32 scales [ceil(N/128), ceil(K/128)], one for
- * each 128 x 128 block, laid out once in the product's tiles, with zeros to whole tiles of 16 x 128;
+ * each 128 x 128 block, laid out once in the product's tiles, with zeros to whole tiles of 32 x 128;
  * asynchronous on `stream`, whose later work may use the weight at once (d_b and d_scales must stay until
  * then). K and N at most 2^22. Free with tmh_fp8_weight_free after that work is done.
  */

@@ -62,9 +62,9 @@ __device__ __forceinline__ float f8_block(const float (&v)[8], uint2& q) {
 }
 
 // Eight elements of type DT: consecutive ones in one or two 16-byte accesses (VEC), or every STEP-th one at a time,
-// those below `n` from the first (past which loads give zeros and stores leave memory alone). Where 16 lanes hold a block
-// of 128 one element at a time, each takes every sixteenth, so that an access is 16 neighbours (quantizing 4096 rows of 2050
-// f16: 16.8 us with eight neighbours to a lane, 11.1 so).
+// those below `n` from the first (past which loads give zeros and stores leave memory alone). Where 16 lanes hold a
+// block of 128 one element at a time, each takes every sixteenth, so that an access is 16 neighbours (quantizing 4096
+// rows of 2050 f16: 16.8 us with eight neighbours to a lane, 11.1 so).
 constexpr int kLaneStep = 16;
 __device__ __forceinline__ int lane_columns(bool vec) {  // a lane's first column of its block
   return vec ? (threadIdx.x & 15) * 8 : threadIdx.x & 15;

@@ -15,10 +15,10 @@
 #include "tmh_f8.h"
 #include "tmh_internal.h"
 
-// Tiles of 16 rows x 128 of K, 2 KiB each in the order [N / 16][K / 128]: two halves (64 of K each) of 1 KiB,
-// lane l = 16 g + r of a wavefront holding row r, k = 64 h + 16 g .. + 15 at offset 16 l of half h. A
-// wavefront's 16-byte loads of a tile are its MFMA operand (the order of k within a block is free, as long as
-// both factors share it), and read 1 KiB in a row. Rows past N and k past K are zeros.
+// Tiles of 16 rows x 128 of K, 2 KiB each in the order [N / 16][K / 128]: two halves (64 of K each) of 1 KiB, lane l
+// = 16 g + r of a wavefront holding row r (of the pair of tiles' 32, tile_row), k = 64 h + 16 g .. + 15 at offset 16
+// l of half h. A wavefront's 16-byte loads of a tile are its MFMA operand (the order of k within a block is free, as
+// long as both factors share it), and read 1 KiB in a row. Rows past N and k past K are zeros; tiles come in pairs.
 struct tmh_fp8_weight {
   int device = 0;
   int64_t K = 0, N = 0;
@@ -175,10 +175,13 @@ __device__ __forceinline__ void wait_vm() {
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | (7 << 4));
 }
 
-// Few rows: a workgroup of KW wavefronts takes NT tiles of 16 columns of Y for 16 MT rows, the
-// wavefronts every KW-th block of K each, and adds their sums in LDS. A wavefront has the next DEPTH - 1 blocks' loads on
-// their way while it multiplies one: W's tiles to registers, A's rows to a place of its own in LDS (no barrier),
-// eight lanes to a row's line (the fragments' own 16 bytes of 16 rows would be 64 lookups a load, k_f8_gemm).
+// Few rows: a workgroup of KW wavefronts takes NT tiles of 16 columns of Y for 16 MT rows, the wavefronts every KW-th
+// block of K each, and adds their sums in LDS. A wavefront has the next DEPTH - 1 blocks' loads on their way while it
+// multiplies one: W's tiles to registers, A's rows to a place of its own in LDS (no barrier), eight lanes to a row's
+// line (the fragments' own 16 bytes of 16 rows would be 64 lookups a load, k_f8_gemm). Bound by the weights' bytes
+// where they are many (one row 2048 -> 22016: 8.7 us, 5.2 TB/s), by what a CU takes in of A and W and the way there
+// where they are few (32 rows 11008 -> 2048 7.1 us, 3.2 TB/s; 13.8 with fragments loaded as they lie, one block at a
+// time).
 template <int MT, int NT, int KW, int DEPTH, bool EXACT>
 __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
   constexpr int STAGE = MT * kTileBytes;
@@ -198,8 +201,9 @@ __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
   uint4_t wr[DEPTH][NT][2];
   float sw[DEPTH], sa[DEPTH][MT];
   constexpr int LOADS = 2 * NT + 1 + 3 * MT;
-  // A block's rows first, then what goes to registers, whose own waits the compiler sees to: so the wait for the rows below
-  // holds with all of them and with fewer. (The scales by vector loads like the others, in this order: they are counted.)
+  // A block's rows first, then what goes to registers, whose own waits the compiler sees to: so the wait for the rows
+  // below holds with all of them and with fewer. (The scales by vector loads like the others, in this order: they are
+  // counted.)
   auto load = [&](int b, int buf) {
     const int k0 = b * kF8Block;
 #pragma unroll
@@ -357,10 +361,17 @@ __device__ __forceinline__ void gemm_outputs(const F8Args& p, const float4_t (&a
   }
 }
 
-// Many rows: BM rows of A times BN of W a workgroup, WM x WN wavefronts of (BM / WM) x (BN / WN) outputs each.
-// A step is one block of K. A's bytes go global -> LDS (buffer_load ... lds), 1 KiB an instruction, DA steps ahead, with
-// the step's row scales; W's tiles, which are operands as they lie, go to registers DW steps ahead and past LDS, whose
+// Many rows: BM rows of A times BN of W a workgroup, WM x WN wavefronts of (BM / WM) x (BN / WN) outputs each. A step
+// is one block of K. A's bytes go global -> LDS (buffer_load ... lds), 1 KiB an instruction, DA steps ahead, with the
+// step's row scales; W's tiles, which are operands as they lie, go to registers DW steps ahead and past LDS, whose
 // reads would bound the loop otherwise. What lies past M, N or K is past the buffers' ranges and arrives as zeros.
+//
+// 4096 x 2048 -> 22016 (f16 Y, 128 x 256): 204 us, 1.8 PFLOP/s, with operands that come from memory, 172 us with
+// those that the last-level cache holds; 8192 x 8192 x 8192 2.25. The matrix unit is busy 54% of the cycles there, at
+// a clock that its own power holds at 1.9 GHz. A block's product needs four FMAs of its own beside it: a loop of
+// nothing but both reaches 3.5 PFLOP/s (4.0 without them). On the way: 16-byte pieces of 64 rows of A an instruction
+// and 8-byte stores 277 us, whole lines 231; two workgroups of 128 x 256 a CU instead of one of 256 x 256 224; the
+// loads one by one between the products 210 (all ahead of them 224).
 template <int BM, int BN, int WM, int WN, int DW, int DA, bool EXACT, bool TOUCH>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   constexpr int NW = WM * WN, TM = BM / 16 / WM, TN = BN / 16 / WN;
@@ -415,8 +426,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   // branches, which the compiler would move the products' FMAs behind: past the last block the loads of A have no
   // range and those of W and the scales are the last block's again.)
   constexpr int LOADS_W = 2 * TN + 1, LOADS_A = A_DMA + 1;
-  // TOUCH: a look at W's lines four blocks further on, a line a lane, each line by one of the row tiles that walk together,
-  // which brings them from memory to the XCD's L2 (the loads of the next block alone would arrive late).
+  // TOUCH: a look at W's lines four blocks further on, a line a lane, each line by one of the row tiles that walk
+  // together, which brings them from memory to the XCD's L2 (the loads of the next block alone would arrive late).
   const bool mine = TOUCH && lane < 16 * TN && (lane >> 3) % group_m == in_group % group_m;
   const uint32_t touch_off = mine ? static_cast<uint32_t>(min(wn * TN + (lane >> 4), p.tiles - 1 - n0 / 16)) * static_cast<uint32_t>(p.kb) * kTileBytes + (lane & 15) * 128
                                   : 0x80000000u;
@@ -457,8 +468,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
   auto step = [&](int b, int buf, auto more) {
     constexpr bool MORE = decltype(more)::value;
     if constexpr (MORE) {
-      // This step's W, scales and A are there: behind them the steps before have asked for later blocks. The barrier: everybody's are,
-      // and everybody has read the stage that is filled next.
+      // This step's W, scales and A are there: behind them the steps before have asked for later blocks. The barrier:
+      // everybody's are, and everybody has read the stage that is filled next.
       constexpr int A_STEP = LOADS_W + LOADS_A + TOUCH;
       wait_vm<(DW - 1) * A_STEP + (DA > DW ? LOADS_A + TOUCH : TOUCH)>();
       barrier();
@@ -568,8 +579,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
 #pragma unroll
     for (int d = 0; d < DW + 1; ++d) step(b + d, d, std::true_type{});
   }
-  // Up to DW steps are left. Their loads have no later ones of a known number behind them (what nobody would read the compiler
-  // leaves out), so they are all waited for.
+  // Up to DW steps are left. Their loads have no later ones of a known number behind them (what nobody would read the
+  // compiler leaves out), so they are all waited for.
   wait_vm<0>();
   barrier();
 #pragma unroll
@@ -613,10 +624,11 @@ struct F8Plan {
 };
 
 // k_f8_gemm: one workgroup's step of 128 of K, in us: alone on its CU (the loads' latency), and with the CU full (the
-// matrix and memory units), as measured over K at sizes that fill the chip once and several times. How far ahead the loads are
-// (DW, DA) is what the registers leave room for, and three blocks with 64 x 64 against one: us, 512 rows 2048 -> 2048 7.1
-// (9.4 with one), 256 rows 4096 -> 4096 10.5 (15.3); two with 64 x 128: 1024 rows 11008 -> 2048 31.5 (41.6); one with 128 x 128, whose
-// third workgroup on a CU two would cost: 2048 rows 2048 -> 22016 109 (115 with two).
+// matrix and memory units), as measured over K at sizes that fill the chip once and several times. How far ahead the
+// loads are (DW, DA) is what the registers leave room for, and three blocks with 64 x 64 against one: us, 512 rows
+// 2048 -> 2048 7.1 (9.4 with one), 256 rows 4096 -> 4096 10.5 (15.3); two with 64 x 128: 1024 rows 11008 -> 2048 31.5
+// (41.6); one with 128 x 128, whose third workgroup on a CU two would cost: 2048 rows 2048 -> 22016 109 (115 with
+// two).
 struct F8Shape {
   int kernel, bm, bn;
   float alone[2], full[2];  // for a 16-bit Y, and for an f32 Y
@@ -627,9 +639,9 @@ constexpr F8Shape kF8Shapes[] = {
     {GEMM_128x128, 128, 128, {0.60f, 1.40f}, {0.54f, 1.05f}},
     {GEMM_128x256, 128, 256, {0.95f, 0.f}, {0.87f, 0.f}},  // (its f32 form's registers would not fit)
 };
-// k_f8_rows by row tiles (of 16), column tiles and wavefronts: a CU takes in 88 KB of weights and rows of A a us, a wavefront
-// a block of K every 0.33 us at most, and a turn of workgroups costs `turn` us beside (ROWS32 and ROWS64 fill a CU's LDS, so
-// that their turns do not overlap).
+// k_f8_rows by row tiles (of 16), column tiles and wavefronts: a CU takes in 88 KB of weights and rows of A a us, a
+// wavefront a block of K every 0.33 us at most, and a turn of workgroups costs `turn` us beside (ROWS32 and ROWS64
+// fill a CU's LDS, so that their turns do not overlap).
 struct F8Rows {
   int kernel, row_tiles, col_tiles, waves;
   double first, turn;
@@ -637,14 +649,15 @@ struct F8Rows {
 constexpr F8Rows kF8Rows[] = {{ROWS16, 1, 1, 8, 2.0, 0.35}, {ROWS16_WIDE, 1, 2, 8, 2.0, 0.35}, {ROWS32, 2, 1, 16, 1.4, 1.0},
                               {ROWS32_WIDE, 2, 2, 8, 2.0, 0.5}, {ROWS64, 4, 1, 8, 1.4, 1.0}};
 
-// The kernel by what it is expected to take; parts of K cost their sums' way to memory and back (4.5 TB/s, 8 TB/s while the
-// last-level cache holds them) and the second launch (2.4 us). Measured, us (f16 Y): one row 2048 -> 22016 8.5 by ROWS16_WIDE, 8.9
-// by ROWS16; 2048 -> 2048 3.7 by ROWS16, 3.9 by ROWS16_WIDE; 32 rows 11008 -> 2048 6.5 by ROWS16 (twice over W), 7.8 by ROWS32; 64
-// rows 8.0 by ROWS16_WIDE, 8.8 by ROWS32, 10.0 by ROWS16, 12.1 by ROWS64, 10.3 by 64x64 in 8 parts; 64 rows 4096 -> 4096 6.1 by
-// ROWS32_WIDE, 7.1 by ROWS64, 9.7 by 64x64 in 4 parts; 64 rows 2048 -> 22016 11.1 by 64x64, 21.9 by ROWS64; 128 rows 11008 -> 2048 14.1 by
-// 64x64 in 8 parts, 15.7 in 4, 39.6 in one of 64x128; 512 rows 2048 -> 2048 6.9 by 64x64, 11.1 by 128x128; 512 rows 2048 -> 22016
-// 27.0 by 128x128, 28.3 by 128x256, 43.9 by 64x64; 4096 rows 11008 -> 2048 81 by 128x256, 87 by 128x128, 119 by a tile of 256 x
-// 256, which no size was best with.
+// The kernel by what it is expected to take; parts of K cost their sums' way to memory and back (4.5 TB/s, 8 TB/s
+// while the last-level cache holds them) and the second launch (2.4 us). Measured, us (f16 Y): one row 2048 -> 22016
+// 8.5 by ROWS16_WIDE, 8.9 by ROWS16; 2048 -> 2048 3.7 by ROWS16, 3.9 by ROWS16_WIDE; 32 rows 11008 -> 2048 6.5 by
+// ROWS16 (twice over W), 7.8 by ROWS32; 64 rows 8.0 by ROWS16_WIDE, 8.8 by ROWS32, 10.0 by ROWS16, 12.1 by ROWS64,
+// 10.3 by 64x64 in 8 parts; 64 rows 4096 -> 4096 6.1 by ROWS32_WIDE, 7.1 by ROWS64, 9.7 by 64x64 in 4 parts; 64 rows
+// 2048 -> 22016 11.1 by 64x64, 21.9 by ROWS64; 128 rows 11008 -> 2048 14.1 by 64x64 in 8 parts, 15.7 in 4, 39.6 in
+// one of 64x128; 512 rows 2048 -> 2048 6.9 by 64x64, 11.1 by 128x128; 512 rows 2048 -> 22016 27.0 by 128x128, 28.3 by
+// 128x256, 43.9 by 64x64; 4096 rows 11008 -> 2048 81 by 128x256, 87 by 128x128, 119 by a tile of 256 x 256, which no
+// size was best with.
 F8Plan plan_of(int64_t M, int64_t N, int kb, int64_t tiles, bool f32, int num_cus) {
   F8Plan best{GEMM_128x128, 1};
   double least = 1e30;
@@ -713,8 +726,8 @@ void launch_plan(const F8Plan& plan, const F8Args& p, hipStream_t s) {
     case GEMM_128x256:
       if constexpr (!F32) {
         // Touches where a call's own operands are a good part of the last-level cache (256 MB), so that W comes from
-        // memory: us, over three sets of them in turn, 4096 rows 2048 -> 22016 (233 MB) 207 (224 without), 1024 rows (92 MB) 57
-        // (62); 4096 rows 11008 -> 2048 (84 MB) 89 (86).
+        // memory: us, over three sets of them in turn, 4096 rows 2048 -> 22016 (233 MB) 207 (224 without), 1024 rows
+        // (92 MB) 57 (62); 4096 rows 11008 -> 2048 (84 MB) 89 (86).
         const int64_t bytes = static_cast<int64_t>(p.M) * p.K + static_cast<int64_t>(p.tiles) * p.kb * kTileBytes + 2 * static_cast<int64_t>(p.M) * p.N;
         if (bytes > 90'000'000) launch_gemm<128, 256, 1, 4, 1, 2, false, true>(p, s);
         else launch_gemm<128, 256, 1, 4, 1, 2, false>(p, s);

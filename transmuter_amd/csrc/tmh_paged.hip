@@ -27,8 +27,8 @@ struct AppendArgs {
   int64_t page_stride, token_stride, head_stride;
   int64_t num_slots;
   int table_dtype, rotary, interleaved, heads, kv_heads;
-  // A token's pieces: of each query and key head (`turned` of them pairs of eight dimensions half a rotary row apart), then
-  // of each value head.
+  // A token's pieces: of each query and key head (`turned` of them pairs of eight dimensions half a rotary row
+  // apart), then of each value head.
   uint32_t pieces, value_pieces;
   int turned, head_dim;
   FastDiv by_pieces, by_head, by_value, by_page;
@@ -45,8 +45,9 @@ __device__ __forceinline__ void load_table(const void* p, int dtype, int64_t at,
   }
 }
 
-// A thread answers eight dimensions of one head of one token, and with VEC of those that turn by halves their partners
-// too. VEC: rows and partners lie on 16 bytes.
+// A thread answers eight dimensions of one head of one token, and with VEC of those that turn by halves their
+// partners too. VEC: rows and partners lie on 16 bytes. Bound by memory: 4096 bf16 tokens of 32 and 4 heads of 128
+// 18.0 us, 4.7 TB/s (20.0 with each half read by two threads).
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs p, int64_t first, uint32_t count, bool table_vec, bool pairs_vec) {
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;
@@ -295,6 +296,11 @@ __device__ __forceinline__ float column_sum(float v) {
 // f16 parts are taken of 2^15 times the probability, so that small ones of long rows do not fall below f16's
 // range; f32 and bf16 ones of 2^-32 times it, so that sums of up to 2^31 values near the type's largest stay
 // finite. The factor is in the running sum too and drops out.
+//
+// Bound by memory where there are many tokens: 4 x 131072 f16 181 us, 5.7 TB/s; 32 x 1..8000 bf16 58.5 us, 4.5 TB/s,
+// of which about 12 us are the way in (lengths, page table, first rows) and out; one sequence of 700 tokens 9.4 us,
+// all of it such ways. Runs of units of equal number to each of two workgroups a CU (their registers' limit) even
+// ragged lengths out; three a CU would spill.
 //
 // What happens to items that several workers share:
 //  JOIN  they meet here. Each leaves its part in memory (stores that pass the XCD's own L2), then counts itself; the one that
@@ -590,9 +596,9 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
     if constexpr (HOW == JOIN) {
       if (!whole) {
         const Parts parts = parts_of(item_first, static_cast<uint32_t>(sp.units), per);
-        // The parts are stored and loaded past the XCDs' L2 caches, so that the order is all that is left to see to: this
-        // thread's stores have arrived, then everybody's, then the count. (Fences of that scope would also write the L2
-        // back and empty it: 32 x 8000 tokens took 163 us with them, 58 without.)
+        // The parts are stored and loaded past the XCDs' L2 caches, so that the order is all that is left to see to:
+        // this thread's stores have arrived, then everybody's, then the count. (Fences of that scope would also write
+        // the L2 back and empty it: 32 x 8000 tokens took 163 us with them, 58 without.)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         __shared__ uint32_t others;
@@ -602,8 +608,8 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
         }
         __syncthreads();
         if (others == parts.count - 1) {
-          // A thread takes four dimensions of one head and every so many parts, BATCH parts' loads at a time, with a running
-          // maximum; the threads of the same dimensions then meet in LDS.
+          // A thread takes four dimensions of one head and every so many parts, BATCH parts' loads at a time, with a
+          // running maximum; the threads of the same dimensions then meet in LDS.
           constexpr int BATCH = F32 && NB == 2 ? 8 : 16;  // (what the registers hold)
           const int all_quads = heads * quads, groups = max(256 / all_quads, 1), mine_group = static_cast<int>(threadIdx.x) / all_quads;
           float4_t* sums = reinterpret_cast<float4_t*>(&lds_o[0][0][0]);
@@ -898,18 +904,19 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
   const int64_t tokens = window > 0 ? std::min(p.most, window) : p.most;
   auto units_of = [&](int64_t u) { return (tokens + u - 1) / u + (tokens < p.most ? 1 : 0); };
   const int64_t all_items = B * cache->kv_heads * chunks;
-  // WHOLE where an item is one unit, which cannot be cut (116 x 1..45, bf16 4 kv heads of 256, 17.1 us as parts, 13.4 whole; one token of f16 4 kv heads of 128 5.5 and 4.7). Few items
-  // of a few units go WHOLE8, where the registers allow it: a turn of 256 tokens (f32: 128) costs 2.6 us more (3.6), parts that meet
-  // 3.3 us, f16 4 kv heads of 128: one sequence of 300 8.4 us (9.2 in parts), of 700 11.3 (9.4); and with workgroups for half the
-  // CUs and more, 32 x 700 12.9 (16.1), 60 x 1..1000 16.7 (20.0), 8 x 1000 15.2 (10.7).
+  // WHOLE where an item is one unit, which cannot be cut (116 x 1..45, bf16 4 kv heads of 256, 17.1 us as parts, 13.4
+  // whole; one token of f16 4 kv heads of 128 5.5 and 4.7). Few items of a few units go WHOLE8, where the registers
+  // allow it: a turn of 256 tokens (f32: 128) costs 2.6 us more (3.6), parts that meet 3.3 us, f16 4 kv heads of 128:
+  // one sequence of 300 8.4 us (9.2 in parts), of 700 11.3 (9.4); and with workgroups for half the CUs and more, 32 x
+  // 700 12.9 (16.1), 60 x 1..1000 16.7 (20.0), 8 x 1000 15.2 (10.7).
   const bool eight = cache->head_dim <= 128 && all_items <= ctx->num_cus &&
                      (units_of(2 * unit) <= 2 || (units_of(2 * unit) <= 4 && all_items >= ctx->num_cus / 2));
   const bool whole = units_of(unit) == 1 ||
                      (!eight && all_items <= ctx->num_cus && (units_of(unit) <= 2 || (units_of(unit) <= 4 && all_items >= ctx->num_cus / 2)));
   if (whole || eight) p.workers = static_cast<uint32_t>(all_items);
-  // JOIN where one workgroup has few parts to read (of equal lengths; of others it may be more): one sequence of 4096 (32 parts of 2
-  // KiB) 9.9 us, 11.8 as PARTS; 32 x 4000 56.6 and 58.7; one of 32768 (128 parts) 25.5 and 24.6, 64 x 2000 with 16 heads of one kv
-  // head (8 parts of 8 KiB) 22.6 and 20.6.
+  // JOIN where one workgroup has few parts to read (of equal lengths; of others it may be more): one sequence of 4096
+  // (32 parts of 2 KiB) 9.9 us, 11.8 as PARTS; 32 x 4000 56.6 and 58.7; one of 32768 (128 parts) 25.5 and 24.6, 64 x
+  // 2000 with 16 heads of one kv head (8 parts of 8 KiB) 22.6 and 20.6.
   const int64_t parts = std::min<int64_t>(units_of(unit), workers / all_items + 2);
   const bool join = parts * std::min(kHeads, group) * cache->head_dim * 4 <= kJoinBytes;
   auto launch = [&](auto dt) {

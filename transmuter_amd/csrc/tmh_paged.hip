@@ -154,6 +154,7 @@ void launch_append(const AppendArgs& p, int64_t T, bool vec, bool table_vec, boo
 
 constexpr int kHeads = 16;  // query heads of one kv head that a workgroup answers (the columns of an MFMA tile)
 constexpr float kNone = -__builtin_inff();
+constexpr uint32_t kNowhere = 1u << 31;  // an offset past every buffer's range here
 constexpr int64_t kJoinBytes = 72 << 10;
 constexpr int kThrough = 16;  // sc1 of a buffer access: past the XCD's L2, to where all XCDs meet
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
@@ -297,8 +298,8 @@ __device__ __forceinline__ float column_sum(float v) {
 // range; f32 and bf16 ones of 2^-32 times it, so that sums of up to 2^31 values near the type's largest stay
 // finite. The factor is in the running sum too and drops out.
 //
-// Bound by memory where there are many tokens: 4 x 131072 f16 181 us, 5.7 TB/s; 32 x 1..8000 bf16 58.5 us, 4.5 TB/s,
-// of which about 12 us are the way in (lengths, page table, first rows) and out; one sequence of 700 tokens 9.4 us,
+// Bound by memory where there are many tokens: 4 x 131072 f16 181 us, 5.7 TB/s; 32 x 1..8000 bf16 57.2 us, 4.6 TB/s,
+// of which about 12 us are the way in (lengths, page table, first rows) and out; one sequence of 700 tokens 8.1 us,
 // all of it such ways. Runs of units of equal number to each of two workgroups a CU (their registers' limit) even
 // ragged lengths out; three a CU would spill.
 //
@@ -608,9 +609,9 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
         }
         __syncthreads();
         if (others == parts.count - 1) {
-          // A thread takes four dimensions of one head and every so many parts, BATCH parts' loads at a time, with a
-          // running maximum; the threads of the same dimensions then meet in LDS.
-          constexpr int BATCH = F32 && NB == 2 ? 8 : 16;  // (what the registers hold)
+          // A thread takes four dimensions of one head and every so many parts, a batch of parts' loads at a time (as many
+          // as the registers hold, or four where that is all), with a running maximum; the threads of the same dimensions
+          // then meet in LDS. What a batch has too many lies past the buffers' ranges: nothing is fetched for it.
           const int all_quads = heads * quads, groups = max(256 / all_quads, 1), mine_group = static_cast<int>(threadIdx.x) / all_quads;
           float4_t* sums = reinterpret_cast<float4_t*>(&lds_o[0][0][0]);
           float2* tops = reinterpret_cast<float2*>(sums + 256);
@@ -619,31 +620,39 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
             const int hd = i / quads, dim = (i - hd * quads) * 4;
             float top = kNone, total = 0.f;
             float4_t o{0.f, 0.f, 0.f, 0.f};
-            if (mine_group < groups && i < all_quads) {
+            auto batches = [&](auto batch) {
+              constexpr int BATCH = decltype(batch)::value;
               for (uint32_t k0 = mine_group; k0 < parts.count; k0 += BATCH * groups) {
                 float2 st[BATCH];
                 float4_t po[BATCH];
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
-                  const uint32_t row = place_of(parts, min(k0 + k * groups, parts.count - 1)) * part_heads + hd;
-                  st[k] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(stats_rsrc, row * 8, 0, kThrough));
-                  po[k] = __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(parts_rsrc, (row * p.head_dim + dim) * 4, 0, kThrough));
+                  const bool there = k0 + k * groups < parts.count;
+                  const uint32_t row = place_of(parts, k0 + k * groups) * part_heads + hd;
+                  st[k] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(stats_rsrc, there ? row * 8 : kNowhere, 0, kThrough));
+                  po[k] = __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(parts_rsrc, there ? (row * p.head_dim + dim) * 4 : kNowhere, 0, kThrough));
                 }
                 float next = top;
 #pragma unroll
-                for (int k = 0; k < BATCH; ++k) next = fmaxf(next, st[k].x);
+                for (int k = 0; k < BATCH; ++k) {
+                  if (k0 + k * groups >= parts.count) st[k].x = kNone;
+                  next = fmaxf(next, st[k].x);
+                }
                 const float keep = top == next ? 1.f : __builtin_amdgcn_exp2f(top - next);
                 total *= keep;
                 o *= keep;
                 top = next;
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
-                  if (k0 + k * groups >= parts.count) continue;
                   const float f = st[k].x == top ? 1.f : __builtin_amdgcn_exp2f(st[k].x - top);
                   total += f * st[k].y;
                   o += f * po[k];
                 }
               }
+            };
+            if (mine_group < groups && i < all_quads) {
+              if (parts.count <= 4u * groups) batches(std::integral_constant<int, 4>{});
+              else batches(std::integral_constant<int, F32 && NB == 2 ? 8 : 12>{});
             }
             if (groups > 1) {
               sums[threadIdx.x] = o;

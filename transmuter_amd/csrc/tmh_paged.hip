@@ -176,6 +176,7 @@ struct AttendArgs {
   int64_t window, most;  // most: max_pages * page_size
   int B, group, kv_heads, chunks, head_dim;
   uint32_t workers;
+  FastDiv by_units, by_items;  // EACH: units of an item, items of a sequence
   float scale;  // of the scores in base-2 logarithms: scale * log2(e)
 };
 
@@ -299,7 +300,7 @@ __device__ __forceinline__ float column_sum(float v) {
 // finite. The factor is in the running sum too and drops out.
 //
 // Bound by memory where there are many tokens: 4 x 131072 f16 181 us, 5.7 TB/s; 32 x 1..8000 bf16 57.2 us, 4.6 TB/s,
-// of which about 12 us are the way in (lengths, page table, first rows) and out; one sequence of 700 tokens 8.1 us,
+// of which about 12 us are the way in (lengths, page table, first rows) and out; one sequence of 700 tokens 7.5 us,
 // all of it such ways. Runs of units of equal number to each of two workgroups a CU (their registers' limit) even
 // ragged lengths out; three a CU would spill.
 //
@@ -309,10 +310,15 @@ __device__ __forceinline__ float column_sum(float v) {
 //        last.
 //  PARTS k_paged_join joins them.
 //  WHOLE there are none: a workgroup (WHOLE8: of eight wavefronts) takes an item, and looks at its own sequence's length only.
-enum : int { JOIN, PARTS, WHOLE, WHOLE8 };
+//  EACH  JOIN with a worker to each unit that the table has room for, where no window moves them: a worker knows its
+//        tokens without the lengths, so that it looks their pages up meanwhile. Those past the length leave.
+enum : int { JOIN, PARTS, WHOLE, WHOLE8, EACH };
 template <int DT, int NB, int HOW>  // NB: blocks of 16 E dimensions
 __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32 && NB == 2) ? 2 : 1) void k_paged_attention(AttendArgs p) {
-  constexpr bool F32 = DT == DT_F32, ALONE = HOW == WHOLE || HOW == WHOLE8;
+  // Every line of the arguments at once: one that is first looked at further on would cost its way then (us: one token of
+  // f16 4.7 without this, 4.5 with it; of f32 and 256 dimensions 8.9 and 8.3).
+  asm volatile("" ::"s"(p.q), "s"(p.part_bytes), "s"(p.window), "s"(p.scale));
+  constexpr bool F32 = DT == DT_F32, ALONE = HOW == WHOLE || HOW == WHOLE8, MEET = HOW == JOIN || HOW == EACH;
   constexpr int WAVES = HOW == WHOLE8 ? 8 : 4, THREADS = 64 * WAVES;
   constexpr int SIZE = F32 ? 4 : 2, E = 16 / SIZE, TILE = F32 ? 16 : 32, UT = WAVES * TILE;
   constexpr int NH = TILE / 16;           // 16-token halves of a tile
@@ -342,7 +348,20 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
   }
   uint32_t per = 0, at, stop, before = 0;
   int b;
-  if constexpr (ALONE) {
+  [[maybe_unused]] uint32_t each_item = 0, each_unit = 0;
+  [[maybe_unused]] int32_t length = 0;
+  if constexpr (HOW == EACH) {
+    const uint32_t of_all = p.by_units.div(worker);
+    each_unit = worker - of_all * p.by_units.d;
+    b = static_cast<int>(p.by_items.div(of_all));
+    each_item = of_all - b * items;
+    int of_lane = b;  // (by a vector load, like the table's below: both are then waited for at once)
+    asm volatile("" : "+v"(of_lane));
+    length = p.lengths[of_lane];
+    per = 1;
+    at = worker;
+    stop = worker + 1;
+  } else if constexpr (ALONE) {
     b = static_cast<int>(worker / items);
     const uint32_t units = static_cast<uint32_t>(span_at<UT>(p, b).units), item = worker - b * items;
     at = item * units;
@@ -375,18 +394,23 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
     }
   }
   [[maybe_unused]] const uint32_t run = at;
-  Span sp = span_at<UT>(p, b);
+  Span sp{};
+  if constexpr (HOW != EACH) sp = span_at<UT>(p, b);
   uint32_t first = before * items;  // the first unit of the sequence's first item
   const int chunks_of_row = (p.head_dim + 4 * E - 1) / (4 * E);
   const bool ragged = p.head_dim % (4 * E) != 0;
   while (at < stop) {
-    while (at >= first + static_cast<uint32_t>(sp.units) * items) {
-      first += static_cast<uint32_t>(sp.units) * items;
-      sp = span_at<UT>(p, ++b);
+    uint32_t item = each_item, item_first = at - each_unit, from = each_unit, to = each_unit + 1;
+    if constexpr (HOW != EACH) {
+      while (at >= first + static_cast<uint32_t>(sp.units) * items) {
+        first += static_cast<uint32_t>(sp.units) * items;
+        sp = span_at<UT>(p, ++b);
+      }
+      item = (at - first) / static_cast<uint32_t>(sp.units);
+      item_first = first + item * sp.units;
+      from = at - item_first;
+      to = min(stop - item_first, static_cast<uint32_t>(sp.units));
     }
-    const uint32_t item = (at - first) / static_cast<uint32_t>(sp.units);
-    const uint32_t item_first = first + item * sp.units;
-    const uint32_t from = at - item_first, to = min(stop - item_first, static_cast<uint32_t>(sp.units));
     const int kv_head = static_cast<int>(item) / p.chunks, chunk = static_cast<int>(item) % p.chunks;
     const int heads = min(kHeads, p.group - chunk * kHeads);
     const int head0 = kv_head * p.group + chunk * kHeads;
@@ -413,7 +437,7 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
     // Lane i looks token i % TILE of a unit's tile up, a unit ahead: its row's offset in bytes, -1 where it is masked.
     auto look = [&](uint32_t u) -> int64_t {
       const int token = (sp.unit + static_cast<int>(u)) * UT + wave * TILE + lane % TILE;
-      if (u >= to || token < sp.begin || token >= sp.end) return -1;
+      if (HOW == EACH ? token >= p.most : (u >= to || token < sp.begin || token >= sp.end)) return -1;
       return token_offset(p.cache, table, static_cast<uint32_t>(token)) * SIZE;  // (a page that is none: negative)
     };
     // The loads are a unit ahead of the products, without more registers: K's next rows follow when the scores have
@@ -441,7 +465,16 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
         }
       }
     };
-    int64_t found = look(from), coming = look(from + 1);
+    int64_t found = look(from), coming = HOW == EACH ? -1 : look(from + 1);
+    if constexpr (HOW == EACH) {
+      sp = span_of(__builtin_amdgcn_readfirstlane(length), p.most, 0, UT);
+      if (from >= static_cast<uint32_t>(sp.units)) {
+        if (from == 0)
+          for (int i = threadIdx.x; i < heads * (p.head_dim / 4); i += THREADS) store(b, head0, 4 * i, float4_t{0.f, 0.f, 0.f, 0.f});
+        return;
+      }
+      if (static_cast<int>(from) * UT + wave * TILE + lane % TILE >= sp.end) found = -1;
+    }
     load_k(found < 0 ? 0 : found);
     load_v(found < 0 ? 0 : found);
     for (uint32_t u = from; u < to; ++u) {
@@ -449,7 +482,7 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
       const int64_t next_row = coming < 0 ? 0 : coming;
       const bool more = u + 1 < to;
       found = coming;
-      coming = look(u + 2);
+      if constexpr (HOW != EACH) coming = look(u + 2);
       const bool full = TILE == 32 ? valid == 0xFFFFFFFFu : (valid & 0xFFFFu) == 0xFFFFu;
       if (ragged) {
 #pragma unroll
@@ -584,7 +617,7 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
       const int64_t row = static_cast<int64_t>(slot) * part_heads + hd;
       if (whole) {
         store(b, head0 + hd, dim, o * (total == 0.f ? 0.f : 1.f / total));
-      } else if constexpr (HOW == JOIN) {
+      } else if constexpr (MEET) {
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4_t, o), parts_rsrc, static_cast<uint32_t>(row * p.head_dim + dim) * 4, 0, kThrough);
         if (dim == 0)
           __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uint2_t, make_float2(top, total)), stats_rsrc, static_cast<uint32_t>(row) * 8, 0, kThrough);
@@ -594,7 +627,7 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
       }
     }
     at = item_first + to;
-    if constexpr (HOW == JOIN) {
+    if constexpr (MEET) {
       if (!whole) {
         const Parts parts = parts_of(item_first, static_cast<uint32_t>(sp.units), per);
         // The parts are stored and loaded past the XCDs' L2 caches, so that the order is all that is left to see to:
@@ -913,25 +946,38 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
   const int64_t tokens = window > 0 ? std::min(p.most, window) : p.most;
   auto units_of = [&](int64_t u) { return (tokens + u - 1) / u + (tokens < p.most ? 1 : 0); };
   const int64_t all_items = B * cache->kv_heads * chunks;
-  // WHOLE where an item is one unit, which cannot be cut (116 x 1..45, bf16 4 kv heads of 256, 17.1 us as parts, 13.4
-  // whole; one token of f16 4 kv heads of 128 5.5 and 4.7). Few items of a few units go WHOLE8, where the registers
-  // allow it: a turn of 256 tokens (f32: 128) costs 2.6 us more (3.6), parts that meet 3.3 us, f16 4 kv heads of 128:
-  // one sequence of 300 8.4 us (9.2 in parts), of 700 11.3 (9.4); and with workgroups for half the CUs and more, 32 x
-  // 700 12.9 (16.1), 60 x 1..1000 16.7 (20.0), 8 x 1000 15.2 (10.7).
-  const bool eight = cache->head_dim <= 128 && all_items <= ctx->num_cus &&
-                     (units_of(2 * unit) <= 2 || (units_of(2 * unit) <= 4 && all_items >= ctx->num_cus / 2));
-  const bool whole = units_of(unit) == 1 ||
-                     (!eight && all_items <= ctx->num_cus && (units_of(unit) <= 2 || (units_of(unit) <= 4 && all_items >= ctx->num_cus / 2)));
-  if (whole || eight) p.workers = static_cast<uint32_t>(all_items);
-  // JOIN where one workgroup has few parts to read (of equal lengths; of others it may be more): one sequence of 4096
-  // (32 parts of 2 KiB) 9.9 us, 11.8 as PARTS; 32 x 4000 56.6 and 58.7; one of 32768 (128 parts) 25.5 and 24.6, 64 x
-  // 2000 with 16 heads of one kv head (8 parts of 8 KiB) 22.6 and 20.6.
+  // JOIN where one workgroup has few parts to read (of equal lengths; of others it may be more): one sequence of
+  // 4096 (32 parts of 2 KiB) 9.9 us, 11.8 as PARTS; 32 x 4000 55.1 and 58.7; one of 32768 (128 parts) 25.5 and
+  // 24.6, 64 x 2000 with 16 heads of one kv head (8 parts of 8 KiB) 22.6 and 20.6. EACH instead where the table's
+  // units are no more than the CUs: one sequence of 700 8.1 us as JOIN, 7.5 so; 8 x 1000 9.4 and 8.6. (With up to
+  // two a CU: 4 x 4000 14.2 and 13.2, but tables that are not full leave the workers unevenly on the CUs: 5 x
+  // 1..2600 9.3 and 9.8, 9 x 1..900 of 256 dimensions 12.3 and 15.2.)
   const int64_t parts = std::min<int64_t>(units_of(unit), workers / all_items + 2);
   const bool join = parts * std::min(kHeads, group) * cache->head_dim * 4 <= kJoinBytes;
+  const bool each = join && tokens == p.most && units > 0 && units <= ctx->num_cus;
+  // WHOLE where an item is one unit, which cannot be cut (116 x 1..45, bf16 4 kv heads of 256, 17.1 us as JOIN, 13.4
+  // whole; one token of f16 4 kv heads of 128 4.5, as EACH 4.7), or two that EACH cannot take (4 x 200 of 256
+  // dimensions 10.8 us, as EACH 9.5). Few items of a few units go WHOLE8, where the registers allow it, if that is one
+  // turn of 256 tokens (f32: 128), as a further one costs 2.6 us (3.6), f16 4 kv heads of 128: 8 x 200 6.1 us (7.4 as
+  // EACH), but 8 x 500 9.4 (7.8); and with workgroups for half the CUs and more, 32 x 400 10.1 (10.2), 32 x 500 10.4
+  // (11.3), 32 x 700 12.8 (16.1 as JOIN), 60 x 1..1000 16.4 (20.0 as JOIN).
+  const bool half = all_items >= ctx->num_cus / 2;
+  const bool eight = cache->head_dim <= 128 && all_items <= ctx->num_cus &&
+                     (units_of(2 * unit) == 1 || (units_of(2 * unit) <= 4 && half));
+  const bool whole = units_of(unit) == 1 || (!eight && all_items <= ctx->num_cus &&
+                                             ((units_of(unit) <= 2 && !each) || (units_of(unit) <= 4 && half)));
+  if (whole || eight) {
+    p.workers = static_cast<uint32_t>(all_items);
+  } else if (each) {
+    p.workers = static_cast<uint32_t>(units);
+    p.by_units = FastDiv(static_cast<uint32_t>(units_of(unit)));
+    p.by_items = FastDiv(static_cast<uint32_t>(cache->kv_heads * chunks));
+  }
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (whole) launch_attention<DT, WHOLE>(p, heads, s);
     else if (eight) launch_attention<DT, WHOLE8>(p, heads, s);
+    else if (each) launch_attention<DT, EACH>(p, heads, s);
     else if (join) launch_attention<DT, JOIN>(p, heads, s);
     else launch_attention<DT, PARTS>(p, heads, s);
   };

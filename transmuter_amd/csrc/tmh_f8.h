@@ -70,29 +70,40 @@ __device__ __forceinline__ int lane_columns(bool vec) {  // a lane's first colum
   return vec ? (threadIdx.x & 15) * 8 : threadIdx.x & 15;
 }
 
+// Eight consecutive elements as they lie (16-bit ones in `lo`), apart from what turns them into floats, so that a
+// thread's loads can all be on their way before the first is waited for.
+struct Raw8 {
+  uint4_t lo{0u, 0u, 0u, 0u}, hi{0u, 0u, 0u, 0u};
+};
+template <int DT>
+__device__ __forceinline__ void load_raw8(const void* p, int64_t at, int n, Raw8& raw) {
+  if (n <= 0) return;
+  const uint4_t* f = reinterpret_cast<const uint4_t*>(static_cast<const char*>(p) + at * (DT == DT_F32 ? 4 : 2));
+  raw.lo = f[0];
+  if constexpr (DT == DT_F32) raw.hi = f[1];
+}
+template <int DT>
+__device__ __forceinline__ void floats_of(const Raw8& raw, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == DT_F32) {
+      const uint32_t a = raw.lo[i], b = raw.hi[i];  // (a bit cast of an element itself would take the first)
+      v[i] = __builtin_bit_cast(float, a);
+      v[4 + i] = __builtin_bit_cast(float, b);
+    } else {
+      const uint32_t w = raw.lo[i];
+      v[2 * i] = DT == DT_F16 ? f16_bits_to_f32(static_cast<uint16_t>(w)) : __builtin_bit_cast(float, w << 16);
+      v[2 * i + 1] = DT == DT_F16 ? f16_bits_to_f32(static_cast<uint16_t>(w >> 16)) : __builtin_bit_cast(float, w & 0xFFFF0000u);
+    }
+  }
+}
+
 template <int DT, bool VEC, int STEP = 1>
 __device__ __forceinline__ void load8(const void* p, int64_t at, int n, float (&v)[8]) {
   if constexpr (VEC) {
-    if (n <= 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    } else if constexpr (DT == DT_F32) {
-      const float4_t* f = reinterpret_cast<const float4_t*>(static_cast<const float*>(p) + at);
-      const float4_t a = f[0], b = f[1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = a[i];
-        v[4 + i] = b[i];
-      }
-    } else {
-      const uint4_t w = *reinterpret_cast<const uint4_t*>(static_cast<const uint16_t*>(p) + at);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = DT == DT_F16 ? f16_bits_to_f32(static_cast<uint16_t>(w[i])) : __builtin_bit_cast(float, w[i] << 16);
-        v[2 * i + 1] = DT == DT_F16 ? f16_bits_to_f32(static_cast<uint16_t>(w[i] >> 16))
-                                    : __builtin_bit_cast(float, w[i] & 0xFFFF0000u);
-      }
-    }
+    Raw8 raw;
+    load_raw8<DT>(p, at, n, raw);
+    floats_of<DT>(raw, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i * STEP < n ? load_as_f32<DT>(p, at + i * STEP) : 0.f;

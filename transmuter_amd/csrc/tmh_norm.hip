@@ -1,6 +1,6 @@
 // The root-mean-square norm with the residual's addition, and rows in 8 bits (tmh_rms_norm, tmh_quantize_rows). Both
 // are bound by memory: each input is read once and each output written once. 4096 x 2048 bf16 with a residual,
-// answered in bf16 and 8 bits: 13.5 us, 5.6 TB/s; the gated 2048 x 11008 f16 22.0 us, 5.1 TB/s (a large copy: 4.8).
+// answered in bf16 and 8 bits: 13.0 us, 5.8 TB/s; the gated 2048 x 11008 f16 20.6 us, 5.5 TB/s (a large copy: 4.8).
 #include <algorithm>
 #include <type_traits>
 
@@ -30,14 +30,18 @@ __device__ __forceinline__ int64_t xcd_row_group(uint32_t block, uint32_t blocks
   return block < 8 * per ? (block & 7) * per + (block >> 3) : block;
 }
 
-__device__ __forceinline__ void load_gamma(const NormArgs& p, int col, int n, float (&g)[8], bool vec) {
-  if (vec && p.gamma_dtype == DT_F16) load8<DT_F16, true>(p.gamma, col, n, g);
-  else if (vec && p.gamma_dtype == DT_BF16) load8<DT_BF16, true>(p.gamma, col, n, g);
-  else if (vec) load8<DT_F32, true>(p.gamma, col, n, g);
-  else {
+__device__ __forceinline__ void load_gamma(const NormArgs& p, int col, int n, Raw8& raw) {
+  if (p.gamma_dtype == DT_F32) load_raw8<DT_F32>(p.gamma, col, n, raw);
+  else load_raw8<DT_F16>(p.gamma, col, n, raw);  // (or bf16: 16 bits)
+}
+__device__ __forceinline__ void gamma_of(const NormArgs& p, const Raw8& raw, float (&g)[8]) {
+  if (p.gamma_dtype == DT_F16) floats_of<DT_F16>(raw, g);
+  else if (p.gamma_dtype == DT_BF16) floats_of<DT_BF16>(raw, g);
+  else floats_of<DT_F32>(raw, g);
+}
+__device__ __forceinline__ void load_gamma(const NormArgs& p, int col, int n, float (&g)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = i * kLaneStep < n ? load_float_rt(p.gamma, p.gamma_dtype, col + i * kLaneStep) : 0.f;
-  }
+  for (int i = 0; i < 8; ++i) g[i] = i * kLaneStep < n ? load_float_rt(p.gamma, p.gamma_dtype, col + i * kLaneStep) : 0.f;
 }
 
 // The sum of a value over the threads of a row (a wavefront, or with WIDE a workgroup), in all of them.
@@ -97,16 +101,38 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void k_rms_norm(NormArgs p) {
   if (row >= p.rows) return;  // (a row of a workgroup always exists)
   auto column = [&](int c) { return c * tpr * 8 + (t >> 4) * kF8Block + lane_columns(VEC); };
   float h[NCH][8], g[NCH][8];
+  if constexpr (VEC) {  // every load, then what waits for them (4096 x 2048 bf16 13.5 us one after another, 13.0 so)
+    Raw8 x[NCH], r[NCH], w[NCH];
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int col = column(c);
-    load8<DT, VEC, kLaneStep>(p.x, row * p.ldx + col, p.cols - col, h[c]);
-    load_gamma(p, col, p.cols - col, g[c], VEC);
-    if (p.residual) {
-      float r[8];
-      load8<DT, VEC, kLaneStep>(p.residual, row * p.ldr + col, p.cols - col, r);
+    for (int c = 0; c < NCH; ++c) {
+      const int col = column(c);
+      load_raw8<DT>(p.x, row * p.ldx + col, p.cols - col, x[c]);
+      if (p.residual) load_raw8<DT>(p.residual, row * p.ldr + col, p.cols - col, r[c]);
+      load_gamma(p, col, p.cols - col, w[c]);
+    }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[c][i] += r[i];
+    for (int c = 0; c < NCH; ++c) {
+      floats_of<DT>(x[c], h[c]);
+      if (p.residual) {
+        float more[8];
+        floats_of<DT>(r[c], more);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[c][i] += more[i];
+      }
+      gamma_of(p, w[c], g[c]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = column(c);
+      load8<DT, false, kLaneStep>(p.x, row * p.ldx + col, p.cols - col, h[c]);
+      load_gamma(p, col, p.cols - col, g[c]);
+      if (p.residual) {
+        float r[8];
+        load8<DT, false, kLaneStep>(p.residual, row * p.ldr + col, p.cols - col, r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[c][i] += r[i];
+      }
     }
   }
   auto squares = [&](float f) {
@@ -162,7 +188,7 @@ __global__ __launch_bounds__(1024) void k_rms_norm_any(NormArgs p) {
   for (int col = own; col - static_cast<int>(threadIdx.x & 15) < p.cols; col += 8 * static_cast<int>(blockDim.x)) {
     float h[8], g[8];
     load(col, h);
-    load_gamma(p, col, p.cols - col, g, false);
+    load_gamma(p, col, p.cols - col, g);
     if (p.sum) store8<DT, false, kLaneStep>(p.sum, row * p.lds + col, p.cols - col, h);
     norm_outputs<DT, false>(p, row, col, p.cols - col, h, g, rstd);
   }
@@ -186,7 +212,7 @@ __device__ __forceinline__ float silu(float g) {
 }
 
 // Sixteen lanes to a block of 128 columns, the blocks of the rows one after another. A gated value took 21
-// instructions with the divisions' general forms (25.5 us where 22.0 are now: it was bound by them).
+// instructions with the divisions' general forms (25.5 us where 20.6 are now: it was bound by them).
 template <int DT, bool VEC, bool GATE>
 __global__ __launch_bounds__(256) void k_quantize_rows(QuantizeArgs p, int64_t first) {
   const int64_t all = p.rows * p.blocks;

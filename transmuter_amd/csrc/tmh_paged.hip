@@ -249,28 +249,20 @@ __device__ __forceinline__ float4_t mfma16(uint4_t a, uint4_t b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
 }
 
-// Two probabilities as the sums of two 16-bit parts each: rounded towards zero, and the rest. Neither part is
-// zero or negative (at least f16's smallest number, of a maximum of 2^15, or bf16's smallest normal one), so that
-// an infinity in V stays what it is in both products.
+// Two probabilities as the sums of two 16-bit parts each: cut off, and the rest, rounded. What is cut is a little less
+// than the probability, so that the rest is not 0 beside a first part that is not, and an infinity in V stays what
+// it is in both products (f16: of probabilities of 2^-23, 2^-38 of the largest, and more; others give NaN with it).
+// A probability of 0 gives zeros: a token without weight has no part in the answer, whatever its value.
 template <int DT>
 __device__ __forceinline__ uint2 split2(float a, float b) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  constexpr uint16_t tiny = DT == DT_F16 ? 0x0001 : 0x0080;
-  uint32_t hi;
-  float ra, rb;
+  constexpr float less = 1.f - 0x1p-20f;
   if constexpr (DT == DT_F16) {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    hi = __builtin_bit_cast(uint32_t, h);
-    ra = a - static_cast<float>(h[0]);
-    rb = b - static_cast<float>(h[1]);
+    const auto h = __builtin_amdgcn_cvt_pkrtz(fmaf(a, less, -0x1p-24f), fmaf(b, less, -0x1p-24f));
+    return make_uint2(__builtin_bit_cast(uint32_t, h), pack2<DT>(a - static_cast<float>(h[0]), b - static_cast<float>(h[1])));
   } else {
-    hi = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
-    ra = a - __builtin_bit_cast(float, hi << 16);
-    rb = b - __builtin_bit_cast(float, hi & 0xFFFF0000u);
+    const uint32_t hi = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b * less), __builtin_bit_cast(uint32_t, a * less), 0x07060302u);
+    return make_uint2(hi, pack2<DT>(a - __builtin_bit_cast(float, hi << 16), b - __builtin_bit_cast(float, hi & 0xFFFF0000u)));
   }
-  const u16x2 least = {tiny, tiny};
-  return make_uint2(__builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, hi), least)),
-                    __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, pack2<DT>(ra, rb)), least)));
 }
 
 // The maximum (sum) over the four lanes of one column of an MFMA tile, in all of them.
@@ -296,8 +288,8 @@ __device__ __forceinline__ float column_sum(float v) {
 // are 16 consecutive bytes.
 // f32: the same with v_mfma_f32_16x16x4_f32, whose operands are single values.
 //
-// Probabilities are split into two 16-bit parts, each multiplied: the sum keeps 16 bits (bf16) or 21 (f16) of
-// each (one part would round each to 8 or 11, as far off as the answer's own type).
+// Probabilities are split into two 16-bit parts, each multiplied: the sum keeps 16 bits (bf16) or 21 (f16, and
+// multiples of 2^-39 of the largest) of each (one part would round each to 8 or 11, as far off as the answer's own type).
 // f16 parts are taken of 2^15 times the probability, so that small ones of long rows do not fall below f16's
 // range; f32 and bf16 ones of 2^-32 times it, so that sums of up to 2^31 values near the type's largest stay
 // finite. The factor is in the running sum too and drops out.
@@ -327,7 +319,7 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
   constexpr int NH = TILE / 16;           // 16-token halves of a tile
   constexpr int NC = 4 * NB;              // chunks of 4 E dimensions of a row
   constexpr int VT = F32 ? 4 : 8;         // tokens a lane reads of V
-  constexpr float BIAS = DT == DT_F16 ? 15.f : -32.f;
+  constexpr float FACTOR = DT == DT_F16 ? 0x1p15f : 0x1p-32f;
   constexpr int ROW = 16 * E * NB + 4;    // floats of a head's answer in LDS (+ 4: off a bank's multiple)
   __shared__ __align__(16) float lds_o[WAVES][kHeads][ROW];
   __shared__ float lds_m[WAVES][kHeads], lds_l[WAVES][kHeads];
@@ -539,15 +531,15 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[nb][e] *= keep;
       }
-      // (f32: the factor by a product, which is exact; 32 more in the exponent's argument would round it at their size:
-      // 1.4e-6 of the answer in the 2-norm over 1000 tokens, 1.0e-6 so.)
-      const float ref = (m == kNone ? 0.f : m) - (F32 ? 0.f : BIAS);
+      // (The factor by a product, which is exact; its exponent in the argument would round that at its size: f32 1.4e-6 of
+      // the answer in the 2-norm over 1000 tokens, 1.0e-6 so.)
+      const float ref = m == kNone ? 0.f : m;
       float pr[NH][4];
 #pragma unroll
       for (int h = 0; h < NH; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          pr[h][i] = __builtin_amdgcn_exp2f(t[h][i] - ref) * (F32 ? 0x1p-32f : 1.f);
+          pr[h][i] = __builtin_amdgcn_exp2f(t[h][i] - ref) * FACTOR;
           l += pr[h][i];
         }
       if constexpr (F32) {

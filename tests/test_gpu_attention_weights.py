@@ -91,3 +91,14 @@ def test_infinite_value_without_weight(ctx, dtype):
     v[9, 5] = np.inf
     got = attend(ctx, dtype, scores, v, 300)
     assert np.isnan(got[5]) and np.isfinite(np.delete(got, 5)).all()
+
+
+@pytest.mark.parametrize("dtype", base.TYPES)
+@pytest.mark.parametrize("tokens,room", [(100, 128), (200, 256), (900, 1024), (5000, 8192), (300, 200000), (100, 200000)])
+def test_nothing_but_scores_of_minus_infinity(ctx, dtype, tokens, room):
+    """A row whose every score is -infinity answers zeros in each way that its work is shared out, infinities and NaN among
+    its values too."""
+    base.say("minus infinity", dtype, tokens, room)
+    v = values(to_type(np.random.default_rng(tokens).standard_normal((tokens, D)), dtype))
+    v[3, 5], v[tokens // 2, 7], v[-1, 9] = np.inf, -np.inf, np.nan
+    assert not attend(ctx, dtype, np.full(tokens, -np.inf), v, room).any()

@@ -268,6 +268,7 @@ class PagedCache:
     def free(self) -> None:
         self.k.free()
         self.v.free()
+        self.desc.k = self.desc.v = None  # (later calls are refused)
 
     def __repr__(self) -> str:
         return (f"PagedCache({self.pages} pages of {self.page_size}, {self.kv_heads} heads of {self.head_dim}, "

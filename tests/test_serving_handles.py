@@ -52,3 +52,22 @@ def test_a_freed_weight_is_refused():
         serving.matmul_fp8(serving.Rows8(_t("f8_e4m3fn", 2, 128), _t("f32", 1, 2)), weight)
     with pytest.raises(TmhArgumentError, match="weight is NULL"):
         weight.device_bytes()
+
+
+def _freed(dtype, *shape):
+    t = _t(dtype, *shape)
+    t.free()
+    return t
+
+
+@pytest.mark.parametrize("call", [
+    lambda: serving.rms_norm(_t("f16", 2, 128), _t("f16", 128), _freed("f16", 2, 128)),
+    lambda: serving.rms_norm(_t("f16", 2, 128), _t("f16", 128), _t("f16", 2, 128), out=serving.Norm(None, None, _freed("f16", 2, 128))),
+    lambda: serving.rms_norm(_t("f16", 2, 128), _t("f16", 128), y=True, out=serving.Norm(_freed("f16", 2, 128), None, None)),
+    lambda: serving.matmul_fp8(serving.Rows8(_t("f8_e4m3fn", 2, 128), _t("f32", 1, 2)), serving.Fp8Weight(CTX, None, 128, 64),
+                               _freed("f16", 64)),
+])
+def test_a_freed_operand_is_not_left_out(call):
+    """A residual, bias or answer that was freed is refused, not taken for one that was not given."""
+    with pytest.raises(TmhArgumentError, match="has been freed"):
+        call()

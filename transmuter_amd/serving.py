@@ -42,10 +42,20 @@ def _at(t: DeviceTensor, elements: int) -> ctypes.c_void_p:
     return ctypes.c_void_p(t.ptr.value + elements * np.dtype(NX_TO_NUMPY[t.dtype]).itemsize)
 
 
+def _given(t: DeviceTensor | None, what: str) -> ctypes.c_void_p | None:
+    """The address of an operand that a call may do without. (A freed one has none, which would leave it out.)"""
+    if t is None:
+        return None
+    if t.ptr is None:
+        _refuse(f"{what} has been freed")
+    return t.ptr
+
+
 def _out(out: DeviceTensor | None, ctx: Context, shape, dtype: str) -> DeviceTensor:
     """The answer's memory: `out`, if it has the answer's shape and type, or new."""
     if out is None:
         return ctx.empty(shape, dtype)
+    _given(out, "out")
     if out.shape != tuple(shape) or out.dtype != dtype:
         _refuse(f"out must be {dtype} {tuple(shape)}, got {out.dtype} {out.shape}")
     return out
@@ -91,7 +101,7 @@ def rms_norm(x: DeviceTensor, gamma: DeviceTensor, residual: DeviceTensor | None
     out = Norm(_out(out.y, ctx, x.shape, x.dtype) if y else None, Rows8._of(ctx, x.shape, out.rows) if rows else None,
                _out(out.sum, ctx, x.shape, x.dtype) if residual is not None else None)
     ctx.check(lib().tmh_rms_norm(
-        ctx.handle, x.ptr, n, residual.ptr if residual is not None else None, n, x.tmh_dtype, t, n, gamma.ptr,
+        ctx.handle, x.ptr, n, _given(residual, "the residual"), n, x.tmh_dtype, t, n, gamma.ptr,
         gamma.tmh_dtype, eps, out.sum.ptr if out.sum else None, n, out.y.ptr if out.y else None, n,
         out.rows.q.ptr if out.rows else None, n, out.rows.scales.ptr if out.rows else None, stream))
     return out
@@ -193,8 +203,9 @@ def matmul_fp8(a: Rows8, w: Fp8Weight, bias: DeviceTensor | None = None, *, y_ty
     if y_type not in FLOAT_TYPES:
         _refuse(f"the 8-bit product's y must be f32, f16 or bf16, got {y_type}")
     y = _out(out, ctx, (*a.q.shape[:-1], w.n), y_type)
-    ctx.check(lib().tmh_matmul_fp8(ctx.handle, w.handle, a.q.ptr, m, w.k, a.scales.ptr, bias.ptr if bias else None,
-                                   bias.tmh_dtype if bias else 0, y.ptr, y.tmh_dtype, w.n, stream))
+    ctx.check(lib().tmh_matmul_fp8(ctx.handle, w.handle, a.q.ptr, m, w.k, a.scales.ptr,
+                                   _given(bias, "the 8-bit product's bias"), bias.tmh_dtype if bias is not None else 0,
+                                   y.ptr, y.tmh_dtype, w.n, stream))
     return y
 
 

@@ -3,6 +3,7 @@ the library refuses arguments ahead of its context (here there is none, which it
 
 import ctypes
 
+import numpy as np
 import pytest
 
 from transmuter_amd import _lib, serving
@@ -71,3 +72,29 @@ def test_a_freed_operand_is_not_left_out(call):
     """A residual, bias or answer that was freed is refused, not taken for one that was not given."""
     with pytest.raises(TmhArgumentError, match="has been freed"):
         call()
+
+
+class _Host(_NoContext):
+    """A context that keeps what is put."""
+
+    def put(self, array, dtype=None):
+        t = self.empty(np.shape(array), dtype or "f32")
+        self.host = array if dtype == "f8_e4m3fn" else self.host
+        return t
+
+
+@pytest.mark.parametrize("b", [np.full((4, 128), 1.5, np.float32), np.ones((4, 128), np.float16), np.ones((4, 128), bool),
+                               np.full((4, 128), 256), np.full((4, 128), -1)])
+def test_a_weight_of_values_is_not_taken_for_bytes(b):
+    with pytest.raises(TmhArgumentError, match="array of f8_e4m3fn bytes"):
+        serving.Fp8Weight.prepare(_Host(), b, np.ones((1, 1), np.float32))
+
+
+@pytest.mark.parametrize("dtype", [np.uint8, np.int8, np.int64])
+def test_a_weight_of_bytes(dtype):
+    """Bytes in any integer type that holds them reach the library as they are."""
+    host = np.arange(4 * 128).reshape(4, 128) % 256
+    ctx = _Host()
+    with pytest.raises(TmhArgumentError, match="context is NULL"):
+        serving.Fp8Weight.prepare(ctx, host.astype(dtype), np.ones((1, 1), np.float32))
+    assert ctx.host.dtype == np.uint8 and np.array_equal(ctx.host, host)

@@ -150,7 +150,12 @@ class Fp8Weight:
     @classmethod
     def prepare(cls, ctx: Context, b, scales) -> "Fp8Weight":
         """From b [N, K] (f8_e4m3fn, or a host array of its bytes) and scales [ceil(N/128), ceil(K/128)] f32."""
-        b_t = b if isinstance(b, DeviceTensor) else ctx.put(np.asarray(b, dtype=np.uint8), "f8_e4m3fn")
+        if not isinstance(b, DeviceTensor):
+            b = np.asarray(b)
+            # (Values of floats would be cut to whole numbers and taken for bits. Signed bytes are bits all the same.)
+            if b.dtype.kind not in "iu" or (b.dtype.itemsize > 1 and b.size and not 0 <= b.min() <= b.max() <= 255):
+                _refuse(f"a host 8-bit weight is an array of f8_e4m3fn bytes, got {b.dtype}")
+        b_t = b if isinstance(b, DeviceTensor) else ctx.put(b.astype(np.uint8), "f8_e4m3fn")
         s_t = scales if isinstance(scales, DeviceTensor) else ctx.put(np.asarray(scales, dtype=np.float32))
         try:
             if len(b_t.shape) != 2 or b_t.dtype != "f8_e4m3fn":

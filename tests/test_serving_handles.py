@@ -98,3 +98,12 @@ def test_a_weight_of_bytes(dtype):
     with pytest.raises(TmhArgumentError, match="context is NULL"):
         serving.Fp8Weight.prepare(ctx, host.astype(dtype), np.ones((1, 1), np.float32))
     assert ctx.host.dtype == np.uint8 and np.array_equal(ctx.host, host)
+
+
+@pytest.mark.parametrize("tables", [(None, True), (True, None)])
+def test_half_the_rotary_tables(tables):
+    """One table without the other is refused, not a step without rotary positions."""
+    cache = serving.PagedCache(CTX, 4, 16, 1, 64)
+    cos, sin = (_t("f32", 100, 32) if given else None for given in tables)
+    with pytest.raises(TmhArgumentError, match="tables cos and sin"):
+        cache.append(_t("f16", 2, 256), 2, _t("s64", 2), _t("s64", 2), cos, sin)

@@ -249,8 +249,8 @@ class PagedCache:
         if slots.dtype != "s64" or slots.size != t:
             _refuse(f"a step of {t} tokens takes {t} s64 slots, got {slots.dtype} {slots.shape}")
         rotary = most = table = 0
-        if cos is not None:
-            if sin is None or positions is None or cos.shape != sin.shape or cos.dtype != sin.dtype or len(cos.shape) != 2:
+        if cos is not None or sin is not None:
+            if cos is None or sin is None or positions is None or cos.shape != sin.shape or cos.dtype != sin.dtype or len(cos.shape) != 2:
                 _refuse("rotary positions take positions and tables cos and sin of one type and shape")
             if positions.dtype != "s64" or positions.size != t:
                 _refuse(f"a step of {t} tokens takes {t} s64 positions, got {positions.dtype} {positions.shape}")

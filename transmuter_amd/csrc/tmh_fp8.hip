@@ -14,6 +14,7 @@
 
 #include "tmh_f8.h"
 #include "tmh_internal.h"
+#include "tmh_launch.h"
 
 // Tiles of 16 rows x 128 of K, 2 KiB each in the order [N / 16][K / 128]: two halves (64 of K each) of 1 KiB, lane l
 // = 16 g + r of a wavefront holding row r (of the pair of tiles' 32, tile_row), k = 64 h + 16 g .. + 15 at offset 16
@@ -79,8 +80,8 @@ __host__ __device__ __forceinline__ int64_t tile_row(int64_t tile, int r) {
 // W [N][K] into its tiles: a workgroup's four wavefronts take a tile each.
 template <bool VEC>
 __global__ __launch_bounds__(256) void k_f8_tile(const uint8_t* __restrict__ w, int64_t N, int64_t K, int64_t kb, int64_t tiles,
-                                                 uint8_t* __restrict__ q) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+                                                 uint8_t* __restrict__ q, int64_t first) {
+  const int64_t at = first + static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (at >= tiles * kb) return;
   const int64_t tile = at / kb, b = at - tile * kb;
   const int lane = threadIdx.x & 63;
@@ -104,8 +105,8 @@ __global__ __launch_bounds__(256) void k_f8_tile(const uint8_t* __restrict__ w, 
 
 // Rows of K bytes at any address and pitch into rows of Kp bytes, a multiple of 16, zeros past K.
 __global__ __launch_bounds__(256) void k_f8_pad_rows(const uint8_t* __restrict__ a, int64_t lda, int64_t M, int64_t K, int64_t Kp,
-                                                     uint8_t* __restrict__ out) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+                                                     uint8_t* __restrict__ out, int64_t first) {
+  const int64_t i = first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = i / (Kp / 16), k = (i - row * (Kp / 16)) * 16;
   if (row >= M) return;
   uint4_t v{0u, 0u, 0u, 0u};
@@ -608,8 +609,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
 
 // Y = the sum of the parts (+ bias), in order. A thread takes four columns (their parts lie on 16 bytes where four
 // divides N).
-__global__ __launch_bounds__(256) void k_f8_reduce(F8Args p) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void k_f8_reduce(F8Args p, int64_t first) {
+  const int64_t i = first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int quads = (p.N + 3) / 4;
   const int64_t m = i / quads;
   if (m >= p.M) return;
@@ -781,10 +782,12 @@ int tmh_fp8_weight_prepare(tmh_ctx* ctx, const void* d_b, const float* d_scales,
   w->device_bytes = bytes + scale_bytes;
   hipStream_t s = pick_stream(ctx, stream);
   if (st == TMH_OK) {
-    const unsigned grid = static_cast<unsigned>((tiles * kb + 3) / 4);
     const auto* b = static_cast<const uint8_t*>(d_b);
-    if (K % 16 == 0 && reinterpret_cast<uintptr_t>(d_b) % 16 == 0) k_f8_tile<true><<<grid, 256, 0, s>>>(b, N, K, kb, tiles, w->d_q);
-    else k_f8_tile<false><<<grid, 256, 0, s>>>(b, N, K, kb, tiles, w->d_q);
+    in_launches(tiles * kb, most_a_launch(256, 4, 1), [&](int64_t first, int64_t count) {
+      const unsigned grid = static_cast<unsigned>((count + 3) / 4);
+      if (K % 16 == 0 && reinterpret_cast<uintptr_t>(d_b) % 16 == 0) k_f8_tile<true><<<grid, 256, 0, s>>>(b, N, K, kb, tiles, w->d_q, first);
+      else k_f8_tile<false><<<grid, 256, 0, s>>>(b, N, K, kb, tiles, w->d_q, first);
+    });
     st = check_launch(ctx, "k_f8_tile");
   }
   if (st == TMH_OK)
@@ -864,7 +867,9 @@ int tmh_matmul_fp8(tmh_ctx* ctx, const tmh_fp8_weight* w, const void* d_a, int64
     if (part_bytes) p.part = reinterpret_cast<float*>(ws + pad_bytes);
   }
   if (pad) {
-    k_f8_pad_rows<<<static_cast<unsigned>((M * (Kp / 16) + 255) / 256), 256, 0, s>>>(p.a, lda, M, w->K, Kp, ws);
+    in_launches(M * (Kp / 16), most_a_launch(256, 256, 1), [&](int64_t first, int64_t count) {
+      k_f8_pad_rows<<<static_cast<unsigned>((count + 255) / 256), 256, 0, s>>>(p.a, lda, M, w->K, Kp, ws, first);
+    });
     TMH_TRY(check_launch(ctx, "k_f8_pad_rows"));
     p.a = ws;
     p.lda = Kp;
@@ -874,7 +879,9 @@ int tmh_matmul_fp8(tmh_ctx* ctx, const tmh_fp8_weight* w, const void* d_a, int64
   else launch_plan<false>(plan, p, s);
   if (p.splits > 1) {
     TMH_TRY(check_launch(ctx, "k_f8_gemm"));
-    k_f8_reduce<<<static_cast<unsigned>((M * ((w->N + 3) / 4) + 255) / 256), 256, 0, s>>>(p);
+    in_launches(M * ((w->N + 3) / 4), most_a_launch(256, 256, 1), [&](int64_t first, int64_t count) {
+      k_f8_reduce<<<static_cast<unsigned>((count + 255) / 256), 256, 0, s>>>(p, first);
+    });
   }
   return check_launch(ctx, "k_f8_gemm");
 }

@@ -489,7 +489,7 @@ int tmh_paged_append(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void* d_k
  * infinity in V is one in the answer where its token weighs 2^-38 of the largest or more; below that it may give NaN, as
  * it does at a weight of 0.
  * A sequence without tokens answers zeros, and so does a row whose every score is -infinity. What lies in
- * masked places of the cache, infinities and NaN too, has no effect. max_pages * page_size below 2^31. The
+ * masked places of the cache, infinities and NaN too, has no effect. max_pages * page_size below 2^31, heads at most 2^20. The
  * context's workspace keeps the parts of long sequences (its size depends on B, heads and head_dim only).
  */
 int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, int heads,

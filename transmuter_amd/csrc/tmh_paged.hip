@@ -155,10 +155,8 @@ void launch_append(const AppendArgs& p, int64_t T, bool vec, bool table_vec, boo
 
 // ------------------------------------------------------------------ attention
 
-constexpr int kHeads = 16;  // query heads of one kv head that a workgroup answers (the columns of an MFMA tile)
 constexpr float kNone = -__builtin_inff();
 constexpr uint32_t kNowhere = 1u << 31;  // an offset past every buffer's range here
-constexpr int64_t kJoinBytes = 72 << 10;
 constexpr int kThrough = 16;  // sc1 of a buffer access: past the XCD's L2, to where all XCDs meet
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 
@@ -307,7 +305,6 @@ __device__ __forceinline__ float column_sum(float v) {
 //  WHOLE there are none: a workgroup (WHOLE8: of eight wavefronts) takes an item, and looks at its own sequence's length only.
 //  EACH  JOIN with a worker to each unit that the table has room for, where no window moves them: a worker knows its
 //        tokens without the lengths, so that it looks their pages up meanwhile. Those past the length leave.
-enum : int { JOIN, PARTS, WHOLE, WHOLE8, EACH };
 template <int DT, int NB, int HOW>  // NB: blocks of 16 E dimensions
 __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32 && NB == 2) ? 2 : 1) void k_paged_attention(AttendArgs p) {
   // Every line of the arguments at once: one that is first looked at further on would cost its way then (us: one token of
@@ -889,6 +886,7 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
   TMH_TRY(check_cache(ctx, cache));
   if (heads < 1 || heads % cache->kv_heads != 0)
     return fail(ctx, TMH_ERR_INVALID, "%d query heads are no multiple of %d kv heads", heads, cache->kv_heads);
+  if (heads > (1 << 20)) return fail(ctx, TMH_ERR_UNSUPPORTED, "attention takes up to 2^20 query heads, got %d", heads);
   if (B < 0 || B > 65535) return fail(ctx, TMH_ERR_INVALID, "attention takes 0 to 65535 sequences, got %lld", (long long)B);
   if (max_pages < 0 || window < 0) return fail(ctx, TMH_ERR_INVALID, "max_pages and window must not be negative");
   if (std::isnan(scale)) return fail(ctx, TMH_ERR_INVALID, "the scale is NaN");
@@ -927,9 +925,8 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
   p.chunks = chunks;
   p.head_dim = cache->head_dim;
   p.scale = scale * 1.44269504088896340736f;
-  // Two workgroups a compute unit, or one a unit of work where the table has room for fewer.
-  const int64_t workers = std::max<int64_t>(1, std::min<int64_t>(2 * ctx->num_cus, units));
-  p.workers = static_cast<uint32_t>(workers);
+  const AttentionPlan plan = attention_plan(B, cache->kv_heads, group, cache->head_dim, p.most, window, cache->dtype == TMH_F32, ctx->num_cus);
+  p.workers = plan.workers;
   hipStream_t s = pick_stream(ctx, stream);
   const size_t rows = 2 * static_cast<size_t>(2 * ctx->num_cus) * std::min(kHeads, group);
   void* ws = workspace(ctx, rows * (cache->head_dim * 4 + sizeof(float2)), s);
@@ -939,44 +936,19 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
   p.meet = ctx->meet;
   p.part_bytes = static_cast<uint32_t>(rows * cache->head_dim * 4);
   p.stats_bytes = static_cast<uint32_t>(rows * sizeof(float2));
-  // Tokens that a sequence may have as far as the host knows (the lengths are the device's), and the units they lie in.
-  const int64_t tokens = window > 0 ? std::min(p.most, window) : p.most;
-  auto units_of = [&](int64_t u) { return (tokens + u - 1) / u + (tokens < p.most ? 1 : 0); };
-  const int64_t all_items = B * cache->kv_heads * chunks;
-  // JOIN where one workgroup has few parts to read (of equal lengths; of others it may be more): one sequence of
-  // 4096 (32 parts of 2 KiB) 9.9 us, 11.8 as PARTS; 32 x 4000 55.1 and 58.7; one of 32768 (128 parts) 25.5 and
-  // 24.6, 64 x 2000 with 16 heads of one kv head (8 parts of 8 KiB) 22.6 and 20.6. EACH instead where the table's
-  // units are no more than the CUs: one sequence of 700 8.1 us as JOIN, 7.5 so; 8 x 1000 9.4 and 8.6. (With up to
-  // two a CU: 4 x 4000 14.2 and 13.2, but tables that are not full leave the workers unevenly on the CUs: 5 x
-  // 1..2600 9.3 and 9.8, 9 x 1..900 of 256 dimensions 12.3 and 15.2.)
-  const int64_t parts = std::min<int64_t>(units_of(unit), workers / all_items + 2);
-  const bool join = parts * std::min(kHeads, group) * cache->head_dim * 4 <= kJoinBytes;
-  const bool each = join && tokens == p.most && units > 0 && units <= ctx->num_cus;
-  // WHOLE where an item is one unit, which cannot be cut (116 x 1..45, bf16 4 kv heads of 256, 17.1 us as JOIN, 13.4
-  // whole; one token of f16 4 kv heads of 128 4.5, as EACH 4.7), or two that EACH cannot take (4 x 200 of 256
-  // dimensions 10.8 us, as EACH 9.5). Few items of a few units go WHOLE8, where the registers allow it, if that is one
-  // turn of 256 tokens (f32: 128), as a further one costs 2.6 us (3.6), f16 4 kv heads of 128: 8 x 200 6.1 us (7.4 as
-  // EACH), but 8 x 500 9.4 (7.8); and with workgroups for half the CUs and more, 32 x 400 10.1 (10.2), 32 x 500 10.4
-  // (11.3), 32 x 700 12.8 (16.1 as JOIN), 60 x 1..1000 16.4 (20.0 as JOIN).
-  const bool half = all_items >= ctx->num_cus / 2;
-  const bool eight = cache->head_dim <= 128 && all_items <= ctx->num_cus &&
-                     (units_of(2 * unit) == 1 || (units_of(2 * unit) <= 4 && half));
-  const bool whole = units_of(unit) == 1 || (!eight && all_items <= ctx->num_cus &&
-                                             ((units_of(unit) <= 2 && !each) || (units_of(unit) <= 4 && half)));
-  if (whole || eight) {
-    p.workers = static_cast<uint32_t>(all_items);
-  } else if (each) {
-    p.workers = static_cast<uint32_t>(units);
-    p.by_units = FastDiv(static_cast<uint32_t>(units_of(unit)));
+  if (plan.way == EACH) {
+    p.by_units = FastDiv(plan.units);
     p.by_items = FastDiv(static_cast<uint32_t>(cache->kv_heads * chunks));
   }
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (whole) launch_attention<DT, WHOLE>(p, heads, s);
-    else if (eight) launch_attention<DT, WHOLE8>(p, heads, s);
-    else if (each) launch_attention<DT, EACH>(p, heads, s);
-    else if (join) launch_attention<DT, JOIN>(p, heads, s);
-    else launch_attention<DT, PARTS>(p, heads, s);
+    switch (plan.way) {
+      case WHOLE: launch_attention<DT, WHOLE>(p, heads, s); break;
+      case WHOLE8: launch_attention<DT, WHOLE8>(p, heads, s); break;
+      case EACH: launch_attention<DT, EACH>(p, heads, s); break;
+      case JOIN: launch_attention<DT, JOIN>(p, heads, s); break;
+      case PARTS: launch_attention<DT, PARTS>(p, heads, s); break;
+    }
   };
   if (cache->dtype == TMH_F32) launch(std::integral_constant<int, DT_F32>{});
   else if (cache->dtype == TMH_F16) launch(std::integral_constant<int, DT_F16>{});

@@ -2,7 +2,10 @@
 // on the host (whose tests go over every case) and on the device.
 #pragma once
 
+#include <algorithm>
 #include <cstdint>
+
+#include "tmh_launch.h"
 
 #if defined(__HIPCC__)
 #define TMH_HD __host__ __device__ __forceinline__
@@ -80,5 +83,56 @@ TMH_HD Parts parts_of(uint32_t first, uint32_t units, uint32_t per) {
 }
 // The place of part i: every part but the item's first is the first of its worker's run.
 TMH_HD uint32_t place_of(const Parts& p, uint32_t i) { return part_place(p.from + i, i > 0 || p.from_first); }
+
+// What happens to items that several workers share:
+//  JOIN  they meet in the kernel: the last worker to finish a part joins an item's parts.
+//  PARTS a second kernel joins them.
+//  WHOLE there are none: a workgroup (WHOLE8: of eight wavefronts) takes an item.
+//  EACH  JOIN with a worker to each unit that the table has room for, where no window moves them.
+enum Way : int { JOIN, PARTS, WHOLE, WHOLE8, EACH };
+
+constexpr int kHeads = 16;  // query heads of one kv head that a workgroup answers (the columns of an MFMA tile)
+constexpr int64_t kJoinBytes = 72 << 10;
+
+struct AttentionPlan {
+  Way way;
+  uint32_t workers;  // workgroups
+  uint32_t units;    // of an item, as far as the host knows
+};
+
+// The way of B sequences whose table has room for `most` tokens each (their lengths are the device's), of kv_heads groups
+// of `group` query heads. B * kv_heads * chunks * units is below 2^31.
+inline AttentionPlan attention_plan(int64_t B, int64_t kv_heads, int64_t group, int head_dim, int64_t most, int64_t window, bool f32,
+                                    int num_cus) {
+  const int64_t unit = f32 ? 64 : 128, chunks = (group + kHeads - 1) / kHeads;
+  const int64_t all_items = B * kv_heads * chunks, units = (most + unit - 1) / unit * all_items;
+  // Two workgroups a compute unit, or one a unit of work where the table has room for fewer.
+  const int64_t workers = std::max<int64_t>(1, std::min<int64_t>(2 * num_cus, units));
+  // Tokens that a sequence may have, and the units they lie in.
+  const int64_t tokens = window > 0 ? std::min(most, window) : most;
+  auto units_of = [&](int64_t u) { return (tokens + u - 1) / u + (tokens < most ? 1 : 0); };
+  // JOIN where one workgroup has few parts to read (of equal lengths; of others it may be more): one sequence of
+  // 4096 (32 parts of 2 KiB) 9.9 us, 11.8 as PARTS; 32 x 4000 55.1 and 58.7; one of 32768 (128 parts) 25.5 and
+  // 24.6, 64 x 2000 with 16 heads of one kv head (8 parts of 8 KiB) 22.6 and 20.6. EACH instead where the table's
+  // units are no more than the CUs: one sequence of 700 8.1 us as JOIN, 7.5 so; 8 x 1000 9.4 and 8.6. (With up to
+  // two a CU: 4 x 4000 14.2 and 13.2, but tables that are not full leave the workers unevenly on the CUs: 5 x
+  // 1..2600 9.3 and 9.8, 9 x 1..900 of 256 dimensions 12.3 and 15.2.)
+  const int64_t parts = std::min<int64_t>(units_of(unit), workers / all_items + 2);
+  const bool join = parts * std::min<int64_t>(kHeads, group) * head_dim * 4 <= kJoinBytes;
+  const bool each = join && tokens == most && units > 0 && units <= num_cus;
+  // WHOLE where an item is one unit, which cannot be cut (116 x 1..45, bf16 4 kv heads of 256, 17.1 us as JOIN, 13.4
+  // whole; one token of f16 4 kv heads of 128 4.5, as EACH 4.7), or two that EACH cannot take (4 x 200 of 256
+  // dimensions 10.8 us, as EACH 9.5). Few items of a few units go WHOLE8, where the registers allow it, if that is one
+  // turn of 256 tokens (f32: 128), as a further one costs 2.6 us (3.6), f16 4 kv heads of 128: 8 x 200 6.1 us (7.4 as
+  // EACH), but 8 x 500 9.4 (7.8); and with workgroups for half the CUs and more, 32 x 400 10.1 (10.2), 32 x 500 10.4
+  // (11.3), 32 x 700 12.8 (16.1 as JOIN), 60 x 1..1000 16.4 (20.0 as JOIN).
+  const bool half = all_items >= num_cus / 2;
+  const bool eight = head_dim <= 128 && all_items <= num_cus && (units_of(2 * unit) == 1 || (units_of(2 * unit) <= 4 && half));
+  // (Of more items than HIP takes workgroups JOIN's share as any others.)
+  const bool whole = (units_of(unit) == 1 && all_items <= most_a_launch(256, 1, 1)) ||
+                     (!eight && all_items <= num_cus && ((units_of(unit) <= 2 && !each) || (units_of(unit) <= 4 && half)));
+  const Way way = whole ? WHOLE : eight ? WHOLE8 : each ? EACH : join ? JOIN : PARTS;
+  return {way, static_cast<uint32_t>(whole || eight ? all_items : each ? units : workers), static_cast<uint32_t>(units_of(unit))};
+}
 
 }  // namespace tmh

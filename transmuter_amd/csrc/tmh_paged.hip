@@ -610,7 +610,11 @@ __global__ __launch_bounds__(HOW == WHOLE8 ? 512 : 256, NB == 1 || (DT == DT_F32
       const float4_t o = joined(hd, dim, top, total);
       const int64_t row = static_cast<int64_t>(slot) * part_heads + hd;
       if (whole) {
-        store(b, head0 + hd, dim, total == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / total));
+        const float each = total == 0.f ? 0.f : 1.f / total;
+        float4_t y = o * each;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = total == 0.f ? 0.f : y[e];  // (0 * an infinity is none)
+        store(b, head0 + hd, dim, y);
       } else if constexpr (MEET) {
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4_t, o), parts_rsrc, static_cast<uint32_t>(row * p.head_dim + dim) * 4, 0, kThrough);
         if (dim == 0)

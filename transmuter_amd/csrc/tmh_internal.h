@@ -32,7 +32,7 @@ struct tmh_ctx {
   std::vector<void*> ws_retired;
   tmh_timeline_state* tl = nullptr;  // while a timeline is recorded
   // Counters of workgroups that meet within a kernel (2 a compute unit): zero between calls, the last of those that
-  // meet clears theirs.
+  // meet clears theirs. They come with the first workspace (a context may be made in another's capture).
   uint32_t* meet = nullptr;
 };
 

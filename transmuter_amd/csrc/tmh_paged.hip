@@ -935,9 +935,9 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
   const size_t rows = 2 * static_cast<size_t>(2 * ctx->num_cus) * std::min(kHeads, group);
   void* ws = workspace(ctx, rows * (cache->head_dim * 4 + sizeof(float2)), s);
   if (!ws) return fail(ctx, TMH_ERR_UNSUPPORTED, "attention's workspace cannot grow here: run one call before the capture");
+  p.meet = ctx->meet;
   p.part = static_cast<float*>(ws);
   p.stats = reinterpret_cast<float2*>(p.part + rows * cache->head_dim);
-  p.meet = ctx->meet;
   p.part_bytes = static_cast<uint32_t>(rows * cache->head_dim * 4);
   p.stats_bytes = static_cast<uint32_t>(rows * sizeof(float2));
   if (plan.way == EACH) {

@@ -62,6 +62,19 @@ int check_launch(tmh_ctx* ctx, const char* kernel) {
   return check_hip(ctx, hipGetLastError(), kernel);
 }
 
+static bool make_counters(tmh_ctx* ctx, hipStream_t stream) {
+  const size_t bytes = 2 * static_cast<size_t>(ctx->num_cus) * sizeof(uint32_t);
+  void* p = nullptr;
+  if (hipMalloc(&p, bytes) == hipSuccess && hipMemsetAsync(p, 0, bytes, stream) == hipSuccess &&
+      hipStreamSynchronize(stream) == hipSuccess) {
+    ctx->meet = static_cast<uint32_t*>(p);
+    return true;
+  }
+  (void)hipGetLastError();
+  if (p) (void)hipFree(p);
+  return false;
+}
+
 void* workspace(tmh_ctx* ctx, size_t bytes, hipStream_t stream) {
   if (ctx->ws_bytes >= bytes) return ctx->ws;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -69,6 +82,7 @@ void* workspace(tmh_ctx* ctx, size_t bytes, hipStream_t stream) {
     (void)hipGetLastError();
     return nullptr;
   }
+  if (!ctx->meet && !make_counters(ctx, stream)) return nullptr;
   // The old workspace is not freed: queued work and graphs captured earlier may still use it.
   // It is retired until tmh_ctx_destroy, and the new one at least doubles, so the retired
   // buffers together stay below the size of the current one.
@@ -182,16 +196,6 @@ int tmh_ctx_create(int device, tmh_ctx** out) {
     delete ctx;
     return check_hip(nullptr, err, "hipStreamCreateWithFlags");
   }
-  const size_t meet_bytes = 2 * static_cast<size_t>(ctx->num_cus) * sizeof(uint32_t);
-  err = hipMalloc(reinterpret_cast<void**>(&ctx->meet), meet_bytes);
-  if (err == hipSuccess) err = hipMemsetAsync(ctx->meet, 0, meet_bytes, ctx->stream);
-  if (err == hipSuccess) err = hipStreamSynchronize(ctx->stream);
-  if (err != hipSuccess) {
-    (void)hipFree(ctx->meet);
-    (void)hipStreamDestroy(ctx->stream);
-    delete ctx;
-    return check_hip(nullptr, err, "the context's counters");
-  }
   *out = ctx;
   return TMH_OK;
 }
@@ -204,7 +208,7 @@ void tmh_ctx_destroy(tmh_ctx* ctx) {
     (void)hipStreamDestroy(ctx->stream);
   }
   if (ctx->ws) (void)hipFree(ctx->ws);
-  (void)hipFree(ctx->meet);
+  if (ctx->meet) (void)hipFree(ctx->meet);
   for (void* p : ctx->ws_retired) (void)hipFree(p);
   delete ctx->tl;
   delete ctx;

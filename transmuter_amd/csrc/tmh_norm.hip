@@ -62,16 +62,23 @@ __device__ __forceinline__ float row_total(float v) {
   return v;
 }
 
-// 1 / sqrt(mean(h^2) + eps) of a row, given a thread's own sum of (f h)^2 for a factor f. Squares of values of 2^64
-// and more overflow f32, though their root would not: such a row (its total is infinite, for all its threads) is
-// summed again with f = 2^-80, which leaves room for 2^30 of the largest numbers; eps is far below its last bits then.
+// r and f with h * f * r = h / sqrt(mean(h^2) + eps) for a row, given a thread's own sum of (f h)^2 for a factor f: 1, but
+// for rows that f32 has no room for. Squares of values of 2^64 and more overflow, though their root would not: a row whose
+// total is infinite (for all its threads) is summed again with f = 2^-80, which leaves room for 2^30 of the largest
+// numbers. Squares below 2^-126 lose bits, and count where the mean and eps are below 2^-96: then f = 2^96, which makes
+// squares of the smallest numbers normal ones and 2^30 of 2^96 at most. (Rows of zeros without an eps are 0 / 0.)
+struct RowScale {
+  float f, r;
+};
 template <bool WIDE, typename Sum>
-__device__ __forceinline__ float row_rstd(const NormArgs& p, Sum sum) {
+__device__ __forceinline__ RowScale row_scale(const NormArgs& p, Sum sum) {
   float total = row_total<WIDE>(sum(1.f));
-  if (total != __builtin_inff()) return 1.f / sqrtf(total / static_cast<float>(p.cols) + p.eps);
+  const float mean = total / static_cast<float>(p.cols) + p.eps;
+  if (total != __builtin_inff() && !(mean < 0x1p-96f)) return {1.f, 1.f / sqrtf(mean)};
+  const float f = total == __builtin_inff() ? 0x1p-80f : 0x1p96f;
   if constexpr (WIDE) __syncthreads();  // every thread has read the wavefronts' sums
-  total = row_total<WIDE>(sum(0x1p-80f));
-  return 0x1p-80f / sqrtf(total / static_cast<float>(p.cols));
+  total = row_total<WIDE>(sum(f));
+  return {f, 1.f / sqrtf(total / static_cast<float>(p.cols) + p.eps * f * f)};
 }
 
 template <int DT, bool VEC>
@@ -154,11 +161,17 @@ __global__ __launch_bounds__(WIDE ? 1024 : 256) void k_rms_norm(NormArgs p) {
       store8<DT, VEC, kLaneStep>(p.sum, row * p.lds + col, p.cols - col, h[c]);
     }
   }
-  const float rstd = row_rstd<WIDE>(p, squares);
+  const RowScale scale = row_scale<WIDE>(p, squares);
+  if (scale.f != 1.f) {
+#pragma unroll
+    for (int c = 0; c < NCH; ++c)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[c][i] *= scale.f;
+  }
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int col = column(c);
-    norm_outputs<DT, VEC>(p, row, col, p.cols - col, h[c], g[c], rstd);
+    norm_outputs<DT, VEC>(p, row, col, p.cols - col, h[c], g[c], scale.r);
   }
 }
 
@@ -178,7 +191,7 @@ __global__ __launch_bounds__(1024) void k_rms_norm_any(NormArgs p) {
       for (int i = 0; i < 8; ++i) h[i] += r[i];
     }
   };
-  const float rstd = row_rstd<true>(p, [&](float f) {
+  const RowScale scale = row_scale<true>(p, [&](float f) {
     float s = 0.f;
     for (int col = own; col < p.cols; col += 8 * static_cast<int>(blockDim.x)) {
       float h[8];
@@ -194,7 +207,11 @@ __global__ __launch_bounds__(1024) void k_rms_norm_any(NormArgs p) {
     load(col, h);
     load_gamma(p, col, p.cols - col, g);
     if (p.sum) store8<DT, false, kLaneStep>(p.sum, row * p.lds + col, p.cols - col, h);
-    norm_outputs<DT, false>(p, row, col, p.cols - col, h, g, rstd);
+    if (scale.f != 1.f) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] *= scale.f;
+    }
+    norm_outputs<DT, false>(p, row, col, p.cols - col, h, g, scale.r);
   }
 }
 

@@ -170,6 +170,9 @@ __device__ __forceinline__ void lds_dma4(__amdgpu_buffer_rsrc_t rsrc, uint8_t* l
 #endif
 }
 
+// No LDS operation of this thread outstanding (any number of vector-memory ones).
+constexpr int kAllLds = 15 | 3 << 14 | 7 << 4;
+
 // At most N (below 64) vector-memory operations of this thread outstanding, and no LDS operation.
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -229,6 +232,8 @@ __global__ __launch_bounds__(64 * KW) void k_f8_rows(F8Args p) {
   auto block = [&](int b, int buf) {
     const int ahead = b + (DEPTH - 1) * KW;
     if (ahead < last) {
+      __builtin_amdgcn_s_waitcnt(kAllLds);  // the block before has been read from the stage that is filled here
+      asm volatile("" ::: "memory");
       load(ahead, (buf + DEPTH - 1) % DEPTH);
       wait_vm<(DEPTH - 1) * LOADS>();  // this block's loads: the later ones' are the youngest
     } else if (DEPTH > 2 && ahead - KW < last) {
@@ -594,8 +599,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_f8_gemm(F8Args p) {
 #pragma unroll
     for (int d = 0; d < DW + 1; ++d) step(b + d, d, std::true_type{});
   }
-  // Up to DW steps are left. Their loads have no later ones of a known number behind them (what nobody would read the
-  // compiler leaves out), so they are all waited for.
+  // Up to DW steps are left. Their loads have no later ones behind them, so they are all waited for. What was loaded has a
+  // reader here on every way out of the loop, so that no load that its waits count can be left out as one that nobody reads.
+#pragma unroll
+  for (int d = 0; d < DW; ++d) {
+    asm volatile("" ::"v"(sw[d]));
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) asm volatile("" ::"v"(wr[d][j][h]));
+  }
   wait_vm<0>();
   barrier();
 #pragma unroll

@@ -1,5 +1,5 @@
 """The way that paged attention's work is shared out (attention_plan in transmuter_amd/csrc/tmh_paged_plan.h) on the host:
-workgroups within what HIP takes, and each way where its kernel can go."""
+workgroups within what HIP takes, each way where its kernel can go, and the ways that the GPU tests' cases reach."""
 
 import ctypes
 import os
@@ -9,6 +9,9 @@ import subprocess
 import numpy as np
 import pytest
 
+import test_gpu_attention_each as each
+import test_gpu_attention_ways as ways
+import test_gpu_serving_norms as norms
 from transmuter_amd import _lib
 from transmuter_amd._lib import PagedCacheDesc, lib
 
@@ -84,6 +87,16 @@ def test_plans(plan, f32):
         check(got, b, g, q, d, m, w, f32)
         seen.add(got[0])
     assert seen == {JOIN, PARTS, WHOLE, WHOLE8, EACH}
+
+
+def test_gpu_cases(plan):
+    """The GPU tests' cases reach each way in each type, for heads in one block of dimensions and in more."""
+    seen = set()
+    for cases in (ways.CASES, each.CASES, norms.ATTENTIONS):
+        for lengths, tokens, h, g, d, page, window in cases.values():
+            for f32 in (False, True):
+                seen.add((f32, d > 128, plan(len(lengths), g, h // g, d, -(-tokens // page) * page, window, f32)[0]))
+    assert seen == {(f32, wide, way) for f32 in (False, True) for wide in (False, True) for way in range(5) if not (wide and way == WHOLE8)}
 
 
 @pytest.mark.parametrize("heads,kv_heads,needle", [(2 ** 20, 2 ** 20, b"context is NULL"), (2 ** 20, 1, b"context is NULL"),

@@ -226,8 +226,8 @@ struct QuantizeArgs {
   FastDiv by_blocks;
 };
 
-// g / (1 + e^-g), as (g / 4) / (1/4 + e^-g / 4): a quarter of the sum's reciprocal does not fall below the normal
-// numbers before the sum is infinite.
+// g / (1 + e^-g), as (g / 4) / (1/4 + e^-g / 4): the reciprocal, which ends at the smallest normal number, is that of a
+// quarter of the sum, and so serves sums up to 2^128, where f32 ends (g of -88.7; the answer is 0 below), not 2^126.
 __device__ __forceinline__ float silu(float g) {
   return 0.25f * g * __builtin_amdgcn_rcpf(0.25f + __builtin_amdgcn_exp2f(fmaf(g, -1.44269504088896340736f, -2.f)));
 }

@@ -426,6 +426,8 @@ int tmh_fp8_weight_info(const tmh_fp8_weight* w, int64_t* K, int64_t* N, size_t*
  * sum over k in b of a[m, k] * w[n, k], summed in f32 and rounded once to y_dtype. With y_dtype F16 or BF16 the
  * 8-bit matrix unit sums a block: it cuts each product to a multiple of 2^-13 of the largest of the eight that
  * it adds first (1.5e-5 to 5e-5 of Y in the 2-norm, below the rounding of Y). With F32 products are exact.
+ * A block's two scales are multiplied first, in f32: what their product loses below the normal numbers, or beyond the
+ * largest, the block loses.
  *  d_a [M, K] F8E4M3, rows lda bytes apart; d_a_scales [ceil(K/128), M]; d_bias NULL or [N] of bias_dtype
  *  d_y [M, N] of y_dtype (F32, F16, BF16), rows ldy elements apart
  * Rows of A that do not start at multiples of 16 bytes, or whose K is no multiple of 16, are copied to the

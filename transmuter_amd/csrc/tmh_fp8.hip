@@ -375,8 +375,8 @@ __device__ __forceinline__ void gemm_outputs(const F8Args& p, const float4_t (&a
 // step's row scales; W's tiles, which are operands as they lie, go to registers DW steps ahead and past LDS, whose
 // reads would bound the loop otherwise. What lies past M, N or K is past the buffers' ranges and arrives as zeros.
 //
-// 4096 x 2048 -> 22016 (f16 Y, 128 x 256): 204 us, 1.8 PFLOP/s, with operands that come from memory, 172 us with
-// those that the last-level cache holds; 8192 x 8192 x 8192 2.25. The matrix unit is busy 54% of the cycles there, at
+// 4096 x 2048 -> 22016 (f16 Y, 128 x 256): 203 to 210 us, 1.8 PFLOP/s, with operands that come from memory, 167 us with
+// those that the last-level cache holds; 8192 x 8192 x 8192 2.4. The matrix unit is busy 54% of the cycles there, at
 // a clock that its own power holds at 1.9 GHz. A block's product needs four FMAs of its own beside it: a loop of
 // nothing but both reaches 3.5 PFLOP/s (4.0 without them). On the way: 16-byte pieces of 64 rows of A an instruction
 // and 8-byte stores 277 us, whole lines 231; two workgroups of 128 x 256 a CU instead of one of 256 x 256 224; the
@@ -666,9 +666,12 @@ void launch_plan(const F8Plan& plan, const F8Args& p, hipStream_t s) {
     case GEMM_128x128: launch_gemm<128, 128, 1, 4, 1, 2, F32>(p, s); break;
     case GEMM_128x256:
       if constexpr (!F32) {
-        // Touches where a call's own operands are a good part of the last-level cache (256 MB), so that W comes from
-        // memory: us, over three sets of them in turn, 4096 rows 2048 -> 22016 (233 MB) 207 (224 without), 1024 rows
-        // (92 MB) 57 (62); 4096 rows 11008 -> 2048 (84 MB) 89 (86).
+        // Touches pay where W comes from memory and cost where the last-level cache (256 MB) holds it, which a call cannot
+        // know: it takes operands of up to 90 MB for held, as those of three calls in turn are. us without touches and
+        // with, 38 sizes from 21 to 234 MB: over nine sets of operands in turn 1024 rows 11008 -> 2048 (38 MB) 0.85 of the
+        // time with, 512 rows 8192 -> 8192 (80 MB) 0.81, 1024 rows 2048 -> 22016 (92 MB) 0.90, 4096 rows (234 MB) 0.92
+        // (1.02 to 0.81 over all); over three, up to 80 MB 1.01 to 1.05, from 84 MB on 0.99 to 0.84, 4096 rows
+        // 2048 -> 22016 222.6 and 203.1; over one, held whole, 1.00 to 1.06, 166.8 and 167.5 there.
         const int64_t bytes = static_cast<int64_t>(p.M) * p.K + static_cast<int64_t>(p.tiles) * p.kb * kTileBytes + 2 * static_cast<int64_t>(p.M) * p.N;
         if (bytes > 90'000'000) launch_gemm<128, 256, 1, 4, 1, 2, false, true>(p, s);
         else launch_gemm<128, 256, 1, 4, 1, 2, false>(p, s);

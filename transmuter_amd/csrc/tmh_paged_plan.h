@@ -111,9 +111,10 @@ inline AttentionPlan attention_plan(int64_t B, int64_t kv_heads, int64_t group, 
   // Tokens that a sequence may have, and the units they lie in.
   const int64_t tokens = window > 0 ? std::min(most, window) : most;
   auto units_of = [&](int64_t u) { return (tokens + u - 1) / u + (tokens < most ? 1 : 0); };
-  // JOIN where one workgroup has few parts to read (of equal lengths; of others it may be more): one sequence of
-  // 4096 (32 parts of 2 KiB) 9.9 us, 11.8 as PARTS; 32 x 4000 55.1 and 58.7; one of 32768 (128 parts) 25.5 and
-  // 24.6, 64 x 2000 with 16 heads of one kv head (8 parts of 8 KiB) 22.6 and 20.6. EACH instead where the table's
+  // JOIN where one workgroup has few parts to read (kJoinBytes of equal lengths; of others it may be more). us as JOIN and
+  // as PARTS: one sequence of 4096 (64 KiB) 9.5 and 11.6, 32 x 4000 55.1 and 57.0, 64 x 2000 with 64 heads of 4 kv
+  // heads 56.6 and 64.0, with 16 heads of one kv head (80 KiB) 20.2 and 20.8; one of 16384 (256 KiB) 20.2 and 19.5, 16 x 4000
+  // with 16 heads of one kv head (256 KiB) 21.0 and 16.1, one of 65536 with those (2 MiB) 82 and 35. EACH instead where the table's
   // units are no more than the CUs: one sequence of 700 8.1 us as JOIN, 7.5 so; 8 x 1000 9.4 and 8.6. (With up to
   // two a CU: 4 x 4000 14.2 and 13.2, but tables that are not full leave the workers unevenly on the CUs: 5 x
   // 1..2600 9.3 and 9.8, 9 x 1..900 of 256 dimensions 12.3 and 15.2.)

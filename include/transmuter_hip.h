@@ -498,6 +498,70 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
                         const tmh_paged_cache* cache, const int32_t* d_page_table, int64_t max_pages,
                         const int32_t* d_lengths, float scale, int64_t window, void* d_y, int64_t ldy, void* stream);
 
+/* ------------------------------------------------------------------ drafted steps and sampling */
+
+/*
+ * The operators of a step that checks several drafted tokens a sequence at once (a tree or a chain of them), over the cache
+ * above: tmh_paged_append_norm for its rows, tmh_paged_tree_attention, and tmh_sample for each row's logits. The tokens
+ * that a tree's path agrees with are kept by appending their rows once more, to the slots that follow each other; a
+ * prompt's chunk is a chain. No reference counterpart: the reference samples and attends on the Nx backend.
+ */
+
+/*
+ * tmh_paged_append for models that norm each query and key head: x * rsqrt(mean(x^2) + eps) * gamma over a head's
+ * head_dim values, in f32, ahead of the rotation, which is rounded once. Values go to the cache as they are.
+ *  d_q_gamma, d_k_gamma [head_dim] of gamma_dtype (F32, F16, BF16), at any address; either may be NULL, whose heads are
+ *    then only turned (without both: tmh_paged_append)
+ * The other arguments are tmh_paged_append's.
+ */
+int tmh_paged_append_norm(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v,
+                          int64_t ldv, int64_t T, int heads, const void* d_q_gamma, const void* d_k_gamma,
+                          int gamma_dtype, float eps, const int64_t* d_positions, const void* d_cos, const void* d_sin,
+                          int table_dtype, int64_t max_positions, int rotary_dim, int interleaved,
+                          const int64_t* d_slots, const tmh_paged_cache* cache, void* d_q_out, int64_t ldqo,
+                          void* stream);
+
+/*
+ * Attention of several new tokens a sequence over the pages of its cache. Sequence b has the n = d_starts[b + 1] -
+ * d_starts[b] rows from d_starts[b] on, which are the last n of its d_lengths[b] tokens, in the order of their slots: row i
+ * of it sees all tokens before them, and of them (nodes 0 .. n - 1) those of its mask; without a mask nodes 0 .. i. With a
+ * window it sees the last `window` of these only (a place whose page is none counts, and is not read). The rest is
+ * tmh_paged_attention's: y = softmax(scale * q . k) v in f32, rounded once, with the weights' parts given there.
+ *  d_q [T, heads, head_dim] of the cache's dtype, 16-byte aligned rows ldq elements apart (ldq a multiple of 16 bytes);
+ *    d_y likewise, ldy
+ *  d_starts [B + 1] S32, not falling, from 0 to at most T. Rows behind the last sequence's are not read or written.
+ *  d_mask [T, mask_words] S64 or NULL: bit j % 64 of word j / 64 of a row is set where the row sees node j of its sequence
+ *    (a tree's ancestors and the node itself). Nodes beyond 64 * mask_words are not seen; bits beyond n mean nothing.
+ *  d_lengths [B] S32, the tokens in the cache, the step's own among them, clamped to [0, max_pages * page_size]; with
+ *    fewer than n the first nodes have no token
+ * A row that sees no token answers zeros. What a row does not see, infinities and NaN too, has no effect on it.
+ * B at most 65535, T * heads / kv_heads below 2^31. The context's workspace keeps the parts of sequences that workgroups
+ * share (its size depends on T / B, heads and head_dim only).
+ */
+int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t T, int heads,
+                             const tmh_paged_cache* cache, const int32_t* d_page_table, int64_t B, int64_t max_pages,
+                             const int32_t* d_lengths, const int32_t* d_starts, const int64_t* d_mask,
+                             int64_t mask_words, float scale, int64_t window, void* d_y, int64_t ldy, void* stream);
+
+/*
+ * One token drawn from each row of logits. With the row's largest logit m and temperature t, token i weighs
+ * w = exp((l_i - m) / t) (computed and summed in 64 bits, as a multiple of 2^-44; a token of less than 2^-44 is not drawn).
+ * Kept are, in this order: of all tokens the top_k largest; of these the fewest, from the largest down, whose weights sum
+ * to top_p of all of these or more; of these the tokens with w >= min_p. Equal logits rank by their index, the lowest
+ * first. The answer is the first kept token, by index, up to which the kept weights sum to more than random times their
+ * whole (the last one where none does).
+ *  d_logits [T, V] of dtype (F32, F16, BF16), rows ld elements apart; V below 2^20. NaN counts as -infinity, which has no
+ *    weight; +infinities have all of it.
+ *  d_temperature [T] F32 or NULL (1): not above 0 (or NaN): the largest logit, whatever else is asked
+ *  d_top_k [T] S32 or NULL: 0 and less, V and more: all;  d_top_p [T] F32 or NULL: 1 and more, NaN: all; the largest is
+ *    always kept;  d_min_p [T] F32 or NULL: 0 and less, NaN: all; 1 and more: the largest and its equals
+ *  d_random [T] F32 in [0, 1)
+ *  d_tokens [T] S64; -1 for a row without any logit above -infinity
+ */
+int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_t T, int64_t V,
+               const float* d_temperature, const int32_t* d_top_k, const float* d_top_p, const float* d_min_p,
+               const float* d_random, int64_t* d_tokens, void* stream);
+
 /* ------------------------------------------------------------------ measurement floors */
 
 /*

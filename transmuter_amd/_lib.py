@@ -114,6 +114,11 @@ SIGNATURES = {
                               _cache, _vp, _i64, _vp]),
     "tmh_paged_attention": (_i, [_vp, _vp, _i64, _i64, _i, _cache, _vp, _i64, _vp, ctypes.c_float, _i64, _vp, _i64,
                                  _vp]),
+    "tmh_paged_append_norm": (_i, [_vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i, _vp, _vp, _i, ctypes.c_float, _vp, _vp,
+                                   _vp, _i, _i64, _i, _i, _vp, _cache, _vp, _i64, _vp]),
+    "tmh_paged_tree_attention": (_i, [_vp, _vp, _i64, _i64, _i, _cache, _vp, _i64, _i64, _vp, _vp, _vp, _i64,
+                                      ctypes.c_float, _i64, _vp, _i64, _vp]),
+    "tmh_sample": (_i, [_vp, _vp, _i64, _i, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 _lock = threading.Lock()

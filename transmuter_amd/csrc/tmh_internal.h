@@ -102,6 +102,9 @@ int check_launch(tmh_ctx* ctx, const char* kernel);
 // would have to grow while the stream is being captured into a graph (or cannot grow).
 void* workspace(tmh_ctx* ctx, size_t bytes, hipStream_t stream);
 
+// What is wrong with the description of a paged cache (tmh_paged.hip).
+int check_cache(tmh_ctx* ctx, const tmh_paged_cache* c);
+
 // Host conversions (round to nearest even).
 float f16_to_f32(uint16_t h);
 uint16_t f32_to_f16(float f);

@@ -4,10 +4,33 @@
 #include <cmath>
 #include <type_traits>
 
-#include "tmh_f8.h"
+#include "tmh_attend.h"
 #include "tmh_internal.h"
+#include "tmh_launch.h"
 
 namespace tmh {
+
+int check_cache(tmh_ctx* ctx, const tmh_paged_cache* c) {
+  if (!c) return fail(ctx, TMH_ERR_INVALID, "the paged cache is NULL");
+  if (!is_float_dtype(c->dtype))
+    return fail(ctx, TMH_ERR_INVALID, "a paged cache holds f32, f16 or bf16 values, got %s", dtype_name(c->dtype));
+  if (c->kv_heads < 1 || c->page_size < 1 || c->pages < 1)
+    return fail(ctx, TMH_ERR_INVALID, "a paged cache needs kv_heads, page_size and pages of at least 1, got %d, %d, %lld",
+                c->kv_heads, c->page_size, (long long)c->pages);
+  if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8 != 0)
+    return fail(ctx, TMH_ERR_UNSUPPORTED, "a paged cache's head_dim must be a multiple of 8 up to 256, got %d", c->head_dim);
+  if (c->pages >= (int64_t{1} << 31) / c->page_size + ((int64_t{1} << 31) % c->page_size != 0))
+    return fail(ctx, TMH_ERR_UNSUPPORTED, "a paged cache needs pages * page_size below 2^31");
+  if (!c->k || !c->v) return fail(ctx, TMH_ERR_INVALID, "a paged cache's k and v must not be NULL");
+  const int64_t e = 16 / dtype_size(c->dtype);
+  if (reinterpret_cast<uintptr_t>(c->k) % 16 != 0 || reinterpret_cast<uintptr_t>(c->v) % 16 != 0 || c->page_stride % e != 0 ||
+      c->token_stride % e != 0 || c->head_stride % e != 0)
+    return fail(ctx, TMH_ERR_UNSUPPORTED, "a paged cache's k, v and strides must be multiples of 16 bytes");
+  if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0)
+    return fail(ctx, TMH_ERR_INVALID, "a paged cache's strides must not be negative");
+  return TMH_OK;
+}
+
 namespace {
 
 // ------------------------------------------------------------------ append
@@ -153,9 +176,191 @@ void launch_append(const AppendArgs& p, int64_t T, bool vec, bool table_vec, boo
   }
 }
 
+// ------------------------------------------------------------------ append with norms
+
+struct AppendNormArgs {
+  AppendArgs a;  // (its `pieces` and what divides by them are not used here)
+  const void* q_gamma;
+  const void* k_gamma;
+  int gamma_dtype, gamma_vec;
+  float eps, each;  // each: 1 / head_dim
+  uint32_t all_heads;  // query, key and value heads
+  FastDiv by_heads;
+};
+
+// The sum of a value over the G lanes of a group, in all of them.
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+  auto add = [](float x, int y) { return x + __builtin_bit_cast(float, y); };
+  v = add(v, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));   // lane ^ 1
+  v = add(v, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));   // lane ^ 2
+  v = add(v, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true));  // 7 - lane
+  if constexpr (G >= 16) v = add(v, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x140, 0xF, 0xF, true));  // 15 - lane
+  if constexpr (G >= 32) v += __shfl_xor(v, 16);
+  return v;
+}
+
+// G lanes answer one head of one token, a lane eight of its dimensions, and with VEC of those that turn by halves their
+// partners too (of a value head: eight more, where G lanes do not hold it). Each row is read once: its squares are summed
+// among the group's lanes while its values stay in registers.
+template <int DT, bool VEC, int G>
+__global__ __launch_bounds__(256) void k_paged_append_norm(AppendNormArgs p, int64_t first, uint32_t count, bool table_vec, bool pairs_vec) {
+  const AppendArgs& a = p.a;
+  const uint32_t i = blockIdx.x * (256 / G) + threadIdx.x / G;
+  if (i >= count) return;
+  const uint32_t tl = p.by_heads.div(i);
+  const int64_t t = first + tl;
+  const int of_all = static_cast<int>(i - tl * p.all_heads), lane = static_cast<int>(threadIdx.x % G);
+  const bool is_q = of_all < a.heads, is_v = of_all >= a.heads + a.kv_heads, is_k = !is_q && !is_v;
+  const int h = is_q ? of_all : is_k ? of_all - a.heads : of_all - a.heads - a.kv_heads;
+  int64_t slot = 0;
+  if (!is_q) {
+    slot = a.slots[t];
+    if (slot < 0 || slot >= a.num_slots) return;
+  }
+  const int half = a.rotary / 2, chunks = a.head_dim / 8;
+  const int at = is_v || lane < a.turned ? lane : lane + a.turned, other = is_v ? lane + G : lane + half / 8;
+  const bool has = at < chunks, pair = is_v ? other < chunks : lane < a.turned;
+  const int dim = 8 * at, dim2 = 8 * other;
+  const void* src = is_q ? a.q : is_k ? a.k : a.v;
+  const int64_t row = (is_q ? a.ldq : is_k ? a.ldk : a.ldv) * t + static_cast<int64_t>(h) * a.head_dim;
+  void* dst;
+  int64_t to;
+  if (is_q) {
+    dst = a.q_out;
+    to = t * a.ldqo + static_cast<int64_t>(h) * a.head_dim;
+  } else {
+    const uint32_t page = a.by_page.div(static_cast<uint32_t>(slot));
+    const uint32_t place = static_cast<uint32_t>(slot) - page * a.by_page.d;
+    dst = is_k ? a.k_cache : a.v_cache;
+    to = page * a.page_stride + place * a.token_stride + h * a.head_stride;
+  }
+  // (The cache's rows lie on 16 bytes whatever the step's do.)
+  auto put = [&](int d, const float (&x)[8]) {
+    if (is_q) store8<DT, VEC>(dst, to + d, 8, x);
+    else store8<DT, true>(dst, to + d, 8, x);
+  };
+  float v[8], o[8];
+  load8<DT, VEC>(src, row + dim, has ? 8 : 0, v);
+  load8<DT, VEC>(src, row + dim2, pair ? 8 : 0, o);
+  if (is_v) {
+    if (has) put(dim, v);
+    if (pair) put(dim2, o);
+    return;
+  }
+  const void* gamma = is_q ? p.q_gamma : p.k_gamma;
+  float f = 1.f, r = 1.f;
+  if (gamma) {
+    // As tmh_rms_norm sums its rows: again with factors of 2^-80 or 2^96 where f32 has no room for the squares.
+    auto squares = [&](float by) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s = fmaf(v[j] * by, v[j] * by, s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s = fmaf(o[j] * by, o[j] * by, s);
+      return group_sum<G>(s);
+    };
+    float total = squares(1.f);
+    float mean = total * p.each + p.eps;
+    if (total == __builtin_inff() || mean < 0x1p-96f) {
+      f = total == __builtin_inff() ? 0x1p-80f : 0x1p96f;
+      mean = squares(f) * p.each + p.eps * f * f;
+    }
+    r = 1.f / sqrtf(mean);
+  }
+  auto gammas = [&](int d, float (&g)[8]) {
+    if (p.gamma_vec) {
+      if (p.gamma_dtype == DT_F32) load8<DT_F32, true>(gamma, d, 8, g);
+      else if (p.gamma_dtype == DT_F16) load8<DT_F16, true>(gamma, d, 8, g);
+      else load8<DT_BF16, true>(gamma, d, 8, g);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = load_float_rt(gamma, p.gamma_dtype, d + j);
+    }
+  };
+  if (!has) return;
+  if (gamma) {
+    float g[8];
+    gammas(dim, g);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * f * r * g[j];
+  }
+  if (dim < a.rotary) {
+    const int64_t position = min(max(a.positions[t], int64_t{0}), a.max_positions - 1);
+    const int64_t table = position * half;
+    if (a.interleaved) {
+      float c[4], s[4];
+      if (pairs_vec) {
+        const float4_t cv = *reinterpret_cast<const float4_t*>(static_cast<const float*>(a.cos) + table + dim / 2);
+        const float4_t sv = *reinterpret_cast<const float4_t*>(static_cast<const float*>(a.sin) + table + dim / 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          c[j] = cv[j];
+          s[j] = sv[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool in = dim + 2 * j < a.rotary;
+          c[j] = in ? load_float_rt(a.cos, a.table_dtype, table + dim / 2 + j) : 1.f;
+          s[j] = in ? load_float_rt(a.sin, a.table_dtype, table + dim / 2 + j) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!pairs_vec && dim + 2 * j >= a.rotary) continue;
+        const float x = v[2 * j], y = v[2 * j + 1];
+        v[2 * j] = x * c[j] - y * s[j];
+        v[2 * j + 1] = fmaf(x, s[j], y * c[j]);
+      }
+    } else if (VEC) {  // a pair
+      float c[8], s[8], high[8];
+      if (gamma) {
+        float g[8];
+        gammas(dim2, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = o[j] * f * r * g[j];
+      }
+      load_table(a.cos, a.table_dtype, table + dim, table_vec, c);
+      load_table(a.sin, a.table_dtype, table + dim, table_vec, s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        high[j] = fmaf(v[j], s[j], o[j] * c[j]);
+        v[j] = v[j] * c[j] - o[j] * s[j];
+      }
+      put(dim2, high);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int d = dim + j;
+        if (d >= a.rotary) continue;
+        const bool low = d < half;
+        const int in_table = low ? d : d - half, partner = low ? d + half : d - half;
+        float x = load_as_f32<DT>(src, row + partner);
+        if (gamma) x = x * f * r * load_float_rt(gamma, p.gamma_dtype, partner);
+        const float c = load_float_rt(a.cos, a.table_dtype, table + in_table);
+        const float s = load_float_rt(a.sin, a.table_dtype, table + in_table);
+        v[j] = low ? v[j] * c - x * s : fmaf(x, s, v[j] * c);
+      }
+    }
+  }
+  put(dim, v);
+}
+
+template <int DT, int G>
+void launch_append_norm(const AppendNormArgs& p, int64_t T, bool vec, bool table_vec, bool pairs_vec, hipStream_t s) {
+  const int64_t most = ((int64_t{1} << 31) - 256) / p.all_heads;  // tokens a launch, within the divisions' range
+  const int64_t threads = most_a_launch(256, 256 / G, p.all_heads);
+  in_launches(T, std::min(most, threads), [&](int64_t first, int64_t tokens) {
+    const uint32_t count = static_cast<uint32_t>(tokens * p.all_heads);
+    const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(count) + 256 / G - 1) / (256 / G));
+    if (vec) k_paged_append_norm<DT, true, G><<<grid, 256, 0, s>>>(p, first, count, table_vec, pairs_vec);
+    else k_paged_append_norm<DT, false, G><<<grid, 256, 0, s>>>(p, first, count, table_vec, pairs_vec);
+  });
+}
+
 // ------------------------------------------------------------------ attention
 
-constexpr float kNone = -__builtin_inff();
 constexpr uint32_t kNowhere = 1u << 31;  // an offset past every buffer's range here
 constexpr int kThrough = 16;  // sc1 of a buffer access: past the XCD's L2, to where all XCDs meet
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
@@ -197,15 +402,6 @@ __device__ __forceinline__ uint32_t units_before(const AttendArgs& p, int b) {
   return n;
 }
 
-__device__ __forceinline__ uint32_t scan64(uint32_t v) {  // the sum over the lanes up to this one
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t up = __shfl_up(v, o);
-    if ((threadIdx.x & 63) >= o) v += up;
-  }
-  return v;
-}
-
 // The sequence whose units hold `target` (below the total), and the units before it.
 template <int UT>
 __device__ __forceinline__ int find_sequence(const AttendArgs& p, uint32_t target, uint32_t& before) {
@@ -224,53 +420,6 @@ __device__ __forceinline__ int find_sequence(const AttendArgs& p, uint32_t targe
   }
   before = base;
   return p.B - 1;  // (not reached: target is below the total)
-}
-
-// (By value: __builtin_bit_cast of a vector's element, an lvalue, reads element 0.)
-__device__ __forceinline__ float as_float(uint32_t v) { return __builtin_bit_cast(float, v); }
-
-template <int DT>
-struct Lane16 {  // 16 bytes of a lane as MFMA operands
-  typedef _Float16 vec __attribute__((ext_vector_type(8)));
-};
-template <>
-struct Lane16<DT_BF16> {
-  typedef __bf16 vec __attribute__((ext_vector_type(8)));
-};
-
-template <int DT>
-__device__ __forceinline__ float4_t mfma16(uint4_t a, uint4_t b, float4_t c) {
-  typedef typename Lane16<DT>::vec vec;
-  if constexpr (DT == DT_F16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
-}
-
-// Two probabilities as the sums of two 16-bit parts each: cut off, and the rest, rounded. What is cut is a little less
-// than the probability, so that the rest is not 0 beside a first part that is not, and an infinity in V stays what
-// it is in both products (f16: of probabilities of 2^-23, 2^-38 of the largest, and more; others give NaN with it).
-// A probability of 0 gives zeros: a token without weight has no part in the answer, whatever its value.
-template <int DT>
-__device__ __forceinline__ uint2 split2(float a, float b) {
-  constexpr float less = 1.f - 0x1p-20f;
-  if constexpr (DT == DT_F16) {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(fmaf(a, less, -0x1p-24f), fmaf(b, less, -0x1p-24f));
-    return make_uint2(__builtin_bit_cast(uint32_t, h), pack2<DT>(a - static_cast<float>(h[0]), b - static_cast<float>(h[1])));
-  } else {
-    const uint32_t hi = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b * less), __builtin_bit_cast(uint32_t, a * less), 0x07060302u);
-    return make_uint2(hi, pack2<DT>(a - __builtin_bit_cast(float, hi << 16), b - __builtin_bit_cast(float, hi & 0xFFFF0000u)));
-  }
-}
-
-// The maximum (sum) over the four lanes of one column of an MFMA tile, in all of them.
-__device__ __forceinline__ float column_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ __forceinline__ float column_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
 }
 
 // One workgroup's share of the units. Four wavefronts take the tiles of a unit (TILE tokens each), with
@@ -773,24 +922,73 @@ __global__ __launch_bounds__(256) void k_paged_join(AttendArgs p) {
   store(dim, total == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / total));
 }
 
-int check_cache(tmh_ctx* ctx, const tmh_paged_cache* c) {
-  if (!c) return fail(ctx, TMH_ERR_INVALID, "the paged cache is NULL");
-  if (!is_float_dtype(c->dtype))
-    return fail(ctx, TMH_ERR_INVALID, "a paged cache holds f32, f16 or bf16 values, got %s", dtype_name(c->dtype));
-  if (c->kv_heads < 1 || c->page_size < 1 || c->pages < 1)
-    return fail(ctx, TMH_ERR_INVALID, "a paged cache needs kv_heads, page_size and pages of at least 1, got %d, %d, %lld",
-                c->kv_heads, c->page_size, (long long)c->pages);
-  if (c->head_dim < 8 || c->head_dim > 256 || c->head_dim % 8 != 0)
-    return fail(ctx, TMH_ERR_UNSUPPORTED, "a paged cache's head_dim must be a multiple of 8 up to 256, got %d", c->head_dim);
-  if (c->pages >= (int64_t{1} << 31) / c->page_size + ((int64_t{1} << 31) % c->page_size != 0))
-    return fail(ctx, TMH_ERR_UNSUPPORTED, "a paged cache needs pages * page_size below 2^31");
-  if (!c->k || !c->v) return fail(ctx, TMH_ERR_INVALID, "a paged cache's k and v must not be NULL");
-  const int64_t e = 16 / dtype_size(c->dtype);
-  if (reinterpret_cast<uintptr_t>(c->k) % 16 != 0 || reinterpret_cast<uintptr_t>(c->v) % 16 != 0 || c->page_stride % e != 0 ||
-      c->token_stride % e != 0 || c->head_stride % e != 0)
-    return fail(ctx, TMH_ERR_UNSUPPORTED, "a paged cache's k, v and strides must be multiples of 16 bytes");
-  if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0)
-    return fail(ctx, TMH_ERR_INVALID, "a paged cache's strides must not be negative");
+// How an append's operands may be read: rows and partners by 16 bytes, tables by eight entries, by four f32 pairs.
+struct AppendForm {
+  bool vec, table_vec, pairs_vec;
+};
+
+// The checks and arguments that the appends share (with T = 0 nothing is filled in).
+int append_args(tmh_ctx* ctx, const char* name, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v,
+                int64_t ldv, int64_t T, int heads, const int64_t* d_positions, const void* d_cos, const void* d_sin,
+                int table_dtype, int64_t max_positions, int rotary_dim, int interleaved, const int64_t* d_slots,
+                const tmh_paged_cache* cache, void* d_q_out, int64_t ldqo, AppendArgs& p, AppendForm& form) {
+  TMH_TRY(check_cache(ctx, cache));
+  const int dim = cache->head_dim;
+  if (T < 0 || heads < 0 || T >= (int64_t{1} << 31) || static_cast<int64_t>(heads) + 2 * static_cast<int64_t>(cache->kv_heads) > (1 << 20))
+    return fail(ctx, TMH_ERR_INVALID, "cannot append %lld tokens of %d query heads", (long long)T, heads);
+  if (rotary_dim < 0 || rotary_dim > dim || rotary_dim % 2 != 0)
+    return fail(ctx, TMH_ERR_INVALID, "rotary_dim must be even and from 0 to head_dim=%d, got %d", dim, rotary_dim);
+  if (rotary_dim && !is_float_dtype(table_dtype))
+    return fail(ctx, TMH_ERR_INVALID, "rotary tables must be f32, f16 or bf16, got %s", dtype_name(table_dtype));
+  if (rotary_dim && max_positions < 1) return fail(ctx, TMH_ERR_INVALID, "rotary tables hold no positions");
+  const int64_t kv_width = static_cast<int64_t>(cache->kv_heads) * dim, q_width = static_cast<int64_t>(heads) * dim;
+  if (ldk < kv_width || ldv < kv_width || (heads && (ldq < q_width || ldqo < q_width)))
+    return fail(ctx, TMH_ERR_INVALID, "the leading dimensions of q, k and v must be at least their heads' widths");
+  TMH_TRY(use_device(ctx));
+  if (T == 0) return TMH_OK;
+  if (!d_k || !d_v || !d_slots || (heads && (!d_q || !d_q_out)) || (rotary_dim && (!d_positions || !d_cos || !d_sin)))
+    return fail(ctx, TMH_ERR_INVALID, "%s: NULL pointer", name);
+  if (heads && rotary_dim && d_q_out == d_q) return fail(ctx, TMH_ERR_INVALID, "rotated queries need a place of their own");
+  p.q = d_q;
+  p.k = d_k;
+  p.v = d_v;
+  p.positions = d_positions;
+  p.cos = d_cos;
+  p.sin = d_sin;
+  p.slots = d_slots;
+  p.q_out = d_q_out;
+  p.k_cache = cache->k;
+  p.v_cache = cache->v;
+  p.ldq = ldq;
+  p.ldk = ldk;
+  p.ldv = ldv;
+  p.ldqo = ldqo;
+  p.max_positions = max_positions;
+  p.page_stride = cache->page_stride;
+  p.token_stride = cache->token_stride;
+  p.head_stride = cache->head_stride;
+  p.num_slots = cache->pages * cache->page_size;
+  p.table_dtype = table_dtype;
+  p.rotary = rotary_dim;
+  p.interleaved = interleaved;
+  p.heads = heads;
+  p.kv_heads = cache->kv_heads;
+  p.by_page = FastDiv(static_cast<uint32_t>(cache->page_size));
+  const int64_t e = 16 / dtype_size(cache->dtype);
+  auto on16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
+  form.vec = on16(d_k) && on16(d_v) && ldk % e == 0 && ldv % e == 0 &&
+                   (!heads || (on16(d_q) && on16(d_q_out) && ldq % e == 0 && ldqo % e == 0)) &&
+                   (interleaved ? true : rotary_dim % 16 == 0);
+  p.head_dim = dim;
+  p.turned = form.vec && !interleaved ? rotary_dim / 16 : 0;
+  const uint32_t of_head = static_cast<uint32_t>(dim / 8 - p.turned);
+  p.value_pieces = static_cast<uint32_t>(cache->kv_heads * (dim / 8));
+  p.pieces = static_cast<uint32_t>(heads + cache->kv_heads) * of_head + p.value_pieces;
+  p.by_pieces = FastDiv(p.pieces);
+  p.by_head = FastDiv(of_head);
+  p.by_value = FastDiv(static_cast<uint32_t>(dim / 8));
+  form.table_vec = on16(d_cos) && on16(d_sin) && rotary_dim % 16 == 0;
+  form.pairs_vec = table_dtype == TMH_F32 && on16(d_cos) && on16(d_sin) && rotary_dim % 8 == 0;  // four pairs an access
   return TMH_OK;
 }
 
@@ -819,69 +1017,53 @@ int tmh_paged_append(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void* d_k
                      int64_t ldv, int64_t T, int heads, const int64_t* d_positions, const void* d_cos,
                      const void* d_sin, int table_dtype, int64_t max_positions, int rotary_dim, int interleaved,
                      const int64_t* d_slots, const tmh_paged_cache* cache, void* d_q_out, int64_t ldqo, void* stream) {
-  TMH_TRY(check_cache(ctx, cache));
-  const int dim = cache->head_dim;
-  if (T < 0 || heads < 0 || T >= (int64_t{1} << 31) || static_cast<int64_t>(heads) + 2 * static_cast<int64_t>(cache->kv_heads) > (1 << 20))
-    return fail(ctx, TMH_ERR_INVALID, "cannot append %lld tokens of %d query heads", (long long)T, heads);
-  if (rotary_dim < 0 || rotary_dim > dim || rotary_dim % 2 != 0)
-    return fail(ctx, TMH_ERR_INVALID, "rotary_dim must be even and from 0 to head_dim=%d, got %d", dim, rotary_dim);
-  if (rotary_dim && !is_float_dtype(table_dtype))
-    return fail(ctx, TMH_ERR_INVALID, "rotary tables must be f32, f16 or bf16, got %s", dtype_name(table_dtype));
-  if (rotary_dim && max_positions < 1) return fail(ctx, TMH_ERR_INVALID, "rotary tables hold no positions");
-  const int64_t kv_width = static_cast<int64_t>(cache->kv_heads) * dim, q_width = static_cast<int64_t>(heads) * dim;
-  if (ldk < kv_width || ldv < kv_width || (heads && (ldq < q_width || ldqo < q_width)))
-    return fail(ctx, TMH_ERR_INVALID, "the leading dimensions of q, k and v must be at least their heads' widths");
-  TMH_TRY(use_device(ctx));
-  if (T == 0) return TMH_OK;
-  if (!d_k || !d_v || !d_slots || (heads && (!d_q || !d_q_out)) || (rotary_dim && (!d_positions || !d_cos || !d_sin)))
-    return fail(ctx, TMH_ERR_INVALID, "tmh_paged_append: NULL pointer");
-  if (heads && rotary_dim && d_q_out == d_q) return fail(ctx, TMH_ERR_INVALID, "rotated queries need a place of their own");
   AppendArgs p;
-  p.q = d_q;
-  p.k = d_k;
-  p.v = d_v;
-  p.positions = d_positions;
-  p.cos = d_cos;
-  p.sin = d_sin;
-  p.slots = d_slots;
-  p.q_out = d_q_out;
-  p.k_cache = cache->k;
-  p.v_cache = cache->v;
-  p.ldq = ldq;
-  p.ldk = ldk;
-  p.ldv = ldv;
-  p.ldqo = ldqo;
-  p.max_positions = max_positions;
-  p.page_stride = cache->page_stride;
-  p.token_stride = cache->token_stride;
-  p.head_stride = cache->head_stride;
-  p.num_slots = cache->pages * cache->page_size;
-  p.table_dtype = table_dtype;
-  p.rotary = rotary_dim;
-  p.interleaved = interleaved;
-  p.heads = heads;
-  p.kv_heads = cache->kv_heads;
-  p.by_page = FastDiv(static_cast<uint32_t>(cache->page_size));
-  const int64_t e = 16 / dtype_size(cache->dtype);
-  auto on16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
-  const bool vec = on16(d_k) && on16(d_v) && ldk % e == 0 && ldv % e == 0 &&
-                   (!heads || (on16(d_q) && on16(d_q_out) && ldq % e == 0 && ldqo % e == 0)) &&
-                   (interleaved ? true : rotary_dim % 16 == 0);
-  p.head_dim = dim;
-  p.turned = vec && !interleaved ? rotary_dim / 16 : 0;
-  const uint32_t of_head = static_cast<uint32_t>(dim / 8 - p.turned);
-  p.value_pieces = static_cast<uint32_t>(cache->kv_heads * (dim / 8));
-  p.pieces = static_cast<uint32_t>(heads + cache->kv_heads) * of_head + p.value_pieces;
-  p.by_pieces = FastDiv(p.pieces);
-  p.by_head = FastDiv(of_head);
-  p.by_value = FastDiv(static_cast<uint32_t>(dim / 8));
-  const bool table_vec = on16(d_cos) && on16(d_sin) && rotary_dim % 16 == 0;
-  const bool pairs_vec = table_dtype == TMH_F32 && on16(d_cos) && on16(d_sin) && rotary_dim % 8 == 0;  // four pairs an access
+  AppendForm form;
+  TMH_TRY(append_args(ctx, "tmh_paged_append", d_q, ldq, d_k, ldk, d_v, ldv, T, heads, d_positions, d_cos, d_sin, table_dtype,
+                      max_positions, rotary_dim, interleaved, d_slots, cache, d_q_out, ldqo, p, form));
+  if (T == 0) return TMH_OK;
   hipStream_t s = pick_stream(ctx, stream);
-  if (cache->dtype == TMH_F32) launch_append<DT_F32>(p, T, vec, table_vec, pairs_vec, s);
-  else if (cache->dtype == TMH_F16) launch_append<DT_F16>(p, T, vec, table_vec, pairs_vec, s);
-  else launch_append<DT_BF16>(p, T, vec, table_vec, pairs_vec, s);
+  if (cache->dtype == TMH_F32) launch_append<DT_F32>(p, T, form.vec, form.table_vec, form.pairs_vec, s);
+  else if (cache->dtype == TMH_F16) launch_append<DT_F16>(p, T, form.vec, form.table_vec, form.pairs_vec, s);
+  else launch_append<DT_BF16>(p, T, form.vec, form.table_vec, form.pairs_vec, s);
   return check_launch(ctx, "k_paged_append");
+}
+
+int tmh_paged_append_norm(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v,
+                          int64_t ldv, int64_t T, int heads, const void* d_q_gamma, const void* d_k_gamma,
+                          int gamma_dtype, float eps, const int64_t* d_positions, const void* d_cos, const void* d_sin,
+                          int table_dtype, int64_t max_positions, int rotary_dim, int interleaved,
+                          const int64_t* d_slots, const tmh_paged_cache* cache, void* d_q_out, int64_t ldqo,
+                          void* stream) {
+  if (!is_float_dtype(gamma_dtype))
+    return fail(ctx, TMH_ERR_INVALID, "the heads' gammas must be f32, f16 or bf16, got %s", dtype_name(gamma_dtype));
+  if (!(eps >= 0.f)) return fail(ctx, TMH_ERR_INVALID, "eps must not be negative, got %g", eps);
+  if (!d_q_gamma && !d_k_gamma) return fail(ctx, TMH_ERR_INVALID, "tmh_paged_append_norm: no gamma (tmh_paged_append norms nothing)");
+  AppendNormArgs p;
+  AppendForm form;
+  TMH_TRY(append_args(ctx, "tmh_paged_append_norm", d_q, ldq, d_k, ldk, d_v, ldv, T, heads, d_positions, d_cos, d_sin, table_dtype,
+                      max_positions, rotary_dim, interleaved, d_slots, cache, d_q_out, ldqo, p.a, form));
+  if (T == 0) return TMH_OK;
+  p.q_gamma = d_q_gamma;
+  p.k_gamma = d_k_gamma;
+  p.gamma_dtype = gamma_dtype;
+  p.gamma_vec = reinterpret_cast<uintptr_t>(d_q_gamma) % 16 == 0 && reinterpret_cast<uintptr_t>(d_k_gamma) % 16 == 0;
+  p.eps = eps;
+  p.each = 1.f / static_cast<float>(cache->head_dim);
+  p.all_heads = static_cast<uint32_t>(heads + 2 * cache->kv_heads);
+  p.by_heads = FastDiv(p.all_heads);
+  hipStream_t s = pick_stream(ctx, stream);
+  const int pieces = cache->head_dim / 8 - p.a.turned;  // of a query's or key's head
+  auto launch = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (pieces <= 8) launch_append_norm<DT, 8>(p, T, form.vec, form.table_vec, form.pairs_vec, s);
+    else if (pieces <= 16) launch_append_norm<DT, 16>(p, T, form.vec, form.table_vec, form.pairs_vec, s);
+    else launch_append_norm<DT, 32>(p, T, form.vec, form.table_vec, form.pairs_vec, s);
+  };
+  if (cache->dtype == TMH_F32) launch(std::integral_constant<int, DT_F32>{});
+  else if (cache->dtype == TMH_F16) launch(std::integral_constant<int, DT_F16>{});
+  else launch(std::integral_constant<int, DT_BF16>{});
+  return check_launch(ctx, "k_paged_append_norm");
 }
 
 int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, int heads, const tmh_paged_cache* cache,

@@ -1,6 +1,7 @@
 """The operators of a decoder layer with 8-bit floating-point weights (include/transmuter_hip.h, "decoder
-layers in 8-bit floating point"): the residual's addition and the root-mean-square norm, rows in 8 bits, the
-8-bit product, and a paged cache of keys and values with the attention that reads it.
+layers in 8-bit floating point", and "drafted steps and sampling"): the residual's addition and the root-mean-square
+norm, rows in 8 bits, the 8-bit product, a paged cache of keys and values with the attentions that read it, and tokens
+drawn from logits.
 
 Rows in 8 bits (`Rows8`) are f8_e4m3fn values with one f32 scale for each block of 128 columns. Every call is
 asynchronous on `stream` (None: the context's); its operands must stay until its work is done. A call's answer is new
@@ -238,10 +239,13 @@ class PagedCache:
 
     def append(self, qkv: DeviceTensor, heads: int, slots: DeviceTensor, positions: DeviceTensor | None = None,
                cos: DeviceTensor | None = None, sin: DeviceTensor | None = None, *, interleaved: bool = False,
+               q_norm: DeviceTensor | None = None, k_norm: DeviceTensor | None = None, eps: float = 1e-6,
                out: DeviceTensor | None = None, stream=None) -> DeviceTensor:
         """The keys and values of a merged q/k/v product [T, (heads + 2 kv_heads) * head_dim] into slots [T] (s64,
         page * page_size + place; outside the cache: not stored), its queries and keys turned by their positions [T]
-        (s64) first where tables cos and sin [max_positions, rotary_dim / 2] are given. Returns the queries."""
+        (s64) first where tables cos and sin [max_positions, rotary_dim / 2] are given. With q_norm or k_norm, gammas
+        [head_dim], each query or key head is normed ahead of that: x * rsqrt(mean(x^2) + eps) * gamma. Returns the
+        queries."""
         t, d, g = math.prod(qkv.shape[:-1]), self.head_dim, self.kv_heads
         width = (heads + 2 * g) * d
         if qkv.dtype != self.dtype or qkv.shape[-1] != width:
@@ -255,9 +259,13 @@ class PagedCache:
             if positions.dtype != "s64" or positions.size != t:
                 _refuse(f"a step of {t} tokens takes {t} s64 positions, got {positions.dtype} {positions.shape}")
             most, rotary, table = cos.shape[0], 2 * cos.shape[1], cos.tmh_dtype
+        gammas = [gamma for gamma in (q_norm, k_norm) if gamma is not None]
+        if any(gamma.shape != (d,) or gamma.dtype != gammas[0].dtype for gamma in gammas):
+            _refuse(f"the heads' norms take gammas [{d}] of one type, got {[(gamma.dtype, gamma.shape) for gamma in gammas]}")
+        norm = (_given(q_norm, "q_norm"), _given(k_norm, "k_norm"), gammas[0].tmh_dtype, eps) if gammas else ()
         q = _out(out, self.ctx, (*qkv.shape[:-1], heads * d), self.dtype)
-        self.ctx.check(lib().tmh_paged_append(
-            self.ctx.handle, qkv.ptr, width, _at(qkv, heads * d), width, _at(qkv, (heads + g) * d), width, t, heads,
+        self.ctx.check((lib().tmh_paged_append_norm if norm else lib().tmh_paged_append)(
+            self.ctx.handle, qkv.ptr, width, _at(qkv, heads * d), width, _at(qkv, (heads + g) * d), width, t, heads, *norm,
             positions.ptr if rotary else None, cos.ptr if rotary else None, sin.ptr if rotary else None, table, most,
             rotary, int(interleaved), slots.ptr, ctypes.byref(self.desc), q.ptr, heads * d, stream))
         return q
@@ -281,6 +289,35 @@ class PagedCache:
             page_table.shape[1], lengths.ptr, scale, window, y.ptr, y.shape[1], stream))
         return y
 
+    def attend_tree(self, q: DeviceTensor, page_table: DeviceTensor, lengths: DeviceTensor, starts: DeviceTensor,
+                    mask: DeviceTensor | None = None, *, scale: float | None = None, window: int = 0,
+                    out: DeviceTensor | None = None, stream=None) -> DeviceTensor:
+        """Attention of several new tokens a sequence: rows starts[b] .. starts[b + 1] - 1 (s32, [B + 1]) of q
+        [T, heads * head_dim] are the last of sequence b's lengths[b] (s32) tokens, in the pages page_table[b] (s32,
+        [B, max_pages]). A row sees its sequence's tokens before them, and of them those whose bits its row of mask
+        [T, words] (s64) has: bit j % 64 of word j // 64 is the sequence's j-th row. Without a mask a row sees those up to
+        itself (a chain of drafts, a prompt's chunk). With a window it sees the last `window` of these. The scale is
+        1 / sqrt(head_dim) by default; rows behind the last sequence's are left as they are."""
+        if q.dtype != self.dtype or len(q.shape) != 2 or q.shape[1] % self.head_dim:
+            _refuse(f"attention takes {self.dtype} queries [T, heads * {self.head_dim}], got {q.dtype} {q.shape}")
+        t = q.shape[0]
+        if page_table.dtype != "s32" or len(page_table.shape) != 2:
+            _refuse(f"the page table is s32 [B, pages], got {page_table.dtype} {page_table.shape}")
+        b = page_table.shape[0]
+        if lengths.dtype != "s32" or lengths.shape != (b,):
+            _refuse(f"the lengths are s32 [{b}], got {lengths.dtype} {lengths.shape}")
+        if starts.dtype != "s32" or starts.shape != (b + 1,):
+            _refuse(f"the starts are s32 [{b + 1}], got {starts.dtype} {starts.shape}")
+        if mask is not None and (mask.dtype != "s64" or len(mask.shape) != 2 or mask.shape[0] != t or mask.shape[1] < 1):
+            _refuse(f"the mask is s64 [{t}, words], got {mask.dtype} {mask.shape}")
+        y = _out(out, self.ctx, q.shape, q.dtype)
+        scale = 1 / math.sqrt(self.head_dim) if scale is None else scale
+        self.ctx.check(lib().tmh_paged_tree_attention(
+            self.ctx.handle, q.ptr, q.shape[1], t, q.shape[1] // self.head_dim, ctypes.byref(self.desc), page_table.ptr, b,
+            page_table.shape[1], lengths.ptr, starts.ptr, _given(mask, "the mask"), mask.shape[1] if mask is not None else 0,
+            scale, window, y.ptr, y.shape[1], stream))
+        return y
+
     def free(self) -> None:
         self.k.free()
         self.v.free()
@@ -289,3 +326,23 @@ class PagedCache:
     def __repr__(self) -> str:
         return (f"PagedCache({self.pages} pages of {self.page_size}, {self.kv_heads} heads of {self.head_dim}, "
                 f"{self.dtype}, {self.order})")
+
+
+def sample(logits: DeviceTensor, random: DeviceTensor, *, temperature: DeviceTensor | None = None,
+           top_k: DeviceTensor | None = None, top_p: DeviceTensor | None = None, min_p: DeviceTensor | None = None,
+           out: DeviceTensor | None = None, stream=None) -> DeviceTensor:
+    """One token (s64) for each row of logits [..., V], drawn by the row's random number in [0, 1) (f32). Each row has its
+    own temperature (f32; 0: the largest logit), top_k (s32; 0: all), top_p (f32; 1: all) and min_p (f32; 0: all), None
+    leaving that out for all rows: of the top_k largest logits' tokens the fewest whose probabilities sum to top_p, and of
+    these those of at least min_p times the most probable one's. -1 for a row without a logit above -infinity."""
+    t, v = _rows(logits, "sampling")
+    for name, tensor, dtype in (("random", random, "f32"), ("temperature", temperature, "f32"), ("top_k", top_k, "s32"),
+                                ("top_p", top_p, "f32"), ("min_p", min_p, "f32")):
+        if tensor is not None and (tensor.dtype != dtype or tensor.size != t):
+            _refuse(f"sampling {t} rows takes {t} {dtype} values of {name}, got {tensor.dtype} {tensor.shape}")
+    ctx = logits.ctx
+    out = _out(out, ctx, logits.shape[:-1], "s64")
+    ctx.check(lib().tmh_sample(ctx.handle, logits.ptr, v, logits.tmh_dtype, t, v, _given(temperature, "temperature"),
+                               _given(top_k, "top_k"), _given(top_p, "top_p"), _given(min_p, "min_p"), random.ptr, out.ptr,
+                               stream))
+    return out

@@ -126,6 +126,20 @@ __device__ __forceinline__ bool not_finite(uint4_t x) {
   return any;
 }
 
+// Two probabilities as the sums of two 16-bit parts each, the first cut off, the second rounded (f16: cut off, at 2^-21 of the
+// probability). Unlike split2's, the second part may be 0 beside a first that is not, and an infinity in V becomes a NaN.
+template <int DT>
+__device__ __forceinline__ uint2 cut2(float a, float b) {
+  if constexpr (DT == DT_F16) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    const auto r = __builtin_amdgcn_cvt_pkrtz(a - static_cast<float>(h[0]), b - static_cast<float>(h[1]));
+    return make_uint2(__builtin_bit_cast(uint32_t, h), __builtin_bit_cast(uint32_t, r));
+  } else {
+    const uint32_t hi = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+    return make_uint2(hi, pack2<DT>(a - __builtin_bit_cast(float, hi << 16), b - __builtin_bit_cast(float, hi & 0xFFFF0000u)));
+  }
+}
+
 // Columns [first, first + columns) of an item over its tokens [from, to), one after another, each product in f32 of what a column
 // sees alone: the workgroups' way where a column does not see a token that holds an infinity or a NaN, which a weight of 0 would
 // leave in a matrix product. put(column of these, dimension, sum) and total(column of these, maximum, sum) take the answers; the
@@ -588,7 +602,7 @@ __device__ __forceinline__ void to_lds16(const char* from, uint8_t* lds) {
 template <int DT, int NB, int C>
 __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs p) {
   constexpr int TW = 64 / NB, UT = 2 * TW, M = 64 * C;  // a wavefront's tokens of a unit
-  constexpr int W = TW / 32, TB = TW / 16, NC = 4 * NB, PITCH = 256 * NB;
+  constexpr int W = TW / 32, NC = 4 * NB, PITCH = 256 * NB;
   constexpr int STAGE = 2 * UT * PITCH;
   constexpr int RI = 4 / NB, RW = TW / 4;  // rows that an instruction brings, and a wavefront
   constexpr float F = DT == DT_F16 ? 15.f : -32.f;
@@ -670,25 +684,34 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs p) {
         for (int e = 0; e < 8; ++e) acc[cb][nb][e] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    // Lane i looks token i % TW of its wavefront's half of a unit up: its row's offset in bytes, -1 where there is none.
+    // Lane i looks token i % TW of its wavefront's half of a unit up, in two steps: the page's number is loaded a unit before it is
+    // looked at, which would wait for the rows that are on their way by then. A row's offset in bytes, -1 where there is none.
     auto first_of = [&](uint32_t u) { return (d.unit + static_cast<int>(u)) * UT + wt * TW; };
-    auto look = [&](uint32_t u) -> int64_t {
+    auto page_of = [&](uint32_t u) { return table[p.cache.by_page.div(static_cast<uint32_t>(min(first_of(u) + lane % TW, d.end - 1)))]; };
+    auto offset_of = [&](uint32_t u, int32_t id) -> int64_t {
       const int token = first_of(u) + lane % TW;
-      if (u >= to || token >= d.end) return -1;
-      return token_offset(p.cache, table, static_cast<uint32_t>(token)) * 2;  // (a page that is none: negative)
+      if (u >= to || token >= d.end || id < 0 || id >= p.cache.pages) return -1;
+      const uint32_t place = static_cast<uint32_t>(token) - p.cache.by_page.div(static_cast<uint32_t>(token)) * p.cache.by_page.d;
+      return (id * p.cache.page_stride + place * p.cache.token_stride) * 2;
     };
     // Brings a unit's rows: a wavefront a quarter of its half's (rows that are masked: row 0 of page 0, not used).
     auto bring = [&](int64_t offset, int stage) {
       const int64_t row = offset < 0 ? 0 : offset;
+      int64_t from_row[RW / RI];
 #pragma unroll
-      for (int j = 0; j < RW / RI; ++j) {
-        const int mine = RW * wc + RI * j + lane / (16 * NB), slot = lane % (16 * NB);  // row of the half, piece of the row
-        const int64_t from_row = __shfl(row, mine);
-        uint8_t* to_k = &lds[stage][(wt * TW + RW * wc + RI * j) * PITCH];
-        const int piece = slot ^ frag_swizzle<16>(mine);
-        if (8 * piece < p.head_dim) to_lds16(kb + from_row + 16 * piece, to_k);
-        if (8 * slot < p.head_dim) to_lds16(vb + from_row + 16 * slot, to_k + UT * PITCH);
-      }
+      for (int j = 0; j < RW / RI; ++j) from_row[j] = __shfl(row, RW * wc + RI * j + lane / (16 * NB));
+      auto each = [&](auto whole) {
+#pragma unroll
+        for (int j = 0; j < RW / RI; ++j) {
+          const int mine = RW * wc + RI * j + lane / (16 * NB), slot = lane % (16 * NB);  // row of the half, piece of the row
+          uint8_t* to_k = &lds[stage][(wt * TW + RW * wc + RI * j) * PITCH];
+          const int piece = slot ^ frag_swizzle<16>(mine);
+          if (whole || 8 * piece < p.head_dim) to_lds16(kb + from_row[j] + 16 * piece, to_k);
+          if (whole || 8 * slot < p.head_dim) to_lds16(vb + from_row[j] + 16 * slot, to_k + UT * PITCH);
+        }
+      };
+      if (p.head_dim == 128 * NB) each(std::true_type{});
+      else each(std::false_type{});
     };
     // All of a workgroup's rows have come, and no wavefront reads the unit before any more.
     auto meet = [&] {
@@ -698,93 +721,64 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs p) {
       asm volatile("" ::: "memory");
     };
 
-    // S^T of the wavefront's half.
-    float4_t s[C][TB];
-    auto scores = [&](int stage) {
-#pragma unroll
-      for (int tb = 0; tb < TB; ++tb) {
-        const uint8_t* row = &lds[stage][(wt * TW + 16 * tb + col) * PITCH];
-#pragma unroll
-        for (int cb = 0; cb < C; ++cb) s[cb][tb] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const uint4_t kf = *reinterpret_cast<const uint4_t*>(row + 16 * ((4 * c + g) ^ frag_swizzle<16>(col)));
-#pragma unroll
-          for (int cb = 0; cb < C; ++cb) s[cb][tb] = mfma16<DT>(kf, qf[cb][c], s[cb][tb]);
-        }
+    // What each of the lane's columns sees of the 32 tokens from `first` on, `valid` of which there are.
+    auto sees = [&](int cb, int first, uint32_t valid) {
+      if (first + 32 > d.prefix) {
+        if (!p.mask) valid &= chain_bits(node[cb], first - d.prefix);
+        else if (p.words == 1) valid &= tree_bits(&word[cb], 1, first - d.prefix);
+        else valid &= tree_bits(p.mask + static_cast<int64_t>(d.row + node[cb]) * p.words, p.words, first - d.prefix);
       }
+      if (p.window > 0) valid &= from_bits(begin[cb], first);
+      return valid;
     };
-    // What each of the lane's columns sees of the tokens from `first` on, `valid` of which there are: false where all see all.
-    uint32_t sees[C][W];
-    auto look_at = [&](int first, uint64_t valid) {
-      const bool masked = valid != (TW == 64 ? ~uint64_t{0} : 0xFFFFFFFFu) || first + TW > d.prefix || p.window > 0;
-#pragma unroll
-      for (int cb = 0; cb < C; ++cb)
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          sees[cb][w] = static_cast<uint32_t>(valid >> 32 * w);
-          if (!masked) continue;
-          const int from = first + 32 * w;
-          if (from + 32 > d.prefix) {
-            if (!p.mask) sees[cb][w] &= chain_bits(node[cb], from - d.prefix);
-            else if (p.words == 1) sees[cb][w] &= tree_bits(&word[cb], 1, from - d.prefix);
-            else sees[cb][w] &= tree_bits(p.mask + static_cast<int64_t>(d.row + node[cb]) * p.words, p.words, from - d.prefix);
-          }
-          if (p.window > 0) sees[cb][w] &= from_bits(begin[cb], from);
-        }
-      return masked;
-    };
-    // 16 bytes of V of each of a lane's tokens 32 w + 16 (j / 4) + 4 g + j % 4 of the half; zeros where there is none.
+    // 16 bytes of V of each of a lane's tokens 32 w + 16 (j / 4) + 4 g + j % 4 of the half.
     auto values_of = [&](int stage, int w, int nb, uint4_t (&vf)[8]) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         vf[j] = *reinterpret_cast<const uint4_t*>(&lds[stage][(UT + wt * TW + 32 * w + 16 * (j / 4) + 4 * g + j % 4) * PITCH + 256 * nb + 16 * col]);
     };
-    auto present = [&](int w, uint64_t valid, uint4_t (&vf)[8]) {
-      asm volatile("");  // (a branch: as selects they would be paid for in every unit)
+    // A step of 32 tokens. Its rows are asked of LDS at once, ahead of all products (the compiler would wait for each by itself).
+    auto step = [&](int stage, int w, int first, uint32_t valid) {
+      uint4_t kf[2][NC], vf[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (!(valid >> (32 * w + 16 * (j / 4) + 4 * g + j % 4) & 1u)) vf[j] = uint4_t{0u, 0u, 0u, 0u};
-    };
-    // Whether a column does not see a token that holds an infinity or a NaN, which a weight of 0 would not hide.
-    auto hides = [&](int stage, uint64_t valid) {
-      bool mixed = false, any = false;
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* row = &lds[stage][(wt * TW + 32 * w + 16 * h + col) * PITCH];
 #pragma unroll
-      for (int cb = 0; cb < C; ++cb)
+        for (int c = 0; c < NC; ++c) kf[h][c] = *reinterpret_cast<const uint4_t*>(row + 16 * ((4 * c + g) ^ frag_swizzle<16>(col)));
+      }
+      values_of(stage, w, 0, vf);
+      __builtin_amdgcn_sched_barrier(0);
+      float4_t s[C][2];
 #pragma unroll
-        for (int w = 0; w < W; ++w) mixed |= sees[cb][w] != static_cast<uint32_t>(valid >> 32 * w);
-      if (!__ballot(mixed)) return false;
-#pragma unroll 1
-      for (int w = 0; w < W; ++w)
-#pragma unroll 1
-        for (int nb = 0; nb < NB; ++nb) {
-          uint4_t vf[8];
-          values_of(stage, w, nb, vf);
-          present(w, valid, vf);
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) any |= not_finite<DT>(vf[j]);
+        for (int cb = 0; cb < C; ++cb) s[cb][h] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int cb = 0; cb < C; ++cb) s[cb][h] = mfma16<DT>(kf[h][c], qf[cb][c], s[cb][h]);
+      }
+      const bool masked = valid != ~0u || first + 32 > d.prefix || p.window > 0;
+      if (masked) {
+        asm volatile("");  // (a branch: as selects it would be paid for in every step)
+#pragma unroll
+        for (int cb = 0; cb < C; ++cb) {
+          const uint32_t some = sees(cb, first, valid);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (!(some >> (16 * h + 4 * g + i) & 1u)) s[cb][h][i] = kNone;
         }
-      return __ballot(any) != 0;
-    };
-    uint4_t parts[C][W][2];  // the probabilities' two parts
-    auto hide = [&] {
-      asm volatile("");  // (as above)
-#pragma unroll
-      for (int cb = 0; cb < C; ++cb)
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!(sees[cb][tb / 2] >> (16 * (tb % 2) + 4 * g + i) & 1u)) s[cb][tb][i] = kNone;
-    };
-    auto softmax = [&] {
+      }
+      uint4_t parts[C][2];  // the probabilities' two parts
 #pragma unroll
       for (int cb = 0; cb < C; ++cb) {
         float top = kNone;
 #pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[cb][tb][i]);
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[cb][h][i]);
         top = column_max(top);
         if (__ballot(top > m[cb])) {
           const float next = fmaxf(m[cb], top);
@@ -798,66 +792,68 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs p) {
         }
         const float c = F - (m[cb] == kNone ? 0.f : m[cb] * a);
 #pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float two[2];
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              two[y] = __builtin_amdgcn_exp2f(fmaf(s[cb][tb][2 * x + y], a, c));
-              l[cb] += two[y];
-            }
-            const uint2 part = split2<DT>(two[0], two[1]);
-            parts[cb][tb / 2][0][2 * (tb % 2) + x] = part.x;
-            parts[cb][tb / 2][1][2 * (tb % 2) + x] = part.y;
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[cb][h][2 * x], a, c)), p1 = __builtin_amdgcn_exp2f(fmaf(s[cb][h][2 * x + 1], a, c));
+            l[cb] += p0 + p1;
+            const uint2 part = cut2<DT>(p0, p1);
+            parts[cb][0][2 * h + x] = part.x;
+            parts[cb][1][2 * h + x] = part.y;
           }
       }
-    };
-    // Of V's dimension 8 (4 g + i) + e (of block nb) the lane's tokens.
-    auto operand = [&](const uint4_t (&vf)[8], int e) {
-      uint4_t vt;
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        vt[x] = __builtin_amdgcn_perm(vf[2 * x + 1][e >> 1], vf[2 * x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-      return vt;
+      for (int nb = 0; nb < NB; ++nb) {
+        if (nb) values_of(stage, w, nb, vf);
+        if (masked) {
+          asm volatile("");  // (as above)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (!(valid >> (16 * (j / 4) + 4 * g + j % 4) & 1u)) vf[j] = uint4_t{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          uint4_t vt;  // of V's dimension 8 (4 g + i) + e (of block nb) the lane's tokens
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            vt[x] = __builtin_amdgcn_perm(vf[2 * x + 1][e >> 1], vf[2 * x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int cb = 0; cb < C; ++cb) {
+            acc[cb][nb][e] = mfma16<DT>(vt, parts[cb][0], acc[cb][nb][e]);
+            acc[cb][nb][e] = mfma16<DT>(vt, parts[cb][1], acc[cb][nb][e]);
+          }
+        }
+      }
     };
 
-    int64_t found = look(from), coming = look(from + 1);
+    int64_t found = offset_of(from, page_of(from));
+    int32_t coming = page_of(from + 1);
     __syncthreads();  // the item before has left LDS
     bring(found, 0);
-    bool alone = false;  // a column does not see an infinity or a NaN
     int stage = 0;
     for (uint32_t u = from; u < to; ++u, stage ^= 1) {
       const uint64_t valid = TW == 64 ? __ballot(found >= 0) : __ballot(found >= 0) & 0xFFFFFFFFu;
       meet();
-      if (u + 1 < to) bring(coming, stage ^ 1);
-      found = coming;
-      coming = look(u + 2);
-      scores(stage);
-      const bool masked = look_at(first_of(u), valid);
-      if (masked) {
-        alone |= hides(stage, valid);
-        hide();
-      }
-      softmax();
-#pragma unroll
-      for (int w = 0; w < W; ++w)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          uint4_t vf[8];
-          values_of(stage, w, nb, vf);
-          if (masked) present(w, valid, vf);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint4_t vt = operand(vf, e);
-#pragma unroll
-            for (int cb = 0; cb < C; ++cb) {
-              acc[cb][nb][e] = mfma16<DT>(vt, parts[cb][w][0], acc[cb][nb][e]);
-              acc[cb][nb][e] = mfma16<DT>(vt, parts[cb][w][1], acc[cb][nb][e]);
-            }
-          }
-        }
+      found = offset_of(u + 1, coming);
+      coming = page_of(u + 2);
+      if (u + 1 < to) bring(found, stage ^ 1);
+#pragma unroll 1
+      for (int w = 0; w < W; ++w) step(stage, w, first_of(u) + 32 * w, static_cast<uint32_t>(valid >> 32 * w));
     }
+    // An infinity or a NaN in V leaves a NaN in every column of its products, whether the column sees it or not (0 times an
+    // infinity): such an item is done again.
+    bool alone = false;
+#pragma unroll
+    for (int cb = 0; cb < C; ++cb)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = acc[cb][nb][e][i];
+            alone |= x != x;
+          }
 
     const bool whole = from == 0 && to == static_cast<uint32_t>(d.units);
     const int64_t slot = part_place(worker, at == run);
@@ -1006,7 +1002,7 @@ struct TreeForm {
 TreeForm tree_form(int64_t columns, bool f32, int head_dim) {
   if (f32) return {false, head_dim <= 128 && columns > 16 ? 32 : 16, 64, 2};
   if (columns <= 16) return {false, 16, 128, 2};
-  return {true, columns <= 64 ? 64 : 128, head_dim <= 128 ? 128 : 64, 1};
+  return {true, columns <= 64 || head_dim > 128 ? 64 : 128, head_dim <= 128 ? 128 : 64, 1};
 }
 
 }  // namespace
@@ -1094,7 +1090,7 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
       else form.columns == 64 ? launch_shared<DT, 1, 1>(p, s) : launch_shared<DT, 1, 2>(p, s);
     } else {
       if (!form.shared) launch_tree<DT, 2, 1>(p, s);
-      else form.columns == 64 ? launch_shared<DT, 2, 1>(p, s) : launch_shared<DT, 2, 2>(p, s);
+      else launch_shared<DT, 2, 1>(p, s);
     }
   };
   if (cache->dtype == TMH_F32) launch(std::integral_constant<int, DT_F32>{});

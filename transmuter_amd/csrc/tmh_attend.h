@@ -7,6 +7,7 @@
 namespace tmh {
 
 constexpr float kNone = -__builtin_inff();
+typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ uint32_t scan64(uint32_t v) {  // the sum over the lanes up to this one
 #pragma unroll

@@ -363,7 +363,6 @@ void launch_append_norm(const AppendNormArgs& p, int64_t T, bool vec, bool table
 
 constexpr uint32_t kNowhere = 1u << 31;  // an offset past every buffer's range here
 constexpr int kThrough = 16;  // sc1 of a buffer access: past the XCD's L2, to where all XCDs meet
-typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 
 struct AttendArgs {
   const void* q;

@@ -37,12 +37,11 @@ __device__ __forceinline__ Draft draft_at(const TreeArgs& p, int b) {
   return draft_of(p.starts[b], p.starts[b + 1], p.rows, p.lengths[b], p.most, p.window, UT, p.group, M);
 }
 template <int UT, int M>
-__device__ __forceinline__ uint32_t work_at(const TreeArgs& p, int b) {  // units of one kv head's tiles
-  const Draft d = draft_at<UT, M>(p, b);
-  return static_cast<uint32_t>(d.units) * static_cast<uint32_t>(d.tiles);
+__device__ __forceinline__ uint32_t work_at(const TreeArgs& p, int b) {
+  return work_of(draft_at<UT, M>(p, b));
 }
 
-// All units of one kv head, by one wavefront.
+// All work of one kv head, by one wavefront.
 template <int UT, int M>
 __device__ __forceinline__ uint32_t all_work(const TreeArgs& p) {
   uint32_t n = 0;
@@ -52,34 +51,41 @@ __device__ __forceinline__ uint32_t all_work(const TreeArgs& p) {
   return __builtin_amdgcn_readfirstlane(n);  // (known to be the same in all lanes, as what follows from it then is)
 }
 
-// The sequence whose units hold `target` (below the total), and the units before it.
-template <int UT, int M>
-__device__ __forceinline__ int find_draft(const TreeArgs& p, uint32_t target, uint32_t& before) {
+// The sequence whose work (BY_ITEM: whose items of one kv head) holds `target`, which is below the total, and the work (before:
+// and the items) ahead of it.
+template <int UT, int M, bool BY_ITEM = false>
+__device__ __forceinline__ int find_draft(const TreeArgs& p, uint32_t target, uint32_t& before, uint32_t* items = nullptr) {
   const int lane = threadIdx.x & 63;
-  uint32_t base = 0;
+  uint32_t base = 0, item_base = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const uint32_t mine = b0 + lane < p.B ? work_at<UT, M>(p, b0 + lane) : 0;
-    const uint32_t sum = scan64(mine);
-    const uint64_t past = __ballot(base + sum > target);
+    uint32_t mine = 0, tiles = 0;
+    if (b0 + lane < p.B) {
+      const Draft d = draft_at<UT, M>(p, b0 + lane);
+      mine = work_of(d);
+      tiles = mine ? static_cast<uint32_t>(d.tiles) : 0;
+    }
+    const uint32_t sum = scan64(mine), item_sum = BY_ITEM ? scan64(tiles) : 0;
+    const uint64_t past = __ballot(BY_ITEM ? item_base + item_sum > target : base + sum > target);
     if (past) {
       const int at = __builtin_ctzll(past);
       before = base + __builtin_amdgcn_readlane(sum - mine, at);
+      if (BY_ITEM) *items = item_base + __builtin_amdgcn_readlane(item_sum - tiles, at);
       return b0 + at;
     }
     base += __builtin_amdgcn_readlane(sum, 63);
+    if (BY_ITEM) item_base += __builtin_amdgcn_readlane(item_sum, 63);
   }
   before = base;
-  return p.B;  // (not reached: target is below the total)
+  return p.B;  // (target is not below the total)
 }
 
-// Where unit `at` lies: its sequence, the item (one kv head and tile of columns) and the item's first unit. An item beyond
-// the sequence's (which only rows that are counted twice, by starts that fall, can give) ends a worker.
+// Where `at` lies in a sequence whose work begins at `before`: the item (one kv head and tile of columns) and where it begins.
 struct Place {
   uint32_t item, first;
 };
 __device__ __forceinline__ Place place_in(const Draft& d, uint32_t before, uint32_t at) {
-  const uint32_t units = static_cast<uint32_t>(d.units), item = (at - before) / units;
-  return {item, before + item * units};
+  const uint32_t each = static_cast<uint32_t>(d.units) + kItem, item = (at - before) / each;
+  return {item, before + item * each};
 }
 
 template <int DT>
@@ -89,27 +95,6 @@ __device__ __forceinline__ void store_answer(const TreeArgs& p, int64_t row, int
     *reinterpret_cast<float4_t*>(static_cast<float*>(p.y) + out) = o;
   else
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + out) = make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
-}
-
-// A lane's answers of one column, dimension 128 nb + 8 (4 g + i) + e in element i of acc[nb][e].
-template <int DT, int NB>
-__device__ __forceinline__ void answer_columns(const TreeArgs& p, const Draft& d, int kv_head, int column, int g, const float4_t (&acc)[NB][8],
-                                               float total) {
-  const int n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(column)));
-  const float each = total == 0.f ? 0.f : 1.f / total;
-  uint16_t* y = static_cast<uint16_t*>(p.y) + (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + column - n * p.group) * p.head_dim;
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int dim = 128 * nb + 8 * (4 * g + i);
-      if (dim >= p.head_dim) continue;
-      uint4_t out;
-#pragma unroll
-      for (int x = 0; x < 4; ++x)  // (0 * an infinity is none)
-        out[x] = total == 0.f ? 0u : pack2<DT>(acc[nb][2 * x][i] * each, acc[nb][2 * x + 1][i] * each);
-      *reinterpret_cast<uint4_t*>(y + dim) = out;
-    }
 }
 
 // Whether 16 bytes hold an infinity or a NaN.
@@ -142,13 +127,17 @@ __device__ __forceinline__ uint2 cut2(float a, float b) {
 
 // Columns [first, first + columns) of an item over its tokens [from, to), one after another, each product in f32 of what a column
 // sees alone: the workgroups' way where a column does not see a token that holds an infinity or a NaN, which a weight of 0 would
-// leave in a matrix product. put(column of these, dimension, sum) and total(column of these, maximum, sum) take the answers; the
-// maxima are of scores in base-2 logarithms. `room` is THREADS floats of LDS.
+// leave in a matrix product. put(column of these, dimension, sum, weights' sum) and total(column of these, maximum, weights' sum)
+// take the answers; the maxima are of scores in base-2 logarithms. Weights are multiplied by `factor`, as the other parts' are;
+// `room` is 3 THREADS + 16 words of LDS.
 template <int DT, int THREADS, typename Put, typename Total>
 __device__ __forceinline__ void each_alone(const TreeArgs& p, const Draft& d, const int32_t* table, int kv_head, int first, int columns, int from,
-                                           int to, float* room, Put put, Total total) {
-  constexpr float FACTOR = DT == DT_F16 ? 0x1p15f : 0x1p-32f;
-  const int tid = threadIdx.x, dim = p.head_dim, groups = THREADS / dim, mine = tid / dim;
+                                           int to, float factor, uint32_t* room, Put put, Total total) {
+  constexpr int EACH = 256 / THREADS > 0 ? 256 / THREADS : 1;  // dimensions a thread may have
+  const int tid = threadIdx.x, dim = p.head_dim, wave = tid >> 6;
+  int64_t* rows = reinterpret_cast<int64_t*>(room);  // of a turn's tokens, negative where one is not seen
+  float* weights = reinterpret_cast<float*>(room + 2 * THREADS);
+  float* tops = weights + THREADS;
   const int64_t head_at = static_cast<int64_t>(kv_head) * p.head_stride;
 #pragma unroll 1
   for (int c = 0; c < columns; ++c) {
@@ -157,50 +146,49 @@ __device__ __forceinline__ void each_alone(const TreeArgs& p, const Draft& d, co
     int begin = 0;
     if (p.window > 0) begin = mask ? tree_begin(mask, p.words, d.prefix, d.nodes, p.window) : chain_begin(node, d.prefix, p.window);
     const int64_t q = (d.row + node) * p.ldq + static_cast<int64_t>(kv_head * p.group + of_all - node * p.group) * dim;
-    float top = kNone, sum = 0.f, o = 0.f;  // o: dimension tid % dim, tokens of this group of threads
+    float top = kNone, sum = 0.f, o[EACH] = {};  // o: dimensions tid + i THREADS
 #pragma unroll 1
     for (int t0 = from; t0 < to; t0 += THREADS) {
       const int token = t0 + tid, some = min(THREADS, to - t0);
       float t = kNone;
-      if (token < to && token >= begin) {
-        const int64_t row = token_offset(p.cache, table, static_cast<uint32_t>(token));
-        const bool seen = row >= 0 && (token < d.prefix || ((mask ? tree_bits(mask, p.words, token - d.prefix) : chain_bits(node, token - d.prefix)) & 1u));
-        if (seen) {
-          float dot = 0.f;
+      int64_t row = -1;
+      if (token < to && token >= begin &&
+          (token < d.prefix || ((mask ? tree_bits(mask, p.words, token - d.prefix) : chain_bits(node, token - d.prefix)) & 1u)))
+        row = token_offset(p.cache, table, static_cast<uint32_t>(token));
+      if (row >= 0) {
+        float dot = 0.f;
 #pragma unroll 1
-          for (int i = 0; i < dim; ++i) dot = fmaf(load_as_f32<DT>(p.q, q + i), load_as_f32<DT>(p.k, row + head_at + i), dot);
-          t = dot * p.scale;
-        }
+        for (int i = 0; i < dim; ++i) dot = fmaf(load_as_f32<DT>(p.q, q + i), load_as_f32<DT>(p.k, row + head_at + i), dot);
+        t = dot * p.scale;
       }
+      float next = t;
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) next = fmaxf(next, __shfl_xor(next, x));
+      __syncthreads();  // the turn before has been read
+      if ((tid & 63) == 0) tops[wave] = next;
       __syncthreads();
-      room[tid] = t;
+      next = top;
+      for (int w = 0; w < THREADS / 64; ++w) next = fmaxf(next, tops[w]);
+      rows[tid] = row;
+      weights[tid] = __builtin_amdgcn_exp2f(t - (next == kNone ? 0.f : next)) * factor;
       __syncthreads();
-      float next = top;
-#pragma unroll 1
-      for (int i = 0; i < some; ++i) next = fmaxf(next, room[i]);
-      const float keep = next == top ? 1.f : __builtin_amdgcn_exp2f(top - next), ref = next == kNone ? 0.f : next;
+      const float keep = next == top ? 1.f : __builtin_amdgcn_exp2f(top - next);
       top = next;
       sum *= keep;
-      o *= keep;
+#pragma unroll
+      for (int x = 0; x < EACH; ++x) o[x] *= keep;
 #pragma unroll 1
       for (int i = 0; i < some; ++i) {
-        const float score = room[i];
-        if (score == kNone) continue;
-        const float w = __builtin_amdgcn_exp2f(score - ref) * FACTOR;
-        sum += w;
-        if (mine < groups && i % groups == mine) {
-          const int64_t row = token_offset(p.cache, table, static_cast<uint32_t>(t0 + i));
-          o = fmaf(w, load_as_f32<DT>(p.v, row + head_at + tid - mine * dim), o);
-        }
+        if (rows[i] < 0) continue;
+        sum += weights[i];
+#pragma unroll
+        for (int x = 0; x < EACH; ++x)
+          if (tid + x * THREADS < dim) o[x] = fmaf(weights[i], load_as_f32<DT>(p.v, rows[i] + head_at + tid + x * THREADS), o[x]);
       }
     }
-    __syncthreads();
-    room[tid] = o;
-    __syncthreads();
-    if (tid < dim) {
-      for (int i = 1; i < groups; ++i) o += room[i * dim + tid];
-      put(c, tid, o, sum);
-    }
+#pragma unroll
+    for (int x = 0; x < EACH; ++x)
+      if (tid + x * THREADS < dim) put(c, tid + x * THREADS, o[x], sum);
     if (tid == 0) total(c, top, sum);
   }
   __syncthreads();
@@ -240,7 +228,7 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
   const uint32_t all = all_work<UT, M>(p) * p.kv_heads, per = units_per_worker(all, p.workers);
   uint32_t at = worker * per;
   if (per == 0 || at >= all) return;
-  const uint32_t stop = min(at + per, all), run = at;
+  const uint32_t stop = min(at + per, all);
   uint32_t before;
   int b = find_draft<UT, M>(p, at / p.kv_heads, before);
   if (b >= p.B) return;
@@ -249,13 +237,16 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
   const int chunks_of_row = (p.head_dim + 4 * E - 1) / (4 * E);
   const bool ragged = p.head_dim % (4 * E) != 0;
   while (at < stop) {
-    while (at - before >= static_cast<uint32_t>(d.units) * d.tiles * p.kv_heads) {
-      before += static_cast<uint32_t>(d.units) * d.tiles * p.kv_heads;
+    while (at - before >= work_of(d) * p.kv_heads) {
+      before += work_of(d) * p.kv_heads;
       if (++b >= p.B) return;
       d = draft_at<UT, M>(p, b);
     }
     const Place place = place_in(d, before, at);
-    const uint32_t from = at - place.first, to = min(stop - place.first, static_cast<uint32_t>(d.units));
+    const Share share = share_of(place.first, static_cast<uint32_t>(d.units), at, stop);
+    const uint32_t from = share.from, to = share.to;
+    at = place.first + kItem + static_cast<uint32_t>(d.units);
+    if (from >= to) continue;
     const int kv_head = static_cast<int>(place.item) / d.tiles, tile = static_cast<int>(place.item) % d.tiles;
     const int columns = min(M, d.nodes * p.group - tile * M);
     const char* kb = static_cast<const char*>(p.k) + static_cast<int64_t>(kv_head) * p.head_stride * SIZE;
@@ -484,12 +475,11 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
     }
 
     const bool whole = from == 0 && to == static_cast<uint32_t>(d.units);
-    const uint32_t slot = part_place(worker, at == run);
-    at = place.first + to;
+    const uint32_t slot = place_of_part(worker, from == 0);
     if (__syncthreads_or(alone)) {
       each_alone<DT, 256>(
           p, d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),
-          &lds_o[0][0][0],
+          FACTOR, reinterpret_cast<uint32_t*>(&lds_o[0][0][0]),
           [&](int c, int dim, float o, float sum) {
             const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
             if (whole) store_as<DT>(p.y, (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + of_all - n * p.group) * p.head_dim + dim, sum == 0.f ? 0.f : o * (1.f / sum));
@@ -548,170 +538,279 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
   }
 }
 
-// The parts of an item that several workers shared: workgroup (w, i) sees to 16 columns of the item that begins in worker w
-// and goes on in the next.
-template <int DT, int M>
-__global__ __launch_bounds__(256) void k_tree_join(TreeArgs p) {
-  constexpr int UT = DT == DT_F32 ? 64 : 128;
+// An item that several workers shared, for the workgroups that join its parts: the `index`-th of all items (BY_ITEM), or the one that
+// begins in worker `index` and goes on in the next. False where there is none.
+struct Joined {
+  Draft d;
+  TreeParts parts;
+  int kv_head, tile;
+};
+template <int UT, int M, bool BY_ITEM>
+__device__ __forceinline__ bool find_joined(const TreeArgs& p, uint32_t index, Joined& j) {
   const uint32_t all = all_work<UT, M>(p) * p.kv_heads, per = units_per_worker(all, p.workers);
-  const uint32_t cut = (blockIdx.x + 1) * per;  // the first unit of the next worker
-  if (per == 0 || cut >= all) return;
-  uint32_t before;
-  const int b = find_draft<UT, M>(p, cut / p.kv_heads, before);
-  if (b >= p.B) return;
-  const Draft d = draft_at<UT, M>(p, b);
-  const Place place = place_in(d, before * p.kv_heads, cut);
-  if (place.item >= static_cast<uint32_t>(d.tiles * p.kv_heads) || place.first >= cut) return;
-  const Parts parts = parts_of(place.first, static_cast<uint32_t>(d.units), per);
-  if (parts.from != blockIdx.x || parts.from + parts.count > p.workers) return;
-  const int kv_head = static_cast<int>(place.item) / d.tiles, tile = static_cast<int>(place.item) % d.tiles;
-  const int first_column = 16 * blockIdx.y, some = min(16, min(M, d.nodes * p.group - tile * M) - first_column);
+  if (per == 0) return false;
+  uint32_t before, items = 0, item, first;
+  if constexpr (BY_ITEM) {
+    const int b = find_draft<UT, M, true>(p, index / p.kv_heads, before, &items);
+    if (b >= p.B) return false;
+    j.d = draft_at<UT, M>(p, b);
+    item = index - items * p.kv_heads;
+    first = before * p.kv_heads + item * (static_cast<uint32_t>(j.d.units) + kItem);
+  } else {
+    const uint32_t cut = (index + 1) * per;  // where the next worker begins
+    if (cut >= all) return false;
+    const int b = find_draft<UT, M>(p, cut / p.kv_heads, before);
+    if (b >= p.B) return false;
+    j.d = draft_at<UT, M>(p, b);
+    const Place place = place_in(j.d, before * p.kv_heads, cut);
+    item = place.item;
+    first = place.first;
+  }
+  if (item >= static_cast<uint32_t>(j.d.tiles * p.kv_heads)) return false;
+  j.parts = tree_parts(first, static_cast<uint32_t>(j.d.units), per);
+  j.kv_head = static_cast<int>(item) / j.d.tiles;
+  j.tile = static_cast<int>(item) % j.d.tiles;
+  return j.parts.count > 1 && j.parts.from + j.parts.count <= p.workers && (BY_ITEM || j.parts.from == index);
+}
+
+// The parts of an item that several workers shared (find_joined): workgroup (index, i) sees to columns 16 i .. 16 i + 15, a thread to
+// four dimensions of one, four parts on their way at once.
+template <int DT, int M, bool BY_ITEM>
+__global__ __launch_bounds__(256) void k_tree_join(TreeArgs p) {
+  constexpr int UT = DT == DT_F32 ? 64 : 128, BATCH = 4;
+  Joined j;
+  if (!find_joined<UT, M, BY_ITEM>(p, blockIdx.x, j)) return;
+  const TreeParts parts = j.parts;
+  const int first_column = 16 * blockIdx.y, some = min(16, min(M, j.d.nodes * p.group - j.tile * M) - first_column);
   const int quads = p.head_dim / 4;
   for (int i = threadIdx.x; i < some * quads; i += 256) {
     const int c = first_column + i / quads, dim = (i % quads) * 4;
-    auto row_of = [&](uint32_t k) { return static_cast<int64_t>(place_of(parts, k)) * M + c; };
     float top = kNone, total = 0.f;
-    for (uint32_t k = 0; k < parts.count; ++k) top = fmaxf(top, p.stats[row_of(k)].x);
     float4_t o{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t k = 0; k < parts.count; ++k) {
-      const float2 st = p.stats[row_of(k)];
-      const float f = st.x == top ? 1.f : __builtin_amdgcn_exp2f(st.x - top);
-      total += f * st.y;
-      o += f * *reinterpret_cast<const float4_t*>(p.part + row_of(k) * p.head_dim + dim);
+    for (uint32_t k0 = 0; k0 < parts.count; k0 += BATCH) {
+      float2 st[BATCH];
+      float4_t po[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {  // (too many: the first again, without a weight)
+        const bool there = k0 + k < parts.count;
+        const uint32_t at = there ? k0 + k : k0;
+        const int64_t row = static_cast<int64_t>(place_of_part(parts.from + at, at == 0)) * M + c;
+        st[k] = p.stats[row];
+        po[k] = *reinterpret_cast<const float4_t*>(p.part + row * p.head_dim + dim);
+        if (!there) {
+          st[k] = make_float2(kNone, 0.f);
+          po[k] = float4_t{0.f, 0.f, 0.f, 0.f};
+        }
+      }
+      float next = top;
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) next = fmaxf(next, st[k].x);
+      const float keep = top == next ? 1.f : __builtin_amdgcn_exp2f(top - next);
+      top = next;
+      total *= keep;
+      o *= keep;
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const float f = st[k].x == top ? 1.f : __builtin_amdgcn_exp2f(st[k].x - top);
+        total += f * st[k].y;
+        o += f * po[k];
+      }
     }
-    const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
-    store_answer<DT>(p, d.row + n, kv_head * p.group + of_all - n * p.group, dim,
+    const int of_all = j.tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
+    store_answer<DT>(p, j.d.row + n, j.kv_head * p.group + of_all - n * p.group, dim,
                      total == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / total));
   }
 }
 
-// Sixteen bytes a lane from memory into LDS at lds + 16 * lane, past the registers. `lds` must be wavefront-uniform.
+// Sixteen bytes a lane from memory into LDS at lds + 16 * lane, past the registers. `lds` must be wavefront-uniform. In assembly,
+// as the compiler would wait for it ahead of every transposed read of LDS, whatever that reads; a wait for all loads and a
+// barrier stand between it and the reads that it is for.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // (m0 is nobody's for longer than an instruction, so that naming it is remarked on)
 __device__ __forceinline__ void to_lds16(const char* from, uint8_t* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+  const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds)));
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "m0");
+#endif
+}
+#pragma clang diagnostic pop
+
+// Of four rows of sixteen 16-bit values, each row by four lanes of eight bytes, to each of sixteen lanes one column.
+__device__ __forceinline__ uint2_t columns_of(const uint8_t* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef short short4_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(lds)));
+#else
+  return uint2_t{0u, 0u};
 #endif
 }
 
-// The same for tiles of many columns, M = 64 C, whose products a wavefront's own columns do not keep waiting for memory: eight
-// wavefronts, four groups of 16 C columns for each half of a unit's tokens, read K and V from LDS, where all of them bring the
-// next unit meanwhile (a stage is 64 KiB, two of them fit a CU). Rows lie in LDS as in memory, K's pieces of 16 bytes moved within
-// their row so that the sixteen rows a product reads at once lie on different banks.
+template <int DT>
+__device__ __forceinline__ float16_t mfma32(uint4_t a, uint4_t b, float16_t c) {
+  typedef typename Lane16<DT>::vec vec;
+  if constexpr (DT == DT_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(vec, a), __builtin_bit_cast(vec, b), c, 0, 0, 0);
+}
+
+// v's upper and lower half's values in both halves.
+__device__ __forceinline__ void both_halves(float v, float& low, float& high) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t a = p[0], b = p[1];
+  low = __builtin_bit_cast(float, a);
+  high = __builtin_bit_cast(float, b);
+}
+
+// A lane's answers of one column, dimensions dim + 8 q + {0 .. 3} in acc[q].
+template <int DT>
+__device__ __forceinline__ void answer_column(const TreeArgs& p, const Draft& d, int kv_head, int column, int dim, const float4_t (&acc)[4], float total) {
+  const int n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(column)));
+  const float each = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float4_t y = acc[q] * each;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) y[x] = total == 0.f ? 0.f : y[x];  // (0 * an infinity is none)
+    if (dim + 8 * q < p.head_dim) store_answer<DT>(p, d.row + n, kv_head * p.group + column - n * p.group, dim + 8 * q, y);
+  }
+}
+__device__ __forceinline__ void quads_of(const float16_t& v, float4_t (&q)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = float4_t{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+}
+
+// What tokens that are none bring to LDS.
+__device__ const uint4_t kZeros[32] = {};
+
+// Tiles of M = 32 WC columns of 16-bit types: WC WT wavefronts, a group of 32 columns each, WT of them sharing a unit's tokens, read K and V
+// from LDS, where all of them bring the next unit meanwhile (two stages of 32 KiB). A step is 32 tokens: S^T = K Q^T, whose
+// lanes then hold sixteen tokens' scores of one column, in the order in which O^T = V^T P^T takes them: no score leaves its
+// lane, and V's columns are read from LDS transposed. Rows lie in LDS as in memory, their pieces of 16 bytes moved within the row,
+// K's by the row's number so that the rows that are read together lie on different banks, V's by four pieces a row of four.
 // Scores' maxima are kept as they come from the products: a probability is 2^(s a - m a + F) with the scale's magnitude a (its
 // sign goes to the queries), one fused multiply-add ahead of the exponential. What m a is rounded by is in all of a column's
-// weights and drops out.
-template <int DT, int NB, int C>
-__global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs p) {
-  constexpr int TW = 64 / NB, UT = 2 * TW, M = 64 * C;  // a wavefront's tokens of a unit
-  constexpr int W = TW / 32, NC = 4 * NB, PITCH = 256 * NB;
-  constexpr int STAGE = 2 * UT * PITCH;
-  constexpr int RI = 4 / NB, RW = TW / 4;  // rows that an instruction brings, and a wavefront
-  constexpr float F = DT == DT_F16 ? 15.f : -32.f;
+// weights and drops out. Probabilities go in two 16-bit parts, as in attention of one token.
+template <int DT, int NB, int WC, int WT>
+__global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(TreeArgs p) {
+  constexpr int THREADS = 64 * WC * WT, UT = 64 / NB, TW = UT / WT, M = 32 * WC;  // TW: a wavefront's tokens of a unit
+  constexpr int W = TW / 32, NC = 8 * NB, DB = 4 * NB, PITCH = 256 * NB, STAGE = 2 * UT * PITCH;
+  constexpr int RI = 4 / NB, RW = TW / WC;  // rows that an instruction brings, and a wavefront
+  constexpr int PLACES = W + 2;             // of a unit's work where loads of the next are asked for
+  constexpr uint32_t kNone16 = ~0u;
+  constexpr float LAG = DT == DT_F16 ? 4.f : 8.f, F = DT == DT_F16 ? 15.f - LAG : -32.f - LAG;
+  static_assert(TW % 32 == 0 && RW % 16 == 0, "");
   __shared__ __align__(16) uint8_t lds[2][STAGE];
-  __shared__ float lds_m[4][16 * C], lds_l[4][16 * C];
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wc = wave & 3, wt = wave >> 2;
+  __shared__ float2 lds_ml[WT][M];
+  const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wc = wave % WC, wt = wave / WC;
   const uint32_t worker = blockIdx.x;
   const int quads = p.head_dim / 4;
   for (int b = static_cast<int>(worker); b < p.B; b += static_cast<int>(p.workers)) {
     const Draft d = draft_at<UT, M>(p, b);
     if (d.units != 0) continue;
     const int64_t of_row = static_cast<int64_t>(p.group) * p.kv_heads * quads;
-    for (int64_t i = threadIdx.x; i < d.nodes * of_row; i += 512)
+    for (int64_t i = threadIdx.x; i < d.nodes * of_row; i += THREADS)
       store_answer<DT>(p, d.row + i / of_row, 0, 4 * static_cast<int>(i % of_row), float4_t{0.f, 0.f, 0.f, 0.f});
   }
   const uint32_t all = all_work<UT, M>(p) * p.kv_heads, per = units_per_worker(all, p.workers);
   uint32_t at = worker * per;
   if (per == 0 || at >= all) return;
-  const uint32_t stop = min(at + per, all), run = at;
+  const uint32_t stop = min(at + per, all);
   uint32_t before;
   int b = find_draft<UT, M>(p, at / p.kv_heads, before);
   if (b >= p.B) return;
   Draft d = draft_at<UT, M>(p, b);
   before *= p.kv_heads;
-  // Pieces of a row past head_dim are brought by nobody: zeros for all units.
-  if (p.head_dim < 128 * NB) {
-    for (int i = threadIdx.x; i < 2 * STAGE / 16; i += 512) reinterpret_cast<uint4_t*>(&lds[0][0])[i] = uint4_t{0u, 0u, 0u, 0u};
+  auto clear = [&] {  // pieces of a row past head_dim are brought by nobody: zeros for all units
+    if (p.head_dim == 128 * NB) return;
+    for (int i = threadIdx.x; i < 2 * STAGE / 16; i += THREADS) reinterpret_cast<uint4_t*>(&lds[0][0])[i] = uint4_t{0u, 0u, 0u, 0u};
     __syncthreads();
-  }
+  };
+  clear();
   // (A scale of 0: queries of zeros, so that -infinity times it stays what it is.)
   const float a = p.scale == 0.f ? 1.f : fabsf(p.scale);
   const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;
+  const uint32_t page16 = static_cast<uint32_t>(p.cache.page_stride / 8), token16 = static_cast<uint32_t>(p.cache.token_stride / 8);
   while (at < stop) {
-    while (at - before >= static_cast<uint32_t>(d.units) * d.tiles * p.kv_heads) {
-      before += static_cast<uint32_t>(d.units) * d.tiles * p.kv_heads;
+    while (at - before >= work_of(d) * p.kv_heads) {
+      before += work_of(d) * p.kv_heads;
       if (++b >= p.B) return;
       d = draft_at<UT, M>(p, b);
     }
     const Place place = place_in(d, before, at);
-    const uint32_t from = at - place.first, to = min(stop - place.first, static_cast<uint32_t>(d.units));
+    const Share share = share_of(place.first, static_cast<uint32_t>(d.units), at, stop);
+    const uint32_t from = share.from, to = share.to;
+    at = place.first + kItem + static_cast<uint32_t>(d.units);
+    if (from >= to) continue;
     const int kv_head = static_cast<int>(place.item) / d.tiles, tile = static_cast<int>(place.item) % d.tiles;
     const int columns = min(M, d.nodes * p.group - tile * M);
     const char* kb = static_cast<const char*>(p.k) + static_cast<int64_t>(kv_head) * p.head_stride * 2;
     const char* vb = static_cast<const char*>(p.v) + static_cast<int64_t>(kv_head) * p.head_stride * 2;
     const int32_t* table = p.table + static_cast<int64_t>(b) * p.max_pages;
+    // Tokens that all columns see, and those that any sees (of chains: up to the tile's first and last nodes).
+    const int first_node = static_cast<int>(p.by_group.div(static_cast<uint32_t>(tile * M)));
+    const int last_node = static_cast<int>(p.by_group.div(static_cast<uint32_t>(tile * M + columns - 1)));
+    const int open = p.mask ? d.prefix : d.prefix + first_node + 1, end = p.mask ? d.end : min(d.end, d.prefix + last_node + 1);
+    const uint32_t needed = end > d.unit * UT ? static_cast<uint32_t>((end + UT - 1) / UT - d.unit) : 0, upto = min(to, needed);
 
-    uint4_t qf[C][NC];
-    int node[C], begin[C];
-    uint64_t word[C];  // of masks of one word
+    const int of_all = tile * M + min(32 * wc + col, columns - 1);  // this lane's column
+    const int node = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
+    const uint64_t* mask = p.mask ? p.mask + static_cast<int64_t>(d.row + node) * p.words : nullptr;
+    const uint64_t word = mask ? mask[0] : 0;  // (all of it, mostly)
+    int begin = 0;
+    if (p.window > 0) begin = mask ? tree_begin(mask, p.words, d.prefix, d.nodes, p.window) : chain_begin(node, d.prefix, p.window);
+    uint4_t qf[NC];
+    float m = kNone, l = 0.f;  // of this lane's column, l over this lane's tokens only
+    float16_t acc[DB];
 #pragma unroll
-    for (int cb = 0; cb < C; ++cb) {
-      const int of_all = tile * M + min(16 * (C * wc + cb) + col, columns - 1);
-      node[cb] = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
-      const int head = kv_head * p.group + of_all - node[cb] * p.group;
-      begin[cb] = 0;
-      const uint64_t* mask = p.mask + static_cast<int64_t>(d.row + node[cb]) * p.words;
-      word[cb] = p.mask ? mask[0] : 0;
-      if (p.window > 0) begin[cb] = p.mask ? tree_begin(mask, p.words, d.prefix, d.nodes, p.window) : chain_begin(node[cb], d.prefix, p.window);
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int x = 0; x < NC; ++x) {
-        const int dim = 32 * x + 8 * g;
-        qf[cb][x] = uint4_t{0u, 0u, 0u, 0u};
-        if (dim < p.head_dim && p.scale != 0.f)
-          qf[cb][x] = *reinterpret_cast<const uint4_t*>(static_cast<const char*>(p.q) +
-                                                        ((d.row + node[cb]) * p.ldq + static_cast<int64_t>(head) * p.head_dim + dim) * 2);
-        qf[cb][x] ^= sign;
-      }
-    }
-    float m[C], l[C];  // of column 16 (C wc + cb) + col, l over this lane's tokens only
-    float4_t acc[C][NB][8];
-#pragma unroll
-    for (int cb = 0; cb < C; ++cb) {
-      m[cb] = kNone;
-      l[cb] = 0.f;
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[cb][nb][e] = float4_t{0.f, 0.f, 0.f, 0.f};
-    }
+      for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
 
-    // Lane i looks token i % TW of its wavefront's half of a unit up, in two steps: the page's number is loaded a unit before it is
-    // looked at, which would wait for the rows that are on their way by then. A row's offset in bytes, -1 where there is none.
+    // Lane i looks token i % TW of its wavefront's part of a unit up, in two steps: the page's number is loaded a unit before it is
+    // looked at, which would wait for the rows that are on their way by then. A row's offset in 16 bytes, kNone16 where there is none.
     auto first_of = [&](uint32_t u) { return (d.unit + static_cast<int>(u)) * UT + wt * TW; };
     auto page_of = [&](uint32_t u) { return table[p.cache.by_page.div(static_cast<uint32_t>(min(first_of(u) + lane % TW, d.end - 1)))]; };
-    auto offset_of = [&](uint32_t u, int32_t id) -> int64_t {
+    auto offset_of = [&](uint32_t u, int32_t id) {
       const int token = first_of(u) + lane % TW;
-      if (u >= to || token >= d.end || id < 0 || id >= p.cache.pages) return -1;
-      const uint32_t place = static_cast<uint32_t>(token) - p.cache.by_page.div(static_cast<uint32_t>(token)) * p.cache.by_page.d;
-      return (id * p.cache.page_stride + place * p.cache.token_stride) * 2;
+      const uint32_t in_page = static_cast<uint32_t>(token) - p.cache.by_page.div(static_cast<uint32_t>(token)) * p.cache.by_page.d;
+      const uint32_t at_row = static_cast<uint32_t>(id) * page16 + in_page * token16;
+      return token < d.end && id >= 0 && id < p.cache.pages ? at_row : kNone16;
     };
-    // Brings a unit's rows: a wavefront a quarter of its half's (rows that are masked: row 0 of page 0, not used).
-    auto bring = [&](int64_t offset, int stage) {
-      const int64_t row = offset < 0 ? 0 : offset;
-      int64_t from_row[RW / RI];
+    // Brings a unit's rows: a wavefront its share of its part's, PIECES instructions, of which those of `place` of all `places`. Rows
+    // that are none bring zeros; where the head is narrower than the unit's rows, lanes past it bring nothing.
+    constexpr int J = RW / RI;
+    const int slot16 = lane % (16 * NB), in_instruction = lane / (16 * NB);
+    const char* k_lane[J];
+    const char* v_lane[RI < 4 ? 4 / RI : 1];
 #pragma unroll
-      for (int j = 0; j < RW / RI; ++j) from_row[j] = __shfl(row, RW * wc + RI * j + lane / (16 * NB));
-      auto each = [&](auto whole) {
+    for (int j = 0; j < J; ++j) k_lane[j] = kb + 16 * (slot16 ^ ((RI * j + in_instruction) & 15));
 #pragma unroll
-        for (int j = 0; j < RW / RI; ++j) {
-          const int mine = RW * wc + RI * j + lane / (16 * NB), slot = lane % (16 * NB);  // row of the half, piece of the row
-          uint8_t* to_k = &lds[stage][(wt * TW + RW * wc + RI * j) * PITCH];
-          const int piece = slot ^ frag_swizzle<16>(mine);
-          if (whole || 8 * piece < p.head_dim) to_lds16(kb + from_row[j] + 16 * piece, to_k);
-          if (whole || 8 * slot < p.head_dim) to_lds16(vb + from_row[j] + 16 * slot, to_k + UT * PITCH);
+    for (int j = 0; j < (RI < 4 ? 4 / RI : 1); ++j) v_lane[j] = vb + 16 * (slot16 ^ (((RI * j + in_instruction) & 3) << 2));
+    uint32_t rows[J];  // of the unit that is brought: the lane's row of each instruction
+    bool plain = true;  // all of its tokens are there, in rows of the full width
+    auto rows_of = [&](uint32_t offset) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) rows[j] = __shfl(offset, RW * wc + RI * j + in_instruction);
+      plain = p.head_dim == 128 * NB && __ballot(offset == kNone16) == 0;
+    };
+    auto bring = [&](int stage, int place, int places) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        if (j * places / J != place) continue;
+        uint8_t* to = &lds[stage][(wt * TW + RW * wc + RI * j) * PITCH];
+        const uint64_t row = static_cast<uint64_t>(rows[j]) << 4;
+        if (plain) {
+          to_lds16(k_lane[j] + row, to);
+          to_lds16(v_lane[j % (4 / RI)] + row, to + UT * PITCH);
+        } else {
+          const char* none = reinterpret_cast<const char*>(kZeros);
+          const int k_piece = slot16 ^ ((RI * j + in_instruction) & 15), v_piece = slot16 ^ (((RI * j + in_instruction) & 3) << 2);
+          if (8 * k_piece < p.head_dim) to_lds16(rows[j] == kNone16 ? none : k_lane[j] + row, to);
+          if (8 * v_piece < p.head_dim) to_lds16(rows[j] == kNone16 ? none : v_lane[j % (4 / RI)] + row, to + UT * PITCH);
         }
-      };
-      if (p.head_dim == 128 * NB) each(std::true_type{});
-      else each(std::false_type{});
+      }
     };
     // All of a workgroup's rows have come, and no wavefront reads the unit before any more.
     auto meet = [&] {
@@ -720,278 +819,300 @@ __global__ __launch_bounds__(512, 2) void k_tree_shared(TreeArgs p) {
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     };
-
-    // What each of the lane's columns sees of the 32 tokens from `first` on, `valid` of which there are.
-    auto sees = [&](int cb, int first, uint32_t valid) {
-      if (first + 32 > d.prefix) {
-        if (!p.mask) valid &= chain_bits(node[cb], first - d.prefix);
-        else if (p.words == 1) valid &= tree_bits(&word[cb], 1, first - d.prefix);
-        else valid &= tree_bits(p.mask + static_cast<int64_t>(d.row + node[cb]) * p.words, p.words, first - d.prefix);
-      }
-      if (p.window > 0) valid &= from_bits(begin[cb], first);
-      return valid;
-    };
-    // 16 bytes of V of each of a lane's tokens 32 w + 16 (j / 4) + 4 g + j % 4 of the half.
-    auto values_of = [&](int stage, int w, int nb, uint4_t (&vf)[8]) {
+    // The TW tokens from `first` on, `valid` of which there are. Meanwhile between() is called PLACES times: a wavefront that
+    // asked for all its share of the next unit at once would wait for the queue of such loads.
+    auto step = [&](int stage, int first, uint64_t valid, auto between) {
+      float16_t s[W];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        vf[j] = *reinterpret_cast<const uint4_t*>(&lds[stage][(UT + wt * TW + 32 * w + 16 * (j / 4) + 4 * g + j % 4) * PITCH + 256 * nb + 16 * col]);
-    };
-    // A step of 32 tokens. Its rows are asked of LDS at once, ahead of all products (the compiler would wait for each by itself).
-    auto step = [&](int stage, int w, int first, uint32_t valid) {
-      uint4_t kf[2][NC], vf[8];
+      for (int w = 0; w < W; ++w) {
+        const uint8_t* k_row = &lds[stage][(wt * TW + 32 * w + col) * PITCH];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* row = &lds[stage][(wt * TW + 32 * w + 16 * h + col) * PITCH];
+        for (int i = 0; i < 16; ++i) s[w][i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) kf[h][c] = *reinterpret_cast<const uint4_t*>(row + 16 * ((4 * c + g) ^ frag_swizzle<16>(col)));
-      }
-      values_of(stage, w, 0, vf);
-      __builtin_amdgcn_sched_barrier(0);
-      float4_t s[C][2];
+        for (int nb = 0; nb < NB; ++nb) {
+          // (Asked of LDS ahead of all products: the compiler would wait for each by itself.)
+          uint4_t kf[8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+          for (int c = 0; c < 8; ++c) kf[c] = *reinterpret_cast<const uint4_t*>(k_row + 16 * ((16 * nb + 2 * c + h) ^ (col & 15)));
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int cb = 0; cb < C; ++cb) s[cb][h] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-          for (int cb = 0; cb < C; ++cb) s[cb][h] = mfma16<DT>(kf[h][c], qf[cb][c], s[cb][h]);
-      }
-      const bool masked = valid != ~0u || first + 32 > d.prefix || p.window > 0;
-      if (masked) {
-        asm volatile("");  // (a branch: as selects it would be paid for in every step)
-#pragma unroll
-        for (int cb = 0; cb < C; ++cb) {
-          const uint32_t some = sees(cb, first, valid);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (!(some >> (16 * h + 4 * g + i) & 1u)) s[cb][h][i] = kNone;
+          for (int c = 0; c < 8; ++c) s[w] = mfma32<DT>(kf[c], qf[8 * nb + c], s[w]);
         }
+        between(w);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      uint4_t parts[C][2];  // the probabilities' two parts
+      if (valid != (TW == 64 ? ~uint64_t{0} : 0xFFFFFFFFu) || first + TW > open || p.window > 0) {
+        asm volatile("");  // (a branch: as selects it would be paid for in every unit)
 #pragma unroll
-      for (int cb = 0; cb < C; ++cb) {
-        float top = kNone;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[cb][h][i]);
-        top = column_max(top);
-        if (__ballot(top > m[cb])) {
-          const float next = fmaxf(m[cb], top);
-          const float keep = next == m[cb] ? 1.f : m[cb] == kNone ? 0.f : __builtin_amdgcn_exp2f((m[cb] - next) * a);
-          m[cb] = next;
-          l[cb] *= keep;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[cb][nb][e] *= keep;
-        }
-        const float c = F - (m[cb] == kNone ? 0.f : m[cb] * a);
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[cb][h][2 * x], a, c)), p1 = __builtin_amdgcn_exp2f(fmaf(s[cb][h][2 * x + 1], a, c));
-            l[cb] += p0 + p1;
-            const uint2 part = cut2<DT>(p0, p1);
-            parts[cb][0][2 * h + x] = part.x;
-            parts[cb][1][2 * h + x] = part.y;
+        for (int w = 0; w < W; ++w) {
+          const int from = first + 32 * w;
+          uint32_t some = static_cast<uint32_t>(valid >> 32 * w);
+          if (from + 32 > d.prefix) {
+            if (!p.mask) some &= chain_bits(node, from - d.prefix);
+            else some &= p.words == 1 ? tree_bits(&word, 1, from - d.prefix) : tree_bits(mask, p.words, from - d.prefix);
           }
+          if (p.window > 0) some &= from_bits(begin, from);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!(some >> (8 * (i / 4) + 4 * h + i % 4) & 1u)) s[w][i] = kNone;
+        }
       }
+      float low, high, top = kNone;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        if (nb) values_of(stage, w, nb, vf);
-        if (masked) {
-          asm volatile("");  // (as above)
+      for (int w = 0; w < W; ++w)
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (!(valid >> (16 * (j / 4) + 4 * g + j % 4) & 1u)) vf[j] = uint4_t{0u, 0u, 0u, 0u};
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[w][i]);
+      both_halves(top, low, high);
+      top = fmaxf(low, high);
+      if (__ballot((top - m) * a > LAG)) {  // (m -infinity: infinity; or NaN where top is so too, or infinite as m is)
+        const float next = fmaxf(m, top);
+        const float keep = next == m ? 1.f : m == kNone ? 0.f : __builtin_amdgcn_exp2f((m - next) * a);
+        m = next;
+        l *= keep;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] *= keep;
+      }
+      const float c = F - (m == kNone ? 0.f : m * a);
+      // Half a step's products: of tokens 16 x + 4 h + {0 .. 3, 8 .. 11} V's dimension 32 db + lane % 32.
+#pragma unroll
+      for (int x = 0; x < 2 * W; ++x) {
+        uint4_t vf[DB], parts[2];
+        const int in_block = lane & 15, token = 16 * x + 4 * h + in_block / 4;
+        const uint8_t* row = &lds[stage][(UT + wt * TW + token) * PITCH];
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const int at = 16 * ((4 * db + 2 * (col >> 4) + (in_block & 3) / 2) ^ ((token & 3) << 2)) + 8 * (in_block & 1);
+          const uint2_t one = columns_of(row + at), two = columns_of(row + 8 * PITCH + at);
+          vf[db] = uint4_t{one.x, one.y, two.x, two.y};
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          uint4_t vt;  // of V's dimension 8 (4 g + i) + e (of block nb) the lane's tokens
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            vt[x] = __builtin_amdgcn_perm(vf[2 * x + 1][e >> 1], vf[2 * x][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-          for (int cb = 0; cb < C; ++cb) {
-            acc[cb][nb][e] = mfma16<DT>(vt, parts[cb][0], acc[cb][nb][e]);
-            acc[cb][nb][e] = mfma16<DT>(vt, parts[cb][1], acc[cb][nb][e]);
-          }
+        for (int y = 0; y < 4; ++y) {
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x % 2) + 2 * y], a, c));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x % 2) + 2 * y + 1], a, c));
+          l += p0 + p1;
+          const uint2 part = cut2<DT>(p0, p1);
+          parts[0][y] = part.x;
+          parts[1][y] = part.y;
         }
+        if (x < 2) between(W + x);
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) acc[db] = mfma32<DT>(vf[db], parts[y], acc[db]);
       }
     };
 
-    int64_t found = offset_of(from, page_of(from));
-    int32_t coming = page_of(from + 1);
+    uint32_t found = kNone16;
+    int32_t coming = 0;
     __syncthreads();  // the item before has left LDS
-    bring(found, 0);
-    int stage = 0;
-    for (uint32_t u = from; u < to; ++u, stage ^= 1) {
-      const uint64_t valid = TW == 64 ? __ballot(found >= 0) : __ballot(found >= 0) & 0xFFFFFFFFu;
-      meet();
-      found = offset_of(u + 1, coming);
-      coming = page_of(u + 2);
-      if (u + 1 < to) bring(found, stage ^ 1);
-#pragma unroll 1
-      for (int w = 0; w < W; ++w) step(stage, w, first_of(u) + 32 * w, static_cast<uint32_t>(valid >> 32 * w));
+    // The queries come by whole rows through the second stage, each wavefront's own columns (by 16 bytes of many rows at a time they
+    // took 5 us, with the first rows of K and V they come in passing).
+    if (from < upto) {
+      const int64_t q_row = (d.row + node) * p.ldq + static_cast<int64_t>(kv_head * p.group + of_all - node * p.group) * p.head_dim;
+#pragma unroll
+      for (int j = 0; j < 32 / RI; ++j) {
+        const int row = RI * j + in_instruction, piece = slot16 ^ (row & 15);
+        const char* q = static_cast<const char*>(p.q) + __shfl(q_row, row) * 2 + 16 * piece;
+        if (8 * piece < p.head_dim) to_lds16(q, &lds[1][(32 * wave + RI * j) * PITCH]);
+      }
+      found = offset_of(from, page_of(from));
+      coming = page_of(from + 1);
+      rows_of(found);
+      bring(0, 0, 1);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      qf[c] = *reinterpret_cast<const uint4_t*>(&lds[1][(32 * wave + col) * PITCH + 16 * ((2 * c + h) ^ (col & 15))]);
+      if (16 * c + 8 * h >= p.head_dim || p.scale == 0.f) qf[c] = uint4_t{0u, 0u, 0u, 0u};
+      qf[c] ^= sign;
+    }
+    int stage = 0;
+    for (uint32_t u = from; u < upto; ++u, stage ^= 1) {
+      const uint64_t valid = TW == 64 ? __ballot(found != kNone16) : __ballot(found != kNone16) & 0xFFFFFFFFu;
+      meet();
+      const bool more = u + 1 < upto;
+      if (more) {
+        found = offset_of(u + 1, coming);
+        coming = page_of(u + 2);
+        rows_of(found);
+      }
+      step(stage, first_of(u), valid, [&](int place) {
+        if (more) bring(stage ^ 1, place, PLACES);
+      });
+    }
+
+    const bool whole = from == 0 && to == static_cast<uint32_t>(d.units);
+    const int64_t slot = place_of_part(worker, from == 0);
     // An infinity or a NaN in V leaves a NaN in every column of its products, whether the column sees it or not (0 times an
     // infinity): such an item is done again.
     bool alone = false;
 #pragma unroll
-    for (int cb = 0; cb < C; ++cb)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = acc[cb][nb][e][i];
-            alone |= x != x;
-          }
-
-    const bool whole = from == 0 && to == static_cast<uint32_t>(d.units);
-    const int64_t slot = part_place(worker, at == run);
-    at = place.first + to;
+      for (int i = 0; i < 16; ++i) {
+        const float x = acc[db][i];
+        alone |= x != x;
+      }
     if (__syncthreads_or(alone)) {
-      each_alone<DT, 512>(
+      each_alone<DT, THREADS>(
           p, d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),
-          reinterpret_cast<float*>(&lds[0][0]),
+          __builtin_ldexpf(1.f, static_cast<int>(F)), reinterpret_cast<uint32_t*>(&lds[0][0]),
           [&](int c, int dim, float o, float sum) {
             const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
             if (whole) store_as<DT>(p.y, (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + of_all - n * p.group) * p.head_dim + dim, sum == 0.f ? 0.f : o * (1.f / sum));
-            else p.part[(((slot * 4 * C + c / 16) * (NB * 8) + dim / 128 * 8 + dim % 8) * 64 + dim % 128 / 32 * 16 + c % 16) * 4 + dim % 32 / 8] = o;
+            else p.part[(((slot * WC + c / 32) * (4 * DB) + dim / 8) * 64 + dim / 4 % 2 * 32 + c % 32) * 4 + dim % 4] = o;
           },
           [&](int c, float top, float sum) {
             if (!whole) p.stats[slot * M + c] = make_float2(top, sum);
           });
-      if (p.head_dim < 128 * NB) {  // (what it used of LDS may have been pieces of zeros)
-        for (int i = threadIdx.x; i < 2 * STAGE / 16; i += 512) reinterpret_cast<uint4_t*>(&lds[0][0])[i] = uint4_t{0u, 0u, 0u, 0u};
-        __syncthreads();
-      }
+      clear();
       continue;
     }
 
-    // The halves' parts meet in LDS, lane by lane; the first half's wavefronts answer.
-    float4_t* mine = reinterpret_cast<float4_t*>(&lds[0][0]) + wc * (C * NB * 8) * 64 + lane;
+    // The wavefronts that share a tile's tokens meet in LDS, lane by lane; the first of them answers.
+    {
+      float low, high;
+      both_halves(l, low, high);
+      l = low + high;
+    }
+    float4_t* sums = reinterpret_cast<float4_t*>(&lds[0][0]);
+    auto place_of_sum = [&](int part, int i) { return ((part * WC + wc) * (4 * DB) + i) * 64 + lane; };
+    lds_ml[wt][32 * wc + col] = make_float2(m, l);
+    if (wt > 0) {
 #pragma unroll
-    for (int cb = 0; cb < C; ++cb) l[cb] = column_sum(l[cb]);
-    if (wt == 1) {
-#pragma unroll
-      for (int cb = 0; cb < C; ++cb) {
-        if (g == 0) {
-          lds_m[wc][16 * cb + col] = m[cb];
-          lds_l[wc][16 * cb + col] = l[cb];
-        }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) mine[((cb * NB + nb) * 8 + e) * 64] = acc[cb][nb][e];
-      }
+      for (int i = 0; i < 4 * DB; ++i)
+        sums[place_of_sum(wt - 1, i)] = float4_t{acc[i / 4][i % 4 * 4], acc[i / 4][i % 4 * 4 + 1], acc[i / 4][i % 4 * 4 + 2], acc[i / 4][i % 4 * 4 + 3]};
     }
     __syncthreads();
-    if (wt == 0) {
+    if (wt == 0 && 32 * wc < columns) {
+      float top = m;
 #pragma unroll
-      for (int cb = 0; cb < C; ++cb) {
-        const int c = 16 * (C * wc + cb) + col;
-        const float other = lds_m[wc][16 * cb + col], top = fmaxf(m[cb], other);
-        const float f0 = m[cb] == top ? 1.f : m[cb] == kNone ? 0.f : __builtin_amdgcn_exp2f((m[cb] - top) * a);
-        const float f1 = other == top ? 1.f : other == kNone ? 0.f : __builtin_amdgcn_exp2f((other - top) * a);
-        const float total = f0 * l[cb] + f1 * lds_l[wc][16 * cb + col];
+      for (int w = 1; w < WT; ++w) top = fmaxf(top, lds_ml[w][32 * wc + col].x);
+      auto weight = [&](float x) { return x == top ? 1.f : x == kNone ? 0.f : __builtin_amdgcn_exp2f((x - top) * a); };
+      const float f0 = weight(m);
+      float total = f0 * l;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+      for (int db = 0; db < DB; ++db) acc[db] *= f0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) acc[cb][nb][e] = f0 * acc[cb][nb][e] + f1 * mine[((cb * NB + nb) * 8 + e) * 64];
-        if (16 * (C * wc + cb) >= columns) continue;
-        if (whole) {
-          if (c < columns) answer_columns<DT, NB>(p, d, kv_head, tile * M + c, g, acc[cb], total);
-        } else {
-          float4_t* part = reinterpret_cast<float4_t*>(p.part) + ((slot * 4 + wc) * (C * NB * 8) + cb * NB * 8) * 64 + lane;
+      for (int w = 1; w < WT; ++w) {
+        const float2 ml = lds_ml[w][32 * wc + col];
+        const float f = weight(ml.x);
+        total += f * ml.y;
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
+        for (int i = 0; i < 4 * DB; ++i) {
+          const float4_t o = sums[place_of_sum(w - 1, i)];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) part[(nb * 8 + e) * 64] = acc[cb][nb][e];
-          if (g == 0) p.stats[slot * M + c] = make_float2(top == kNone ? kNone : top * a, total);
+          for (int x = 0; x < 4; ++x) acc[i / 4][i % 4 * 4 + x] += f * o[x];
         }
+      }
+      if (whole) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          float4_t four[4];
+          quads_of(acc[db], four);
+          if (32 * wc + col < columns) answer_column<DT>(p, d, kv_head, tile * M + 32 * wc + col, 32 * db + 4 * h, four, total);
+        }
+      } else {
+        float4_t* part = reinterpret_cast<float4_t*>(p.part) + (slot * WC + wc) * (4 * DB) * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < 4 * DB; ++i)
+          part[i * 64] = float4_t{acc[i / 4][i % 4 * 4], acc[i / 4][i % 4 * 4 + 1], acc[i / 4][i % 4 * 4 + 2], acc[i / 4][i % 4 * 4 + 3]};
+        if (h == 0) p.stats[slot * M + 32 * wc + col] = make_float2(top == kNone ? kNone : top * a, total);
       }
     }
   }
 }
 
-// The parts of an item that several workers shared: workgroup (w, i) sees to 16 columns of the item that begins in worker w
-// and goes on in the next, its four wavefronts to every fourth part.
-template <int DT, int NB, int C>
-__global__ __launch_bounds__(256) void k_tree_shared_join(TreeArgs p) {
-  constexpr int UT = 128 / NB, M = 64 * C;
-  const uint32_t all = all_work<UT, M>(p) * p.kv_heads, per = units_per_worker(all, p.workers);
-  const uint32_t cut = (blockIdx.x + 1) * per;  // the first unit of the next worker
-  if (per == 0 || cut >= all) return;
-  uint32_t before;
-  const int b = find_draft<UT, M>(p, cut / p.kv_heads, before);
-  if (b >= p.B) return;
-  const Draft d = draft_at<UT, M>(p, b);
-  const Place place = place_in(d, before * p.kv_heads, cut);
-  if (place.item >= static_cast<uint32_t>(d.tiles * p.kv_heads) || place.first >= cut) return;
-  const Parts parts = parts_of(place.first, static_cast<uint32_t>(d.units), per);
-  if (parts.from != blockIdx.x || parts.from + parts.count > p.workers) return;
-  const int kv_head = static_cast<int>(place.item) / d.tiles, tile = static_cast<int>(place.item) % d.tiles;
-  const int block = blockIdx.y;  // 16 columns
-  const int columns = min(M, d.nodes * p.group - tile * M);
-  if (16 * block >= columns) return;
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// The parts of an item that several workers shared (find_joined): workgroup (index, wc, z) sees to columns 32 wc .. 32 wc + 31 and
+// dimensions 128 z .. 128 z + 127, four wavefronts to each 32 of these, each to every fourth part, four of them on their way at once.
+template <int DT, int NB, int WC, bool BY_ITEM>
+__global__ __launch_bounds__(1024) void k_tree_shared_join(TreeArgs p) {
+  constexpr int UT = 64 / NB, M = 32 * WC, BATCH = 4;
+  __shared__ __align__(16) float4_t sums[4][3][4][64];
+  __shared__ float2 stats[4][3][64];
+  Joined j;
+  if (!find_joined<UT, M, BY_ITEM>(p, blockIdx.x, j)) return;
+  const TreeParts parts = j.parts;
+  auto slot_of = [&](uint32_t k) { return static_cast<int64_t>(place_of_part(parts.from + k, k == 0)); };
+  const int wc = blockIdx.y, columns = min(M, j.d.nodes * p.group - j.tile * M);
+  if (32 * wc >= columns) return;
+  const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave & 3, quarter = wave >> 2;
+  const int db = 4 * blockIdx.z + quarter;
   float top = kNone, total = 0.f;
-  float4_t acc[NB][8];
+  float4_t acc[4];
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
+  for (int q = 0; q < 4; ++q) acc[q] = float4_t{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t k0 = mine; k0 < parts.count; k0 += 4 * BATCH) {
+    float2 st[BATCH];
+    float4_t o[BATCH][4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[nb][e] = float4_t{0.f, 0.f, 0.f, 0.f};
-  auto join = [&](float other, float sum, auto from) {
-    const float next = fmaxf(top, other);
-    const float f0 = top == next ? 1.f : __builtin_amdgcn_exp2f(top - next), f1 = other == next ? 1.f : __builtin_amdgcn_exp2f(other - next);
+    for (int k = 0; k < BATCH; ++k) {  // (too many: the first again, without a weight)
+      const bool there = k0 + 4 * k < parts.count;
+      const int64_t slot = slot_of(there ? k0 + 4 * k : k0);
+      st[k] = p.stats[slot * M + 32 * wc + col];
+      if (!there) st[k] = make_float2(kNone, 0.f);
+      const float4_t* part = reinterpret_cast<const float4_t*>(p.part) + ((slot * WC + wc) * (16 * NB) + 4 * db) * 64 + lane;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[k][q] = part[q * 64];
+    }
+    float next = top;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) next = fmaxf(next, st[k].x);
+    const float keep = top == next ? 1.f : __builtin_amdgcn_exp2f(top - next);
     top = next;
-    total = f0 * total + f1 * sum;
+    total *= keep;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int q = 0; q < 4; ++q) acc[q] *= keep;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[nb][e] = f0 * acc[nb][e] + f1 * from(nb * 8 + e);
-  };
-#pragma unroll 2
-  for (uint32_t k = wave; k < parts.count; k += 4) {
-    const int64_t slot = place_of(parts, k);
-    const float2 st = p.stats[slot * M + 16 * block + col];
-    const float4_t* part = reinterpret_cast<const float4_t*>(p.part) + (slot * 4 * C + block) * (NB * 8) * 64 + lane;
-    join(st.x, st.y, [&](int i) { return part[i * 64]; });
+    for (int k = 0; k < BATCH; ++k) {
+      if (k0 + 4 * k >= parts.count) continue;
+      const float f = st[k].x == top ? 1.f : __builtin_amdgcn_exp2f(st[k].x - top);
+      total += f * st[k].y;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) acc[q] += f * o[k][q];
+    }
   }
-  __shared__ __align__(16) float4_t sums[3][NB * 8][64];
-  __shared__ float2 stats[3][64];
-  if (wave) {
-    stats[wave - 1][lane] = make_float2(top, total);
+  if (mine) {
+    stats[quarter][mine - 1][lane] = make_float2(top, total);
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sums[wave - 1][nb * 8 + e][lane] = acc[nb][e];
+    for (int q = 0; q < 4; ++q) sums[quarter][mine - 1][q][lane] = acc[q];
   }
   __syncthreads();
-  if (wave) return;
-  for (int w = 0; w < 3; ++w) join(stats[w][lane].x, stats[w][lane].y, [&](int i) { return sums[w][i][lane]; });
-  if (16 * block + col < columns) answer_columns<DT, NB>(p, d, kv_head, tile * M + 16 * block + col, g, acc, total);
+  if (mine) return;
+  float most = top;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) most = fmaxf(most, stats[quarter][w][lane].x);
+  const float keep = top == most ? 1.f : __builtin_amdgcn_exp2f(top - most);
+  total *= keep;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) acc[q] *= keep;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+    const float2 st = stats[quarter][w][lane];
+    const float f = st.x == most ? 1.f : __builtin_amdgcn_exp2f(st.x - most);
+    total += f * st.y;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[q] += f * sums[quarter][w][q][lane];
+  }
+  if (32 * wc + col < columns) answer_column<DT>(p, j.d, j.kv_head, j.tile * M + 32 * wc + col, 32 * db + 4 * h, acc, total);
 }
 
+// Items that several workers shared are found among all items, or among the workers' ends, whichever are fewer.
 template <int DT, int NB, int CB>
-void launch_tree(const TreeArgs& p, hipStream_t s) {
+void launch_tree(const TreeArgs& p, int64_t items, hipStream_t s) {
   k_tree_attention<DT, NB, CB><<<p.workers, 256, 0, s>>>(p);
-  if (p.workers > 1) k_tree_join<DT, 16 * CB><<<dim3(p.workers - 1, CB), 256, 0, s>>>(p);
+  if (p.workers == 1) return;
+  if (items < p.workers) k_tree_join<DT, 16 * CB, true><<<dim3(static_cast<unsigned>(items), CB), 256, 0, s>>>(p);
+  else k_tree_join<DT, 16 * CB, false><<<dim3(p.workers - 1, CB), 256, 0, s>>>(p);
 }
-template <int DT, int NB, int C>
-void launch_shared(const TreeArgs& p, hipStream_t s) {
-  k_tree_shared<DT, NB, C><<<p.workers, 512, 0, s>>>(p);
-  if (p.workers > 1) k_tree_shared_join<DT, NB, C><<<dim3(p.workers - 1, 4 * C), 256, 0, s>>>(p);
+template <int DT, int NB, int WC, int WT>
+void launch_shared(const TreeArgs& p, int64_t items, hipStream_t s) {
+  k_tree_shared<DT, NB, WC, WT><<<p.workers, 64 * WC * WT, 0, s>>>(p);
+  if (p.workers == 1) return;
+  if (items < p.workers) k_tree_shared_join<DT, NB, WC, true><<<dim3(static_cast<unsigned>(items), WC, NB), 1024, 0, s>>>(p);
+  else k_tree_shared_join<DT, NB, WC, false><<<dim3(p.workers - 1, WC, NB), 1024, 0, s>>>(p);
 }
 
 // How columns go to workgroups, by the columns that a sequence has in the mean (all the host knows).
@@ -999,10 +1120,12 @@ struct TreeForm {
   bool shared;
   int columns, unit, per_cu;  // columns of a tile, tokens of a unit, workgroups a CU
 };
-TreeForm tree_form(int64_t columns, bool f32, int head_dim) {
+// `near`: rows' offsets fit 32 bits, counted in 16 bytes.
+TreeForm tree_form(int64_t columns, bool f32, int head_dim, bool near) {
   if (f32) return {false, head_dim <= 128 && columns > 16 ? 32 : 16, 64, 2};
-  if (columns <= 16) return {false, 16, 128, 2};
-  return {true, columns <= 64 || head_dim > 128 ? 64 : 128, head_dim <= 128 ? 128 : 64, 1};
+  if (columns <= 16 || !near) return {false, 16, 128, 2};
+  if (head_dim > 128) return {true, 64, 32, 2};
+  return {true, columns <= 64 ? 64 : 128, 64, 2};
 }
 
 }  // namespace
@@ -1041,11 +1164,15 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
   const int group = heads / cache->kv_heads;
   if (T * group >= (int64_t{1} << 31)) return fail(ctx, TMH_ERR_UNSUPPORTED, "attention over too many rows at once");
   const bool f32 = cache->dtype == TMH_F32;
-  const TreeForm form = tree_form((T * group + B - 1) / B, f32, cache->head_dim);
+  const unsigned __int128 last_row = static_cast<unsigned __int128>(cache->pages - 1) * cache->page_stride +
+                                     static_cast<unsigned __int128>(cache->page_size - 1) * cache->token_stride;
+  const bool near = last_row / 8 < (uint64_t{1} << 32) - 1;
+  const TreeForm form = tree_form((T * group + B - 1) / B, f32, cache->head_dim, near);
   const int64_t unit = form.unit;
   const int64_t most = max_pages * cache->page_size;
   const int64_t items = (T * group / form.columns + B) * cache->kv_heads;
-  if ((most + unit - 1) / unit >= (int64_t{1} << 31) / items)
+  const int64_t each = (most + unit - 1) / unit + kItem;  // of an item
+  if (each >= (int64_t{1} << 31) / items)
     return fail(ctx, TMH_ERR_UNSUPPORTED, "attention over too many rows and tokens at once");
   TreeArgs p;
   p.q = d_q;
@@ -1082,15 +1209,15 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if constexpr (DT == DT_F32) {
-      if (cache->head_dim <= 64) form.columns == 16 ? launch_tree<DT, 1, 1>(p, s) : launch_tree<DT, 1, 2>(p, s);
-      else if (cache->head_dim <= 128) form.columns == 16 ? launch_tree<DT, 2, 1>(p, s) : launch_tree<DT, 2, 2>(p, s);
-      else launch_tree<DT, 4, 1>(p, s);
+      if (cache->head_dim <= 64) form.columns == 16 ? launch_tree<DT, 1, 1>(p, items, s) : launch_tree<DT, 1, 2>(p, items, s);
+      else if (cache->head_dim <= 128) form.columns == 16 ? launch_tree<DT, 2, 1>(p, items, s) : launch_tree<DT, 2, 2>(p, items, s);
+      else launch_tree<DT, 4, 1>(p, items, s);
     } else if (cache->head_dim <= 128) {
-      if (!form.shared) launch_tree<DT, 1, 1>(p, s);
-      else form.columns == 64 ? launch_shared<DT, 1, 1>(p, s) : launch_shared<DT, 1, 2>(p, s);
+      if (!form.shared) launch_tree<DT, 1, 1>(p, items, s);
+      else form.columns == 64 ? launch_shared<DT, 1, 2, 2>(p, items, s) : launch_shared<DT, 1, 4, 1>(p, items, s);
     } else {
-      if (!form.shared) launch_tree<DT, 2, 1>(p, s);
-      else launch_shared<DT, 2, 1>(p, s);
+      if (!form.shared) launch_tree<DT, 2, 1>(p, items, s);
+      else launch_shared<DT, 2, 2, 1>(p, items, s);
     }
   };
   if (cache->dtype == TMH_F32) launch(std::integral_constant<int, DT_F32>{});

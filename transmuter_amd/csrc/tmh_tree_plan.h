@@ -74,4 +74,32 @@ TMH_HD int chain_begin(int node, int prefix, int window) {
   return end > window ? end - window : 0;
 }
 
+// How the work is shared out. An item, one kv head's tile of columns over all units of its sequence, counts as kItem units more
+// than it has, ahead of them: the way in (its queries, masks and first rows, one after another from memory) and out. All items lie
+// in order and are cut into equal runs, one a worker, which so may begin or end within what only counts. What a worker has of an
+// item that it does not have whole is a part, of which it keeps two at most: in place 2 w one that does not begin the item, in
+// 2 w + 1 one that does.
+constexpr uint32_t kItem = 4;
+TMH_HD uint32_t work_of(const Draft& d) {  // of one kv head
+  return d.units ? (static_cast<uint32_t>(d.units) + kItem) * static_cast<uint32_t>(d.tiles) : 0;
+}
+// The units [from, to) of an item whose work begins at `first` that lie in [at, stop) (none: from >= to).
+struct Share {
+  uint32_t from, to;
+};
+TMH_HD Share share_of(uint32_t first, uint32_t units, uint32_t at, uint32_t stop) {
+  const uint32_t begin = first + kItem, end = begin + units;
+  const uint32_t from = at > begin ? at : begin, to = stop < end ? stop : end;
+  return {from - begin, to > begin ? to - begin : 0};
+}
+TMH_HD uint32_t place_of_part(uint32_t worker, bool begins) { return 2 * worker + (begins ? 1 : 0); }
+// The parts of an item: those of the workers `from` .. `from + count - 1` (count 1: the worker has it whole).
+struct TreeParts {
+  uint32_t from, count;
+};
+TMH_HD TreeParts tree_parts(uint32_t first, uint32_t units, uint32_t per) {
+  const uint32_t from = (first + kItem) / per;
+  return {from, (first + kItem + units - 1) / per - from + 1};
+}
+
 }  // namespace tmh

@@ -23,6 +23,8 @@ struct TreeArgs {
   void* y;
   float* part;    // [2 workers][columns of a tile][head_dim], then their (maximum, sum) pairs
   float2* stats;
+  uint32_t part_bytes, stats_bytes;
+  uint32_t* meet;  // [workers] parts of the item that begins in a worker, kept so far; zero between calls
   int64_t ldq, ldy, max_pages, rows, most;  // most: max_pages * page_size
   PageShape cache;
   int64_t head_stride;
@@ -51,29 +53,21 @@ __device__ __forceinline__ uint32_t all_work(const TreeArgs& p) {
   return __builtin_amdgcn_readfirstlane(n);  // (known to be the same in all lanes, as what follows from it then is)
 }
 
-// The sequence whose work (BY_ITEM: whose items of one kv head) holds `target`, which is below the total, and the work (before:
-// and the items) ahead of it.
-template <int UT, int M, bool BY_ITEM = false>
-__device__ __forceinline__ int find_draft(const TreeArgs& p, uint32_t target, uint32_t& before, uint32_t* items = nullptr) {
+// The sequence whose work holds `target`, and the work before it.
+template <int UT, int M>
+__device__ __forceinline__ int find_draft(const TreeArgs& p, uint32_t target, uint32_t& before) {
   const int lane = threadIdx.x & 63;
-  uint32_t base = 0, item_base = 0;
+  uint32_t base = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    uint32_t mine = 0, tiles = 0;
-    if (b0 + lane < p.B) {
-      const Draft d = draft_at<UT, M>(p, b0 + lane);
-      mine = work_of(d);
-      tiles = mine ? static_cast<uint32_t>(d.tiles) : 0;
-    }
-    const uint32_t sum = scan64(mine), item_sum = BY_ITEM ? scan64(tiles) : 0;
-    const uint64_t past = __ballot(BY_ITEM ? item_base + item_sum > target : base + sum > target);
+    const uint32_t mine = b0 + lane < p.B ? work_at<UT, M>(p, b0 + lane) : 0;
+    const uint32_t sum = scan64(mine);
+    const uint64_t past = __ballot(base + sum > target);
     if (past) {
       const int at = __builtin_ctzll(past);
       before = base + __builtin_amdgcn_readlane(sum - mine, at);
-      if (BY_ITEM) *items = item_base + __builtin_amdgcn_readlane(item_sum - tiles, at);
       return b0 + at;
     }
     base += __builtin_amdgcn_readlane(sum, 63);
-    if (BY_ITEM) item_base += __builtin_amdgcn_readlane(item_sum, 63);
   }
   before = base;
   return p.B;  // (target is not below the total)
@@ -86,6 +80,110 @@ struct Place {
 __device__ __forceinline__ Place place_in(const Draft& d, uint32_t before, uint32_t at) {
   const uint32_t each = static_cast<uint32_t>(d.units) + kItem, item = (at - before) / each;
   return {item, before + item * each};
+}
+
+// Parts of items that several workers shared. Each worker leaves its part in memory (stores that pass the XCD's own L2), then counts
+// itself; the one that finds all others counted joins the parts, in their order, whoever it is. Items of more than MOST parts, which
+// would keep one workgroup too long, are left to a second kernel (join_most: half a MiB of parts).
+constexpr int kThrough = 16;                // sc1 of a buffer access: past the XCD's L2, to where all XCDs meet
+constexpr uint32_t kNowhere = 0xFFFFFFF0u;  // an offset past every buffer's range here
+constexpr uint32_t join_most(int columns, int blocks) { return 1024u / (columns * blocks); }
+
+__device__ __forceinline__ void put_part(const TreeArgs& p, uint32_t quad, float4_t v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uint4_t, v), buffer_rsrc(p.part, p.part_bytes), quad * 16, 0, kThrough);
+}
+__device__ __forceinline__ void put_stats(const TreeArgs& p, uint32_t at, float top, float total) {
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uint2_t, make_float2(top, total)), buffer_rsrc(p.stats, p.stats_bytes), at * 8, 0, kThrough);
+}
+template <int AUX>
+__device__ __forceinline__ float4_t get_part(const TreeArgs& p, uint32_t quad, bool there) {
+  return __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(buffer_rsrc(p.part, p.part_bytes), there ? quad * 16 : kNowhere, 0, AUX));
+}
+template <int AUX>
+__device__ __forceinline__ float2 get_stats(const TreeArgs& p, uint32_t at, bool there) {
+  return __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(buffer_rsrc(p.stats, p.stats_bytes), there ? at * 8 : kNowhere, 0, AUX));
+}
+
+// Whether this worker is the last of an item's to have left its part. (As k_paged_attention counts: this thread's stores have arrived,
+// then everybody's, then the count.)
+__device__ __forceinline__ bool last_of(const TreeArgs& p, const TreeParts& parts) {
+  __shared__ uint32_t others;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    others = __hip_atomic_fetch_add(p.meet + parts.from, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (others == parts.count - 1) __hip_atomic_store(p.meet + parts.from, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return others == parts.count - 1;
+}
+
+// The sum of parts k = first, first + step, ..: QUADS quads of a lane each, at quads quad_at(place of the part, i), with the statistics
+// at stats_at(place of the part); four parts on their way at once. AUX: kThrough where other
+// workgroups of the same kernel have written them.
+template <int AUX, int QUADS, typename QuadAt, typename StatsAt>
+__device__ __forceinline__ void join_parts(const TreeArgs& p, const TreeParts& parts, uint32_t first, uint32_t step, float4_t (&acc)[QUADS], float& top,
+                                           float& total, QuadAt quad_at, StatsAt stats_at) {
+  constexpr int BATCH = 4;
+  top = kNone;
+  total = 0.f;
+#pragma unroll
+  for (int i = 0; i < QUADS; ++i) acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (uint32_t k0 = first; k0 < parts.count; k0 += BATCH * step) {
+    float2 st[BATCH];
+    float4_t o[BATCH][QUADS];
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {  // (what a batch has too many lies past the buffers' ranges: zeros)
+      const uint32_t k = k0 + b * step, place = place_of_part(parts.from + k, k == 0);
+      const bool there = k < parts.count;
+      st[b] = get_stats<AUX>(p, stats_at(place), there);
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) o[b][i] = get_part<AUX>(p, quad_at(place, i), there);
+    }
+    float next = top;
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      if (k0 + b * step >= parts.count) st[b].x = kNone;
+      next = fmaxf(next, st[b].x);
+    }
+    const float keep = top == next ? 1.f : __builtin_amdgcn_exp2f(top - next);
+    top = next;
+    total *= keep;
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) acc[i] *= keep;
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const float f = st[b].x == top ? 1.f : __builtin_amdgcn_exp2f(st[b].x - top);
+      total += f * st[b].y;
+#pragma unroll
+      for (int i = 0; i < QUADS; ++i) acc[i] += f * o[b][i];
+    }
+  }
+}
+
+// The item of more than MOST parts, if there is one, whose first part is one of the workers MOST index .. MOST index + MOST - 1's: it
+// is what the next such run of workers begins with.
+struct Joined {
+  Draft d;
+  TreeParts parts;
+  int kv_head, tile;
+};
+template <int UT, int M, uint32_t MOST>
+__device__ __forceinline__ bool find_joined(const TreeArgs& p, uint32_t index, Joined& j) {
+  const uint32_t all = all_work<UT, M>(p) * p.kv_heads, per = units_per_worker(all, p.workers);
+  const uint32_t cut = MOST * (index + 1) * per;
+  if (per == 0 || cut >= all) return false;
+  uint32_t before;
+  const int b = find_draft<UT, M>(p, cut / p.kv_heads, before);
+  if (b >= p.B) return false;
+  j.d = draft_at<UT, M>(p, b);
+  const Place place = place_in(j.d, before * p.kv_heads, cut);
+  if (place.item >= static_cast<uint32_t>(j.d.tiles * p.kv_heads)) return false;
+  j.parts = tree_parts(place.first, static_cast<uint32_t>(j.d.units), per);
+  j.kv_head = static_cast<int>(place.item) / j.d.tiles;
+  j.tile = static_cast<int>(place.item) % j.d.tiles;
+  return j.parts.count > MOST && j.parts.from / MOST == index && j.parts.from + j.parts.count <= p.workers;
 }
 
 template <int DT>
@@ -192,6 +290,17 @@ __device__ __forceinline__ void each_alone(const TreeArgs& p, const Draft& d, co
     if (tid == 0) total(c, top, sum);
   }
   __syncthreads();
+}
+
+// Four dimensions of one column of an item whose parts are rows.
+template <int AUX, int DT, int M>
+__device__ __forceinline__ void join_item(const TreeArgs& p, const Draft& d, const TreeParts& parts, int kv_head, int tile, int c, int quad, int quads) {
+  float4_t o[1];
+  float top, total;
+  join_parts<AUX, 1>(p, parts, 0, 1, o, top, total, [&](uint32_t place, int) { return (place * M + c) * quads + quad; }, [&](uint32_t place) { return place * M + c; });
+  const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
+  store_answer<DT>(p, d.row + n, kv_head * p.group + of_all - n * p.group, 4 * quad,
+                   total == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o[0] * (1.f / total));
 }
 
 // A tile of M = 16 CB columns (a column: one query head of one node) over a run of units of its sequence's tokens, four
@@ -476,6 +585,14 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
 
     const bool whole = from == 0 && to == static_cast<uint32_t>(d.units);
     const uint32_t slot = place_of_part(worker, from == 0);
+    const TreeParts all_parts = tree_parts(place.first, static_cast<uint32_t>(d.units), per);
+    auto join_here = [&] {
+      if (whole || all_parts.count > join_most(M, 1) || !last_of(p, all_parts)) return;
+      for (int i = threadIdx.x; i < columns * quads; i += 256) {
+        const int c = i / quads, quad = i - c * quads;
+        join_item<kThrough, DT, M>(p, d, all_parts, kv_head, tile, c, quad, quads);
+      }
+    };
     if (__syncthreads_or(alone)) {
       each_alone<DT, 256>(
           p, d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),
@@ -488,6 +605,8 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
           [&](int c, float top, float sum) {
             if (!whole) p.stats[static_cast<int64_t>(slot) * M + c] = make_float2(top, sum);
           });
+      __threadfence();  // (these stores went by the XCD's L2)
+      join_here();
       continue;
     }
     // The wavefronts' parts of the item meet in LDS, sixteen columns at a time.
@@ -528,97 +647,27 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
           for (int e = 0; e < 4; ++e) y[e] = total == 0.f ? 0.f : y[e];  // (0 * an infinity is none)
           store_answer<DT>(p, d.row + n, kv_head * p.group + of_all - n * p.group, dim, y);
         } else {
-          const int64_t row = static_cast<int64_t>(slot) * M + 16 * cb + c;
-          *reinterpret_cast<float4_t*>(p.part + row * p.head_dim + dim) = o;
-          if (dim == 0) p.stats[row] = make_float2(top, total);
+          const uint32_t row = slot * M + 16 * cb + c;
+          put_part(p, row * quads + dim / 4, o);
+          if (dim == 0) put_stats(p, row, top, total);
         }
       }
       __syncthreads();
     }
+    join_here();
   }
 }
 
-// An item that several workers shared, for the workgroups that join its parts: the `index`-th of all items (BY_ITEM), or the one that
-// begins in worker `index` and goes on in the next. False where there is none.
-struct Joined {
-  Draft d;
-  TreeParts parts;
-  int kv_head, tile;
-};
-template <int UT, int M, bool BY_ITEM>
-__device__ __forceinline__ bool find_joined(const TreeArgs& p, uint32_t index, Joined& j) {
-  const uint32_t all = all_work<UT, M>(p) * p.kv_heads, per = units_per_worker(all, p.workers);
-  if (per == 0) return false;
-  uint32_t before, items = 0, item, first;
-  if constexpr (BY_ITEM) {
-    const int b = find_draft<UT, M, true>(p, index / p.kv_heads, before, &items);
-    if (b >= p.B) return false;
-    j.d = draft_at<UT, M>(p, b);
-    item = index - items * p.kv_heads;
-    first = before * p.kv_heads + item * (static_cast<uint32_t>(j.d.units) + kItem);
-  } else {
-    const uint32_t cut = (index + 1) * per;  // where the next worker begins
-    if (cut >= all) return false;
-    const int b = find_draft<UT, M>(p, cut / p.kv_heads, before);
-    if (b >= p.B) return false;
-    j.d = draft_at<UT, M>(p, b);
-    const Place place = place_in(j.d, before * p.kv_heads, cut);
-    item = place.item;
-    first = place.first;
-  }
-  if (item >= static_cast<uint32_t>(j.d.tiles * p.kv_heads)) return false;
-  j.parts = tree_parts(first, static_cast<uint32_t>(j.d.units), per);
-  j.kv_head = static_cast<int>(item) / j.d.tiles;
-  j.tile = static_cast<int>(item) % j.d.tiles;
-  return j.parts.count > 1 && j.parts.from + j.parts.count <= p.workers && (BY_ITEM || j.parts.from == index);
-}
-
-// The parts of an item that several workers shared (find_joined): workgroup (index, i) sees to columns 16 i .. 16 i + 15, a thread to
-// four dimensions of one, four parts on their way at once.
-template <int DT, int M, bool BY_ITEM>
+// Items of many parts (find_joined): workgroup (i, index) sees to columns 16 i .. 16 i + 15.
+template <int DT, int M>
 __global__ __launch_bounds__(256) void k_tree_join(TreeArgs p) {
-  constexpr int UT = DT == DT_F32 ? 64 : 128, BATCH = 4;
+  constexpr int UT = DT == DT_F32 ? 64 : 128;
   Joined j;
-  if (!find_joined<UT, M, BY_ITEM>(p, blockIdx.x, j)) return;
-  const TreeParts parts = j.parts;
-  const int first_column = 16 * blockIdx.y, some = min(16, min(M, j.d.nodes * p.group - j.tile * M) - first_column);
-  const int quads = p.head_dim / 4;
+  if (!find_joined<UT, M, join_most(M, 1)>(p, blockIdx.y, j)) return;
+  const int first_column = 16 * blockIdx.x, some = min(16, min(M, j.d.nodes * p.group - j.tile * M) - first_column), quads = p.head_dim / 4;
   for (int i = threadIdx.x; i < some * quads; i += 256) {
-    const int c = first_column + i / quads, dim = (i % quads) * 4;
-    float top = kNone, total = 0.f;
-    float4_t o{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t k0 = 0; k0 < parts.count; k0 += BATCH) {
-      float2 st[BATCH];
-      float4_t po[BATCH];
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k) {  // (too many: the first again, without a weight)
-        const bool there = k0 + k < parts.count;
-        const uint32_t at = there ? k0 + k : k0;
-        const int64_t row = static_cast<int64_t>(place_of_part(parts.from + at, at == 0)) * M + c;
-        st[k] = p.stats[row];
-        po[k] = *reinterpret_cast<const float4_t*>(p.part + row * p.head_dim + dim);
-        if (!there) {
-          st[k] = make_float2(kNone, 0.f);
-          po[k] = float4_t{0.f, 0.f, 0.f, 0.f};
-        }
-      }
-      float next = top;
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k) next = fmaxf(next, st[k].x);
-      const float keep = top == next ? 1.f : __builtin_amdgcn_exp2f(top - next);
-      top = next;
-      total *= keep;
-      o *= keep;
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        const float f = st[k].x == top ? 1.f : __builtin_amdgcn_exp2f(st[k].x - top);
-        total += f * st[k].y;
-        o += f * po[k];
-      }
-    }
-    const int of_all = j.tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
-    store_answer<DT>(p, j.d.row + n, j.kv_head * p.group + of_all - n * p.group, dim,
-                     total == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / total));
+    const int c = i / quads;
+    join_item<0, DT, M>(p, j.d, j.parts, j.kv_head, j.tile, first_column + c, i - c * quads, quads);
   }
 }
 
@@ -678,6 +727,14 @@ __device__ __forceinline__ void answer_column(const TreeArgs& p, const Draft& d,
 __device__ __forceinline__ void quads_of(const float16_t& v, float4_t (&q)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) q[i] = float4_t{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+}
+
+// 32 dimensions (block db) of 32 columns (wc) of an item whose parts lie lane by lane.
+template <int AUX, int DB, int WC>
+__device__ __forceinline__ void join_block(const TreeArgs& p, const TreeParts& parts, int wc, int db, int lane, uint32_t first, uint32_t step, float4_t (&o)[4],
+                                           float& top, float& total) {
+  join_parts<AUX, 4>(p, parts, first, step, o, top, total, [&](uint32_t place, int i) { return ((place * WC + wc) * (4 * DB) + 4 * db + i) * 64 + lane; },
+                [&](uint32_t place) { return place * (32 * WC) + 32 * wc + (lane & 31); });
 }
 
 // What tokens that are none bring to LDS.
@@ -943,7 +1000,18 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
     }
 
     const bool whole = from == 0 && to == static_cast<uint32_t>(d.units);
-    const int64_t slot = place_of_part(worker, from == 0);
+    const uint32_t slot = place_of_part(worker, from == 0);
+    const TreeParts parts = tree_parts(place.first, static_cast<uint32_t>(d.units), per);
+    auto join_here = [&] {
+      if (whole || parts.count > join_most(M, NB) || !last_of(p, parts)) return;
+      for (int i = wave; i < WC * DB; i += WC * WT)
+        if (32 * (i / DB) < columns && 32 * (i % DB) < p.head_dim) {
+          float4_t o[4];
+          float top, total;
+          join_block<kThrough, DB, WC>(p, parts, i / DB, i % DB, lane, 0, 1, o, top, total);
+          if (32 * (i / DB) + col < columns) answer_column<DT>(p, d, kv_head, tile * M + 32 * (i / DB) + col, 32 * (i % DB) + 4 * h, o, total);
+        }
+    };
     // An infinity or a NaN in V leaves a NaN in every column of its products, whether the column sees it or not (0 times an
     // infinity): such an item is done again.
     bool alone = false;
@@ -961,12 +1029,14 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
           [&](int c, int dim, float o, float sum) {
             const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
             if (whole) store_as<DT>(p.y, (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + of_all - n * p.group) * p.head_dim + dim, sum == 0.f ? 0.f : o * (1.f / sum));
-            else p.part[(((slot * WC + c / 32) * (4 * DB) + dim / 8) * 64 + dim / 4 % 2 * 32 + c % 32) * 4 + dim % 4] = o;
+            else p.part[static_cast<int64_t>(((slot * WC + c / 32) * (4 * DB) + dim / 8) * 64 + dim / 4 % 2 * 32 + c % 32) * 4 + dim % 4] = o;
           },
           [&](int c, float top, float sum) {
             if (!whole) p.stats[slot * M + c] = make_float2(top, sum);
           });
       clear();
+      __threadfence();  // (these stores went by the XCD's L2)
+      join_here();
       continue;
     }
 
@@ -1014,105 +1084,70 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
           if (32 * wc + col < columns) answer_column<DT>(p, d, kv_head, tile * M + 32 * wc + col, 32 * db + 4 * h, four, total);
         }
       } else {
-        float4_t* part = reinterpret_cast<float4_t*>(p.part) + (slot * WC + wc) * (4 * DB) * 64 + lane;
 #pragma unroll
         for (int i = 0; i < 4 * DB; ++i)
-          part[i * 64] = float4_t{acc[i / 4][i % 4 * 4], acc[i / 4][i % 4 * 4 + 1], acc[i / 4][i % 4 * 4 + 2], acc[i / 4][i % 4 * 4 + 3]};
-        if (h == 0) p.stats[slot * M + 32 * wc + col] = make_float2(top == kNone ? kNone : top * a, total);
+          put_part(p, ((slot * WC + wc) * (4 * DB) + i) * 64 + lane, float4_t{acc[i / 4][i % 4 * 4], acc[i / 4][i % 4 * 4 + 1], acc[i / 4][i % 4 * 4 + 2], acc[i / 4][i % 4 * 4 + 3]});
+        if (h == 0) put_stats(p, slot * M + 32 * wc + col, top == kNone ? kNone : top * a, total);
       }
     }
+    join_here();
   }
 }
 
-// The parts of an item that several workers shared (find_joined): workgroup (index, wc, z) sees to columns 32 wc .. 32 wc + 31 and
-// dimensions 128 z .. 128 z + 127, four wavefronts to each 32 of these, each to every fourth part, four of them on their way at once.
-template <int DT, int NB, int WC, bool BY_ITEM>
-__global__ __launch_bounds__(1024) void k_tree_shared_join(TreeArgs p) {
-  constexpr int UT = 64 / NB, M = 32 * WC, BATCH = 4;
-  __shared__ __align__(16) float4_t sums[4][3][4][64];
-  __shared__ float2 stats[4][3][64];
+// Items of many parts (find_joined): workgroup (wc, db, index) sees to 32 dimensions of 32 columns, its wavefronts to every fourth part.
+// (The index last: workgroups go to the XCDs in turn, and items of one length begin in workers that many apart. By index first all of the
+// work was one XCD's, 21 us for 8 items of 64 parts.)
+template <int DT, int NB, int WC>
+__global__ __launch_bounds__(256) void k_tree_shared_join(TreeArgs p) {
+  constexpr int UT = 64 / NB, M = 32 * WC;
+  __shared__ __align__(16) float4_t sums[3][4][64];
+  __shared__ float2 stats[3][64];
   Joined j;
-  if (!find_joined<UT, M, BY_ITEM>(p, blockIdx.x, j)) return;
-  const TreeParts parts = j.parts;
-  auto slot_of = [&](uint32_t k) { return static_cast<int64_t>(place_of_part(parts.from + k, k == 0)); };
-  const int wc = blockIdx.y, columns = min(M, j.d.nodes * p.group - j.tile * M);
-  if (32 * wc >= columns) return;
+  if (!find_joined<UT, M, join_most(M, NB)>(p, blockIdx.z, j)) return;
+  const int wc = blockIdx.x, db = blockIdx.y, columns = min(M, j.d.nodes * p.group - j.tile * M);
+  if (32 * wc >= columns || 32 * db >= p.head_dim) return;
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = wave & 3, quarter = wave >> 2;
-  const int db = 4 * blockIdx.z + quarter;
-  float top = kNone, total = 0.f;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float4_t acc[4];
+  float top, total;
+  join_block<0, 4 * NB, WC>(p, j.parts, wc, db, lane, wave, 4, acc, top, total);
+  if (wave) {
+    stats[wave - 1][lane] = make_float2(top, total);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) acc[q] = float4_t{0.f, 0.f, 0.f, 0.f};
-  for (uint32_t k0 = mine; k0 < parts.count; k0 += 4 * BATCH) {
-    float2 st[BATCH];
-    float4_t o[BATCH][4];
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) {  // (too many: the first again, without a weight)
-      const bool there = k0 + 4 * k < parts.count;
-      const int64_t slot = slot_of(there ? k0 + 4 * k : k0);
-      st[k] = p.stats[slot * M + 32 * wc + col];
-      if (!there) st[k] = make_float2(kNone, 0.f);
-      const float4_t* part = reinterpret_cast<const float4_t*>(p.part) + ((slot * WC + wc) * (16 * NB) + 4 * db) * 64 + lane;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) o[k][q] = part[q * 64];
-    }
-    float next = top;
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) next = fmaxf(next, st[k].x);
-    const float keep = top == next ? 1.f : __builtin_amdgcn_exp2f(top - next);
-    top = next;
-    total *= keep;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) acc[q] *= keep;
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) {
-      if (k0 + 4 * k >= parts.count) continue;
-      const float f = st[k].x == top ? 1.f : __builtin_amdgcn_exp2f(st[k].x - top);
-      total += f * st[k].y;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) acc[q] += f * o[k][q];
-    }
-  }
-  if (mine) {
-    stats[quarter][mine - 1][lane] = make_float2(top, total);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) sums[quarter][mine - 1][q][lane] = acc[q];
+    for (int q = 0; q < 4; ++q) sums[wave - 1][q][lane] = acc[q];
   }
   __syncthreads();
-  if (mine) return;
+  if (wave) return;
   float most = top;
 #pragma unroll
-  for (int w = 0; w < 3; ++w) most = fmaxf(most, stats[quarter][w][lane].x);
+  for (int w = 0; w < 3; ++w) most = fmaxf(most, stats[w][lane].x);
   const float keep = top == most ? 1.f : __builtin_amdgcn_exp2f(top - most);
   total *= keep;
 #pragma unroll
   for (int q = 0; q < 4; ++q) acc[q] *= keep;
 #pragma unroll
   for (int w = 0; w < 3; ++w) {
-    const float2 st = stats[quarter][w][lane];
+    const float2 st = stats[w][lane];
     const float f = st.x == most ? 1.f : __builtin_amdgcn_exp2f(st.x - most);
     total += f * st.y;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) acc[q] += f * sums[quarter][w][q][lane];
+    for (int q = 0; q < 4; ++q) acc[q] += f * sums[w][q][lane];
   }
   if (32 * wc + col < columns) answer_column<DT>(p, j.d, j.kv_head, j.tile * M + 32 * wc + col, 32 * db + 4 * h, acc, total);
 }
 
-// Items that several workers shared are found among all items, or among the workers' ends, whichever are fewer.
+// (`units`: of an item, as far as the host knows. Without items of many parts there is nothing for the second kernel to do.)
 template <int DT, int NB, int CB>
-void launch_tree(const TreeArgs& p, int64_t items, hipStream_t s) {
+void launch_tree(const TreeArgs& p, int64_t units, hipStream_t s) {
+  constexpr uint32_t MOST = join_most(16 * CB, 1);
   k_tree_attention<DT, NB, CB><<<p.workers, 256, 0, s>>>(p);
-  if (p.workers == 1) return;
-  if (items < p.workers) k_tree_join<DT, 16 * CB, true><<<dim3(static_cast<unsigned>(items), CB), 256, 0, s>>>(p);
-  else k_tree_join<DT, 16 * CB, false><<<dim3(p.workers - 1, CB), 256, 0, s>>>(p);
+  if (p.workers > MOST && units > MOST) k_tree_join<DT, 16 * CB><<<dim3(CB, p.workers / MOST), 256, 0, s>>>(p);
 }
 template <int DT, int NB, int WC, int WT>
-void launch_shared(const TreeArgs& p, int64_t items, hipStream_t s) {
+void launch_shared(const TreeArgs& p, int64_t units, hipStream_t s) {
+  constexpr uint32_t MOST = join_most(32 * WC, NB);
   k_tree_shared<DT, NB, WC, WT><<<p.workers, 64 * WC * WT, 0, s>>>(p);
-  if (p.workers == 1) return;
-  if (items < p.workers) k_tree_shared_join<DT, NB, WC, true><<<dim3(static_cast<unsigned>(items), WC, NB), 1024, 0, s>>>(p);
-  else k_tree_shared_join<DT, NB, WC, false><<<dim3(p.workers - 1, WC, NB), 1024, 0, s>>>(p);
+  if (p.workers > MOST && units > MOST) k_tree_shared_join<DT, NB, WC><<<dim3(WC, 4 * NB, p.workers / MOST), 256, 0, s>>>(p);
 }
 
 // How columns go to workgroups, by the columns that a sequence has in the mean (all the host knows).
@@ -1171,8 +1206,8 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
   const int64_t unit = form.unit;
   const int64_t most = max_pages * cache->page_size;
   const int64_t items = (T * group / form.columns + B) * cache->kv_heads;
-  const int64_t each = (most + unit - 1) / unit + kItem;  // of an item
-  if (each >= (int64_t{1} << 31) / items)
+  const int64_t units = (most + unit - 1) / unit;  // of an item
+  if (units + kItem >= (int64_t{1} << 31) / items)
     return fail(ctx, TMH_ERR_UNSUPPORTED, "attention over too many rows and tokens at once");
   TreeArgs p;
   p.q = d_q;
@@ -1198,7 +1233,7 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
   p.head_dim = cache->head_dim;
   p.by_group = FastDiv(static_cast<uint32_t>(group));
   p.scale = scale * 1.44269504088896340736f;
-  p.workers = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(form.per_cu * ctx->num_cus, (most + unit - 1) / unit * items)));
+  p.workers = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(form.per_cu * ctx->num_cus, units * items)));
   hipStream_t s = pick_stream(ctx, stream);
   const size_t rows = 2 * static_cast<size_t>(form.per_cu * ctx->num_cus) * form.columns;
   const int width_of_part = form.shared ? (cache->head_dim <= 128 ? 128 : 256) : cache->head_dim;
@@ -1206,18 +1241,21 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
   if (!ws) return fail(ctx, TMH_ERR_UNSUPPORTED, "attention's workspace cannot grow here: run one call before the capture");
   p.part = static_cast<float*>(ws);
   p.stats = reinterpret_cast<float2*>(p.part + rows * width_of_part);
+  p.part_bytes = static_cast<uint32_t>(rows * width_of_part * 4);
+  p.stats_bytes = static_cast<uint32_t>(rows * sizeof(float2));
+  p.meet = ctx->meet;
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if constexpr (DT == DT_F32) {
-      if (cache->head_dim <= 64) form.columns == 16 ? launch_tree<DT, 1, 1>(p, items, s) : launch_tree<DT, 1, 2>(p, items, s);
-      else if (cache->head_dim <= 128) form.columns == 16 ? launch_tree<DT, 2, 1>(p, items, s) : launch_tree<DT, 2, 2>(p, items, s);
-      else launch_tree<DT, 4, 1>(p, items, s);
+      if (cache->head_dim <= 64) form.columns == 16 ? launch_tree<DT, 1, 1>(p, units, s) : launch_tree<DT, 1, 2>(p, units, s);
+      else if (cache->head_dim <= 128) form.columns == 16 ? launch_tree<DT, 2, 1>(p, units, s) : launch_tree<DT, 2, 2>(p, units, s);
+      else launch_tree<DT, 4, 1>(p, units, s);
     } else if (cache->head_dim <= 128) {
-      if (!form.shared) launch_tree<DT, 1, 1>(p, items, s);
-      else form.columns == 64 ? launch_shared<DT, 1, 2, 2>(p, items, s) : launch_shared<DT, 1, 4, 1>(p, items, s);
+      if (!form.shared) launch_tree<DT, 1, 1>(p, units, s);
+      else form.columns == 64 ? launch_shared<DT, 1, 2, 2>(p, units, s) : launch_shared<DT, 1, 4, 1>(p, units, s);
     } else {
-      if (!form.shared) launch_tree<DT, 2, 1>(p, items, s);
-      else launch_shared<DT, 2, 2, 1>(p, items, s);
+      if (!form.shared) launch_tree<DT, 2, 1>(p, units, s);
+      else launch_shared<DT, 2, 2, 1>(p, units, s);
     }
   };
   if (cache->dtype == TMH_F32) launch(std::integral_constant<int, DT_F32>{});

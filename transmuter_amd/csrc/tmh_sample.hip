@@ -1,4 +1,16 @@
 // Tokens drawn from rows of logits by temperature, top-k, top-p, min-p and given random numbers (tmh_sample).
+//
+// A row's weights are whole numbers (units of 2^-44 of the largest), so that sums of them do not depend on an order. Three kernels,
+// each with `slices` workgroups a row, the last of which to finish does what needs the whole row:
+//  k_sample_top   the largest logit.
+//  k_sample_sum   rows that keep all tokens, or those of min-p: the weights of every chunk of tokens, and the draw. Rows by top-k: how
+//                 many tokens lie in each bin (a sixteenth of a factor of two in weight), and down to which bin the k largest reach.
+//                 Others, by top-p alone: the weights of each bin, and the bin in which they reach top-p of the whole.
+//  k_sample_draw  rows by top-k: the tokens down to that bin go to a list. By top-p alone: those of that bin do, and the weights above
+//                 it to chunks. The list, sorted out in LDS, gives the least logit kept and how many of its equals are; then the draw.
+// A list that does not fit (thousands of tokens of almost the same logit) leaves its row to the last workgroup, which goes over all
+// of it a few times.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -9,6 +21,16 @@
 namespace tmh {
 namespace {
 
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kUnit = 44;
+constexpr int kPerOctave = 16, kWeightBins = kPerOctave * kUnit + 4;  // (a few more than have weights: bins are found in f32)
+constexpr int kList = 4096;        // tokens of a row's list
+constexpr int kDigits = 2048;      // of a selection's turn
+constexpr int kMostChunks = (1 << 20) / 256 + 1;
+constexpr int kMostRows = 512;     // of a launch: each has a counter
+
+enum Mode : int { GREEDY, ALL, TOP_K, TOP_P };
+
 struct SampleArgs {
   const void* x;
   const float* temperature;
@@ -18,14 +40,17 @@ struct SampleArgs {
   const float* u;
   int64_t* tokens;
   int64_t ld;
-  int vocabulary;
+  int vocabulary, slices, chunks;  // chunks: of a row
+  // The workspace: of each row and slice the largest logit and its place, the bins and the list with its count; of each row the chunks'
+  // weights and what k_sample_sum tells k_sample_draw.
+  uint64_t* best;    // [rows][slices]
+  uint64_t* bins;    // [rows][slices][kWeightBins]
+  uint64_t* list;    // [rows][slices][kList]
+  uint32_t* counts;  // [rows][slices]
+  uint64_t* sums;    // [rows][chunks]
+  uint64_t* told;    // [rows][4]: border bin, weight above it, weight of all
+  uint32_t* meet;    // [rows] slices that have finished; zero between launches
 };
-
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kUnit = 44;  // weights are multiples of 2^-44 (of the largest's): sums of up to 2^20 of them in 64 bits
-constexpr int kSegment = 512;
-constexpr int kMostSegments = (1 << 20) / kSegment;
-constexpr int kBins = 2048;
 
 // Logits as numbers that order as they do, NaN with -infinity, the lowest.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -37,13 +62,13 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
+constexpr uint32_t kLowestKey = 0x007FFFFFu;  // of -infinity
 
-// 2^x, x <= 0, in 64 bits: 2^n e^y with y = (x - n) ln 2 of magnitude up to 0.35, whose series ends with y^12 / 12! (the
-// next term is 2^-52).
+// 2^x, x <= 0, in 64 bits: 2^n e^y with y = (x - n) ln 2 of magnitude up to 0.35, whose series ends with y^11 / 11! (the
+// next term is 2^-47, an eighth of a unit).
 __device__ __forceinline__ double exp2_of(double x) {
   const double n = __builtin_rint(x), y = (x - n) * 0.69314718055994530942;
-  double s = 1.0 / 479001600.0;
-  s = fma(s, y, 1.0 / 39916800.0);
+  double s = 1.0 / 39916800.0;
   s = fma(s, y, 1.0 / 3628800.0);
   s = fma(s, y, 1.0 / 362880.0);
   s = fma(s, y, 1.0 / 40320.0);
@@ -58,17 +83,36 @@ __device__ __forceinline__ double exp2_of(double x) {
   return __builtin_amdgcn_ldexp(s, static_cast<int>(n));
 }
 
-struct Weigh {
-  float top;  // the row's largest logit
-  double c;   // log2(e) / temperature
-  double least;
-  // exp((x - top) / temperature) in units of 2^-44; 0 where it is less than one, or less than `least`.
-  __device__ __forceinline__ uint64_t operator()(float x) const {
+// What a row's WG knows of its row.
+struct Row {
+  Mode mode;
+  int k;
+  float top;          // the largest logit
+  uint32_t top_key, top_index;
+  double c;           // log2(e) / temperature
+  float per_bin;      // bins a logit
+  double top_p, least;  // least: the smallest weight that min-p keeps
+  float u;
+  // exp((x - top) / temperature) in units of 2^-44; 0 where it is less than one.
+  __device__ __forceinline__ uint64_t weight(float x) const {
+    if (top == __builtin_inff()) return x == top ? uint64_t{1} << kUnit : 0;
+    const double e = (static_cast<double>(x) - static_cast<double>(top)) * c;
+    if (!(e >= -kUnit)) return 0;
+    return static_cast<uint64_t>(__builtin_rint(exp2_of(e) * 0x1p44));
+  }
+  // The same, 0 where min-p leaves the token out.
+  __device__ __forceinline__ uint64_t kept_weight(float x) const {
     if (top == __builtin_inff()) return x == top ? uint64_t{1} << kUnit : 0;
     const double e = (static_cast<double>(x) - static_cast<double>(top)) * c;
     if (!(e >= -kUnit)) return 0;
     const double w = exp2_of(e);
     return w >= least ? static_cast<uint64_t>(__builtin_rint(w * 0x1p44)) : 0;
+  }
+  // The bin of a logit: of the largest 0, kWeightBins and more where it has no weight. Not falling as logits fall.
+  __device__ __forceinline__ int bin(float x) const {
+    if (!(x > -__builtin_inff())) return kWeightBins;
+    if (x == top) return 0;
+    return static_cast<int>(fminf((top - x) * per_bin, static_cast<float>(kWeightBins)));
   }
 };
 
@@ -91,198 +135,517 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
   }
   return v;
 }
+__device__ __forceinline__ void put64(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t get64(const uint64_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// One workgroup a row. Weights are whole numbers, so that their sums do not depend on an order.
+// A row in chunks of 64 E tokens, a wavefront's 16 bytes a lane; chunk 0 begins with the 16 bytes that the row's first token lies in.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void k_sample(SampleArgs p, int64_t first) {
-  __shared__ uint64_t bins[kBins];
-  __shared__ uint64_t red[kWaves];
-  __shared__ uint64_t seg_sum[kMostSegments];
-  __shared__ uint32_t seg_ties[kMostSegments];
-  __shared__ uint64_t found[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = p.vocabulary;
-  const int64_t row = first + blockIdx.x;
-  const int64_t base = row * p.ld;
-  auto logit = [&](int i) { return load_as_f32<DT>(p.x, base + i); };
-  auto block = [&](uint64_t v, auto join) {  // (all threads)
-    __syncthreads();
-    if (lane == 0) red[wave] = v;
-    __syncthreads();
-    uint64_t all = red[0];
-    for (int w = 1; w < kWaves; ++w) all = join(all, red[w]);
-    return all;
-  };
-  // The largest logit, and of equal ones the first.
-  uint64_t best = 0;
-  for (int i = tid; i < n; i += kThreads) best = max(best, static_cast<uint64_t>(key_of(logit(i))) << 32 | static_cast<uint32_t>(~i));
-  best = block(wave_max(best), [](uint64_t a, uint64_t b) { return max(a, b); });
-  const uint32_t top_key = static_cast<uint32_t>(best >> 32);
-  const float temperature = p.temperature ? p.temperature[row] : 1.f;
-  if (top_key == key_of(-__builtin_inff())) {  // no token
-    if (tid == 0) p.tokens[row] = -1;
-    return;
+struct Chunks {
+  static constexpr int E = DT == DT_F32 ? 4 : 8, SIZE = DT == DT_F32 ? 4 : 2;
+  const char* row;  // chunk 0
+  int before, n;    // places of chunk 0 ahead of the row, tokens
+  __device__ Chunks(const SampleArgs& p, int64_t r) : n(p.vocabulary) {
+    const char* first = static_cast<const char*>(p.x) + r * p.ld * SIZE;
+    before = static_cast<int>(reinterpret_cast<uintptr_t>(first) % 16) / SIZE;
+    row = first - before * SIZE;
   }
-  if (!(temperature > 0.f)) {
-    if (tid == 0) p.tokens[row] = static_cast<uint32_t>(~best);
-    return;
-  }
-  Weigh weigh{value_of(top_key), 1.4426950408889634074 / static_cast<double>(temperature), 0.0};
-
-  // Kept are the keys above `edge`, and the first `ties` tokens of that key.
-  uint32_t edge = 0;
-  uint64_t ties = ~uint64_t{0};
-  // The key at which the sum of measure(key) over kept keys, from the largest down, reaches `need`, and the sum above it.
-  auto select = [&](auto measure, auto reached, uint64_t& above) {
-    uint32_t prefix = 0, mask = 0;
-    above = 0;
-#pragma unroll 1
-    for (int shift : {21, 10, 0}) {
-      const uint32_t digits = shift ? 2047u : 1023u;
-      __syncthreads();
-      for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < n; i += kThreads) {
-        const uint32_t key = key_of(logit(i));
-        if (key < edge || (key & mask) != prefix) continue;
-        atomicAdd(reinterpret_cast<unsigned long long*>(&bins[key >> shift & digits]), static_cast<unsigned long long>(measure(key)));
+  // The lane's first token of chunk q (its E tokens may begin before 0 or end past n).
+  __device__ __forceinline__ int token(int q) const { return (q * 64 + static_cast<int>(threadIdx.x & 63)) * E - before; }
+  __device__ __forceinline__ uint4_t raw(int q) const {
+    const int t = token(q);
+    if (t >= 0 && t + E <= n) return *reinterpret_cast<const uint4_t*>(row + static_cast<int64_t>(t + before) * SIZE);
+    uint4_t v = uint4_t{0u, 0u, 0u, 0u};  // (16 bytes that are not all the row's: one token after another)
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (t + e >= 0 && t + e < n) {
+        const char* at = row + static_cast<int64_t>(t + e + before) * SIZE;
+        if constexpr (DT == DT_F32) v[e] = *reinterpret_cast<const uint32_t*>(at);
+        else v[e / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at)) << 16 * (e % 2);
       }
-      __syncthreads();
-      if (wave == 0) {  // lane l: bins from digits - 32 l down
-        uint64_t mine = 0;
-        for (int i = 0; i < 32; ++i)
-          if (static_cast<int>(digits) - 32 * lane - i >= 0) mine += bins[digits - 32 * lane - i];
-        const uint64_t upto = wave_scan(mine) + above;
-        const uint64_t past = __ballot(reached(upto));
-        const int at = past ? __builtin_ctzll(past) : digits / 32;  // (always reached by the last)
-        if (lane == at) {
-          uint64_t sum = upto - mine;
-          int i = 0;
-          for (; i < 31 && static_cast<int>(digits) - 32 * lane - i > 0; ++i) {
-            if (reached(sum + bins[digits - 32 * lane - i])) break;
-            sum += bins[digits - 32 * lane - i];
-          }
-          found[0] = digits - 32 * lane - i;
-          found[1] = sum;
-        }
+    return v;
+  }
+  // Its E logits, -infinity in the place of tokens that there are not.
+  __device__ __forceinline__ void logits(int q, uint4_t v, float (&x)[E]) const {
+    const int t = token(q);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if constexpr (DT == DT_F32) {
+        const uint32_t w = v[e];
+        x[e] = __builtin_bit_cast(float, w);
+      } else {
+        const uint32_t w = v[e / 2] >> 16 * (e % 2);
+        x[e] = DT == DT_F16 ? f16_bits_to_f32(static_cast<uint16_t>(w)) : __builtin_bit_cast(float, w << 16);
       }
-      __syncthreads();
-      prefix |= static_cast<uint32_t>(found[0]) << shift;
-      mask |= digits << shift;
-      above = found[1];
+      if (t + e < 0 || t + e >= n) x[e] = -__builtin_inff();
     }
-    return prefix;
-  };
-  const int k = p.top_k ? p.top_k[row] : 0;
-  if (k > 0 && k < n) {
-    uint64_t above;
-    edge = select([](uint32_t) { return uint64_t{1}; }, [&](uint64_t sum) { return sum >= static_cast<uint64_t>(k); }, above);
-    ties = static_cast<uint64_t>(k) - above;
   }
-  const float top_p = p.top_p ? p.top_p[row] : 1.f;
-  if (top_p < 1.f) {
-    // Of tokens at the edge only `ties` count: they weigh the same, so the rest of theirs is taken off the sum.
-    uint64_t sum = 0, at_edge = 0;
-    for (int i = tid; i < n; i += kThreads) {
-      const float x = logit(i);
-      const uint32_t key = key_of(x);
-      if (key > edge) sum += weigh(x);
-      at_edge += key == edge;
-    }
-    auto add = [](uint64_t a, uint64_t b) { return a + b; };
-    sum = block(wave_sum(sum), add);
-    at_edge = min(block(wave_sum(at_edge), add), ties);
-    sum += at_edge * weigh(value_of(edge));
-    const double need = fmax(static_cast<double>(top_p) * static_cast<double>(sum), 1.0);  // (one token at least)
-    uint64_t above;
-    const uint32_t last = edge;
-    const uint64_t last_ties = at_edge;
-    edge = select([&](uint32_t key) { return weigh(value_of(key)); }, [&](uint64_t s) { return static_cast<double>(s) >= need; }, above);
-    const uint64_t each = weigh(value_of(edge));
-    ties = 1;
-    if (each && static_cast<double>(above + each) < need) {
-      ties = static_cast<uint64_t>((need - static_cast<double>(above)) / static_cast<double>(each));
-      if (ties) --ties;  // (the quotient is rounded: counted up from just below)
-      while (static_cast<double>(above + ties * each) < need) ++ties;
-    }
-    if (edge == last) ties = min(ties, last_ties);
-  }
-  if (p.min_p && p.min_p[row] > 0.f) weigh.least = fmin(static_cast<double>(p.min_p[row]), 1.0);
-  const uint64_t each = weigh(value_of(edge));
+};
 
-  // Sums of segments in the order of the tokens, then the segment where they pass u of the whole.
-  const int segments = (n + kSegment - 1) / kSegment;
+// Calls each(q, logits) for the chunks [from, to), a wavefront taking every kWaves-th, with four loads on their way.
+template <int DT, typename Each>
+__device__ __forceinline__ void over_chunks(const Chunks<DT>& row, int from, int to, Each each) {
+  constexpr int AHEAD = 4;
+  const int wave = threadIdx.x >> 6;
+  for (int q0 = from + wave; q0 < to; q0 += AHEAD * kWaves) {
+    uint4_t v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (q0 + i * kWaves < to) v[i] = row.raw(q0 + i * kWaves);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int q = q0 + i * kWaves;
+      if (q >= to) break;
+      float x[Chunks<DT>::E];
+      row.logits(q, v[i], x);
+      each(q, x);
+    }
+  }
+}
+
+struct Slice {
+  int64_t row;
+  int at, from, to;  // which, its chunks
+};
+__device__ __forceinline__ Slice slice_of(const SampleArgs& p) {
+  Slice s;
+  s.row = blockIdx.x / p.slices;
+  s.at = static_cast<int>(blockIdx.x - s.row * p.slices);
+  s.from = static_cast<int>(static_cast<int64_t>(p.chunks) * s.at / p.slices);
+  s.to = static_cast<int>(static_cast<int64_t>(p.chunks) * (s.at + 1) / p.slices);
+  return s;
+}
+
+// Whether this workgroup is the last of its row's. What the others have stored (past their XCD's L2, put64) it may load (get64).
+__device__ __forceinline__ bool last_of_row(const SampleArgs& p, int64_t row) {
+  __shared__ uint32_t others;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  for (int s = wave; s < segments; s += kWaves) {
+  if (threadIdx.x == 0) {
+    others = p.slices == 1 ? 0 : __hip_atomic_fetch_add(p.meet + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (p.slices > 1 && others == static_cast<uint32_t>(p.slices) - 1) __hip_atomic_store(p.meet + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return others == static_cast<uint32_t>(p.slices) - 1;
+}
+
+template <typename Join>
+__device__ __forceinline__ uint64_t block_join(uint64_t v, Join join) {  // (of all threads; v is its wavefront's)
+  __shared__ uint64_t red[kWaves];
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  uint64_t all = red[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) all = join(all, red[w]);
+  return all;
+}
+__device__ __forceinline__ uint64_t block_sum(uint64_t v) {
+  return block_join(wave_sum(v), [](uint64_t a, uint64_t b) { return a + b; });
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_sample_top(SampleArgs p) {
+  const Slice s = slice_of(p);
+  const Chunks<DT> row(p, s.row);
+  uint64_t best = 0;
+  over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[Chunks<DT>::E]) {
+    const int t = row.token(q);
+#pragma unroll
+    for (int e = 0; e < Chunks<DT>::E; ++e) best = max(best, static_cast<uint64_t>(key_of(x[e])) << 32 | static_cast<uint32_t>(~(t + e)));
+  });
+  best = block_join(wave_max(best), [](uint64_t a, uint64_t b) { return max(a, b); });
+  if (threadIdx.x == 0) p.best[s.row * p.slices + s.at] = best;
+}
+
+// A row's choices; in GREEDY rows the token is known (the largest; -1 where no logit is above -infinity).
+__device__ __forceinline__ Row row_of(const SampleArgs& p, int64_t r) {
+  Row row;
+  uint64_t best = 0;
+  for (int i = 0; i < p.slices; ++i) best = max(best, p.best[r * p.slices + i]);
+  row.top_key = static_cast<uint32_t>(best >> 32);
+  row.top_index = static_cast<uint32_t>(~best);
+  row.top = value_of(row.top_key);
+  const float temperature = p.temperature ? p.temperature[r] : 1.f;
+  row.c = 1.4426950408889634074 / static_cast<double>(temperature);
+  row.per_bin = static_cast<float>(row.c * kPerOctave);
+  row.k = p.top_k ? p.top_k[r] : 0;
+  row.top_p = p.top_p ? p.top_p[r] : 1.0;
+  const float min_p = p.min_p ? p.min_p[r] : 0.f;
+  row.least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+  row.u = p.u[r];
+  row.mode = !(temperature > 0.f) || row.top_key == kLowestKey ? GREEDY : row.k > 0 && row.k < p.vocabulary ? TOP_K : row.top_p < 1.0 ? TOP_P : ALL;
+  return row;
+}
+
+// The draw: the first token, by index, up to which the weights sum to more than u of their whole. sums: of each chunk, in LDS.
+// weight(token, logit, equal, ties_before): a token's, given the equals of the edge ahead of it.
+template <int DT, typename Weight, typename TiesBefore>
+__device__ __forceinline__ void draw(const SampleArgs& p, const Row& r, const Chunks<DT>& row, int64_t at_row, const uint64_t* sums, uint32_t edge,
+                                     Weight weight, TiesBefore ties_before) {
+  constexpr int E = Chunks<DT>::E;
+  __shared__ uint64_t parts[kWaves];
+  __shared__ uint64_t found_before;
+  __shared__ int found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // Each thread some chunks in a row.
+  const int each = (p.chunks + kThreads - 1) / kThreads, first = tid * each;
+  uint64_t mine = 0;
+  for (int i = 0; i < each; ++i)
+    if (first + i < p.chunks) mine += sums[first + i];
+  const uint64_t upto = wave_scan(mine);
+  __syncthreads();
+  if (lane == 63) parts[wave] = upto;
+  if (tid == 0) found = -1;
+  __syncthreads();
+  uint64_t before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += parts[w];
+    total += parts[w];
+  }
+  const double target = static_cast<double>(r.u) * static_cast<double>(total);
+  // (Where no sum is above the target, as for u >= 1, the last token of any weight is taken. A NaN is above nothing.)
+  auto past = [&](uint64_t sum) { return static_cast<double>(sum) > target || sum == total; };
+  if (mine && past(before + mine) && !(before && past(before))) {
+    for (int i = 0; i < each && first + i < p.chunks; ++i) {
+      const uint64_t w = sums[first + i];
+      if (w && past(before + w)) {
+        found = first + i;
+        found_before = before;
+        break;
+      }
+      before += w;
+    }
+  }
+  __syncthreads();
+  if (wave != 0 || found < 0) return;
+  const int q = found, t = row.token(q);
+  float x[E];
+  row.logits(q, row.raw(q), x);
+  uint64_t equal = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) equal += key_of(x[e]) == edge && x[e] > -__builtin_inff();
+  uint64_t ties = wave_scan(equal) - equal + ties_before(q * 64 * E - row.before);
+  uint64_t w[E], sum = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const uint32_t key = key_of(x[e]);
+    w[e] = x[e] > -__builtin_inff() ? weight(x[e], key, ties) : 0;
+    ties += key == edge && x[e] > -__builtin_inff();
+    sum += w[e];
+  }
+  uint64_t so_far = wave_scan(sum) - sum + found_before;
+  int token = -1;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    so_far += w[e];
+    if (token < 0 && w[e] && past(so_far)) token = t + e;
+  }
+  const uint64_t any = __ballot(token >= 0);
+  if (any && lane == __builtin_ctzll(any)) p.tokens[at_row] = token;
+}
+
+// The key at which the sum of measures over items of falling keys reaches `need`, and the sum above it. items(each): calls
+// each(key, measure) for the thread's items, those whose keys are below `least` left out by it.
+template <typename Items, typename Reached>
+__device__ __forceinline__ uint32_t select(uint64_t* bins, Items items, Reached reached, uint64_t& above) {
+  __shared__ uint64_t found[2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint32_t prefix = 0, mask = 0;
+  above = 0;
+#pragma unroll 1
+  for (int shift : {21, 10, 0}) {
+    const uint32_t digits = shift ? 2047u : 1023u;
+    __syncthreads();
+    for (int i = tid; i < kDigits; i += kThreads) bins[i] = 0;
+    __syncthreads();
+    items([&](uint32_t key, uint64_t measure) {
+      if ((key & mask) == prefix) atomicAdd(reinterpret_cast<unsigned long long*>(&bins[key >> shift & digits]), static_cast<unsigned long long>(measure));
+    });
+    __syncthreads();
+    if (tid < 64) {  // lane l: bins from digits - 32 l down
+      uint64_t mine = 0;
+      for (int i = 0; i < 32; ++i)
+        if (static_cast<int>(digits) - 32 * lane - i >= 0) mine += bins[digits - 32 * lane - i];
+      const uint64_t upto = wave_scan(mine) + above;
+      const uint64_t past = __ballot(reached(upto));
+      const int at = past ? __builtin_ctzll(past) : digits / 32;  // (always reached by the last)
+      if (lane == at) {
+        uint64_t sum = upto - mine;
+        int i = 0;
+        for (; i < 31 && static_cast<int>(digits) - 32 * lane - i > 0; ++i) {
+          if (reached(sum + bins[digits - 32 * lane - i])) break;
+          sum += bins[digits - 32 * lane - i];
+        }
+        found[0] = digits - 32 * lane - i;
+        found[1] = sum;
+      }
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(found[0]) << shift;
+    mask |= digits << shift;
+    above = found[1];
+  }
+  return prefix;
+}
+
+// How many of equal weights `each` it takes, beside `above`, to reach `need`.
+__device__ __forceinline__ uint64_t equals_needed(double need, uint64_t above, uint64_t each) {
+  if (!each || static_cast<double>(above + each) >= need) return 1;
+  uint64_t n = static_cast<uint64_t>((need - static_cast<double>(above)) / static_cast<double>(each));
+  if (n) --n;  // (the quotient is rounded: counted up from just below)
+  while (static_cast<double>(above + n * each) < need) ++n;
+  return n;
+}
+
+// The least key kept by top-k and top-p, and how many of its equals, among items of falling keys of which those above have the weight
+// `above`: items(each) as select takes them, with each(key) alone. `whole`: the weight that top-p is of, or 0: that of what top-k keeps.
+struct Edge {
+  uint32_t key;
+  uint64_t ties;
+};
+template <typename Items>
+__device__ __forceinline__ Edge edge_of(const Row& r, uint64_t* bins, Items items, uint64_t above, uint64_t whole) {
+  Edge edge{0, ~uint64_t{0}};
+  if (r.mode == TOP_K) {
+    uint64_t more;
+    edge.key = select(bins, [&](auto each) { items([&](uint32_t key) { each(key, uint64_t{1}); }); },
+                      [&](uint64_t sum) { return sum >= static_cast<uint64_t>(r.k); }, more);
+    edge.ties = static_cast<uint64_t>(r.k) - more;
+  }
+  if (r.top_p < 1.0) {
+    uint64_t at_edge = edge.ties;
+    if (!whole) {
+      // Of tokens at the edge only `ties` count.
+      uint64_t sum = 0, equal = 0;
+      items([&](uint32_t key) {
+        if (key > edge.key) sum += r.weight(value_of(key));
+        equal += key == edge.key;
+      });
+      whole = block_sum(sum);
+      at_edge = min(block_sum(equal), edge.ties);
+      whole += at_edge * r.weight(value_of(edge.key));
+    }
+    const double need = fmax(r.top_p * static_cast<double>(whole), 1.0);  // (one token at least)
+    const Edge by_k = edge;
+    uint64_t more;
+    edge.key = select(bins, [&](auto each) { items([&](uint32_t key) { if (key >= by_k.key) each(key, r.weight(value_of(key))); }); },
+                      [&](uint64_t sum) { return static_cast<double>(above + sum) >= need; }, more);
+    edge.ties = equals_needed(need, above + more, r.weight(value_of(edge.key)));
+    if (edge.key == by_k.key) edge.ties = min(edge.ties, at_edge);
+  }
+  return edge;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_sample_sum(SampleArgs p) {
+  constexpr int E = Chunks<DT>::E;
+  __shared__ uint64_t bins[kMostChunks];  // (or, for the draw, the chunks' weights)
+  static_assert(kMostChunks >= kWeightBins, "");
+  const Slice s = slice_of(p);
+  const Row r = row_of(p, s.row);
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (r.mode == GREEDY) {
+    if (s.at == 0 && tid == 0) p.tokens[s.row] = r.top_key == kLowestKey ? -1 : static_cast<int64_t>(r.top_index);
+    return;
+  }
+  const Chunks<DT> row(p, s.row);
+  uint64_t* sums = p.sums + s.row * p.chunks;
+  if (r.mode == ALL) {
+    over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[E]) {
+      uint64_t sum = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += r.kept_weight(x[e]);
+      sum = wave_sum(sum);
+      if (lane == 0) put64(sums + q, sum);
+    });
+    if (!last_of_row(p, s.row)) return;
+    for (int i = tid; i < p.chunks; i += kThreads) bins[i] = get64(sums + i);
+    __syncthreads();
+    draw<DT>(p, r, row, s.row, bins, 0u, [&](float x, uint32_t, uint64_t) { return r.kept_weight(x); }, [](int) { return uint64_t{0}; });
+    return;
+  }
+  for (int i = tid; i < kWeightBins; i += kThreads) bins[i] = 0;
+  __syncthreads();
+  over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int b = r.bin(x[e]);
+      if (b >= kWeightBins) continue;
+      atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b]), static_cast<unsigned long long>(r.mode == TOP_K ? 1 : r.weight(x[e])));
+    }
+  });
+  __syncthreads();
+  uint64_t* all = p.bins + s.row * p.slices * kWeightBins;
+  for (int i = tid; i < kWeightBins; i += kThreads) put64(all + s.at * kWeightBins + i, bins[i]);
+  if (!last_of_row(p, s.row)) return;
+  uint64_t mine = 0;
+  if (tid < kWeightBins)
+    for (int i = 0; i < p.slices; ++i) mine += get64(all + i * kWeightBins + tid);
+  static_assert(kWeightBins <= kThreads, "");
+  // The first bin with which the sum of the bins reaches k tokens, or top-p of the whole.
+  __shared__ uint64_t parts[kWaves];
+  __shared__ uint32_t border;
+  __shared__ uint64_t above;
+  const uint64_t upto = wave_scan(mine);
+  if (lane == 63) parts[tid >> 6] = upto;
+  if (tid == 0) {
+    border = kWeightBins;
+    above = 0;
+  }
+  __syncthreads();
+  uint64_t before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < (tid >> 6)) before += parts[w];
+    total += parts[w];
+  }
+  const double need = fmax(r.top_p * static_cast<double>(total), 1.0);
+  auto reached = [&](uint64_t sum) { return r.mode == TOP_K ? sum >= static_cast<uint64_t>(r.k) : static_cast<double>(sum) >= need; };
+  if (mine && reached(before + mine) && !(before && reached(before))) {
+    border = tid;
+    above = before;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    p.told[4 * s.row] = border;
+    p.told[4 * s.row + 1] = r.mode == TOP_K ? 0 : above;
+    p.told[4 * s.row + 2] = r.mode == TOP_K ? 0 : total;
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
+  constexpr int E = Chunks<DT>::E;
+  __shared__ uint64_t bins[kDigits];
+  __shared__ uint64_t list[kList];  // key << 32 | token
+  __shared__ uint64_t sums[kMostChunks];
+  __shared__ uint32_t count;
+  const Slice s = slice_of(p);
+  const Row r = row_of(p, s.row);
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (r.mode == GREEDY || r.mode == ALL) return;
+  const Chunks<DT> row(p, s.row);
+  const uint32_t border = static_cast<uint32_t>(p.told[4 * s.row]);
+  const uint64_t above = p.told[4 * s.row + 1], whole = p.told[4 * s.row + 2];
+  uint64_t* all_sums = p.sums + s.row * p.chunks;
+  uint64_t* lists = p.list + s.row * p.slices * kList;
+  uint32_t* counts = p.counts + s.row * p.slices;
+  if (tid == 0) count = 0;
+  __syncthreads();
+  over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[E]) {
+    const int t = row.token(q);
     uint64_t sum = 0;
-    uint32_t equal = 0;
-    for (int j = 0; j < kSegment / 64; ++j) {
-      const int i = s * kSegment + j * 64 + lane;
-      if (i >= n) continue;
-      const float x = logit(i);
-      const uint32_t key = key_of(x);
-      if (key > edge) sum += weigh(x);
-      equal += key == edge;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t b = static_cast<uint32_t>(r.bin(x[e]));
+      if (b > border || b >= kWeightBins) continue;
+      if (b == border || r.mode == TOP_K) {
+        const uint32_t at = atomicAdd(&count, 1u);
+        if (at < kList) list[at] = static_cast<uint64_t>(key_of(x[e])) << 32 | static_cast<uint32_t>(t + e);
+      } else {
+        sum += r.kept_weight(x[e]);
+      }
+    }
+    if (r.mode == TOP_P) {
+      sum = wave_sum(sum);
+      if (lane == 0) put64(all_sums + q, sum);
+    }
+  });
+  __syncthreads();
+  if (p.slices > 1) {
+    for (uint32_t i = tid; i < min(count, static_cast<uint32_t>(kList)); i += kThreads) put64(lists + s.at * kList + i, list[i]);
+    if (tid == 0) __hip_atomic_store(counts + s.at, count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!last_of_row(p, s.row)) return;
+    // All slices' lists (a slice's that did not fit: neither does the whole).
+    uint32_t n = 0;
+    for (int i = 0; i < p.slices; ++i) {
+      const uint32_t some = __hip_atomic_load(counts + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      for (uint32_t k = tid; k < some && n + k < kList; k += kThreads) list[n + k] = get64(lists + i * kList + k);
+      n += some;
+    }
+    __syncthreads();
+    if (tid == 0) count = n;
+    __syncthreads();
+  }
+  const uint32_t n = count;
+  const bool fits = n <= kList;
+  for (int i = tid; i < p.chunks; i += kThreads) sums[i] = fits && r.mode == TOP_P ? get64(all_sums + i) : 0;
+  // The edge, from the list or from the whole row.
+  auto from_list = [&](auto each) {
+    for (uint32_t i = tid; i < n; i += kThreads) each(static_cast<uint32_t>(list[i] >> 32));
+  };
+  auto from_row = [&](auto each) {
+    over_chunks<DT>(row, 0, p.chunks, [&](int, const float (&x)[E]) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (x[e] > -__builtin_inff()) each(key_of(x[e]));
+    });
+  };
+  const bool cut = border < kWeightBins;  // (without, all tokens of any weight are kept: fewer than k, as it is)
+  Edge edge{0, ~uint64_t{0}};
+  if (cut || r.top_p < 1.0) {
+    Row rr = r;
+    if (!cut) rr.mode = TOP_P;  // (fewer tokens of any weight than k)
+    edge = fits ? edge_of(rr, bins, from_list, r.mode == TOP_P ? above : 0, whole) : edge_of(rr, bins, from_row, 0, whole);
+  }
+  const uint64_t at_edge = r.kept_weight(value_of(edge.key));
+  __syncthreads();
+  auto chunk_of = [&](uint32_t token) { return (token + row.before) / (64 * E); };
+  auto add = [&](uint32_t chunk, uint64_t w) { atomicAdd(reinterpret_cast<unsigned long long*>(&sums[chunk]), static_cast<unsigned long long>(w)); };
+  auto weight = [&](float x, uint32_t key, uint64_t ties) { return key > edge.key ? r.kept_weight(x) : key == edge.key && ties < edge.ties ? at_edge : 0; };
+  if (fits) {
+    // A token of the edge is kept if fewer than `ties` of its equals come before it.
+    for (uint32_t i = tid; i < n; i += kThreads) {
+      const uint32_t key = static_cast<uint32_t>(list[i] >> 32), token = static_cast<uint32_t>(list[i]);
+      if (key < edge.key) continue;
+      uint64_t ties = 0;
+      if (key == edge.key && edge.ties < n)
+        for (uint32_t j = 0; j < n; ++j) ties += (list[j] >> 32) == key && static_cast<uint32_t>(list[j]) < token;
+      const uint64_t w = weight(value_of(key), key, ties);
+      if (w) add(chunk_of(token), w);
+    }
+    __syncthreads();
+    draw<DT>(p, r, row, s.row, sums, edge.key, weight, [&](int first) {
+      uint64_t ties = 0;
+      for (uint32_t j = lane; j < n; j += 64) ties += (list[j] >> 32) == edge.key && static_cast<int>(static_cast<uint32_t>(list[j])) < first;
+      return wave_sum(ties);
+    });
+    return;
+  }
+  // The whole row again: chunks' weights above the edge and equals of it, then how many of those are kept.
+  uint32_t* equals = reinterpret_cast<uint32_t*>(list);
+  static_assert(sizeof(list) >= kMostChunks * sizeof(uint32_t), "");
+  over_chunks<DT>(row, 0, p.chunks, [&](int q, const float (&x)[E]) {
+    uint64_t sum = 0, equal = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint32_t key = key_of(x[e]);
+      if (!(x[e] > -__builtin_inff())) continue;
+      if (key > edge.key) sum += r.kept_weight(x[e]);
+      equal += key == edge.key;
     }
     sum = wave_sum(sum);
-    equal = static_cast<uint32_t>(wave_sum(equal));
+    equal = wave_sum(equal);
     if (lane == 0) {
-      seg_sum[s] = sum;
-      seg_ties[s] = equal;
+      sums[q] = sum;
+      equals[q] = static_cast<uint32_t>(equal);
+    }
+  });
+  __syncthreads();
+  if (tid < 64) {  // equals[q] becomes how many come before chunk q
+    uint64_t before = 0;
+    for (int q0 = 0; q0 < p.chunks; q0 += 64) {
+      const uint64_t equal = q0 + lane < p.chunks ? equals[q0 + lane] : 0, upto = wave_scan(equal) + before, start = upto - equal;
+      if (q0 + lane < p.chunks) {
+        sums[q0 + lane] += (min(upto, edge.ties) - min(start, edge.ties)) * at_edge;
+        equals[q0 + lane] = static_cast<uint32_t>(start);
+      }
+      before = __shfl(upto, 63);
     }
   }
   __syncthreads();
-  if (wave != 0) return;
-  // (A segment's kept ties: as many of its own as `ties` has left for it.)
-  uint64_t total = 0, before_ties = 0;
-  for (int s0 = 0; s0 < segments; s0 += 64) {
-    const int s = s0 + lane;
-    const uint64_t equal = s < segments ? seg_ties[s] : 0, upto = wave_scan(equal) + before_ties;
-    const uint64_t start = min(upto - equal, ties), kept = min(upto, ties) - start;
-    if (s < segments) seg_sum[s] += kept * each;
-    total += wave_sum(s < segments ? seg_sum[s] : 0);
-    before_ties = __shfl(upto, 63);
-  }
-  const float u = p.u[row];
-  const double target = static_cast<double>(u) * static_cast<double>(total);
-  uint64_t before = 0, ties_before = 0;
-  int segment = -1;
-  for (int s0 = 0; s0 < segments; s0 += 64) {
-    const int s = s0 + lane;
-    const uint64_t mine = s < segments ? seg_sum[s] : 0, upto = wave_scan(mine) + before;
-    const uint64_t equal = s < segments ? seg_ties[s] : 0, ties_upto = wave_scan(equal) + ties_before;
-    // (Where no sum is above the target, as for u >= 1, the last token of any weight is taken.)
-    const uint64_t past = __ballot(mine != 0 && (static_cast<double>(upto) > target || upto == total));
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      segment = s0 + at;
-      before = __shfl(upto - mine, at);
-      ties_before = __shfl(ties_upto - equal, at);
-      break;
-    }
-    before = __shfl(upto, 63);
-    ties_before = __shfl(ties_upto, 63);
-  }
-  if (segment < 0) return;  // (not reached: the largest logit has a weight)
-  for (int j = 0; j < kSegment / 64; ++j) {
-    const int i = segment * kSegment + j * 64 + lane;
-    uint64_t w = 0, equal = 0;
-    if (i < n) {
-      const float x = logit(i);
-      const uint32_t key = key_of(x);
-      equal = key == edge;
-      if (key > edge) w = weigh(x);
-    }
-    const uint64_t ties_upto = wave_scan(equal) + ties_before;
-    if (equal && ties_upto <= ties) w = each;
-    const uint64_t upto = wave_scan(w) + before;
-    const uint64_t past = __ballot(w != 0 && (static_cast<double>(upto) > target || upto == total));
-    if (past) {
-      if (lane == __builtin_ctzll(past)) p.tokens[row] = i;
-      return;
-    }
-    before = __shfl(upto, 63);
-    ties_before = __shfl(ties_upto, 63);
-  }
+  draw<DT>(p, r, row, s.row, sums, edge.key, weight, [&](int first) { return static_cast<uint64_t>(equals[chunk_of(static_cast<uint32_t>(first < 0 ? 0 : first))]); });
 }
 
 }  // namespace
@@ -303,15 +666,49 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
   TMH_TRY(use_device(ctx));
   if (T == 0) return TMH_OK;
   if (!d_logits || !d_random || !d_tokens) return fail(ctx, TMH_ERR_INVALID, "tmh_sample: NULL pointer");
-  SampleArgs p{d_logits, d_temperature, d_top_k, d_top_p, d_min_p, d_random, d_tokens, ld, static_cast<int>(V)};
+  const int64_t size = dtype_size(dtype), chunk = 64 * 16 / size;
+  if (reinterpret_cast<uintptr_t>(d_logits) % size != 0) return fail(ctx, TMH_ERR_UNSUPPORTED, "the logits must lie on multiples of their size");
   hipStream_t s = pick_stream(ctx, stream);
-  in_launches(T, most_a_launch(kThreads, 1, 1), [&](int64_t first, int64_t rows) {
-    const unsigned grid = static_cast<unsigned>(rows);
-    if (dtype == TMH_F32) k_sample<DT_F32><<<grid, kThreads, 0, s>>>(p, first);
-    else if (dtype == TMH_F16) k_sample<DT_F16><<<grid, kThreads, 0, s>>>(p, first);
-    else k_sample<DT_BF16><<<grid, kThreads, 0, s>>>(p, first);
+  const int64_t most_rows = std::min<int64_t>(kMostRows, 2 * ctx->num_cus);
+  const int64_t rows = std::min(T, most_rows);
+  SampleArgs p{};
+  p.ld = ld;
+  p.vocabulary = static_cast<int>(V);
+  p.chunks = static_cast<int>((V + 16 / size - 1 + chunk - 1) / chunk);  // (rows that begin inside 16 bytes may take one more)
+  // Two workgroups a CU in all, of a chunk a wavefront at least.
+  p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * ctx->num_cus / rows, p.chunks / kWaves)));
+  const size_t of_rows = static_cast<size_t>(rows) * p.slices;
+  const size_t bytes = 8 * (of_rows * (1 + kWeightBins + (p.slices > 1 ? kList : 0)) + static_cast<size_t>(rows) * (p.chunks + 4)) + 4 * of_rows;
+  void* ws = workspace(ctx, bytes, s);
+  if (!ws) return fail(ctx, TMH_ERR_UNSUPPORTED, "sampling's workspace cannot grow here: run one call before the capture");
+  p.best = static_cast<uint64_t*>(ws);
+  p.bins = p.best + of_rows;
+  p.list = p.bins + of_rows * kWeightBins;
+  p.sums = p.list + (p.slices > 1 ? of_rows * kList : 0);
+  p.told = p.sums + static_cast<size_t>(rows) * p.chunks;
+  p.counts = reinterpret_cast<uint32_t*>(p.told + static_cast<size_t>(rows) * 4);
+  p.meet = ctx->meet;
+  in_launches(T, most_rows, [&](int64_t first, int64_t some) {
+    auto from = [&](auto* a) { return a ? a + first : a; };
+    p.x = static_cast<const char*>(d_logits) + first * ld * size;
+    p.temperature = from(d_temperature);
+    p.top_k = from(d_top_k);
+    p.top_p = from(d_top_p);
+    p.min_p = from(d_min_p);
+    p.u = from(d_random);
+    p.tokens = d_tokens + first;
+    const unsigned grid = static_cast<unsigned>(some * p.slices);
+    auto launch = [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      k_sample_top<DT><<<grid, kThreads, 0, s>>>(p);
+      k_sample_sum<DT><<<grid, kThreads, 0, s>>>(p);
+      if (d_top_k || d_top_p) k_sample_draw<DT><<<grid, kThreads, 0, s>>>(p);
+    };
+    if (dtype == TMH_F32) launch(std::integral_constant<int, DT_F32>{});
+    else if (dtype == TMH_F16) launch(std::integral_constant<int, DT_F16>{});
+    else launch(std::integral_constant<int, DT_BF16>{});
   });
-  return check_launch(ctx, "k_sample");
+  return check_launch(ctx, "k_sample_draw");
 }
 
 }  // extern "C"

@@ -7,7 +7,7 @@
 //                 many tokens lie in each bin (a sixteenth of a factor of two in weight), and down to which bin the k largest reach.
 //                 Others, by top-p alone: the weights of each bin, and the bin in which they reach top-p of the whole.
 //  k_sample_draw  rows by top-k: the tokens down to that bin go to a list. By top-p alone: those of that bin do, and the weights above
-//                 it to chunks. The list, sorted out in LDS, gives the least logit kept and how many of its equals are; then the draw.
+//                 it to chunks. The list, sorted out in LDS, gives the least logit kept and the last of its equals that is; then the draw.
 // A list that does not fit (thousands of tokens of almost the same logit) leaves its row to the last workgroup, which goes over all
 // of it a few times.
 #include <algorithm>
@@ -92,6 +92,7 @@ struct Row {
   double c;           // log2(e) / temperature
   float per_bin;      // bins a logit
   double top_p, least;  // least: the smallest weight that min-p keeps
+  float low;          // logits below it are certainly left out by min-p, or weigh nothing
   float u;
   // exp((x - top) / temperature) in units of 2^-44; 0 where it is less than one.
   __device__ __forceinline__ uint64_t weight(float x) const {
@@ -243,16 +244,39 @@ __device__ __forceinline__ uint64_t block_sum(uint64_t v) {
   return block_join(wave_sum(v), [](uint64_t a, uint64_t b) { return a + b; });
 }
 
+// The sum over the threads before this one, and over all.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t& all) {
+  __shared__ uint64_t parts[kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint64_t upto = wave_scan(v);
+  __syncthreads();
+  if (lane == 63) parts[wave] = upto;
+  __syncthreads();
+  uint64_t before = upto - v;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += parts[w];
+    all += parts[w];
+  }
+  return before;
+}
+
 template <int DT>
 __global__ __launch_bounds__(kThreads) void k_sample_top(SampleArgs p) {
   const Slice s = slice_of(p);
   const Chunks<DT> row(p, s.row);
-  uint64_t best = 0;
+  uint32_t top = 0, at = 0;  // (a thread's tokens come in their order: the first of equals stays)
   over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[Chunks<DT>::E]) {
     const int t = row.token(q);
 #pragma unroll
-    for (int e = 0; e < Chunks<DT>::E; ++e) best = max(best, static_cast<uint64_t>(key_of(x[e])) << 32 | static_cast<uint32_t>(~(t + e)));
+    for (int e = 0; e < Chunks<DT>::E; ++e) {
+      const uint32_t key = key_of(x[e]);
+      at = key > top ? t + e : at;
+      top = max(top, key);
+    }
   });
+  uint64_t best = static_cast<uint64_t>(top) << 32 | static_cast<uint32_t>(~at);
   best = block_join(wave_max(best), [](uint64_t a, uint64_t b) { return max(a, b); });
   if (threadIdx.x == 0) p.best[s.row * p.slices + s.at] = best;
 }
@@ -273,17 +297,17 @@ __device__ __forceinline__ Row row_of(const SampleArgs& p, int64_t r) {
   const float min_p = p.min_p ? p.min_p[r] : 0.f;
   row.least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
   row.u = p.u[r];
+  // (A factor of two below: more than f32's roundings are.)
+  row.low = row.top == __builtin_inff() ? row.top : row.top - static_cast<float>((1.0 - (row.least > 0.0 ? fmax(log2(row.least), -1.0 * kUnit) : -1.0 * kUnit)) / row.c);
   row.mode = !(temperature > 0.f) || row.top_key == kLowestKey ? GREEDY : row.k > 0 && row.k < p.vocabulary ? TOP_K : row.top_p < 1.0 ? TOP_P : ALL;
   return row;
 }
 
 // The draw: the first token, by index, up to which the weights sum to more than u of their whole. sums: of each chunk, in LDS.
-// weight(token, logit, equal, ties_before): a token's, given the equals of the edge ahead of it.
-template <int DT, typename Weight, typename TiesBefore>
-__device__ __forceinline__ void draw(const SampleArgs& p, const Row& r, const Chunks<DT>& row, int64_t at_row, const uint64_t* sums, uint32_t edge,
-                                     Weight weight, TiesBefore ties_before) {
+// weight(logit, token): a token's, 0 where it is not kept.
+template <int DT, typename Weight>
+__device__ __forceinline__ void draw(const SampleArgs& p, const Row& r, const Chunks<DT>& row, int64_t at_row, const uint64_t* sums, Weight weight) {
   constexpr int E = Chunks<DT>::E;
-  __shared__ uint64_t parts[kWaves];
   __shared__ uint64_t found_before;
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -292,17 +316,9 @@ __device__ __forceinline__ void draw(const SampleArgs& p, const Row& r, const Ch
   uint64_t mine = 0;
   for (int i = 0; i < each; ++i)
     if (first + i < p.chunks) mine += sums[first + i];
-  const uint64_t upto = wave_scan(mine);
-  __syncthreads();
-  if (lane == 63) parts[wave] = upto;
   if (tid == 0) found = -1;
-  __syncthreads();
-  uint64_t before = upto - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += parts[w];
-    total += parts[w];
-  }
+  uint64_t total;
+  uint64_t before = block_scan(mine, total);
   const double target = static_cast<double>(r.u) * static_cast<double>(total);
   // (Where no sum is above the target, as for u >= 1, the last token of any weight is taken. A NaN is above nothing.)
   auto past = [&](uint64_t sum) { return static_cast<double>(sum) > target || sum == total; };
@@ -322,16 +338,10 @@ __device__ __forceinline__ void draw(const SampleArgs& p, const Row& r, const Ch
   const int q = found, t = row.token(q);
   float x[E];
   row.logits(q, row.raw(q), x);
-  uint64_t equal = 0;
-#pragma unroll
-  for (int e = 0; e < E; ++e) equal += key_of(x[e]) == edge && x[e] > -__builtin_inff();
-  uint64_t ties = wave_scan(equal) - equal + ties_before(q * 64 * E - row.before);
   uint64_t w[E], sum = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const uint32_t key = key_of(x[e]);
-    w[e] = x[e] > -__builtin_inff() ? weight(x[e], key, ties) : 0;
-    ties += key == edge && x[e] > -__builtin_inff();
+    w[e] = x[e] > -__builtin_inff() ? weight(x[e], t + e) : 0;
     sum += w[e];
   }
   uint64_t so_far = wave_scan(sum) - sum + found_before;
@@ -345,48 +355,68 @@ __device__ __forceinline__ void draw(const SampleArgs& p, const Row& r, const Ch
   if (any && lane == __builtin_ctzll(any)) p.tokens[at_row] = token;
 }
 
-// The key at which the sum of measures over items of falling keys reaches `need`, and the sum above it. items(each): calls
-// each(key, measure) for the thread's items, those whose keys are below `least` left out by it.
+// The key at which the sum of measures over items of falling keys reaches `need` (reached(sum)), and the sum above it, by 11 bits of the
+// keys a turn, of those in which they differ. items(each) calls each(key, measure) for the thread's items.
 template <typename Items, typename Reached>
 __device__ __forceinline__ uint32_t select(uint64_t* bins, Items items, Reached reached, uint64_t& above) {
-  __shared__ uint64_t found[2];
-  const int tid = threadIdx.x, lane = tid & 63;
-  uint32_t prefix = 0, mask = 0;
+  static_assert(kDigits == 2 * kThreads, "");
+  __shared__ uint32_t found_digit;
+  __shared__ uint64_t found_sum;
+  const uint32_t tid = threadIdx.x;
+  uint32_t low = ~0u, high = 0;
+  items([&](uint32_t key, uint64_t) {
+    low = min(low, key);
+    high = max(high, key);
+  });
+  // (Both ends' largest in one number: the low half holds the complement of the lowest.)
+  auto both = [](uint64_t a, uint64_t b) {
+    const uint32_t x = max(static_cast<uint32_t>(a >> 32), static_cast<uint32_t>(b >> 32)), y = max(static_cast<uint32_t>(a), static_cast<uint32_t>(b));
+    return static_cast<uint64_t>(x) << 32 | y;
+  };
+  uint64_t ends = static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(~low);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) ends = both(ends, __shfl_xor(ends, o));
+  ends = block_join(ends, both);
+  low = ~static_cast<uint32_t>(ends);
+  high = static_cast<uint32_t>(ends >> 32);
   above = 0;
+  int shift = high > low ? max(32 - __builtin_clz(high - low) - 11, 0) : 0;
+  uint32_t base = low, span = high - low;  // the keys that are left are base .. base + span
 #pragma unroll 1
-  for (int shift : {21, 10, 0}) {
-    const uint32_t digits = shift ? 2047u : 1023u;
-    __syncthreads();
-    for (int i = tid; i < kDigits; i += kThreads) bins[i] = 0;
+  while (true) {
+    bins[2 * tid] = 0;
+    bins[2 * tid + 1] = 0;
     __syncthreads();
     items([&](uint32_t key, uint64_t measure) {
-      if ((key & mask) == prefix) atomicAdd(reinterpret_cast<unsigned long long*>(&bins[key >> shift & digits]), static_cast<unsigned long long>(measure));
+      if (key >= base && key - base <= span)
+        atomicAdd(reinterpret_cast<unsigned long long*>(&bins[(key - base) >> shift]), static_cast<unsigned long long>(measure));
     });
     __syncthreads();
-    if (tid < 64) {  // lane l: bins from digits - 32 l down
-      uint64_t mine = 0;
-      for (int i = 0; i < 32; ++i)
-        if (static_cast<int>(digits) - 32 * lane - i >= 0) mine += bins[digits - 32 * lane - i];
-      const uint64_t upto = wave_scan(mine) + above;
-      const uint64_t past = __ballot(reached(upto));
-      const int at = past ? __builtin_ctzll(past) : digits / 32;  // (always reached by the last)
-      if (lane == at) {
-        uint64_t sum = upto - mine;
-        int i = 0;
-        for (; i < 31 && static_cast<int>(digits) - 32 * lane - i > 0; ++i) {
-          if (reached(sum + bins[digits - 32 * lane - i])) break;
-          sum += bins[digits - 32 * lane - i];
-        }
-        found[0] = digits - 32 * lane - i;
-        found[1] = sum;
-      }
+    // Each thread two digits, from the highest down.
+    const uint32_t digit = kDigits - 1 - 2 * tid;
+    const uint64_t first = bins[digit], second = bins[digit - 1];
+    uint64_t all;
+    uint64_t before = block_scan(first + second, all) + above;
+    // (The first to reach it; the lowest that there is, should the sums not.)
+    const bool here = (first + second) && reached(before + first + second) && !(before != above && reached(before));
+    if (tid == 0) {
+      found_digit = 0;
+      found_sum = above + all - (bins[0]);
     }
     __syncthreads();
-    prefix |= static_cast<uint32_t>(found[0]) << shift;
-    mask |= digits << shift;
-    above = found[1];
+    if (here) {
+      const bool upper = first && reached(before + first);
+      found_digit = upper ? digit : digit - 1;
+      found_sum = upper ? before : before + first;
+    }
+    __syncthreads();
+    above = found_sum;
+    base += found_digit << shift;
+    if (shift == 0) return base;
+    span = (1u << shift) - 1;
+    shift = max(shift - 11, 0);
+    __syncthreads();
   }
-  return prefix;
 }
 
 // How many of equal weights `each` it takes, beside `above`, to reach `need`.
@@ -398,43 +428,50 @@ __device__ __forceinline__ uint64_t equals_needed(double need, uint64_t above, u
   return n;
 }
 
-// The least key kept by top-k and top-p, and how many of its equals, among items of falling keys of which those above have the weight
-// `above`: items(each) as select takes them, with each(key) alone. `whole`: the weight that top-p is of, or 0: that of what top-k keeps.
+// What top-k and top-p keep: keys above `key`, and of its equals the tokens up to `last`. items(each) calls each(key, token) for the
+// thread's items, the tokens that may be the border's; those above all of them weigh `above`. `whole`: the weight that top-p is of, or
+// 0: that of what top-k keeps.
 struct Edge {
-  uint32_t key;
-  uint64_t ties;
+  uint32_t key, last;
+  __device__ __forceinline__ bool keeps(uint32_t k, uint32_t token) const { return k > key || (k == key && token <= last); }
 };
 template <typename Items>
 __device__ __forceinline__ Edge edge_of(const Row& r, uint64_t* bins, Items items, uint64_t above, uint64_t whole) {
-  Edge edge{0, ~uint64_t{0}};
+  uint32_t edge = 0;
+  uint64_t ties = ~uint64_t{0};
   if (r.mode == TOP_K) {
     uint64_t more;
-    edge.key = select(bins, [&](auto each) { items([&](uint32_t key) { each(key, uint64_t{1}); }); },
-                      [&](uint64_t sum) { return sum >= static_cast<uint64_t>(r.k); }, more);
-    edge.ties = static_cast<uint64_t>(r.k) - more;
+    edge = select(bins, [&](auto each) { items([&](uint32_t key, uint32_t) { each(key, uint64_t{1}); }); },
+                  [&](uint64_t sum) { return sum >= static_cast<uint64_t>(r.k); }, more);
+    ties = static_cast<uint64_t>(r.k) - more;
   }
   if (r.top_p < 1.0) {
-    uint64_t at_edge = edge.ties;
+    uint64_t at_edge = ties;
     if (!whole) {
       // Of tokens at the edge only `ties` count.
       uint64_t sum = 0, equal = 0;
-      items([&](uint32_t key) {
-        if (key > edge.key) sum += r.weight(value_of(key));
-        equal += key == edge.key;
+      items([&](uint32_t key, uint32_t) {
+        if (key > edge) sum += r.weight(value_of(key));
+        equal += key == edge;
       });
       whole = block_sum(sum);
-      at_edge = min(block_sum(equal), edge.ties);
-      whole += at_edge * r.weight(value_of(edge.key));
+      at_edge = min(block_sum(equal), ties);
+      whole += at_edge * r.weight(value_of(edge));
     }
     const double need = fmax(r.top_p * static_cast<double>(whole), 1.0);  // (one token at least)
-    const Edge by_k = edge;
+    const uint32_t by_k = edge;
     uint64_t more;
-    edge.key = select(bins, [&](auto each) { items([&](uint32_t key) { if (key >= by_k.key) each(key, r.weight(value_of(key))); }); },
-                      [&](uint64_t sum) { return static_cast<double>(above + sum) >= need; }, more);
-    edge.ties = equals_needed(need, above + more, r.weight(value_of(edge.key)));
-    if (edge.key == by_k.key) edge.ties = min(edge.ties, at_edge);
+    edge = select(bins, [&](auto each) { items([&](uint32_t key, uint32_t) { if (key >= by_k) each(key, r.weight(value_of(key))); }); },
+                  [&](uint64_t sum) { return static_cast<double>(above + sum) >= need; }, more);
+    ties = equals_needed(need, above + more, r.weight(value_of(edge)));
+    if (edge == by_k) ties = min(ties, at_edge);
   }
-  return edge;
+  uint64_t equal = 0;
+  items([&](uint32_t key, uint32_t) { equal += key == edge; });
+  if (block_sum(equal) <= ties) return {edge, ~0u};
+  uint64_t more;
+  return {edge, ~select(bins, [&](auto each) { items([&](uint32_t key, uint32_t token) { if (key == edge) each(~token, uint64_t{1}); }); },
+                        [&](uint64_t sum) { return sum >= ties; }, more)};
 }
 
 template <int DT>
@@ -455,14 +492,15 @@ __global__ __launch_bounds__(kThreads) void k_sample_sum(SampleArgs p) {
     over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[E]) {
       uint64_t sum = 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) sum += r.kept_weight(x[e]);
-      sum = wave_sum(sum);
+      for (int e = 0; e < E; ++e)
+        if (!(x[e] < r.low)) sum += r.kept_weight(x[e]);
+      if (__ballot(sum != 0)) sum = wave_sum(sum);
       if (lane == 0) put64(sums + q, sum);
     });
     if (!last_of_row(p, s.row)) return;
     for (int i = tid; i < p.chunks; i += kThreads) bins[i] = get64(sums + i);
     __syncthreads();
-    draw<DT>(p, r, row, s.row, bins, 0u, [&](float x, uint32_t, uint64_t) { return r.kept_weight(x); }, [](int) { return uint64_t{0}; });
+    draw<DT>(p, r, row, s.row, bins, [&](float x, int) { return r.kept_weight(x); });
     return;
   }
   for (int i = tid; i < kWeightBins; i += kThreads) bins[i] = 0;
@@ -481,25 +519,18 @@ __global__ __launch_bounds__(kThreads) void k_sample_sum(SampleArgs p) {
   if (!last_of_row(p, s.row)) return;
   uint64_t mine = 0;
   if (tid < kWeightBins)
+#pragma unroll 8
     for (int i = 0; i < p.slices; ++i) mine += get64(all + i * kWeightBins + tid);
   static_assert(kWeightBins <= kThreads, "");
   // The first bin with which the sum of the bins reaches k tokens, or top-p of the whole.
-  __shared__ uint64_t parts[kWaves];
   __shared__ uint32_t border;
   __shared__ uint64_t above;
-  const uint64_t upto = wave_scan(mine);
-  if (lane == 63) parts[tid >> 6] = upto;
   if (tid == 0) {
     border = kWeightBins;
     above = 0;
   }
-  __syncthreads();
-  uint64_t before = upto - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < (tid >> 6)) before += parts[w];
-    total += parts[w];
-  }
+  uint64_t total;
+  const uint64_t before = block_scan(mine, total);
   const double need = fmax(r.top_p * static_cast<double>(total), 1.0);
   auto reached = [&](uint64_t sum) { return r.mode == TOP_K ? sum >= static_cast<uint64_t>(r.k) : static_cast<double>(sum) >= need; };
   if (mine && reached(before + mine) && !(before && reached(before))) {
@@ -557,15 +588,19 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
     for (uint32_t i = tid; i < min(count, static_cast<uint32_t>(kList)); i += kThreads) put64(lists + s.at * kList + i, list[i]);
     if (tid == 0) __hip_atomic_store(counts + s.at, count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (!last_of_row(p, s.row)) return;
-    // All slices' lists (a slice's that did not fit: neither does the whole).
-    uint32_t n = 0;
-    for (int i = 0; i < p.slices; ++i) {
-      const uint32_t some = __hip_atomic_load(counts + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      for (uint32_t k = tid; k < some && n + k < kList; k += kThreads) list[n + k] = get64(lists + i * kList + k);
-      n += some;
+    // All slices' lists, one behind the other (a slice's that did not fit: neither does the whole).
+    const uint32_t some = tid < p.slices ? __hip_atomic_load(counts + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    uint64_t all;
+    const uint64_t before = block_scan(some, all);
+    uint32_t* begins = reinterpret_cast<uint32_t*>(bins);  // (and ends)
+    if (tid < p.slices) {
+      begins[2 * tid] = static_cast<uint32_t>(min(before, uint64_t{kList}));
+      begins[2 * tid + 1] = static_cast<uint32_t>(min(before + some, uint64_t{kList}));
     }
+    if (tid == 0) count = static_cast<uint32_t>(min(all, uint64_t{kList} + 1));
     __syncthreads();
-    if (tid == 0) count = n;
+    for (int i = tid >> 6; i < p.slices; i += kWaves)
+      for (uint32_t k = begins[2 * i] + lane; k < begins[2 * i + 1]; k += 64) list[k] = get64(lists + i * kList + k - begins[2 * i]);
     __syncthreads();
   }
   const uint32_t n = count;
@@ -573,79 +608,44 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
   for (int i = tid; i < p.chunks; i += kThreads) sums[i] = fits && r.mode == TOP_P ? get64(all_sums + i) : 0;
   // The edge, from the list or from the whole row.
   auto from_list = [&](auto each) {
-    for (uint32_t i = tid; i < n; i += kThreads) each(static_cast<uint32_t>(list[i] >> 32));
+    for (uint32_t i = tid; i < n; i += kThreads) each(static_cast<uint32_t>(list[i] >> 32), static_cast<uint32_t>(list[i]));
   };
   auto from_row = [&](auto each) {
-    over_chunks<DT>(row, 0, p.chunks, [&](int, const float (&x)[E]) {
+    over_chunks<DT>(row, 0, p.chunks, [&](int q, const float (&x)[E]) {
+      const int t = row.token(q);
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (x[e] > -__builtin_inff()) each(key_of(x[e]));
+        if (x[e] > -__builtin_inff()) each(key_of(x[e]), static_cast<uint32_t>(t + e));
     });
   };
-  const bool cut = border < kWeightBins;  // (without, all tokens of any weight are kept: fewer than k, as it is)
-  Edge edge{0, ~uint64_t{0}};
+  const bool cut = border < kWeightBins;  // (without: fewer than k tokens have a weight)
+  Edge edge{0, ~0u};
   if (cut || r.top_p < 1.0) {
     Row rr = r;
-    if (!cut) rr.mode = TOP_P;  // (fewer tokens of any weight than k)
+    if (!cut) rr.mode = TOP_P;
     edge = fits ? edge_of(rr, bins, from_list, r.mode == TOP_P ? above : 0, whole) : edge_of(rr, bins, from_row, 0, whole);
   }
-  const uint64_t at_edge = r.kept_weight(value_of(edge.key));
   __syncthreads();
-  auto chunk_of = [&](uint32_t token) { return (token + row.before) / (64 * E); };
-  auto add = [&](uint32_t chunk, uint64_t w) { atomicAdd(reinterpret_cast<unsigned long long*>(&sums[chunk]), static_cast<unsigned long long>(w)); };
-  auto weight = [&](float x, uint32_t key, uint64_t ties) { return key > edge.key ? r.kept_weight(x) : key == edge.key && ties < edge.ties ? at_edge : 0; };
+  auto weight = [&](float x, int token) { return edge.keeps(key_of(x), static_cast<uint32_t>(token)) ? r.kept_weight(x) : 0; };
   if (fits) {
-    // A token of the edge is kept if fewer than `ties` of its equals come before it.
     for (uint32_t i = tid; i < n; i += kThreads) {
-      const uint32_t key = static_cast<uint32_t>(list[i] >> 32), token = static_cast<uint32_t>(list[i]);
-      if (key < edge.key) continue;
-      uint64_t ties = 0;
-      if (key == edge.key && edge.ties < n)
-        for (uint32_t j = 0; j < n; ++j) ties += (list[j] >> 32) == key && static_cast<uint32_t>(list[j]) < token;
-      const uint64_t w = weight(value_of(key), key, ties);
-      if (w) add(chunk_of(token), w);
+      const uint32_t token = static_cast<uint32_t>(list[i]);
+      const uint64_t w = weight(value_of(static_cast<uint32_t>(list[i] >> 32)), static_cast<int>(token));
+      if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sums[(token + row.before) / (64 * E)]), static_cast<unsigned long long>(w));
     }
-    __syncthreads();
-    draw<DT>(p, r, row, s.row, sums, edge.key, weight, [&](int first) {
-      uint64_t ties = 0;
-      for (uint32_t j = lane; j < n; j += 64) ties += (list[j] >> 32) == edge.key && static_cast<int>(static_cast<uint32_t>(list[j])) < first;
-      return wave_sum(ties);
-    });
-    return;
-  }
-  // The whole row again: chunks' weights above the edge and equals of it, then how many of those are kept.
-  uint32_t* equals = reinterpret_cast<uint32_t*>(list);
-  static_assert(sizeof(list) >= kMostChunks * sizeof(uint32_t), "");
-  over_chunks<DT>(row, 0, p.chunks, [&](int q, const float (&x)[E]) {
-    uint64_t sum = 0, equal = 0;
+  } else {
+    over_chunks<DT>(row, 0, p.chunks, [&](int q, const float (&x)[E]) {
+      const int t = row.token(q);
+      uint64_t sum = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint32_t key = key_of(x[e]);
-      if (!(x[e] > -__builtin_inff())) continue;
-      if (key > edge.key) sum += r.kept_weight(x[e]);
-      equal += key == edge.key;
-    }
-    sum = wave_sum(sum);
-    equal = wave_sum(equal);
-    if (lane == 0) {
-      sums[q] = sum;
-      equals[q] = static_cast<uint32_t>(equal);
-    }
-  });
-  __syncthreads();
-  if (tid < 64) {  // equals[q] becomes how many come before chunk q
-    uint64_t before = 0;
-    for (int q0 = 0; q0 < p.chunks; q0 += 64) {
-      const uint64_t equal = q0 + lane < p.chunks ? equals[q0 + lane] : 0, upto = wave_scan(equal) + before, start = upto - equal;
-      if (q0 + lane < p.chunks) {
-        sums[q0 + lane] += (min(upto, edge.ties) - min(start, edge.ties)) * at_edge;
-        equals[q0 + lane] = static_cast<uint32_t>(start);
-      }
-      before = __shfl(upto, 63);
-    }
+      for (int e = 0; e < E; ++e)
+        if (x[e] > -__builtin_inff()) sum += weight(x[e], t + e);
+      sum = wave_sum(sum);
+      if (lane == 0) sums[q] = sum;
+    });
   }
   __syncthreads();
-  draw<DT>(p, r, row, s.row, sums, edge.key, weight, [&](int first) { return static_cast<uint64_t>(equals[chunk_of(static_cast<uint32_t>(first < 0 ? 0 : first))]); });
+  draw<DT>(p, r, row, s.row, sums, weight);
 }
 
 }  // namespace

@@ -285,7 +285,8 @@ __global__ __launch_bounds__(kThreads) void k_sample_top(SampleArgs p) {
 __device__ __forceinline__ Row row_of(const SampleArgs& p, int64_t r) {
   Row row;
   uint64_t best = 0;
-  for (int i = 0; i < p.slices; ++i) best = max(best, p.best[r * p.slices + i]);
+  for (int i = threadIdx.x & 63; i < p.slices; i += 64) best = max(best, p.best[r * p.slices + i]);
+  best = wave_max(best);
   row.top_key = static_cast<uint32_t>(best >> 32);
   row.top_index = static_cast<uint32_t>(~best);
   row.top = value_of(row.top_key);
@@ -545,6 +546,44 @@ __global__ __launch_bounds__(kThreads) void k_sample_sum(SampleArgs p) {
   }
 }
 
+// A row by top-k whose list has up to 64 tokens, a lane each, by one wavefront: what comes before a token by logit, and of what is kept
+// by index, is summed over the lanes one after another.
+__device__ __forceinline__ void draw_few(const SampleArgs& p, const Row& r, int64_t at_row, const uint64_t* list, int n, int lane) {
+  const bool there = lane < n;
+  const uint64_t mine = there ? list[lane] : 0;
+  const uint32_t key = static_cast<uint32_t>(mine >> 32), token = static_cast<uint32_t>(mine);
+  uint64_t w = there ? r.weight(value_of(key)) : 0;
+  auto of_lane = [](uint64_t v, int i) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), i))) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), i));
+  };
+  int rank = 0;
+  uint64_t before = 0;
+  for (int i = 0; i < n; ++i) {
+    const uint64_t other = of_lane(mine, i), weight = of_lane(w, i);
+    const uint32_t k = static_cast<uint32_t>(other >> 32), t = static_cast<uint32_t>(other);
+    const bool ahead = k > key || (k == key && t < token);
+    rank += ahead;
+    before += ahead ? weight : 0;
+  }
+  bool kept = there && rank < r.k;
+  if (r.top_p < 1.0) {
+    const double need = fmax(r.top_p * static_cast<double>(wave_sum(kept ? w : 0)), 1.0);
+    kept = kept && static_cast<double>(before) < need;
+  }
+  w = kept ? r.kept_weight(value_of(key)) : 0;
+  const uint64_t total = wave_sum(w);
+  before = 0;
+  for (int i = 0; i < n; ++i) {
+    const uint64_t weight = of_lane(w, i);
+    const uint32_t t = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(token), i));
+    before += t < token ? weight : 0;
+  }
+  const double target = static_cast<double>(r.u) * static_cast<double>(total);
+  auto past = [&](uint64_t sum) { return static_cast<double>(sum) > target || sum == total; };
+  if (w && past(before + w) && !(before && past(before))) p.tokens[at_row] = token;
+}
+
 template <int DT>
 __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
   constexpr int E = Chunks<DT>::E;
@@ -620,6 +659,10 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
   };
   const bool cut = border < kWeightBins;  // (without: fewer than k tokens have a weight)
   Edge edge{0, ~0u};
+  if (n <= 64 && r.mode == TOP_K) {
+    if (tid < 64) draw_few(p, r, s.row, list, static_cast<int>(n), lane);
+    return;
+  }
   if (cut || r.top_p < 1.0) {
     Row rr = r;
     if (!cut) rr.mode = TOP_P;

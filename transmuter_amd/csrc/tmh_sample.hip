@@ -64,23 +64,23 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 constexpr uint32_t kLowestKey = 0x007FFFFFu;  // of -infinity
 
-// 2^x, x <= 0, in 64 bits: 2^n e^y with y = (x - n) ln 2 of magnitude up to 0.35, whose series ends with y^11 / 11! (the
-// next term is 2^-47, an eighth of a unit).
-__device__ __forceinline__ double exp2_of(double x) {
-  const double n = __builtin_rint(x), y = (x - n) * 0.69314718055994530942;
-  double s = 1.0 / 39916800.0;
-  s = fma(s, y, 1.0 / 3628800.0);
-  s = fma(s, y, 1.0 / 362880.0);
-  s = fma(s, y, 1.0 / 40320.0);
-  s = fma(s, y, 1.0 / 5040.0);
-  s = fma(s, y, 1.0 / 720.0);
-  s = fma(s, y, 1.0 / 120.0);
-  s = fma(s, y, 1.0 / 24.0);
-  s = fma(s, y, 1.0 / 6.0);
-  s = fma(s, y, 0.5);
-  s = fma(s, y, 1.0);
-  s = fma(s, y, 1.0);
-  return __builtin_amdgcn_ldexp(s, static_cast<int>(n));
+// 2^(j / 128) in units of 2^-44 of 1, j < 128, in LDS: e^y with y = j ln 2 / 128 up to 0.7, whose series ends with y^15 / 15! (the next
+// term is below 2^-53).
+constexpr int kSteps = 128;
+__device__ __forceinline__ const double* powers() {
+  __shared__ double table[kSteps];
+  if (threadIdx.x < kSteps) {
+    const double y = threadIdx.x * (0.69314718055994530942 / kSteps);
+    double term = 0x1p44, sum = 0x1p44;
+#pragma unroll
+    for (int i = 1; i <= 15; ++i) {
+      term *= y * (1.0 / i);
+      sum += term;
+    }
+    table[threadIdx.x] = sum;
+  }
+  __syncthreads();
+  return table;
 }
 
 // What a row's WG knows of its row.
@@ -89,51 +89,67 @@ struct Row {
   int k;
   float top;          // the largest logit
   uint32_t top_key, top_index;
-  double c;           // log2(e) / temperature
+  double c;           // 128 log2(e) / temperature
+  const double* table;  // of powers()
   float per_bin;      // bins a logit
-  double top_p, least;  // least: the smallest weight that min-p keeps
+  double top_p, least;  // least: the smallest weight that min-p keeps, in units
   float low;          // logits below it are certainly left out by min-p, or weigh nothing
   float u;
-  // exp((x - top) / temperature) in units of 2^-44; 0 where it is less than one.
-  __device__ __forceinline__ uint64_t weight(float x) const {
-    if (top == __builtin_inff()) return x == top ? uint64_t{1} << kUnit : 0;
-    const double e = (static_cast<double>(x) - static_cast<double>(top)) * c;
-    if (!(e >= -kUnit)) return 0;
-    return static_cast<uint64_t>(__builtin_rint(exp2_of(e) * 0x1p44));
+  // exp((x - top) / temperature) in units of 2^-44, not rounded; 0 where it is less than one. It is 2^(t / 128): the whole part n of t gives
+  // a power of two and a place of the table, the rest z, up to a half, 2^(z / 128) by its series up to z^4 (the next term is 2^-49).
+  __device__ __forceinline__ double units(float x) const {
+    constexpr double kRound = 0x1.8p52;  // (added, its low bits are the whole part)
+    if (top == __builtin_inff()) return x == top ? 0x1p44 : 0.0;
+    const double t = (static_cast<double>(x) - static_cast<double>(top)) * c;
+    if (!(t >= -kUnit * kSteps)) return 0.0;
+    const double whole = t + kRound, z = t - (whole - kRound);
+    const int n = static_cast<int>(__builtin_bit_cast(uint64_t, whole));
+    constexpr double l = 0.69314718055994530942 / kSteps;
+    double s = fma(z, l * l * l * l / 24.0, l * l * l / 6.0);
+    s = fma(s, z, l * l / 2.0);
+    s = fma(s, z, l);
+    s = fma(s, z, 1.0) * table[n & (kSteps - 1)];
+    return __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, s) + (static_cast<uint64_t>(static_cast<uint32_t>(n >> 7) << 20) << 32));
   }
+  // A whole number of units: added to 2^52, the low bits.
+  static __device__ __forceinline__ uint64_t rounded(double units) { return __builtin_bit_cast(uint64_t, units + 0x1p52) & ((uint64_t{1} << 52) - 1); }
+  __device__ __forceinline__ uint64_t weight(float x) const { return rounded(units(x)); }
   // The same, 0 where min-p leaves the token out.
   __device__ __forceinline__ uint64_t kept_weight(float x) const {
-    if (top == __builtin_inff()) return x == top ? uint64_t{1} << kUnit : 0;
-    const double e = (static_cast<double>(x) - static_cast<double>(top)) * c;
-    if (!(e >= -kUnit)) return 0;
-    const double w = exp2_of(e);
-    return w >= least ? static_cast<uint64_t>(__builtin_rint(w * 0x1p44)) : 0;
+    const double w = units(x);
+    return w >= least ? rounded(w) : 0;
   }
   // The bin of a logit: of the largest 0, kWeightBins and more where it has no weight. Not falling as logits fall.
   __device__ __forceinline__ int bin(float x) const {
-    if (!(x > -__builtin_inff())) return kWeightBins;
-    if (x == top) return 0;
-    return static_cast<int>(fminf((top - x) * per_bin, static_cast<float>(kWeightBins)));
+    const float b = fminf((top - x) * per_bin, static_cast<float>(kWeightBins));  // (of NaN the other)
+    return x == top ? 0 : static_cast<int>(b);
   }
 };
 
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  return v;
+// The sum over the lanes up to this one: within rows of 16 lanes, then the rows' last lanes to the rows behind (DPP moves; a lane that
+// a move does not reach adds 0).
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ uint64_t moved(uint64_t v) {
+  const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CONTROL, ROWS, 0xF, false);
+  const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CONTROL, ROWS, 0xF, false);
+  return static_cast<uint64_t>(high) << 32 | low;
 }
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
+  v += moved<0x111, 0xF>(v);
+  v += moved<0x112, 0xF>(v);
+  v += moved<0x114, 0xF>(v);
+  v += moved<0x118, 0xF>(v);
+  v += moved<0x142, 0xA>(v);
+  return v + moved<0x143, 0xC>(v);
+}
+__device__ __forceinline__ uint64_t of_lane(uint64_t v, int i) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), i))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), i));
+}
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return of_lane(wave_scan(v), 63); }
 __device__ __forceinline__ uint64_t wave_max(uint64_t v) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) v = max(v, static_cast<uint64_t>(__shfl_xor(v, o)));
-  return v;
-}
-// The sum over the lanes up to this one.
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t up = __shfl_up(v, o);
-    if ((threadIdx.x & 63) >= o) v += up;
-  }
   return v;
 }
 __device__ __forceinline__ void put64(uint64_t* p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -182,26 +198,37 @@ struct Chunks {
   }
 };
 
-// Calls each(q, logits) for the chunks [from, to), a wavefront taking every kWaves-th, with four loads on their way.
-template <int DT, typename Each>
-__device__ __forceinline__ void over_chunks(const Chunks<DT>& row, int from, int to, Each each) {
-  constexpr int AHEAD = 4;
-  const int wave = threadIdx.x >> 6;
-  for (int q0 = from + wave; q0 < to; q0 += AHEAD * kWaves) {
-    uint4_t v[AHEAD];
+// Calls each(q, logits) for the chunks [from, to), a wavefront taking every kWaves-th, with kAhead loads on their way; the first of them
+// are loaded where it is made.
+constexpr int kAhead = 4;
+template <int DT>
+struct OverChunks {
+  const Chunks<DT>& row;
+  int from, to;
+  uint4_t v[kAhead];
+  __device__ __forceinline__ void load(int q0) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
+    for (int i = 0; i < kAhead; ++i)
       if (q0 + i * kWaves < to) v[i] = row.raw(q0 + i * kWaves);
+  }
+  __device__ __forceinline__ OverChunks(const Chunks<DT>& r, int first, int end) : row(r), from(first + static_cast<int>(threadIdx.x >> 6)), to(end) {
+    load(from);
+  }
+  template <typename Each>
+  __device__ __forceinline__ void operator()(Each each) {
+    for (int q0 = from; q0 < to; q0 += kAhead * kWaves) {
+      if (q0 != from) load(q0);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const int q = q0 + i * kWaves;
-      if (q >= to) break;
-      float x[Chunks<DT>::E];
-      row.logits(q, v[i], x);
-      each(q, x);
+      for (int i = 0; i < kAhead; ++i) {
+        const int q = q0 + i * kWaves;
+        if (q >= to) break;
+        float x[Chunks<DT>::E];
+        row.logits(q, v[i], x);
+        each(q, x);
+      }
     }
   }
-}
+};
 
 struct Slice {
   int64_t row;
@@ -267,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_top(SampleArgs p) {
   const Slice s = slice_of(p);
   const Chunks<DT> row(p, s.row);
   uint32_t top = 0, at = 0;  // (a thread's tokens come in their order: the first of equals stays)
-  over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[Chunks<DT>::E]) {
+  OverChunks<DT>(row, s.from, s.to)([&](int q, const float (&x)[Chunks<DT>::E]) {
     const int t = row.token(q);
 #pragma unroll
     for (int e = 0; e < Chunks<DT>::E; ++e) {
@@ -284,6 +311,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_top(SampleArgs p) {
 // A row's choices; in GREEDY rows the token is known (the largest; -1 where no logit is above -infinity).
 __device__ __forceinline__ Row row_of(const SampleArgs& p, int64_t r) {
   Row row;
+  row.table = powers();
   uint64_t best = 0;
   for (int i = threadIdx.x & 63; i < p.slices; i += 64) best = max(best, p.best[r * p.slices + i]);
   best = wave_max(best);
@@ -291,15 +319,16 @@ __device__ __forceinline__ Row row_of(const SampleArgs& p, int64_t r) {
   row.top_index = static_cast<uint32_t>(~best);
   row.top = value_of(row.top_key);
   const float temperature = p.temperature ? p.temperature[r] : 1.f;
-  row.c = 1.4426950408889634074 / static_cast<double>(temperature);
-  row.per_bin = static_cast<float>(row.c * kPerOctave);
+  row.c = kSteps * 1.4426950408889634074 / static_cast<double>(temperature);
+  row.per_bin = static_cast<float>(row.c * (1.0 * kPerOctave / kSteps));
   row.k = p.top_k ? p.top_k[r] : 0;
   row.top_p = p.top_p ? p.top_p[r] : 1.0;
   const float min_p = p.min_p ? p.min_p[r] : 0.f;
-  row.least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+  row.least = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) * 0x1p44 : 0.0;
   row.u = p.u[r];
   // (A factor of two below: more than f32's roundings are.)
-  row.low = row.top == __builtin_inff() ? row.top : row.top - static_cast<float>((1.0 - (row.least > 0.0 ? fmax(log2(row.least), -1.0 * kUnit) : -1.0 * kUnit)) / row.c);
+  const float octaves = 1.f + (min_p > 0.f ? fminf(-log2f(fminf(min_p, 1.f)), kUnit) : kUnit);
+  row.low = row.top == __builtin_inff() ? row.top : static_cast<float>(row.top - octaves * kSteps / row.c);
   row.mode = !(temperature > 0.f) || row.top_key == kLowestKey ? GREEDY : row.k > 0 && row.k < p.vocabulary ? TOP_K : row.top_p < 1.0 ? TOP_P : ALL;
   return row;
 }
@@ -375,9 +404,13 @@ __device__ __forceinline__ uint32_t select(uint64_t* bins, Items items, Reached 
     return static_cast<uint64_t>(x) << 32 | y;
   };
   uint64_t ends = static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(~low);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) ends = both(ends, __shfl_xor(ends, o));
-  ends = block_join(ends, both);
+  ends = both(ends, moved<0x111, 0xF>(ends));
+  ends = both(ends, moved<0x112, 0xF>(ends));
+  ends = both(ends, moved<0x114, 0xF>(ends));
+  ends = both(ends, moved<0x118, 0xF>(ends));
+  ends = both(ends, moved<0x142, 0xA>(ends));
+  ends = both(ends, moved<0x143, 0xC>(ends));
+  ends = block_join(of_lane(ends, 63), both);
   low = ~static_cast<uint32_t>(ends);
   high = static_cast<uint32_t>(ends >> 32);
   above = 0;
@@ -387,6 +420,7 @@ __device__ __forceinline__ uint32_t select(uint64_t* bins, Items items, Reached 
   while (true) {
     bins[2 * tid] = 0;
     bins[2 * tid + 1] = 0;
+    if (tid == 0) found_digit = ~0u;
     __syncthreads();
     items([&](uint32_t key, uint64_t measure) {
       if (key >= base && key - base <= span)
@@ -395,24 +429,19 @@ __device__ __forceinline__ uint32_t select(uint64_t* bins, Items items, Reached 
     __syncthreads();
     // Each thread two digits, from the highest down.
     const uint32_t digit = kDigits - 1 - 2 * tid;
-    const uint64_t first = bins[digit], second = bins[digit - 1];
+    const uint64_t first = bins[digit], second = bins[digit - 1], lowest = bins[0];
     uint64_t all;
-    uint64_t before = block_scan(first + second, all) + above;
-    // (The first to reach it; the lowest that there is, should the sums not.)
-    const bool here = (first + second) && reached(before + first + second) && !(before != above && reached(before));
-    if (tid == 0) {
-      found_digit = 0;
-      found_sum = above + all - (bins[0]);
-    }
-    __syncthreads();
-    if (here) {
+    const uint64_t before = block_scan(first + second, all) + above;
+    // The first to reach it.
+    if ((first + second) && reached(before + first + second) && !(before != above && reached(before))) {
       const bool upper = first && reached(before + first);
       found_digit = upper ? digit : digit - 1;
       found_sum = upper ? before : before + first;
     }
     __syncthreads();
-    above = found_sum;
-    base += found_digit << shift;
+    const uint32_t found = found_digit;
+    above = found == ~0u ? above + all - lowest : found_sum;  // (the lowest that there is, should the sums not reach it)
+    base += (found == ~0u ? 0 : found) << shift;
     if (shift == 0) return base;
     span = (1u << shift) - 1;
     shift = max(shift - 11, 0);
@@ -436,14 +465,17 @@ struct Edge {
   uint32_t key, last;
   __device__ __forceinline__ bool keeps(uint32_t k, uint32_t token) const { return k > key || (k == key && token <= last); }
 };
-template <typename Items>
+template <int DT, typename Items>
 __device__ __forceinline__ Edge edge_of(const Row& r, uint64_t* bins, Items items, uint64_t above, uint64_t whole) {
+  // (The low bits of 16-bit types' keys are all alike, 0 or, of numbers below 0, 1.)
+  constexpr int QUIET = DT == DT_F32 ? 0 : DT == DT_F16 ? 13 : 16;
+  auto key_again = [](uint32_t k) { return k << QUIET | (k >> (31 - QUIET) ? 0 : (1u << QUIET) - 1); };
   uint32_t edge = 0;
   uint64_t ties = ~uint64_t{0};
   if (r.mode == TOP_K) {
     uint64_t more;
-    edge = select(bins, [&](auto each) { items([&](uint32_t key, uint32_t) { each(key, uint64_t{1}); }); },
-                  [&](uint64_t sum) { return sum >= static_cast<uint64_t>(r.k); }, more);
+    edge = key_again(select(bins, [&](auto each) { items([&](uint32_t key, uint32_t) { each(key >> QUIET, uint64_t{1}); }); },
+                            [&](uint64_t sum) { return sum >= static_cast<uint64_t>(r.k); }, more));
     ties = static_cast<uint64_t>(r.k) - more;
   }
   if (r.top_p < 1.0) {
@@ -462,8 +494,8 @@ __device__ __forceinline__ Edge edge_of(const Row& r, uint64_t* bins, Items item
     const double need = fmax(r.top_p * static_cast<double>(whole), 1.0);  // (one token at least)
     const uint32_t by_k = edge;
     uint64_t more;
-    edge = select(bins, [&](auto each) { items([&](uint32_t key, uint32_t) { if (key >= by_k) each(key, r.weight(value_of(key))); }); },
-                  [&](uint64_t sum) { return static_cast<double>(above + sum) >= need; }, more);
+    edge = key_again(select(bins, [&](auto each) { items([&](uint32_t key, uint32_t) { if (key >= by_k) each(key >> QUIET, r.weight(value_of(key))); }); },
+                            [&](uint64_t sum) { return static_cast<double>(above + sum) >= need; }, more));
     ties = equals_needed(need, above + more, r.weight(value_of(edge)));
     if (edge == by_k) ties = min(ties, at_edge);
   }
@@ -481,16 +513,17 @@ __global__ __launch_bounds__(kThreads) void k_sample_sum(SampleArgs p) {
   __shared__ uint64_t bins[kMostChunks];  // (or, for the draw, the chunks' weights)
   static_assert(kMostChunks >= kWeightBins, "");
   const Slice s = slice_of(p);
+  const Chunks<DT> row(p, s.row);
+  OverChunks<DT> over(row, s.from, s.to);
   const Row r = row_of(p, s.row);
   const int tid = threadIdx.x, lane = tid & 63;
   if (r.mode == GREEDY) {
     if (s.at == 0 && tid == 0) p.tokens[s.row] = r.top_key == kLowestKey ? -1 : static_cast<int64_t>(r.top_index);
     return;
   }
-  const Chunks<DT> row(p, s.row);
   uint64_t* sums = p.sums + s.row * p.chunks;
   if (r.mode == ALL) {
-    over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[E]) {
+    over([&](int q, const float (&x)[E]) {
       uint64_t sum = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e)
@@ -506,7 +539,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_sum(SampleArgs p) {
   }
   for (int i = tid; i < kWeightBins; i += kThreads) bins[i] = 0;
   __syncthreads();
-  over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[E]) {
+  over([&](int q, const float (&x)[E]) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int b = r.bin(x[e]);
@@ -553,10 +586,6 @@ __device__ __forceinline__ void draw_few(const SampleArgs& p, const Row& r, int6
   const uint64_t mine = there ? list[lane] : 0;
   const uint32_t key = static_cast<uint32_t>(mine >> 32), token = static_cast<uint32_t>(mine);
   uint64_t w = there ? r.weight(value_of(key)) : 0;
-  auto of_lane = [](uint64_t v, int i) {
-    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), i))) << 32 |
-           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), i));
-  };
   int rank = 0;
   uint64_t before = 0;
   for (int i = 0; i < n; ++i) {
@@ -592,10 +621,11 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
   __shared__ uint64_t sums[kMostChunks];
   __shared__ uint32_t count;
   const Slice s = slice_of(p);
+  const Chunks<DT> row(p, s.row);
+  OverChunks<DT> over(row, s.from, s.to);
   const Row r = row_of(p, s.row);
   const int tid = threadIdx.x, lane = tid & 63;
   if (r.mode == GREEDY || r.mode == ALL) return;
-  const Chunks<DT> row(p, s.row);
   const uint32_t border = static_cast<uint32_t>(p.told[4 * s.row]);
   const uint64_t above = p.told[4 * s.row + 1], whole = p.told[4 * s.row + 2];
   uint64_t* all_sums = p.sums + s.row * p.chunks;
@@ -603,7 +633,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
   uint32_t* counts = p.counts + s.row * p.slices;
   if (tid == 0) count = 0;
   __syncthreads();
-  over_chunks<DT>(row, s.from, s.to, [&](int q, const float (&x)[E]) {
+  over([&](int q, const float (&x)[E]) {
     const int t = row.token(q);
     uint64_t sum = 0;
 #pragma unroll
@@ -650,7 +680,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
     for (uint32_t i = tid; i < n; i += kThreads) each(static_cast<uint32_t>(list[i] >> 32), static_cast<uint32_t>(list[i]));
   };
   auto from_row = [&](auto each) {
-    over_chunks<DT>(row, 0, p.chunks, [&](int q, const float (&x)[E]) {
+    OverChunks<DT>(row, 0, p.chunks)([&](int q, const float (&x)[E]) {
       const int t = row.token(q);
 #pragma unroll
       for (int e = 0; e < E; ++e)
@@ -666,7 +696,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
   if (cut || r.top_p < 1.0) {
     Row rr = r;
     if (!cut) rr.mode = TOP_P;
-    edge = fits ? edge_of(rr, bins, from_list, r.mode == TOP_P ? above : 0, whole) : edge_of(rr, bins, from_row, 0, whole);
+    edge = fits ? edge_of<DT>(rr, bins, from_list, r.mode == TOP_P ? above : 0, whole) : edge_of<DT>(rr, bins, from_row, 0, whole);
   }
   __syncthreads();
   auto weight = [&](float x, int token) { return edge.keeps(key_of(x), static_cast<uint32_t>(token)) ? r.kept_weight(x) : 0; };
@@ -677,7 +707,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
       if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sums[(token + row.before) / (64 * E)]), static_cast<unsigned long long>(w));
     }
   } else {
-    over_chunks<DT>(row, 0, p.chunks, [&](int q, const float (&x)[E]) {
+    OverChunks<DT>(row, 0, p.chunks)([&](int q, const float (&x)[E]) {
       const int t = row.token(q);
       uint64_t sum = 0;
 #pragma unroll

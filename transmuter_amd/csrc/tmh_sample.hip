@@ -26,7 +26,6 @@ constexpr int kUnit = 44;
 constexpr int kPerOctave = 16, kWeightBins = kPerOctave * kUnit + 4;  // (a few more than have weights: bins are found in f32)
 constexpr int kList = 4096;        // tokens of a row's list
 constexpr int kDigits = 2048;      // of a selection's turn
-constexpr int kMostChunks = (1 << 20) / 256 + 1;
 constexpr int kMostRows = 512;     // of a launch: each has a counter
 
 enum Mode : int { GREEDY, ALL, TOP_K, TOP_P };
@@ -198,17 +197,16 @@ struct Chunks {
   }
 };
 
-// Calls each(q, logits) for the chunks [from, to), a wavefront taking every kWaves-th, with kAhead loads on their way; the first of them
+// Calls each(q, logits) for the chunks [from, to), a wavefront taking every kWaves-th, with AHEAD loads on their way; the first of them
 // are loaded where it is made.
-constexpr int kAhead = 4;
-template <int DT>
+template <int DT, int AHEAD = 4>
 struct OverChunks {
   const Chunks<DT>& row;
   int from, to;
-  uint4_t v[kAhead];
+  uint4_t v[AHEAD];
   __device__ __forceinline__ void load(int q0) {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
+    for (int i = 0; i < AHEAD; ++i)
       if (q0 + i * kWaves < to) v[i] = row.raw(q0 + i * kWaves);
   }
   __device__ __forceinline__ OverChunks(const Chunks<DT>& r, int first, int end) : row(r), from(first + static_cast<int>(threadIdx.x >> 6)), to(end) {
@@ -216,10 +214,10 @@ struct OverChunks {
   }
   template <typename Each>
   __device__ __forceinline__ void operator()(Each each) {
-    for (int q0 = from; q0 < to; q0 += kAhead * kWaves) {
+    for (int q0 = from; q0 < to; q0 += AHEAD * kWaves) {
       if (q0 != from) load(q0);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
+      for (int i = 0; i < AHEAD; ++i) {
         const int q = q0 + i * kWaves;
         if (q >= to) break;
         float x[Chunks<DT>::E];
@@ -510,8 +508,7 @@ __device__ __forceinline__ Edge edge_of(const Row& r, uint64_t* bins, Items item
 template <int DT>
 __global__ __launch_bounds__(kThreads) void k_sample_sum(SampleArgs p) {
   constexpr int E = Chunks<DT>::E;
-  __shared__ uint64_t bins[kMostChunks];  // (or, for the draw, the chunks' weights)
-  static_assert(kMostChunks >= kWeightBins, "");
+  extern __shared__ uint64_t bins[];  // kWeightBins (or, for the draw, the chunks' weights)
   const Slice s = slice_of(p);
   const Chunks<DT> row(p, s.row);
   OverChunks<DT> over(row, s.from, s.to);
@@ -618,7 +615,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
   constexpr int E = Chunks<DT>::E;
   __shared__ uint64_t bins[kDigits];
   __shared__ uint64_t list[kList];  // key << 32 | token
-  __shared__ uint64_t sums[kMostChunks];
+  extern __shared__ uint64_t sums[];  // of each chunk
   __shared__ uint32_t count;
   const Slice s = slice_of(p);
   const Chunks<DT> row(p, s.row);
@@ -680,7 +677,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
     for (uint32_t i = tid; i < n; i += kThreads) each(static_cast<uint32_t>(list[i] >> 32), static_cast<uint32_t>(list[i]));
   };
   auto from_row = [&](auto each) {
-    OverChunks<DT>(row, 0, p.chunks)([&](int q, const float (&x)[E]) {
+    OverChunks<DT, 1>(row, 0, p.chunks)([&](int q, const float (&x)[E]) {
       const int t = row.token(q);
 #pragma unroll
       for (int e = 0; e < E; ++e)
@@ -707,7 +704,7 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
       if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sums[(token + row.before) / (64 * E)]), static_cast<unsigned long long>(w));
     }
   } else {
-    OverChunks<DT>(row, 0, p.chunks)([&](int q, const float (&x)[E]) {
+    OverChunks<DT, 1>(row, 0, p.chunks)([&](int q, const float (&x)[E]) {
       const int t = row.token(q);
       uint64_t sum = 0;
 #pragma unroll
@@ -748,8 +745,9 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
   p.ld = ld;
   p.vocabulary = static_cast<int>(V);
   p.chunks = static_cast<int>((V + 16 / size - 1 + chunk - 1) / chunk);  // (rows that begin inside 16 bytes may take one more)
-  // Two workgroups a CU in all, of a chunk a wavefront at least.
-  p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2 * ctx->num_cus / rows, p.chunks / kWaves)));
+  // A workgroup a CU in all (the registers of the weights' pass leave room for one; 64 rows of 151936 bf16 in us: 68 so, 81 with
+  // two a CU, that take turns), of a chunk a wavefront at least.
+  p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctx->num_cus / rows, p.chunks / kWaves)));
   const size_t of_rows = static_cast<size_t>(rows) * p.slices;
   const size_t bytes = 8 * (of_rows * (1 + kWeightBins + (p.slices > 1 ? kList : 0)) + static_cast<size_t>(rows) * (p.chunks + 4)) + 4 * of_rows;
   void* ws = workspace(ctx, bytes, s);
@@ -774,8 +772,8 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
     auto launch = [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
       k_sample_top<DT><<<grid, kThreads, 0, s>>>(p);
-      k_sample_sum<DT><<<grid, kThreads, 0, s>>>(p);
-      if (d_top_k || d_top_p) k_sample_draw<DT><<<grid, kThreads, 0, s>>>(p);
+      k_sample_sum<DT><<<grid, kThreads, 8 * std::max(kWeightBins, p.chunks), s>>>(p);
+      if (d_top_k || d_top_p) k_sample_draw<DT><<<grid, kThreads, 8 * p.chunks, s>>>(p);
     };
     if (dtype == TMH_F32) launch(std::integral_constant<int, DT_F32>{});
     else if (dtype == TMH_F16) launch(std::integral_constant<int, DT_F16>{});

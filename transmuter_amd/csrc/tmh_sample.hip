@@ -8,6 +8,7 @@
 //                 Others, by top-p alone: the weights of each bin, and the bin in which they reach top-p of the whole.
 //  k_sample_draw  rows by top-k: the tokens down to that bin go to a list. By top-p alone: those of that bin do, and the weights above
 //                 it to chunks. The list, sorted out in LDS, gives the least logit kept and the last of its equals that is; then the draw.
+// Rows of at most kList tokens are a list from the start: k_sample_short, one kernel and a workgroup a row.
 // A list that does not fit (thousands of tokens of almost the same logit) leaves its row to the last workgroup, which goes over all
 // of it a few times.
 #include <algorithm>
@@ -307,12 +308,9 @@ __global__ __launch_bounds__(kThreads) void k_sample_top(SampleArgs p) {
 }
 
 // A row's choices; in GREEDY rows the token is known (the largest; -1 where no logit is above -infinity).
-__device__ __forceinline__ Row row_of(const SampleArgs& p, int64_t r) {
+__device__ __forceinline__ Row row_of(const SampleArgs& p, int64_t r, uint64_t best) {
   Row row;
   row.table = powers();
-  uint64_t best = 0;
-  for (int i = threadIdx.x & 63; i < p.slices; i += 64) best = max(best, p.best[r * p.slices + i]);
-  best = wave_max(best);
   row.top_key = static_cast<uint32_t>(best >> 32);
   row.top_index = static_cast<uint32_t>(~best);
   row.top = value_of(row.top_key);
@@ -329,6 +327,12 @@ __device__ __forceinline__ Row row_of(const SampleArgs& p, int64_t r) {
   row.low = row.top == __builtin_inff() ? row.top : static_cast<float>(row.top - octaves * kSteps / row.c);
   row.mode = !(temperature > 0.f) || row.top_key == kLowestKey ? GREEDY : row.k > 0 && row.k < p.vocabulary ? TOP_K : row.top_p < 1.0 ? TOP_P : ALL;
   return row;
+}
+
+__device__ __forceinline__ Row row_of(const SampleArgs& p, int64_t r) {
+  uint64_t best = 0;
+  for (int i = threadIdx.x & 63; i < p.slices; i += 64) best = max(best, p.best[r * p.slices + i]);
+  return row_of(p, r, wave_max(best));
 }
 
 // The draw: the first token, by index, up to which the weights sum to more than u of their whole. sums: of each chunk, in LDS.
@@ -610,6 +614,58 @@ __device__ __forceinline__ void draw_few(const SampleArgs& p, const Row& r, int6
   if (w && past(before + w) && !(before && past(before))) p.tokens[at_row] = token;
 }
 
+// A row of up to kList tokens by one workgroup, as the others do the tokens of a list.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_sample_short(SampleArgs p) {
+  constexpr int E = Chunks<DT>::E;
+  __shared__ uint64_t bins[kDigits];
+  __shared__ uint32_t keys[kList];
+  extern __shared__ uint64_t sums[];  // of each chunk
+  const int64_t at = blockIdx.x;
+  const Chunks<DT> row(p, at);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const uint32_t n = static_cast<uint32_t>(p.vocabulary);
+  uint64_t best = 0;
+  OverChunks<DT>(row, 0, p.chunks)([&](int q, const float (&x)[E]) {
+    const int t = row.token(q);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (t + e < 0 || t + e >= row.n) continue;
+      const uint32_t key = key_of(x[e]);
+      keys[t + e] = key;
+      best = max(best, static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~(t + e)));
+    }
+  });
+  const Row r = row_of(p, at, block_join(wave_max(best), [](uint64_t a, uint64_t b) { return max(a, b); }));
+  if (r.mode == GREEDY) {
+    if (tid == 0) p.tokens[at] = r.top_key == kLowestKey ? -1 : static_cast<int64_t>(r.top_index);
+    return;
+  }
+  auto items = [&](auto each) {
+    for (uint32_t i = tid; i < n; i += kThreads) each(keys[i], i);
+  };
+  Edge edge{0, ~0u};
+  if (r.mode == TOP_P) {  // (of all)
+    uint64_t sum = 0;
+    items([&](uint32_t key, uint32_t) { sum += r.weight(value_of(key)); });
+    edge = edge_of<DT>(r, bins, items, 0, block_sum(sum));
+  } else if (r.mode == TOP_K) {
+    edge = edge_of<DT>(r, bins, items, 0, 0);
+  }
+  auto weight = [&](float x, int token) { return edge.keeps(key_of(x), static_cast<uint32_t>(token)) ? r.kept_weight(x) : 0; };
+  for (int q = tid >> 6; q < p.chunks; q += kWaves) {
+    const int t = row.token(q);
+    uint64_t sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (t + e >= 0 && t + e < row.n) sum += weight(value_of(keys[t + e]), t + e);
+    sum = wave_sum(sum);
+    if (lane == 0) sums[q] = sum;
+  }
+  __syncthreads();
+  draw<DT>(p, r, row, at, sums, weight);
+}
+
 template <int DT>
 __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
   constexpr int E = Chunks<DT>::E;
@@ -739,6 +795,9 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
   const int64_t size = dtype_size(dtype), chunk = 64 * 16 / size;
   if (reinterpret_cast<uintptr_t>(d_logits) % size != 0) return fail(ctx, TMH_ERR_UNSUPPORTED, "the logits must lie on multiples of their size");
   hipStream_t s = pick_stream(ctx, stream);
+  // In us, by one workgroup a row and by the three kernels: 31 x 703 f16 17.7 and 30.4, 174 x 196 f32 13.5 and 22.4, 64 x 4096 bf16
+  // 18.5 and 25.5, 500 x 4096 of all kinds 37.2 and 48.9; but one row of 4096 by top-k and top-p 19.9 and 16.2.
+  const bool is_short = V <= kList;
   const int64_t most_rows = std::min<int64_t>(kMostRows, 2 * ctx->num_cus);
   const int64_t rows = std::min(T, most_rows);
   SampleArgs p{};
@@ -748,18 +807,20 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
   // A workgroup a CU in all (the registers of the weights' pass leave room for one; 64 rows of 151936 bf16 in us: 68 so, 81 with
   // two a CU, that take turns), of a chunk a wavefront at least.
   p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctx->num_cus / rows, p.chunks / kWaves)));
-  const size_t of_rows = static_cast<size_t>(rows) * p.slices;
-  const size_t bytes = 8 * (of_rows * (1 + kWeightBins + (p.slices > 1 ? kList : 0)) + static_cast<size_t>(rows) * (p.chunks + 4)) + 4 * of_rows;
-  void* ws = workspace(ctx, bytes, s);
-  if (!ws) return fail(ctx, TMH_ERR_UNSUPPORTED, "sampling's workspace cannot grow here: run one call before the capture");
-  p.best = static_cast<uint64_t*>(ws);
-  p.bins = p.best + of_rows;
-  p.list = p.bins + of_rows * kWeightBins;
-  p.sums = p.list + (p.slices > 1 ? of_rows * kList : 0);
-  p.told = p.sums + static_cast<size_t>(rows) * p.chunks;
-  p.counts = reinterpret_cast<uint32_t*>(p.told + static_cast<size_t>(rows) * 4);
-  p.meet = ctx->meet;
-  in_launches(T, most_rows, [&](int64_t first, int64_t some) {
+  if (!is_short) {
+    const size_t of_rows = static_cast<size_t>(rows) * p.slices;
+    const size_t bytes = 8 * (of_rows * (1 + kWeightBins + (p.slices > 1 ? kList : 0)) + static_cast<size_t>(rows) * (p.chunks + 4)) + 4 * of_rows;
+    void* ws = workspace(ctx, bytes, s);
+    if (!ws) return fail(ctx, TMH_ERR_UNSUPPORTED, "sampling's workspace cannot grow here: run one call before the capture");
+    p.best = static_cast<uint64_t*>(ws);
+    p.bins = p.best + of_rows;
+    p.list = p.bins + of_rows * kWeightBins;
+    p.sums = p.list + (p.slices > 1 ? of_rows * kList : 0);
+    p.told = p.sums + static_cast<size_t>(rows) * p.chunks;
+    p.counts = reinterpret_cast<uint32_t*>(p.told + static_cast<size_t>(rows) * 4);
+    p.meet = ctx->meet;
+  }
+  in_launches(T, is_short ? most_a_launch(kThreads, 1, 1) : most_rows, [&](int64_t first, int64_t some) {
     auto from = [&](auto* a) { return a ? a + first : a; };
     p.x = static_cast<const char*>(d_logits) + first * ld * size;
     p.temperature = from(d_temperature);
@@ -771,6 +832,10 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
     const unsigned grid = static_cast<unsigned>(some * p.slices);
     auto launch = [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
+      if (is_short) {
+        k_sample_short<DT><<<static_cast<unsigned>(some), kThreads, 8 * p.chunks, s>>>(p);
+        return;
+      }
       k_sample_top<DT><<<grid, kThreads, 0, s>>>(p);
       k_sample_sum<DT><<<grid, kThreads, 8 * std::max(kWeightBins, p.chunks), s>>>(p);
       if (d_top_k || d_top_p) k_sample_draw<DT><<<grid, kThreads, 8 * p.chunks, s>>>(p);
@@ -779,7 +844,7 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
     else if (dtype == TMH_F16) launch(std::integral_constant<int, DT_F16>{});
     else launch(std::integral_constant<int, DT_BF16>{});
   });
-  return check_launch(ctx, "k_sample_draw");
+  return check_launch(ctx, "sampling");
 }
 
 }  // extern "C"

@@ -12,9 +12,10 @@ import pytest
 import drafts_plain as drafts
 import serving_plain as plain
 from serving_plain import HALF, TINY, to_type, values
-from test_gpu_serving import APPENDS, attention_inputs, by_token, filled_cache
+from test_gpu_serving import APPENDS, attention_inputs, by_token, filled_cache, fp8_weight
 from transmuter_amd import _lib, serving
 from transmuter_amd._lib import TmhArgumentError, lib
+from transmuter_amd.serving import Fp8Weight, Rows8
 
 pytestmark = pytest.mark.gpu
 
@@ -339,6 +340,78 @@ def test_tree_of_one_is_attention(ctx):
         assert (np.abs(one - tree) <= 2 * HALF[dtype] * np.abs(one) + 2.0 ** -18 * np.abs(v[np.isfinite(v)]).max()).all()
 
 
+LONG = [  # sequences that many workgroups share, steps of many sequences: (length, nodes), heads, kv heads, dim, page, window
+    ([(60000, 4)], 2, 1, 64, 64, 0), ([(30000, 20)], 8, 1, 64, 16, 0), ([(20000, 40)], 4, 1, 128, 16, 0), ([(9000, 9)], 16, 1, 256, 32, 0),
+    ([(20000, 2), (3, 3), (20000, 64)], 6, 2, 72, 20, 15000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"{max(c[0])}_h{c[1]}_g{c[2]}_d{c[3]}")
+def test_tree_attention_long(ctx, case, dtype):
+    shapes, h, g, d, page, window = case
+    say("long tree attention", case, dtype)
+    rng = np.random.default_rng(d + h)
+    cache, k, v, table, q, starts, mask = draft_inputs(ctx, rng, shapes, h, g, d, page, "token", dtype, "tree")
+    rows = {(b, i) for b, (_, n) in enumerate(shapes) for i in (0, 1, n // 2, n - 1)}
+    args = (ctx, cache, q, table, [n for n, _ in shapes], starts, mask)
+    y = attend_tree(*args, window=window).numpy()
+    check_draft(y, q, k, v, table, shapes, starts, mask, page, h, g, d, dtype, 1 / math.sqrt(d), window, rows=rows)
+    assert np.array_equal(np.asarray(attend_tree(*args, window=window).numpy()), np.asarray(y))  # (whoever joins the parts)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_tree_attention_many_sequences(ctx, dtype):
+    say("many sequences", dtype)
+    rng = np.random.default_rng(9)
+    for b, h, g, d in ((3000, 2, 1, 16), (700, 24, 1, 40)):
+        shapes = [(int(n), int(m)) for n, m in zip(rng.integers(0, 30, b), rng.integers(0, 4, b))]
+        cache, k, v, table, q, starts, mask = draft_inputs(ctx, rng, shapes, h, g, d, 8, "head", dtype, "tree")
+        y = attend_tree(ctx, cache, q, table, [n for n, _ in shapes], starts, mask).numpy()
+        check_draft(y, q, k, v, table, shapes, starts, mask, 8, h, g, d, dtype, 1 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("heads", [2, 12, 40])
+def test_tree_attention_far_offsets(ctx, heads):
+    """Pages further apart than 32 bits of elements can say, as columns of one tile and of several."""
+    say("tree far offsets", heads)
+    d, page, stride, n = 64, 4, 2 ** 31 + 64, 3
+    rng = np.random.default_rng(1)
+    blocks = {p: to_type(rng.standard_normal((2, page, 1, d)), "f16") for p in range(3)}
+    half = (2 * stride + page * d) * 2
+    pool = ctx.alloc(2 * half)
+    try:
+        for p in range(3):
+            for i in range(2):
+                block = np.ascontiguousarray(blocks[p][i])
+                ctx.check(lib().tmh_upload(ctx.handle, ctypes.c_void_p(pool.value + i * half + p * stride * 2),
+                                           block.ctypes.data_as(ctypes.c_void_p), block.nbytes))
+        desc = _lib.PagedCacheDesc(k=pool.value, v=pool.value + half, dtype=_lib.F16, kv_heads=1, head_dim=d, page_size=page,
+                                   pages=3, page_stride=stride, token_stride=d, head_stride=0)
+        q, table = to_type(rng.standard_normal((n, heads * d)), "f16"), np.array([[2, 0, 1]], np.int32)
+        starts = np.array([0, n], np.int32)
+        qt, tt, lt, st = ctx.put(q), ctx.put(table), ctx.put(np.array([11], np.int32)), ctx.put(starts)
+        y = ctx.empty((n, heads * d), "f16")
+        ctx.check(lib().tmh_paged_tree_attention(ctx.handle, qt.ptr, heads * d, n, heads, ctypes.byref(desc), tt.ptr, 1, 3, lt.ptr, st.ptr,
+                                                 None, 0, 0.125, 0, y.ptr, heads * d, None))
+        k, v = (np.stack([values(blocks[p][i]) for p in range(3)]) for i in range(2))
+        check_draft(y.numpy(), q, k, v, table, [(11, n)], starts, None, page, heads, 1, d, "f16", 0.125)
+        # ... and written there, the keys normed.
+        x, gamma = to_type(rng.standard_normal((1, 2 * d)), "f16"), to_type(rng.random(d) + 0.5, "f16")
+        xt, gt, slot = ctx.put(x), ctx.put(gamma), ctx.put(np.array([9], np.int64))
+        ctx.check(lib().tmh_paged_append_norm(ctx.handle, None, 0, xt.ptr, 2 * d, ctypes.c_void_p(xt.ptr.value + 2 * d), 2 * d, 1, 0, None,
+                                              gt.ptr, _lib.F16, 1e-6, None, None, None, 0, 0, 0, 0, slot.ptr, ctypes.byref(desc), None, 0, None))
+        back = np.empty((2, d), np.float16)
+        for i in range(2):
+            where = ctypes.c_void_p(pool.value + i * half + (2 * stride + d) * 2)
+            ctx.check(lib().tmh_download(ctx.handle, back[i].ctypes.data_as(ctypes.c_void_p), where, back[i].nbytes))
+        want = drafts.head_norm(values(x)[:, None, :d], values(gamma), 1e-6)[0, 0]
+        assert np.array_equal(back[1], x[0, d:])
+        assert (np.abs(values(back[0]) - want) <= (HALF["f16"] + NORM + 3 * E32) * np.abs(want) + TINY["f16"]).all()
+    finally:
+        ctx.synchronize()
+        ctx.free(pool)
+
+
 # ---------------------------------------------------------------- sampling
 
 
@@ -377,6 +450,17 @@ def test_sample(ctx, t, n, dtype):
     check_sample(ctx, x, u, temperature=temperature, top_p=top_p)
     check_sample(ctx, x, u, min_p=min_p)
     check_sample(ctx, x, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("t,n", [(5, 4095), (5, 4096), (5, 4097), (600, 4200), (1030, 20)])
+def test_sample_sizes(ctx, t, n, dtype):
+    """About the longest row of one workgroup, and more rows than a launch takes."""
+    say("sample sizes", t, n, dtype)
+    rng = np.random.default_rng(t * n)
+    x = logits_rows(rng, t, n, dtype)
+    check_sample(ctx, x, rng.random(t), temperature=rng.choice([0.0, 0.5, 1.0, 4.0], t), top_k=rng.choice([0, 1, 64, 65, 900], t),
+                 top_p=rng.choice([0.2, 0.9, 0.9999, 1.0], t), min_p=rng.choice([0.0, 0.01, 0.3], t))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -462,6 +546,207 @@ def test_sample_is_as_likely_as_its_weights(ctx):
     w /= w.sum()
     # Evenly spaced random numbers: each token as often as its share, to one at either end.
     assert (np.abs(np.bincount(tokens, minlength=40) - t * w) <= 2).all()
+
+
+# ---------------------------------------------------------------- a drafted step, streams and graphs
+
+
+class Step:
+    """A step of drafted tokens over one cache as a program runs it: append with head norms, attention, logits, tokens, and the rows of
+    a path appended once more to the slots that follow each other."""
+
+    SHAPES = [(45, 5), (708, 8), (3, 3), (0, 0), (130, 1)]  # tokens with the step's own, of those the step's
+    H, G, D, PAGE, V = 4, 2, 64, 16, 5000
+
+    def __init__(self, ctx, rng):
+        h, g, d, page = self.H, self.G, self.D, self.PAGE
+        self.ctx = ctx
+        self.cache, _, _, self.table, _, self.starts, _ = draft_inputs(ctx, rng, self.SHAPES, h, g, d, page, "token", "f16", "chain")
+        self.t = t = int(self.starts[-1])
+        self.first = [n - m for n, m in self.SHAPES]
+        parents = [[-1] + [int(rng.integers(0, i)) for i in range(1, m)] for _, m in self.SHAPES]
+        seen, depth = np.zeros((t, 64), bool), np.zeros(t, np.int64)
+        self.paths, slots, kept = [], np.zeros(t, np.int64), np.full(t, -1, np.int64)
+        for b, (_, m) in enumerate(self.SHAPES):
+            for i in range(m):
+                r, up = self.starts[b] + i, parents[b][i]
+                if up >= 0:
+                    seen[r], depth[r] = seen[self.starts[b] + up], depth[self.starts[b] + up] + 1
+                seen[r, i] = True
+                slots[r] = self.slot(b, self.first[b] + i)
+            path = np.flatnonzero(seen[self.starts[b] + m - 1]) if m else np.zeros(0, int)
+            self.paths.append(self.starts[b] + path)
+            for j, i in enumerate(path):
+                kept[self.starts[b] + i] = self.slot(b, self.first[b] + j)
+        self.mask = drafts.pack(seen)
+        first = np.repeat(self.first, [m for _, m in self.SHAPES])
+        angle = rng.random((800, d // 2)) * 6
+        self.gammas = [to_type(rng.random(d) + 0.5, "f16") for _ in range(2)]
+        put = ctx.put
+        self.dev = dict(qkv=ctx.empty((t, (h + 2 * g) * d), "f16"), u=ctx.empty((t,), "f32"), positions=put(first + depth), slots=put(slots),
+                        kept=put(kept), table=put(self.table), lengths=put(np.array([n for n, _ in self.SHAPES], np.int32)),
+                        starts=put(self.starts), mask=put(self.mask), cos=put(np.cos(angle).astype(np.float32)),
+                        sin=put(np.sin(angle).astype(np.float32)), gq=put(self.gammas[0]), gk=put(self.gammas[1]),
+                        p=put(np.full(t, 0.9, np.float32)), k=put(np.where(np.arange(t) % 2, 50, 0).astype(np.int32)))
+        w, sw = fp8_weight(rng, self.V, h * d)
+        self.head = Fp8Weight.prepare(ctx, w, sw * np.float32(0.02))
+        self.q, self.y = ctx.empty((t, h * d), "f16"), ctx.empty((t, h * d), "f16")
+        self.rows, self.logits, self.tokens = Rows8.empty(ctx, (t, h * d)), ctx.empty((t, self.V), "f16"), ctx.empty((t,), "s64")
+
+    def slot(self, b, token):
+        return int(self.table[b, token // self.PAGE]) * self.PAGE + token % self.PAGE
+
+    def fill(self, rng):
+        qkv, u = to_type(rng.standard_normal((self.t, self.dev["qkv"].shape[1])), "f16"), rng.random(self.t).astype(np.float32)
+        for name, v in (("qkv", qkv), ("u", u)):
+            self.ctx.check(lib().tmh_upload(self.ctx.handle, self.dev[name].ptr, v.ctypes.data_as(ctypes.c_void_p), v.nbytes))
+        return u
+
+    def append(self, slots):
+        v, c = self.dev, self.cache
+        c.append(v["qkv"], self.H, slots, v["positions"], v["cos"], v["sin"], q_norm=v["gq"], k_norm=v["gk"], out=self.q)
+
+    def run(self):
+        v, ctx, c, w = self.dev, self.ctx, self.cache, self.H * self.D
+        self.append(v["slots"])
+        c.attend_tree(self.q, v["table"], v["lengths"], v["starts"], v["mask"], out=self.y)
+        ctx.check(lib().tmh_quantize_rows(ctx.handle, self.y.ptr, w, None, 0, _lib.F16, self.t, w, self.rows.q.ptr, w, self.rows.scales.ptr, None))
+        ctx.check(lib().tmh_matmul_fp8(ctx.handle, self.head.handle, self.rows.q.ptr, self.t, w, self.rows.scales.ptr, None, 0, self.logits.ptr,
+                                       _lib.F16, self.V, None))
+        serving.sample(self.logits, v["u"], top_k=v["k"], top_p=v["p"], out=self.tokens)
+        self.append(v["kept"])
+
+    def results(self):
+        return [np.asarray(v.numpy()).copy() for v in (self.q, self.y, self.logits, self.tokens, self.cache.k, self.cache.v)]
+
+    def clear(self):
+        for v in (self.q, self.y, self.logits, self.tokens):
+            zero = np.zeros(v.nbytes, np.uint8)
+            self.ctx.check(lib().tmh_upload(self.ctx.handle, v.ptr, zero.ctypes.data_as(ctypes.c_void_p), v.nbytes))
+
+    def graph(self):
+        graph = ctypes.c_void_p()
+        self.ctx.check(lib().tmh_graph_begin(self.ctx.handle, None))
+        self.run()
+        self.ctx.check(lib().tmh_graph_end(self.ctx.handle, None, ctypes.byref(graph)))
+        return graph
+
+
+def same(a, b):
+    return all(np.array_equal(x, y, equal_nan=x.dtype.kind == "f") for x, y in zip(a, b))
+
+
+def test_drafted_step(ctx):
+    """Its answers, its tokens, and that the path that was kept answers afterwards as a chain what it did as a branch of its tree."""
+    say("drafted step")
+    rng = np.random.default_rng(6)
+    s = Step(ctx, rng)
+    u = s.fill(rng)
+    s.append(s.dev["slots"])
+    k, v = (values(np.asarray(x.numpy())) for x in (s.cache.k, s.cache.v))
+    s.run()
+    q, y, logits, tokens, k_then, v_then = s.results()
+    geometry = (s.PAGE, s.H, s.G, s.D, "f16", 1 / math.sqrt(s.D))
+    check_draft(y, q, k, v, s.table, s.SHAPES, s.starts, s.mask, *geometry)
+    rows = values(logits)
+    assert tokens.tolist() == [drafts.sample(rows[i], top_k=50 * (i % 2), top_p=float(np.float32(0.9)), u=float(u[i])) for i in range(s.t)]
+    lengths = [a + len(path) for a, path in zip(s.first, s.paths)]
+    starts = np.concatenate([[0], np.cumsum([len(path) for path in s.paths])]).astype(np.int32)
+    chosen = q[np.concatenate(s.paths)]
+    chain = s.cache.attend_tree(ctx.put(chosen), s.dev["table"], ctx.put(np.array(lengths, np.int32)), ctx.put(starts)).numpy()
+    check_draft(chain, chosen, values(k_then), values(v_then), s.table, [(n, len(path)) for n, path in zip(lengths, s.paths)], starts, None, *geometry)
+    # (Over the same keys and values, bit for bit, so both are within those bounds of the same numbers.)
+    slots, kept = s.dev["slots"].numpy(), s.dev["kept"].numpy()
+    r = np.flatnonzero(kept >= 0)
+    for before, then in ((k, k_then), (v, v_then)):
+        at, to = ((x[r] // s.PAGE, x[r] % s.PAGE) for x in (slots, kept))
+        assert np.array_equal(before[at], values(then)[to])
+
+
+def test_drafted_step_in_graphs(ctx):
+    """The step recorded twice on one context, whose workspace both graphs share and larger calls between the replays let grow: every
+    replay gives the eager calls' bits."""
+    say("drafted step in graphs")
+    rng = np.random.default_rng(7)
+    steps = [Step(ctx, rng), Step(ctx, rng)]
+    for s in steps:
+        s.fill(rng)
+        s.run()
+    first = steps[0].results()
+    steps[0].run()
+    assert same(first, steps[0].results())
+    graphs = [s.graph() for s in steps]
+    for replay in range(4):
+        wants = []
+        for s in steps:
+            s.fill(rng)
+            s.run()
+            wants.append(s.results())
+            s.clear()
+        serving.sample(ctx.put(to_type(rng.standard_normal((8 << replay, 9000)), "f32")), ctx.put(rng.random(8 << replay).astype(np.float32)),
+                       top_k=ctx.put(np.full(8 << replay, 9, np.int32)))
+        for graph in graphs:
+            ctx.check(lib().tmh_graph_launch(ctx.handle, graph, None))
+        for s, want in zip(steps, wants):
+            assert same(want, s.results()), replay
+        ctx.synchronize()
+    for graph in graphs:
+        ctx.check(lib().tmh_graph_destroy(ctx.handle, graph))
+
+
+def test_drafts_on_another_stream(ctx):
+    """The calls run on the stream they are given: a second context's, fenced by the host."""
+    from transmuter_amd import Context
+
+    say("drafts on another stream")
+    rng = np.random.default_rng(8)
+    cache, k, v, table, q, starts, mask = draft_inputs(ctx, rng, [(300, 9), (20, 3)], 8, 2, 64, 16, "token", "f16", "tree")
+    args = ctx.put(q), ctx.put(table), ctx.put(np.array([300, 20], np.int32)), ctx.put(starts), ctx.put(mask)
+    x, u = ctx.put(logits_rows(rng, 3, 9000, "f16")), ctx.put(rng.random(3).astype(np.float32))
+    qkv, slots = ctx.put(to_type(rng.standard_normal((2, 12 * 64)), "f16")), ctx.put(np.array([-1, -1], np.int64))
+    gamma = ctx.put(to_type(rng.random(64), "f16"))
+
+    def calls(stream):
+        return (cache.attend_tree(*args, stream=stream), serving.sample(x, u, stream=stream),
+                cache.append(qkv, 8, slots, q_norm=gamma, stream=stream))
+
+    want = [y.numpy() for y in calls(None)]
+    other = Context(0)
+    try:
+        got = calls(other.stream)
+        other.synchronize()
+        assert all(np.array_equal(y.numpy(), w) for y, w in zip(got, want))
+    finally:
+        other.close()
+
+
+def test_drafts_refused_in_a_capture():
+    """A fresh context's capture finds no workspace for the attention or for long rows of logits: refused, not run. Short rows need none."""
+    from transmuter_amd import Context
+
+    say("drafts refused in a capture")
+    c = Context(0)
+    try:
+        cache = serving.PagedCache(c, 4, 16, 1, 64)
+        q, table, lengths, y = c.empty((1, 64), "f16"), c.put(np.array([[0]], np.int32)), c.put(np.array([3], np.int32)), c.empty((1, 64), "f16")
+        starts, x, u, token = c.put(np.array([0, 1], np.int32)), c.put(np.zeros((1, 9000), np.float32)), c.put(np.zeros(1, np.float32)), c.empty((1,), "s64")
+        x.numpy()
+        c.check(lib().tmh_graph_begin(c.handle, None))
+        one = lib().tmh_paged_tree_attention(c.handle, q.ptr, 64, 1, 1, ctypes.byref(cache.desc), table.ptr, 1, 1, lengths.ptr, starts.ptr, None, 0, 1.0,
+                                             0, y.ptr, 64, None)
+        needle = lib().tmh_last_error(c.handle)
+        two = lib().tmh_sample(c.handle, x.ptr, 9000, _lib.F32, 1, 9000, None, None, None, None, u.ptr, token.ptr, None)
+        needles = needle, lib().tmh_last_error(c.handle)
+        three = lib().tmh_sample(c.handle, x.ptr, 4096, _lib.F32, 1, 4096, None, None, None, None, u.ptr, token.ptr, None)
+        graph = ctypes.c_void_p()
+        c.check(lib().tmh_graph_end(c.handle, None, ctypes.byref(graph)))
+        c.check(lib().tmh_graph_launch(c.handle, graph, None))
+        assert token.numpy().tolist() == [0]
+        c.check(lib().tmh_graph_destroy(c.handle, graph))
+        assert (one, two, three) == (_lib.ERR_UNSUPPORTED, _lib.ERR_UNSUPPORTED, 0)
+        assert all(b"before the capture" in n for n in needles)
+    finally:
+        c.close()
 
 
 # ---------------------------------------------------------------- refusals that need a device

@@ -27,6 +27,21 @@ void draft(int32_t start, int32_t stop, int64_t rows, int32_t length, int64_t mo
   int* o = out;
   *o++ = d.row, *o++ = d.nodes, *o++ = d.prefix, *o++ = d.end, *o++ = d.unit, *o++ = d.units, *o++ = d.tiles;
 }
+uint32_t item_work() { return kItem; }
+uint32_t work(int units, int tiles) {
+  Draft d{};
+  d.units = units, d.tiles = tiles;
+  return work_of(d);
+}
+void share(uint32_t first, uint32_t units, uint32_t at, uint32_t stop, uint32_t* out) {
+  const Share s = share_of(first, units, at, stop);
+  out[0] = s.from, out[1] = s.to;
+}
+uint32_t place(uint32_t worker, int begins) { return place_of_part(worker, begins != 0); }
+void parts(uint32_t first, uint32_t units, uint32_t per, uint32_t* out) {
+  const TreeParts t = tree_parts(first, units, per);
+  out[0] = t.from, out[1] = t.count;
+}
 }
 """
 
@@ -107,3 +122,40 @@ def test_drafts(plan):
             assert units == 0
     plan.draft(2, 7, 100, 50, 1000, 0, 128, 4, 16, out.ctypes.data_as(ctypes.c_void_p))
     assert out.tolist() == [2, 5, 45, 50, 0, 1, 2]
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_shares(plan, seed):
+    """Every unit of every item goes to one worker; the workers of an item are those that its parts name, and no two parts lie in one
+    place."""
+    rng = np.random.default_rng(seed)
+    out = np.zeros(2, np.uint32)
+    at = out.ctypes.data_as(ctypes.c_void_p)
+    plan.place.restype = plan.work.restype = plan.item_work.restype = ctypes.c_uint32
+    way = plan.item_work()
+    for _ in range(40):
+        items = [int(x) for x in rng.integers(1, int(rng.choice([2, 6, 300])), int(rng.choice([1, 3, 40])))]
+        assert plan.work(items[0], 3) == 3 * (items[0] + way) and plan.work(0, 3) == 0
+        begins = np.concatenate([[0], np.cumsum([n + way for n in items])])
+        workers = int(rng.choice([1, 2, 7, 64, 512]))
+        per = -(-int(begins[-1]) // workers)
+        places = set()
+        for first, n in zip(begins.tolist(), items):
+            plan.parts(first, n, per, at)
+            start, count = (int(x) for x in out)
+            have, covered = [], 0
+            for w in range(workers):
+                if (w + 1) * per <= first or w * per >= first + n + way:
+                    continue
+                plan.share(first, n, w * per, (w + 1) * per, at)
+                lo, hi = (int(x) for x in out)
+                if lo >= hi:
+                    continue
+                assert lo == covered and hi <= n
+                covered = hi
+                have.append(w)
+                if hi - lo < n:
+                    place = plan.place(w, lo == 0)
+                    assert place not in places and place < 2 * workers
+                    places.add(place)
+            assert covered == n and have == list(range(start, start + count))

@@ -5,6 +5,7 @@ Tolerances are sums of half steps, as for the decoder-layer operators (test_gpu_
 
 import ctypes
 import math
+import sys
 
 import numpy as np
 import pytest
@@ -338,6 +339,91 @@ def test_tree_of_one_is_attention(ctx):
         one = values(cache.attend(ctx.put(q), ctx.put(table), ctx.put(np.asarray(lengths, np.int32))).numpy())
         tree = values(attend_tree(ctx, cache, q, table, lengths, np.arange(6, dtype=np.int32), None).numpy())
         assert (np.abs(one - tree) <= 2 * HALF[dtype] * np.abs(one) + 2.0 ** -18 * np.abs(v[np.isfinite(v)]).max()).all()
+
+
+WIDE = 10 ** 6  # tokens that a table has room for: of such tables tiles of many columns are worth their while
+
+
+def attend_tree_wide(ctx, cache, q, table, *args, **kw):
+    table = np.pad(table, ((0, 0), (0, WIDE // cache.page_size - table.shape[1])), constant_values=-1)
+    return narrow(ctx, cache, q, table, *args, **kw)
+
+
+narrow = attend_tree
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("kind", ["chain", "tree", "holes"])
+@pytest.mark.parametrize("case", TREES, ids=lambda c: f"b{len(c[0])}_{max(c[0])}_h{c[1]}_g{c[2]}_d{c[3]}_p{c[4]}_{c[5]}_w{c[6]}")
+def test_tree_attention_wide_tables(ctx, case, kind, dtype):
+    shapes, h, g, d, page, order, window = case
+    say("tree attention, wide table", case if len(shapes) < 20 else (len(shapes), *case[1:]), kind, dtype)
+    rng = np.random.default_rng(sum(n + m for n, m in shapes) + h + d + 1)
+    cache, k, v, table, q, starts, mask = draft_inputs(ctx, rng, shapes, h, g, d, page, order, dtype, kind)
+    if not len(q):
+        return
+    y = attend_tree_wide(ctx, cache, q, table, [n for n, _ in shapes], starts, mask, window=window).numpy()
+    check_draft(y, q, k, v, table, shapes, starts, mask, page, h, g, d, dtype, 1 / math.sqrt(d), window)
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_random_tree_attention_wide_tables(ctx, seed):
+    rng = np.random.default_rng(7700 + seed)
+    dtype = TYPES[1 + seed % 2]
+    d, g = int(rng.choice([8, 64, 104, 128, 128, 200, 256])), int(rng.choice([1, 2, 4]))
+    h = g * int(rng.choice([1, 2, 4, 7, 8, 16, 17]))
+    page, order, most = int(rng.choice([1, 5, 16, 64])), str(rng.choice(["token", "head"])), int(rng.choice([5, 40, 100]))
+    shapes = [(int(n), int(m)) for n, m in zip(rng.integers(0, int(rng.choice([3, 150, 3000])) + 1, 9), rng.integers(0, most + 1, 9))]
+    shapes, kind = shapes[:int(rng.choice([1, 2, 9]))], str(rng.choice(["chain", "tree", "holes"]))
+    say("random tree attention, wide table", seed, shapes, h, g, d, page, order, kind, dtype)
+    cache, k, v, table, q, starts, mask = draft_inputs(ctx, rng, shapes, h, g, d, page, order, dtype, kind)
+    if not len(q):
+        return
+    scale = float(rng.choice([1 / math.sqrt(d), 0.01, -0.1]))
+    y = attend_tree_wide(ctx, cache, q, table, [n for n, _ in shapes], starts, mask, scale=scale).numpy()
+    check_draft(y, q, k, v, table, shapes, starts, mask, page, h, g, d, dtype, scale)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 256])
+def test_tree_attention_bad_pages_in_wide_tables(ctx, dtype, d):
+    say("tree bad pages, wide table", dtype, d)
+    rng = np.random.default_rng(5)
+    h, g, page = 8, 2, 16
+    shapes = [(100, 15), (100, 13), (164, 70), (40, 0)]
+    cache, k, v, table, q, starts, mask = draft_inputs(ctx, rng, shapes, h, g, d, page, "token", dtype, "tree", words=1, behind=4)
+    table[0, 2], table[0, 6] = -1, 10 ** 6
+    table[1, :] = -7
+    table[2, 0] = np.int32(2 ** 31 - 1)
+    out = ctx.put(to_type(np.full(q.shape, 7.0), dtype))
+    for m in (mask, None):
+        y = attend_tree_wide(ctx, cache, q, table, [100, 100, 164, 40], starts, m, out=out).numpy()
+        check_draft(y, q, k, v, table, shapes, starts, m, page, h, g, d, dtype, 1 / math.sqrt(d))
+        assert not values(y)[15:28].any() and (values(y)[starts[-1]:] == 7).all()
+    y = attend_tree_wide(ctx, cache, q[:15], table[:1], [-3], starts[:2], mask[:15]).numpy()
+    assert not values(y).any()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("h,g,d", [(4, 2, 64), (16, 1, 128), (2, 1, 256), (8, 1, 40)])
+def test_tree_attention_hides_infinities_in_wide_tables(ctx, dtype, h, g, d, monkeypatch):
+    monkeypatch.setattr(sys.modules[__name__], "attend_tree", attend_tree_wide)
+    test_tree_attention_hides_infinities(ctx, dtype, h, g, d, 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["chain", "tree"])
+@pytest.mark.parametrize("b,n,h,g,d,window", [(30, 70, 8, 4, 64, 100), (30, 40, 16, 4, 128, 37), (10, 70, 8, 4, 128, 1500), (16, 36, 8, 4, 256, 1100),
+                                              (8, 64, 16, 4, 128, 0)])
+def test_tree_attention_many_columns(ctx, b, n, h, g, d, window, kind, dtype):
+    """Steps with work enough for tiles of many columns, with windows."""
+    say("many columns", b, n, h, g, d, window, kind, dtype)
+    rng = np.random.default_rng(b + n + window)
+    shapes = [(int(x), n) for x in rng.integers(n - 3, max(1000, 2 * window), b)]
+    cache, k, v, table, q, starts, mask = draft_inputs(ctx, rng, shapes, h, g, d, 16, "token", dtype, kind)
+    y = attend_tree(ctx, cache, q, table, [x for x, _ in shapes], starts, mask, window=window).numpy()
+    rows = {(i, j) for i in range(b) for j in (0, 1, n // 2, n - 1)}
+    check_draft(y, q, k, v, table, shapes, starts, mask, 16, h, g, d, dtype, 1 / math.sqrt(d), window, rows=rows)
 
 
 LONG = [  # sequences that many workgroups share, steps of many sequences: (length, nodes), heads, kv heads, dim, page, window

@@ -1150,17 +1150,34 @@ void launch_shared(const TreeArgs& p, int64_t units, hipStream_t s) {
   if (p.workers > MOST && units > MOST) k_tree_shared_join<DT, NB, WC><<<dim3(WC, 4 * NB, p.workers / MOST), 256, 0, s>>>(p);
 }
 
-// How columns go to workgroups, by the columns that a sequence has in the mean (all the host knows).
+// How columns go to workgroups, by the columns that a sequence has in the mean and the tokens that the table or the window leaves it
+// (all the host knows).
 struct TreeForm {
   bool shared;
-  int columns, unit, per_cu;  // columns of a tile, tokens of a unit, workgroups a CU
+  int columns, unit;  // columns of a tile, tokens of a unit
 };
+constexpr int kPerCu = 2;  // workgroups a CU
 // `near`: rows' offsets fit 32 bits, counted in 16 bytes.
-TreeForm tree_form(int64_t columns, bool f32, int head_dim, bool near) {
-  if (f32) return {false, head_dim <= 128 && columns > 16 ? 32 : 16, 64, 2};
-  if (columns <= 16 || !near) return {false, 16, 128, 2};
-  if (head_dim > 128) return {true, 64, 32, 2};
-  return {true, columns <= 64 ? 64 : 128, 64, 2};
+// Wide tiles read K and V less often, narrow ones give every workgroup work where there is little. What little is, by the work of a
+// worker in narrow tiles, is from measurements, us in tiles of 16 columns, 64 and 128 (16-bit types, 128 dimensions, sequences x
+// nodes over tokens):
+//   up to 10 units of 16 columns: 4 x 32 over 500 with 8 kv heads of 4 heads 21, 24, 37; 16 x 30 over 64 to 128 13, 19, 17;
+//     4 x 30 over 2000 26, 35, 31; 9 x 40 over 1 to 900 26, 28, 42; past it 8 x 32 over 4000 59, 47, 43;
+//   up to 16 units of 64 columns, of sequences of up to 1024 tokens (where more of a worker's time goes to the ways in and out): 512
+//     over 512 41, 31, 37; two of them 74, 31, 44; 8 x 64 over 1000 86, 44, 55; past it 8 of 512 327, 109, 82;
+//   others: 128 over 4096 60, 48, 44; 8 x 64 over 4000 94, 65, 69.
+//   of 256 dimensions, in tiles of 16 and 64: 4 x 32 over 500 48 and 53, 16 x 30 over 64 to 128 29 and 39, 4 x 30 over 2000 61 and 45.
+// Columns that fill no second tile of 16 stay in one (32 x 4 over 4000 with 4 heads a kv head 62, 80, 90; 6 nodes 94, 78, 87); up to
+// 64 go to tiles of 64 (16 nodes 90, 52, 60; 20 nodes 105, 66, 65). In f32, tiles of 16 and 32: 4 x 8 over 2000 35 and 41, 64 over
+// 1000 35 and 38; 8 x 32 over 1000 76 and 65, 32 x 8 over 4000 259 and 196.
+TreeForm tree_form(int64_t B, int64_t columns, int64_t tokens, int kv_heads, int64_t workers, bool f32, int head_dim, bool near) {
+  auto work = [&](int64_t tile, int64_t unit) {  // of a worker
+    return B * kv_heads * ((columns + tile - 1) / tile) * ((tokens + unit - 1) / unit + kItem) / workers;
+  };
+  if (f32) return {false, head_dim <= 128 && columns > 16 && work(16, 64) > 5 ? 32 : 16, 64};
+  if (columns <= 16 || !near || (work(16, 128) <= 10 && (head_dim <= 128 || tokens <= 1024))) return {false, 16, 128};
+  if (head_dim > 128) return {true, 64, 32};
+  return {true, columns <= 64 || (tokens <= 1024 && work(64, 64) <= 16) ? 64 : 128, 64};
 }
 
 }  // namespace
@@ -1202,9 +1219,10 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
   const unsigned __int128 last_row = static_cast<unsigned __int128>(cache->pages - 1) * cache->page_stride +
                                      static_cast<unsigned __int128>(cache->page_size - 1) * cache->token_stride;
   const bool near = last_row / 8 < (uint64_t{1} << 32) - 1;
-  const TreeForm form = tree_form((T * group + B - 1) / B, f32, cache->head_dim, near);
+  const int64_t most = max_pages * cache->page_size, nodes = (T + B - 1) / B, workers = kPerCu * ctx->num_cus;
+  const int64_t tokens = window > 0 && window < most ? std::min(most, window + nodes) : most;
+  const TreeForm form = tree_form(B, (T * group + B - 1) / B, tokens, cache->kv_heads, workers, f32, cache->head_dim, near);
   const int64_t unit = form.unit;
-  const int64_t most = max_pages * cache->page_size;
   const int64_t items = (T * group / form.columns + B) * cache->kv_heads;
   const int64_t units = (most + unit - 1) / unit;  // of an item
   if (units + kItem >= (int64_t{1} << 31) / items)
@@ -1233,9 +1251,9 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
   p.head_dim = cache->head_dim;
   p.by_group = FastDiv(static_cast<uint32_t>(group));
   p.scale = scale * 1.44269504088896340736f;
-  p.workers = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(form.per_cu * ctx->num_cus, units * items)));
+  p.workers = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(workers, units * items)));
   hipStream_t s = pick_stream(ctx, stream);
-  const size_t rows = 2 * static_cast<size_t>(form.per_cu * ctx->num_cus) * form.columns;
+  const size_t rows = 2 * static_cast<size_t>(workers) * form.columns;
   const int width_of_part = form.shared ? (cache->head_dim <= 128 ? 128 : 256) : cache->head_dim;
   void* ws = workspace(ctx, rows * (width_of_part * 4 + sizeof(float2)), s);
   if (!ws) return fail(ctx, TMH_ERR_UNSUPPORTED, "attention's workspace cannot grow here: run one call before the capture");

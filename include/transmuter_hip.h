@@ -19,7 +19,8 @@
  *    on that stream unless stated otherwise.
  *  - Shapes are int64_t element counts; no call reads or writes outside the extents given.
  *  - Prefill MatMulNBits (split K), DynamicQuantizeLinear, QMoE, the 8-bit product (rows at any
- *    address, parts of K) and paged attention (parts of sequences, and counters beside) keep
+ *    address, parts of K), paged attention of one and of several tokens a sequence (parts of
+ *    sequences, and counters beside) and sampling from rows of more than 4096 logits keep
  *    intermediates in one workspace per context, grown outside graph capture. Calls of one
  *    context on two streams must not run at the same time; use a context per concurrent stream.
  *    A call that would have to grow the workspace while its stream is being captured into a
@@ -526,7 +527,9 @@ int tmh_paged_append_norm(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void
  * d_starts[b] rows from d_starts[b] on, which are the last n of its d_lengths[b] tokens, in the order of their slots: row i
  * of it sees all tokens before them, and of them (nodes 0 .. n - 1) those of its mask; without a mask nodes 0 .. i. With a
  * window it sees the last `window` of these only (a place whose page is none counts, and is not read). The rest is
- * tmh_paged_attention's: y = softmax(scale * q . k) v in f32, rounded once, with the weights' parts given there.
+ * tmh_paged_attention's: y = softmax(scale * q . k) v in f32, rounded once, with the weights in two 16-bit parts as there;
+ * F16's end at 2^-35 of the largest weight. An infinity in V is one in the answer of a row that sees it with a weight of
+ * 2^-90 of the largest or more; below that it may give NaN.
  *  d_q [T, heads, head_dim] of the cache's dtype, 16-byte aligned rows ldq elements apart (ldq a multiple of 16 bytes);
  *    d_y likewise, ldy
  *  d_starts [B + 1] S32, not falling, from 0 to at most T. Rows behind the last sequence's are not read or written.
@@ -536,7 +539,7 @@ int tmh_paged_append_norm(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void
  *    fewer than n the first nodes have no token
  * A row that sees no token answers zeros. What a row does not see, infinities and NaN too, has no effect on it.
  * B at most 65535, T * heads / kv_heads below 2^31. The context's workspace keeps the parts of sequences that workgroups
- * share (its size depends on T / B, heads and head_dim only).
+ * share. How columns and tokens are shared out, and so the last bits, follows T / B, heads, max_pages and the window.
  */
 int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t T, int heads,
                              const tmh_paged_cache* cache, const int32_t* d_page_table, int64_t B, int64_t max_pages,
@@ -550,13 +553,15 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
  * to top_p of all of these or more; of these the tokens with w >= min_p. Equal logits rank by their index, the lowest
  * first. The answer is the first kept token, by index, up to which the kept weights sum to more than random times their
  * whole (the last one where none does).
- *  d_logits [T, V] of dtype (F32, F16, BF16), rows ld elements apart; V below 2^20. NaN counts as -infinity, which has no
+ *  d_logits [T, V] of dtype (F32, F16, BF16), on a multiple of its size, rows ld elements apart; V below 2^20. NaN counts as -infinity, which has no
  *    weight; +infinities have all of it.
  *  d_temperature [T] F32 or NULL (1): not above 0 (or NaN): the largest logit, whatever else is asked
  *  d_top_k [T] S32 or NULL: 0 and less, V and more: all;  d_top_p [T] F32 or NULL: 1 and more, NaN: all; the largest is
  *    always kept;  d_min_p [T] F32 or NULL: 0 and less, NaN: all; 1 and more: the largest and its equals
  *  d_random [T] F32 in [0, 1)
  *  d_tokens [T] S64; -1 for a row without any logit above -infinity
+ * Sums are of whole numbers, so a row's answer depends on no order, and on no other row. Rows of more than 4096 logits use
+ * the context's workspace.
  */
 int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_t T, int64_t V,
                const float* d_temperature, const int32_t* d_top_k, const float* d_top_p, const float* d_min_p,

@@ -9,6 +9,9 @@
 //  k_sample_draw  rows by top-k: the tokens down to that bin go to a list. By top-p alone: those of that bin do, and the weights above
 //                 it to chunks. The list, sorted out in LDS, gives the least logit kept and the last of its equals that is; then the draw.
 // Rows of at most kList tokens are a list from the start: k_sample_short, one kernel and a workgroup a row.
+// Bound by latency (what one kernel leaves the next, a row's last workgroup alone) and by the weights' exponentials in 64 bits; in us
+// k_sample_top, k_sample_sum, k_sample_draw: 1 x 151936 f32 by top-k and top-p 4, 12, 10; 64 x 151936 bf16 by top-p 10, 21, 36;
+// 500 x 32003 f16 of all kinds 14, 36, 42; 256 x 151936 f32 by min-p 34, 36: 4.6 and 4.3 TB/s.
 // A list that does not fit (thousands of tokens of almost the same logit) leaves its row to the last workgroup, which goes over all
 // of it a few times.
 #include <algorithm>

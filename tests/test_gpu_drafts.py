@@ -539,9 +539,9 @@ def test_sample(ctx, t, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("t,n", [(5, 4095), (5, 4096), (5, 4097), (600, 4200), (1030, 20)])
+@pytest.mark.parametrize("t,n", [(5, 4095), (5, 4096), (5, 4097), (600, 4200), (1030, 20), (2, 2 ** 20 - 1)])
 def test_sample_sizes(ctx, t, n, dtype):
-    """About the longest row of one workgroup, and more rows than a launch takes."""
+    """About the longest row of one workgroup, more rows than a launch takes, and the longest row."""
     say("sample sizes", t, n, dtype)
     rng = np.random.default_rng(t * n)
     x = logits_rows(rng, t, n, dtype)

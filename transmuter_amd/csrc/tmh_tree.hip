@@ -1180,7 +1180,7 @@ constexpr int kPerCu = 2;  // workgroups a CU
 // 1000 35 and 38; 8 x 32 over 1000 76 and 65, 32 x 8 over 4000 259 and 196.
 TreeForm tree_form(int64_t B, int64_t columns, int64_t tokens, int kv_heads, int64_t workers, bool f32, int head_dim, bool near) {
   auto work = [&](int64_t tile, int64_t unit) {  // of a worker
-    return B * kv_heads * ((columns + tile - 1) / tile) * ((tokens + unit - 1) / unit + kItem) / workers;
+    return 1.0 * B * kv_heads * ((columns + tile - 1) / tile) * ((tokens + unit - 1) / unit + kItem) / workers;
   };
   if (f32) return {false, head_dim <= 128 && columns > 16 && work(16, 64) > 5 ? 32 : 16, 64};
   if (columns <= 16 || !near || (work(16, 128) <= 10 && (head_dim <= 128 || tokens <= 1024))) return {false, 16, 128};

@@ -20,7 +20,7 @@
  *  - Shapes are int64_t element counts; no call reads or writes outside the extents given.
  *  - Prefill MatMulNBits (split K), DynamicQuantizeLinear, QMoE, the 8-bit product (rows at any
  *    address, parts of K), paged attention of one and of several tokens a sequence (parts of
- *    sequences, and counters beside) and sampling from rows of more than 4096 logits keep
+ *    sequences, and counters beside) and sampling from rows of more than 8192 logits keep
  *    intermediates in one workspace per context, grown outside graph capture. Calls of one
  *    context on two streams must not run at the same time; use a context per concurrent stream.
  *    A call that would have to grow the workspace while its stream is being captured into a
@@ -560,7 +560,7 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
  *    always kept;  d_min_p [T] F32 or NULL: 0 and less, NaN: all; 1 and more: the largest and its equals
  *  d_random [T] F32 in [0, 1)
  *  d_tokens [T] S64; -1 for a row without any logit above -infinity
- * Sums are of whole numbers, so a row's answer depends on no order, and on no other row. Rows of more than 4096 logits use
+ * Sums are of whole numbers, so a row's answer depends on no order, and on no other row. Rows of more than 8192 logits use
  * the context's workspace.
  */
 int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_t T, int64_t V,

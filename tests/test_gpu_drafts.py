@@ -539,7 +539,7 @@ def test_sample(ctx, t, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("t,n", [(5, 4095), (5, 4096), (5, 4097), (600, 4200), (1030, 20), (2, 2 ** 20 - 1)])
+@pytest.mark.parametrize("t,n", [(5, 4095), (5, 4096), (5, 4097), (5, 8191), (5, 8192), (5, 8193), (600, 8300), (1030, 20), (2, 2 ** 20 - 1)])
 def test_sample_sizes(ctx, t, n, dtype):
     """About the longest row of one workgroup, more rows than a launch takes, and the longest row."""
     say("sample sizes", t, n, dtype)
@@ -642,7 +642,7 @@ class Step:
     a path appended once more to the slots that follow each other."""
 
     SHAPES = [(45, 5), (708, 8), (3, 3), (0, 0), (130, 1)]  # tokens with the step's own, of those the step's
-    H, G, D, PAGE, V = 4, 2, 64, 16, 5000
+    H, G, D, PAGE, V = 4, 2, 64, 16, 9000
 
     def __init__(self, ctx, rng):
         h, g, d, page = self.H, self.G, self.D, self.PAGE

@@ -8,7 +8,7 @@
 //                 Others, by top-p alone: the weights of each bin, and the bin in which they reach top-p of the whole.
 //  k_sample_draw  rows by top-k: the tokens down to that bin go to a list. By top-p alone: those of that bin do, and the weights above
 //                 it to chunks. The list, sorted out in LDS, gives the least logit kept and the last of its equals that is; then the draw.
-// Rows of at most kList tokens are a list from the start: k_sample_short, one kernel and a workgroup a row.
+// Rows of at most kShort tokens are a list from the start: k_sample_short, one kernel and a workgroup a row.
 // Bound by latency (what one kernel leaves the next, a row's last workgroup alone) and by the weights' exponentials in 64 bits; in us
 // k_sample_top, k_sample_sum, k_sample_draw: 1 x 151936 f32 by top-k and top-p 4, 12, 10; 64 x 151936 bf16 by top-p 10, 21, 36;
 // 500 x 32003 f16 of all kinds 14, 36, 42; 256 x 151936 f32 by min-p 34, 36: 4.6 and 4.3 TB/s.
@@ -29,6 +29,7 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kUnit = 44;
 constexpr int kPerOctave = 16, kWeightBins = kPerOctave * kUnit + 4;  // (a few more than have weights: bins are found in f32)
 constexpr int kList = 4096;        // tokens of a row's list
+constexpr int kShort = 8192;       // tokens of a row that one workgroup takes
 constexpr int kDigits = 2048;      // of a selection's turn
 constexpr int kMostRows = 512;     // of a launch: each has a counter
 
@@ -617,13 +618,13 @@ __device__ __forceinline__ void draw_few(const SampleArgs& p, const Row& r, int6
   if (w && past(before + w) && !(before && past(before))) p.tokens[at_row] = token;
 }
 
-// A row of up to kList tokens by one workgroup, as the others do the tokens of a list.
+// A row of up to kShort tokens by one workgroup, as the others do the tokens of a list.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void k_sample_short(SampleArgs p) {
   constexpr int E = Chunks<DT>::E;
   __shared__ uint64_t bins[kDigits];
-  __shared__ uint32_t keys[kList];
   extern __shared__ uint64_t sums[];  // of each chunk
+  uint32_t* keys = reinterpret_cast<uint32_t*>(sums + p.chunks);
   const int64_t at = blockIdx.x;
   const Chunks<DT> row(p, at);
   const int tid = threadIdx.x, lane = tid & 63;
@@ -798,9 +799,10 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
   const int64_t size = dtype_size(dtype), chunk = 64 * 16 / size;
   if (reinterpret_cast<uintptr_t>(d_logits) % size != 0) return fail(ctx, TMH_ERR_UNSUPPORTED, "the logits must lie on multiples of their size");
   hipStream_t s = pick_stream(ctx, stream);
-  // In us, by one workgroup a row and by the three kernels: 31 x 703 f16 17.7 and 30.4, 174 x 196 f32 13.5 and 22.4, 64 x 4096 bf16
-  // 18.5 and 25.5, 500 x 4096 of all kinds 37.2 and 48.9; but one row of 4096 by top-k and top-p 19.9 and 16.2.
-  const bool is_short = V <= kList;
+  // In us, by one workgroup a row and by the three kernels: 31 x 703 f16 17.7 and 30.4, 174 x 196 f32 13.5 and 22.4; of all kinds 24 x
+  // 8192 bf16 22.4 and 29.6, 193 f32 31.4 and 34.9, 500 f16 47.2 and 52.5, 24 x 16384 31.6 and 32.3, 193 44.6 and 41.1, 500 71.4 and
+  // 63.4. (One row by top-k and top-p, of 8192, 23.8 and 19.5.)
+  const bool is_short = V <= kShort;
   const int64_t most_rows = std::min<int64_t>(kMostRows, 2 * ctx->num_cus);
   const int64_t rows = std::min(T, most_rows);
   SampleArgs p{};
@@ -836,7 +838,7 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
     auto launch = [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
       if (is_short) {
-        k_sample_short<DT><<<static_cast<unsigned>(some), kThreads, 8 * p.chunks, s>>>(p);
+        k_sample_short<DT><<<static_cast<unsigned>(some), kThreads, 8 * p.chunks + 4 * p.vocabulary, s>>>(p);
         return;
       }
       k_sample_top<DT><<<grid, kThreads, 0, s>>>(p);

@@ -787,16 +787,17 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
   if (b >= p.B) return;
   Draft d = draft_at<UT, M>(p, b);
   before *= p.kv_heads;
-  auto clear = [&] {  // pieces of a row past head_dim are brought by nobody: zeros for all units
+  auto clear = [&](int stages) {  // pieces of a row past head_dim are brought by nobody: zeros for all units
     if (p.head_dim == 128 * NB) return;
-    for (int i = threadIdx.x; i < 2 * STAGE / 16; i += THREADS) reinterpret_cast<uint4_t*>(&lds[0][0])[i] = uint4_t{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < stages * STAGE / 16; i += THREADS) reinterpret_cast<uint4_t*>(&lds[0][0])[i] = uint4_t{0u, 0u, 0u, 0u};
     __syncthreads();
   };
-  clear();
+  clear(2);
   // (A scale of 0: queries of zeros, so that -infinity times it stays what it is.)
   const float a = p.scale == 0.f ? 1.f : fabsf(p.scale);
   const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;
   const uint32_t page16 = static_cast<uint32_t>(p.cache.page_stride / 8), token16 = static_cast<uint32_t>(p.cache.token_stride / 8);
+  bool used = false;  // stage 0, by an item's sums
   while (at < stop) {
     while (at - before >= work_of(d) * p.kv_heads) {
       before += work_of(d) * p.kv_heads;
@@ -970,6 +971,8 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
     uint32_t found = kNone16;
     int32_t coming = 0;
     __syncthreads();  // the item before has left LDS
+    if (WT > 1 && used) clear(1);  // (its sums: as 16-bit values NaN among them, for which it would all be done again)
+    used = true;
     // The queries come by whole rows through the second stage, each wavefront's own columns (by 16 bytes of many rows at a time they
     // took 5 us, with the first rows of K and V they come in passing).
     if (from < upto) {
@@ -1042,7 +1045,7 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
           [&](int c, float top, float sum) {
             if (!whole) p.stats[slot * M + c] = make_float2(top, sum);
           });
-      clear();
+      clear(2);
       __threadfence();  // (these stores went by the XCD's L2)
       join_here();
       continue;

@@ -778,6 +778,22 @@ __global__ __launch_bounds__(kThreads) void k_sample_draw(SampleArgs p) {
   draw<DT>(p, r, row, s.row, sums, weight);
 }
 
+// The workgroups of a row, of `most` at most. One fits a CU (the weights' pass has registers for one), so that they take turns of
+// what a slice's tokens take and its ways in and out beside, which cost as much as 24000 tokens. (In us, with the CUs' share of
+// workgroups a row rounded down and so: 132 x 139374 f16 by top-p 153 and 117, 300 x 150000 bf16 269 and 227, 160 x 100000 117 and 105,
+// by top-k and top-p 69 and 77; 64 x 151936 with 8 a row, in two turns, 81, with 4 68.)
+int slices_of(int64_t rows, int64_t vocabulary, int64_t most, int64_t cus) {
+  int64_t best = 1, least = INT64_MAX;
+  for (int64_t s = 1; s <= std::max<int64_t>(most, 1) && (s == 1 || rows * s <= 4 * cus); ++s) {
+    const int64_t cost = (rows * s + cus - 1) / cus * (vocabulary / s + 24000);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return static_cast<int>(best);
+}
+
 }  // namespace
 }  // namespace tmh
 
@@ -809,9 +825,7 @@ int tmh_sample(tmh_ctx* ctx, const void* d_logits, int64_t ld, int dtype, int64_
   p.ld = ld;
   p.vocabulary = static_cast<int>(V);
   p.chunks = static_cast<int>((V + 16 / size - 1 + chunk - 1) / chunk);  // (rows that begin inside 16 bytes may take one more)
-  // A workgroup a CU in all (the registers of the weights' pass leave room for one; 64 rows of 151936 bf16 in us: 68 so, 81 with
-  // two a CU, that take turns), of a chunk a wavefront at least.
-  p.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctx->num_cus / rows, p.chunks / kWaves)));
+  p.slices = is_short ? 1 : slices_of(rows, V, p.chunks / kWaves, ctx->num_cus);
   if (!is_short) {
     const size_t of_rows = static_cast<size_t>(rows) * p.slices;
     const size_t bytes = 8 * (of_rows * (1 + kWeightBins + (p.slices > 1 ? kList : 0)) + static_cast<size_t>(rows) * (p.chunks + 4)) + 4 * of_rows;

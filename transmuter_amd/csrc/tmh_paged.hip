@@ -314,7 +314,7 @@ __global__ __launch_bounds__(256) void k_paged_append_norm(AppendNormArgs p, int
         v[2 * j] = x * c[j] - y * s[j];
         v[2 * j + 1] = fmaf(x, s[j], y * c[j]);
       }
-    } else if (VEC) {  // a pair
+    } else if (VEC && a.turned) {  // a pair
       float c[8], s[8], high[8];
       if (gamma) {
         float g[8];
@@ -922,9 +922,9 @@ __global__ __launch_bounds__(256) void k_paged_join(AttendArgs p) {
   store(dim, total == 0.f ? float4_t{0.f, 0.f, 0.f, 0.f} : o * (1.f / total));
 }
 
-// How an append's operands may be read: rows and partners by 16 bytes, tables by eight entries, by four f32 pairs.
+// How an append's operands may be read: rows by 16 bytes, rows and partners so, tables by eight entries, by four f32 pairs.
 struct AppendForm {
-  bool vec, table_vec, pairs_vec;
+  bool rows, vec, table_vec, pairs_vec;
 };
 
 // The checks and arguments that the appends share (with T = 0 nothing is filled in).
@@ -976,9 +976,9 @@ int append_args(tmh_ctx* ctx, const char* name, const void* d_q, int64_t ldq, co
   p.by_page = FastDiv(static_cast<uint32_t>(cache->page_size));
   const int64_t e = 16 / dtype_size(cache->dtype);
   auto on16 = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
-  form.vec = on16(d_k) && on16(d_v) && ldk % e == 0 && ldv % e == 0 &&
-                   (!heads || (on16(d_q) && on16(d_q_out) && ldq % e == 0 && ldqo % e == 0)) &&
-                   (interleaved ? true : rotary_dim % 16 == 0);
+  form.rows = on16(d_k) && on16(d_v) && ldk % e == 0 && ldv % e == 0 &&
+              (!heads || (on16(d_q) && on16(d_q_out) && ldq % e == 0 && ldqo % e == 0));
+  form.vec = form.rows && (interleaved ? true : rotary_dim % 16 == 0);
   p.head_dim = dim;
   p.turned = form.vec && !interleaved ? rotary_dim / 16 : 0;
   const uint32_t of_head = static_cast<uint32_t>(dim / 8 - p.turned);
@@ -1056,9 +1056,9 @@ int tmh_paged_append_norm(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void
   const int pieces = cache->head_dim / 8 - p.a.turned;  // of a query's or key's head
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (pieces <= 8) launch_append_norm<DT, 8>(p, T, form.vec, form.table_vec, form.pairs_vec, s);
-    else if (pieces <= 16) launch_append_norm<DT, 16>(p, T, form.vec, form.table_vec, form.pairs_vec, s);
-    else launch_append_norm<DT, 32>(p, T, form.vec, form.table_vec, form.pairs_vec, s);
+    if (pieces <= 8) launch_append_norm<DT, 8>(p, T, form.rows, form.table_vec, form.pairs_vec, s);
+    else if (pieces <= 16) launch_append_norm<DT, 16>(p, T, form.rows, form.table_vec, form.pairs_vec, s);
+    else launch_append_norm<DT, 32>(p, T, form.rows, form.table_vec, form.pairs_vec, s);
   };
   if (cache->dtype == TMH_F32) launch(std::integral_constant<int, DT_F32>{});
   else if (cache->dtype == TMH_F16) launch(std::integral_constant<int, DT_F16>{});

@@ -32,6 +32,7 @@ struct TreeArgs {
   uint32_t workers;
   FastDiv by_group;
   float scale;  // of the scores in base-2 logarithms: scale * log2(e)
+  float unit;   // base-2 logarithms to one of the parts' maxima: 1, or, of tiles that keep maxima as the products have them, |scale|
 };
 
 template <int UT, int M>
@@ -148,14 +149,14 @@ __device__ __forceinline__ void join_parts(const TreeArgs& p, const TreeParts& p
       if (k0 + b * step >= parts.count) st[b].x = kNone;
       next = fmaxf(next, st[b].x);
     }
-    const float keep = top == next ? 1.f : __builtin_amdgcn_exp2f(top - next);
+    const float keep = top == next ? 1.f : __builtin_amdgcn_exp2f((top - next) * p.unit);
     top = next;
     total *= keep;
 #pragma unroll
     for (int i = 0; i < QUADS; ++i) acc[i] *= keep;
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
-      const float f = st[b].x == top ? 1.f : __builtin_amdgcn_exp2f(st[b].x - top);
+      const float f = st[b].x == top ? 1.f : __builtin_amdgcn_exp2f((st[b].x - top) * p.unit);
       total += f * st[b].y;
 #pragma unroll
       for (int i = 0; i < QUADS; ++i) acc[i] += f * o[b][i];
@@ -227,11 +228,11 @@ __device__ __forceinline__ uint2 cut2(float a, float b) {
 // Columns [first, first + columns) of an item over its tokens [from, to), one after another, each product in f32 of what a column
 // sees alone: the workgroups' way where a column does not see a token that holds an infinity or a NaN, which a weight of 0 would
 // leave in a matrix product. put(column of these, dimension, sum, weights' sum) and total(column of these, maximum, weights' sum)
-// take the answers; the maxima are of scores in base-2 logarithms. Weights are multiplied by `factor`, as the other parts' are;
-// `room` is 3 THREADS + 16 words of LDS.
+// take the answers; the maxima are of products times `scale`, each worth p.unit base-2 logarithms. Weights are multiplied by `factor`,
+// as the other parts' are; `room` is 3 THREADS + 16 words of LDS.
 template <int DT, int THREADS, typename Put, typename Total>
 __device__ __forceinline__ void each_alone(const TreeArgs& p, const Draft& d, const int32_t* table, int kv_head, int first, int columns, int from,
-                                           int to, float factor, uint32_t* room, Put put, Total total) {
+                                           int to, float scale, float factor, uint32_t* room, Put put, Total total) {
   constexpr int EACH = 256 / THREADS > 0 ? 256 / THREADS : 1;  // dimensions a thread may have
   const int tid = threadIdx.x, dim = p.head_dim, wave = tid >> 6;
   int64_t* rows = reinterpret_cast<int64_t*>(room);  // of a turn's tokens, negative where one is not seen
@@ -258,7 +259,7 @@ __device__ __forceinline__ void each_alone(const TreeArgs& p, const Draft& d, co
         float dot = 0.f;
 #pragma unroll 1
         for (int i = 0; i < dim; ++i) dot = fmaf(load_as_f32<DT>(p.q, q + i), load_as_f32<DT>(p.k, row + head_at + i), dot);
-        t = dot * p.scale;
+        t = dot * scale;
       }
       float next = t;
 #pragma unroll
@@ -269,9 +270,9 @@ __device__ __forceinline__ void each_alone(const TreeArgs& p, const Draft& d, co
       next = top;
       for (int w = 0; w < THREADS / 64; ++w) next = fmaxf(next, tops[w]);
       rows[tid] = row;
-      weights[tid] = __builtin_amdgcn_exp2f(t - (next == kNone ? 0.f : next)) * factor;
+      weights[tid] = __builtin_amdgcn_exp2f((t - (next == kNone ? 0.f : next)) * p.unit) * factor;
       __syncthreads();
-      const float keep = next == top ? 1.f : __builtin_amdgcn_exp2f(top - next);
+      const float keep = next == top ? 1.f : __builtin_amdgcn_exp2f((top - next) * p.unit);
       top = next;
       sum *= keep;
 #pragma unroll
@@ -599,7 +600,7 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
     if (__syncthreads_or(alone)) {
       each_alone<DT, 256>(
           p, d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),
-          FACTOR, reinterpret_cast<uint32_t*>(&lds_o[0][0][0]),
+          p.scale, FACTOR, reinterpret_cast<uint32_t*>(&lds_o[0][0][0]),
           [&](int c, int dim, float o, float sum) {
             const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
             if (whole) store_as<DT>(p.y, (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + of_all - n * p.group) * p.head_dim + dim, sum == 0.f ? 0.f : o * (1.f / sum));
@@ -748,9 +749,11 @@ __device__ const uint4_t kZeros[32] = {};
 // lanes then hold sixteen tokens' scores of one column, in the order in which O^T = V^T P^T takes them: no score leaves its
 // lane, and V's columns are read from LDS transposed. Rows lie in LDS as in memory, their pieces of 16 bytes moved within the row,
 // K's by the row's number so that the rows that are read together lie on different banks, V's by four pieces a row of four.
-// Scores' maxima are kept as they come from the products: a probability is 2^(s a - m a + F) with the scale's magnitude a (its
-// sign goes to the queries), one fused multiply-add ahead of the exponential. What m a is rounded by is in all of a column's
-// weights and drops out. Probabilities go in two 16-bit parts, as in attention of one token (one part would make 4 x 512 over
+// Scores' maxima are kept as they come from the products, in the parts too: a probability is 2^((s - m) a + F) with the scale's
+// magnitude a (its sign goes to the queries), at most 2^(F + LAG) whatever size the scores have. It is computed as s a + (F - m a), one
+// instruction, up to maxima of FAR, where the roundings move weights by 2^-18 at most (from 2^27 on they would leave the 16-bit
+// parts' range); past that a branch subtracts the maximum from the scores first (always so, 4 x 512 over 4096 took 168 us for 164).
+// Probabilities go in two 16-bit parts, as in attention of one token (one part would make 4 x 512 over
 // 4096 13% faster, and show in the answer). Maxima are followed where they grow by more than LAG only, as a rule never after a
 // column's first unit (0 instead, one of 64 over 131072 f16: 310 us with 32 heads and so, 297 with 4).
 // Bound by the products: 8192 more tokens of 4 x 512 bf16 rows cost 395 us, 1.04 PFLOP/s in all, where a large library product
@@ -763,7 +766,7 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
   constexpr int RI = 4 / NB, RW = TW / WC;  // rows that an instruction brings, and a wavefront
   constexpr int PLACES = W + 2;             // of a unit's work where loads of the next are asked for
   constexpr uint32_t kNone16 = ~0u;
-  constexpr float LAG = DT == DT_F16 ? 4.f : 8.f, F = DT == DT_F16 ? 15.f - LAG : -32.f - LAG;
+  constexpr float LAG = DT == DT_F16 ? 4.f : 8.f, F = DT == DT_F16 ? 15.f - LAG : -32.f - LAG, FAR = 64.f;
   static_assert(TW % 32 == 0 && RW % 16 == 0, "");
   __shared__ __align__(16) uint8_t lds[2][STAGE];
   __shared__ float2 lds_ml[WT][M];
@@ -793,8 +796,7 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
     __syncthreads();
   };
   clear(2);
-  // (A scale of 0: queries of zeros, so that -infinity times it stays what it is.)
-  const float a = p.scale == 0.f ? 1.f : fabsf(p.scale);
+  const float a = p.unit;
   const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;
   const uint32_t page16 = static_cast<uint32_t>(p.cache.page_stride / 8), token16 = static_cast<uint32_t>(p.cache.token_stride / 8);
   bool used = false;  // stage 0, by an item's sums
@@ -828,6 +830,7 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
     if (p.window > 0) begin = mask ? tree_begin(mask, p.words, d.prefix, d.nodes, p.window) : chain_begin(node, d.prefix, p.window);
     uint4_t qf[NC];
     float m = kNone, l = 0.f;  // of this lane's column, l over this lane's tokens only
+    bool far = false;          // a column's maximum is past FAR
     float16_t acc[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -937,8 +940,18 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
         l *= keep;
 #pragma unroll
         for (int db = 0; db < DB; ++db) acc[db] *= keep;
+        far = __ballot(m != kNone && fabsf(m * a) > FAR) != 0;
       }
-      const float c = F - (m == kNone ? 0.f : m * a);
+      const float ref = m == kNone ? 0.f : m;
+      float c = F - ref * a;
+      if (far) {
+        asm volatile("");
+        c = F;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[w][i] -= ref;
+      }
       // Half a step's products: of tokens 16 x + 4 h + {0 .. 3, 8 .. 11} V's dimension 32 db + lane % 32.
 #pragma unroll
       for (int x = 0; x < 2 * W; ++x) {
@@ -1036,7 +1049,7 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
     if (__syncthreads_or(alone)) {
       each_alone<DT, THREADS>(
           p, d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),
-          __builtin_ldexpf(1.f, static_cast<int>(F)), reinterpret_cast<uint32_t*>(&lds[0][0]),
+          p.scale == 0.f ? 0.f : copysignf(1.f, p.scale), __builtin_ldexpf(1.f, static_cast<int>(F)), reinterpret_cast<uint32_t*>(&lds[0][0]),
           [&](int c, int dim, float o, float sum) {
             const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
             if (whole) store_as<DT>(p.y, (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + of_all - n * p.group) * p.head_dim + dim, sum == 0.f ? 0.f : o * (1.f / sum));
@@ -1098,7 +1111,7 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
 #pragma unroll
         for (int i = 0; i < 4 * DB; ++i)
           put_part(p, ((slot * WC + wc) * (4 * DB) + i) * 64 + lane, float4_t{acc[i / 4][i % 4 * 4], acc[i / 4][i % 4 * 4 + 1], acc[i / 4][i % 4 * 4 + 2], acc[i / 4][i % 4 * 4 + 3]});
-        if (h == 0) put_stats(p, slot * M + 32 * wc + col, top == kNone ? kNone : top * a, total);
+        if (h == 0) put_stats(p, slot * M + 32 * wc + col, top, total);
       }
     }
     join_here();
@@ -1132,14 +1145,14 @@ __global__ __launch_bounds__(256) void k_tree_shared_join(TreeArgs p) {
   float most = top;
 #pragma unroll
   for (int w = 0; w < 3; ++w) most = fmaxf(most, stats[w][lane].x);
-  const float keep = top == most ? 1.f : __builtin_amdgcn_exp2f(top - most);
+  const float keep = top == most ? 1.f : __builtin_amdgcn_exp2f((top - most) * p.unit);
   total *= keep;
 #pragma unroll
   for (int q = 0; q < 4; ++q) acc[q] *= keep;
 #pragma unroll
   for (int w = 0; w < 3; ++w) {
     const float2 st = stats[w][lane];
-    const float f = st.x == most ? 1.f : __builtin_amdgcn_exp2f(st.x - most);
+    const float f = st.x == most ? 1.f : __builtin_amdgcn_exp2f((st.x - most) * p.unit);
     total += f * st.y;
 #pragma unroll
     for (int q = 0; q < 4; ++q) acc[q] += f * sums[w][q][lane];
@@ -1262,6 +1275,8 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
   p.head_dim = cache->head_dim;
   p.by_group = FastDiv(static_cast<uint32_t>(group));
   p.scale = scale * 1.44269504088896340736f;
+  // (A scale of 0: queries of zeros, so that -infinity times the unit stays what it is.)
+  p.unit = !form.shared || p.scale == 0.f ? 1.f : std::fabs(p.scale);
   p.workers = static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(workers, units * items)));
   hipStream_t s = pick_stream(ctx, stream);
   const size_t rows = 2 * static_cast<size_t>(workers) * form.columns;

@@ -538,7 +538,7 @@ int tmh_paged_append_norm(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void
  *  d_lengths [B] S32, the tokens in the cache, the step's own among them, clamped to [0, max_pages * page_size]; with
  *    fewer than n the first nodes have no token
  * A row that sees no token answers zeros. What a row does not see, infinities and NaN too, has no effect on it.
- * B at most 65535, T * heads / kv_heads below 2^31. The context's workspace keeps the parts of sequences that workgroups
+ * B at most 65535, T * heads / kv_heads below 2^31, max_pages * page_size up to 2^31 - 1024. The context's workspace keeps the parts of sequences that workgroups
  * share. How columns and tokens are shared out, and so the last bits, follows T / B, heads, max_pages and the window.
  */
 int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t T, int heads,

@@ -1228,8 +1228,9 @@ int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t
   const int64_t width = static_cast<int64_t>(heads) * cache->head_dim;
   if (ldq < width || ldy < width)
     return fail(ctx, TMH_ERR_INVALID, "the leading dimensions of q and y must be at least %lld", (long long)width);
-  if (max_pages >= (int64_t{1} << 31) / cache->page_size)
-    return fail(ctx, TMH_ERR_UNSUPPORTED, "attention needs max_pages * page_size below 2^31");
+  // (A workgroup counts up to two units past its last, and tokens in 32 bits.)
+  if (max_pages > ((int64_t{1} << 31) - 1024) / cache->page_size)
+    return fail(ctx, TMH_ERR_UNSUPPORTED, "attention of several tokens needs max_pages * page_size of up to 2^31 - 1024");
   TMH_TRY(use_device(ctx));
   if (B == 0 || T == 0) return TMH_OK;
   if (!d_q || !d_y || !d_lengths || !d_starts || (max_pages && !d_page_table))

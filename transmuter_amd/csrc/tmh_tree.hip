@@ -197,20 +197,6 @@ __device__ __forceinline__ void store_answer(const TreeArgs& p, int64_t row, int
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.y) + out) = make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
 }
 
-// Whether 16 bytes hold an infinity or a NaN.
-template <int DT>
-__device__ __forceinline__ bool not_finite(uint4_t x) {
-  constexpr uint32_t e = DT == DT_F32 ? 0x7F800000u : DT == DT_F16 ? 0x7C00u : 0x7F80u;
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t w = x[i];
-    if constexpr (DT == DT_F32) any |= (w & e) == e;
-    else any |= (w & e) == e || (w >> 16 & e) == e;
-  }
-  return any;
-}
-
 // Two probabilities as the sums of two 16-bit parts each, the first cut off, the second rounded (f16: cut off, at 2^-21 of the
 // probability). Unlike split2's, the second part may be 0 beside a first that is not, and an infinity in V becomes a NaN.
 template <int DT>
@@ -311,7 +297,7 @@ __device__ __forceinline__ void join_item(const TreeArgs& p, const Draft& d, con
 // computed them, in two 16-bit parts. K's and V's 16 bytes a lane are used for CB products each, so that a tree's
 // rows read the cache once together.
 // What a column sees of the step's own tokens is 32 bits a tile; what it does not see has a weight of 0, and where
-// an infinity or NaN is there (found by looking at V where the columns differ) the item is done again, by each_alone.
+// an infinity or NaN is there (found by the NaN that it leaves) the item is done again, by each_alone.
 // Bound by memory where tokens are many, else by the ways in and out: 32 x 4 nodes over 4000 bf16 (4 kv heads of 4 heads of 128,
 // 262 MB of K and V) 62 us, 4.2 TB/s; one of 8 nodes over 700 f16 12.
 template <int DT, int NB, int CB>  // NB: blocks of 16 E dimensions
@@ -484,18 +470,6 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
       }
       return true;
     };
-    // Whether a column does not see a token of the tile that holds an infinity or a NaN, which a weight of 0 would not hide.
-    auto hides = [&](uint32_t valid) {
-      bool mixed = false, any = false;
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) mixed |= sees[cb] != valid;
-      if (!__ballot(mixed)) return false;
-#pragma unroll
-      for (int j = 0; j < VT; ++j)
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) any |= not_finite<DT>(vf[j][nb]);
-      return __ballot(any) != 0;
-    };
     float pr[F32 ? CB : 1][4];        // the probabilities, or
     uint4_t parts[F32 ? 1 : CB][2];   // their two parts
     auto softmax = [&](bool masked) {
@@ -564,7 +538,6 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
     int64_t found = look(from), coming = look(from + 1);
     load_k(found < 0 ? 0 : found);
     load_v(found < 0 ? 0 : found);
-    bool alone = false;  // a column does not see an infinity or a NaN
     for (uint32_t u = from; u < to; ++u) {
       const uint32_t valid = static_cast<uint32_t>(__ballot(found >= 0)) & WHOLE;  // (TILE 16: the four copies agree)
       const int64_t next_row = coming < 0 ? 0 : coming;
@@ -573,9 +546,7 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
       coming = look(u + 2);
       scores();
       if (more) load_k(next_row);
-      const bool masked = look_at(first_of(u), valid);
-      if (masked) alone |= hides(valid);
-      softmax(masked);
+      softmax(look_at(first_of(u), valid));
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -597,6 +568,20 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
         join_item<kThrough, DT, M>(p, d, all_parts, kv_head, tile, c, quad, quads);
       }
     };
+    // An infinity or a NaN in V leaves a NaN in every column that does not see it (0 times an infinity), and an infinity may in one that
+    // sees it with little weight, of which a 16-bit part is 0: such an item is done again.
+    bool alone = false;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = acc[cb][nb][e][i];
+            alone |= x != x;
+          }
     if (__syncthreads_or(alone)) {
       each_alone<DT, 256>(
           p, d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),

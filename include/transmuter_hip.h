@@ -538,6 +538,9 @@ int tmh_paged_append_norm(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void
  *  d_lengths [B] S32, the tokens in the cache, the step's own among them, clamped to [0, max_pages * page_size]; with
  *    fewer than n the first nodes have no token
  * A row that sees no token answers zeros. What a row does not see, infinities and NaN too, has no effect on it.
+ * It may have one on the time: rows that do not see an infinity or a NaN in V that others of their tile (up to 128 rows times query heads of a
+ * kv head) see, and rows that see one, are computed a second time token by token, which takes 5 to 40 times as long as the call. One in a
+ * query or a key costs nothing.
  * B at most 65535, T * heads / kv_heads below 2^31, max_pages * page_size up to 2^31 - 1024. The context's workspace keeps the parts of sequences that workgroups
  * share. How columns and tokens are shared out, and so the last bits, follows T / B, heads, max_pages and the window.
  */

@@ -97,6 +97,9 @@ __device__ __forceinline__ void put_part(const TreeArgs& p, uint32_t quad, float
 __device__ __forceinline__ void put_stats(const TreeArgs& p, uint32_t at, float top, float total) {
   __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(uint2_t, make_float2(top, total)), buffer_rsrc(p.stats, p.stats_bytes), at * 8, 0, kThrough);
 }
+__device__ __forceinline__ void put_value(const TreeArgs& p, uint32_t at, float v) {  // (of a part, counted in values)
+  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), buffer_rsrc(p.part, p.part_bytes), at * 4, 0, kThrough);
+}
 template <int AUX>
 __device__ __forceinline__ float4_t get_part(const TreeArgs& p, uint32_t quad, bool there) {
   return __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(buffer_rsrc(p.part, p.part_bytes), there ? quad * 16 : kNowhere, 0, AUX));
@@ -211,73 +214,184 @@ __device__ __forceinline__ uint2 cut2(float a, float b) {
   }
 }
 
-// Columns [first, first + columns) of an item over its tokens [from, to), one after another, each product in f32 of what a column
-// sees alone: the workgroups' way where a column does not see a token that holds an infinity or a NaN, which a weight of 0 would
-// leave in a matrix product. put(column of these, dimension, sum, weights' sum) and total(column of these, maximum, weights' sum)
-// take the answers; the maxima are of products times `scale`, each worth p.unit base-2 logarithms. Weights are multiplied by `factor`,
-// as the other parts' are; `room` is 3 THREADS + 16 words of LDS.
+// An infinity or a NaN in V leaves a NaN in every column of its products that does not see it (0 times an infinity), and an infinity may in
+// one that sees it with little weight, of which a 16-bit part is 0. Such columns are done again, by each_alone: those whose sums have a NaN
+// while the sum of their weights, in which V has no part, has none. (Where it has one, as for a NaN in the query, the answer is NaN
+// whatever V holds.) mark: the bits `first` and up of `words`, in LDS, for the GROUP columns of a wavefront in which a lane says so.
+template <int GROUP>
+__device__ __forceinline__ void mark(uint32_t* words, int first, bool flag) {
+  uint64_t b = __ballot(flag);
+#pragma unroll
+  for (int o = 32; o >= GROUP; o /= 2) b |= b >> o;
+  const uint32_t some = static_cast<uint32_t>(b & ((uint64_t{1} << GROUP) - 1));
+  if (some && (threadIdx.x & 63) == 0) atomicOr(&words[first / 32], some << (first % 32));
+}
+
+// The marked columns of an item's [first, first + columns) over its tokens [from, to), in f32, of the tokens that each sees alone, eight columns
+// at a time: a thread takes a token for their scores, then a dimension for their sums. put(column of these, dimension, sum,
+// weights' sum) and total(column of these, maximum, weights' sum) take the answers; the maxima are of products times `scale`, each worth
+// p.unit base-2 logarithms. Weights are multiplied by `factor`, as the other columns' are. It is slow (4 x 512 over 4096 bf16 with one NaN in
+// each kv head's V 9.6 ms, 0.16 without): for columns that need it only. `room`: kAloneRoom(THREADS, head_dim) bytes of LDS;
+// `marked` lies in LDS too.
+constexpr int kAlone = 8;
+constexpr int kAloneRoom(int threads, int dim) { return threads * (12 + 4 * kAlone) + (dim + threads / 64 + 3) * 4 * kAlone; }
 template <int DT, int THREADS, typename Put, typename Total>
-__device__ __forceinline__ void each_alone(const TreeArgs& p, const Draft& d, const int32_t* table, int kv_head, int first, int columns, int from,
-                                           int to, float scale, float factor, uint32_t* room, Put put, Total total) {
+__device__ __forceinline__ void each_alone(const Draft& d, const int32_t* table, int kv_head, int first, int columns, int from,
+                                           int to, float scale, float factor, const uint32_t* marked, void* room, Put put, Total total) {
   constexpr int EACH = 256 / THREADS > 0 ? 256 / THREADS : 1;  // dimensions a thread may have
-  const int tid = threadIdx.x, dim = p.head_dim, wave = tid >> 6;
-  int64_t* rows = reinterpret_cast<int64_t*>(room);  // of a turn's tokens, negative where one is not seen
-  float* weights = reinterpret_cast<float*>(room + 2 * THREADS);
-  float* tops = weights + THREADS;
+  constexpr int BATCH = 8;                                      // loads of V on their way at once
+  // The kernel's arguments (its only one is a TreeArgs) once more, and the thread, as nothing that the compiler knows: what follows from
+  // them it would compute ahead of all work and keep in registers (3 x 13 over 1000 f32 13.3 us, so 11.8).
+  const auto* args = (const __attribute__((address_space(4))) void*)__builtin_amdgcn_kernarg_segment_ptr();
+  int tid = threadIdx.x;
+  asm volatile("" : "+s"(args), "+v"(tid));
+  TreeArgs p;
+  __builtin_memcpy(&p, (const void*)args, sizeof(p));
+  const int dim = p.head_dim, wave = tid >> 6;
+  int64_t* rows = static_cast<int64_t*>(room);  // of a turn's tokens, negative where there is none
+  auto weights = reinterpret_cast<float(*)[kAlone]>(rows + THREADS);
+  float* q = &weights[THREADS][0];  // [dim][kAlone]
+  auto meet = reinterpret_cast<float(*)[kAlone]>(q + dim * kAlone);                           // [THREADS / 64]
+  uint32_t* seen = reinterpret_cast<uint32_t*>(&meet[THREADS / 64][0]);  // by which of the columns, of a turn's tokens
+  // The columns (-1: none), their nodes, and the first token that the window leaves them.
+  int *column = reinterpret_cast<int*>(seen + THREADS), *node = column + kAlone, *begin = node + kAlone;
   const int64_t head_at = static_cast<int64_t>(kv_head) * p.head_stride;
+  int next_column = 0;
 #pragma unroll 1
-  for (int c = 0; c < columns; ++c) {
-    const int of_all = first + c, node = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
-    const uint64_t* mask = p.mask ? p.mask + static_cast<int64_t>(d.row + node) * p.words : nullptr;
-    int begin = 0;
-    if (p.window > 0) begin = mask ? tree_begin(mask, p.words, d.prefix, d.nodes, p.window) : chain_begin(node, d.prefix, p.window);
-    const int64_t q = (d.row + node) * p.ldq + static_cast<int64_t>(kv_head * p.group + of_all - node * p.group) * dim;
-    float top = kNone, sum = 0.f, o[EACH] = {};  // o: dimensions tid + i THREADS
+  while (true) {
+    if (tid < kAlone) {
+      int c = next_column;
+      for (int left = tid; c < columns; ++c)
+        if ((marked[c / 32] >> (c % 32) & 1u) && left-- == 0) break;
+      const int n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(first + min(c, columns - 1))));
+      column[tid] = c < columns ? c : -1;
+      node[tid] = n;
+      begin[tid] = 0;
+      if (p.window > 0) {
+        if (p.mask) begin[tid] = tree_begin(p.mask + static_cast<int64_t>(d.row + n) * p.words, p.words, d.prefix, d.nodes, p.window);
+        else begin[tid] = chain_begin(n, d.prefix, p.window);
+      }
+    }
+    __syncthreads();
+    if (column[0] < 0) break;
+    next_column = column[kAlone - 1] < 0 ? columns : column[kAlone - 1] + 1;
+    for (int i = tid; i < dim * kAlone; i += THREADS) {
+      const int k = i % kAlone;
+      const int head = kv_head * p.group + first + max(column[k], 0) - node[k] * p.group;
+      q[i] = column[k] < 0 ? 0.f : load_as_f32<DT>(p.q, (d.row + node[k]) * p.ldq + static_cast<int64_t>(head) * dim + i / kAlone);
+    }
+    float top[kAlone], sum[kAlone], o[kAlone][EACH];  // sum: of this thread's tokens, o: dimensions tid + x THREADS
+#pragma unroll
+    for (int k = 0; k < kAlone; ++k) {
+      top[k] = kNone;
+      sum[k] = 0.f;
+#pragma unroll
+      for (int x = 0; x < EACH; ++x) o[k][x] = 0.f;
+    }
+    __syncthreads();
 #pragma unroll 1
     for (int t0 = from; t0 < to; t0 += THREADS) {
       const int token = t0 + tid, some = min(THREADS, to - t0);
-      float t = kNone;
-      int64_t row = -1;
-      if (token < to && token >= begin &&
-          (token < d.prefix || ((mask ? tree_bits(mask, p.words, token - d.prefix) : chain_bits(node, token - d.prefix)) & 1u)))
-        row = token_offset(p.cache, table, static_cast<uint32_t>(token));
+      const int64_t row = token < to ? token_offset(p.cache, table, static_cast<uint32_t>(token)) : -1;
+      float t[kAlone] = {};
       if (row >= 0) {
-        float dot = 0.f;
-#pragma unroll 1
-        for (int i = 0; i < dim; ++i) dot = fmaf(load_as_f32<DT>(p.q, q + i), load_as_f32<DT>(p.k, row + head_at + i), dot);
-        t = dot * scale;
-      }
-      float next = t;
+#pragma unroll 2
+        for (int i = 0; i < dim; i += 8) {
+          float y[8];
+          load8<DT, true>(p.k, row + head_at + i, 8, y);
 #pragma unroll
-      for (int x = 1; x < 64; x <<= 1) next = fmaxf(next, __shfl_xor(next, x));
-      __syncthreads();  // the turn before has been read
-      if ((tid & 63) == 0) tops[wave] = next;
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int k = 0; k < kAlone; ++k) t[k] = fmaf(q[(i + j) * kAlone + k], y[j], t[k]);
+        }
+      }
+      uint32_t by = 0;
+#pragma unroll
+      for (int k = 0; k < kAlone; ++k) {
+        bool sees = column[k] >= 0 && row >= 0 && token >= begin[k];
+        if (sees && token >= d.prefix) {
+          const uint64_t* mask = p.mask ? p.mask + static_cast<int64_t>(d.row + node[k]) * p.words : nullptr;
+          sees = (mask ? tree_bits(mask, p.words, token - d.prefix) : chain_bits(node[k], token - d.prefix)) & 1u;
+        }
+        by |= sees ? 1u << k : 0u;
+        t[k] = sees ? t[k] * scale : kNone;
+        float most = t[k];
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) most = fmaxf(most, __shfl_xor(most, x));
+        if ((tid & 63) == 0) meet[wave][k] = most;
+      }
       __syncthreads();
-      next = top;
-      for (int w = 0; w < THREADS / 64; ++w) next = fmaxf(next, tops[w]);
       rows[tid] = row;
-      weights[tid] = __builtin_amdgcn_exp2f((t - (next == kNone ? 0.f : next)) * p.unit) * factor;
-      __syncthreads();
-      const float keep = next == top ? 1.f : __builtin_amdgcn_exp2f((top - next) * p.unit);
-      top = next;
-      sum *= keep;
+      seen[tid] = by;
 #pragma unroll
-      for (int x = 0; x < EACH; ++x) o[x] *= keep;
-#pragma unroll 1
-      for (int i = 0; i < some; ++i) {
-        if (rows[i] < 0) continue;
-        sum += weights[i];
+      for (int k = 0; k < kAlone; ++k) {
+        float next = top[k];
 #pragma unroll
-        for (int x = 0; x < EACH; ++x)
-          if (tid + x * THREADS < dim) o[x] = fmaf(weights[i], load_as_f32<DT>(p.v, rows[i] + head_at + tid + x * THREADS), o[x]);
+        for (int w = 0; w < THREADS / 64; ++w) next = fmaxf(next, meet[w][k]);
+        const float keep = next == top[k] ? 1.f : __builtin_amdgcn_exp2f((top[k] - next) * p.unit);
+        top[k] = next;
+        const float w = by >> k & 1u ? __builtin_amdgcn_exp2f((t[k] - (next == kNone ? 0.f : next)) * p.unit) * factor : 0.f;
+        weights[tid][k] = w;
+        sum[k] = fmaf(sum[k], keep, w);
+#pragma unroll
+        for (int x = 0; x < EACH; ++x) o[k][x] *= keep;
       }
+      __syncthreads();
+      if (64 * wave < dim) {
+#pragma unroll 1
+        for (int i = 0; i < some; i += BATCH) {  // (tokens past `some` are seen by none; the cache's first row is in their place, not used)
+          float v[EACH][BATCH];
+          bool special = false;
+#pragma unroll
+          for (int j = 0; j < BATCH; ++j)
+#pragma unroll
+            for (int x = 0; x < EACH; ++x) {
+              v[x][j] = load_as_f32<DT>(p.v, max(rows[i + j], int64_t{0}) + head_at + min(tid + x * THREADS, dim - 1));
+              special |= !(fabsf(v[x][j]) < __builtin_inff());
+            }
+          if (__ballot(special)) {
+#pragma unroll
+            for (int j = 0; j < BATCH; ++j)
+#pragma unroll
+              for (int x = 0; x < EACH; ++x) {
+                if (fabsf(v[x][j]) < __builtin_inff()) continue;
+#pragma unroll
+                for (int k = 0; k < kAlone; ++k)
+                  if (seen[i + j] >> k & 1u) o[k][x] = fmaf(weights[i + j][k], v[x][j], o[k][x]);
+                v[x][j] = 0.f;
+              }
+          }
+#pragma unroll
+          for (int j = 0; j < BATCH; ++j)
+#pragma unroll
+            for (int k = 0; k < kAlone; ++k)
+#pragma unroll
+              for (int x = 0; x < EACH; ++x) o[k][x] = fmaf(weights[i + j][k], v[x][j], o[k][x]);
+        }
+      }
+      __syncthreads();
     }
 #pragma unroll
-    for (int x = 0; x < EACH; ++x)
-      if (tid + x * THREADS < dim) put(c, tid + x * THREADS, o[x], sum);
-    if (tid == 0) total(c, top, sum);
+    for (int k = 0; k < kAlone; ++k) {
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) sum[k] += __shfl_xor(sum[k], x);
+      if ((tid & 63) == 0) meet[wave][k] = sum[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kAlone; ++k) {
+      if (column[k] < 0) continue;
+      sum[k] = meet[0][k];
+#pragma unroll
+      for (int w = 1; w < THREADS / 64; ++w) sum[k] += meet[w][k];
+#pragma unroll
+      for (int x = 0; x < EACH; ++x)
+        if (tid + x * THREADS < dim) put(column[k], tid + x * THREADS, o[k][x], sum[k]);
+      if (tid == 0) total(column[k], top[k], sum[k]);
+    }
+    __syncthreads();  // the columns have been read
   }
-  __syncthreads();
+  __syncthreads();  // that there are no more, too
 }
 
 // Four dimensions of one column of an item whose parts are rows.
@@ -297,7 +411,7 @@ __device__ __forceinline__ void join_item(const TreeArgs& p, const Draft& d, con
 // computed them, in two 16-bit parts. K's and V's 16 bytes a lane are used for CB products each, so that a tree's
 // rows read the cache once together.
 // What a column sees of the step's own tokens is 32 bits a tile; what it does not see has a weight of 0, and where
-// an infinity or NaN is there (found by the NaN that it leaves) the item is done again, by each_alone.
+// an infinity or NaN is there (found by the NaN that it leaves) a column is done again (mark).
 // Bound by memory where tokens are many, else by the ways in and out: 32 x 4 nodes over 4000 bf16 (4 kv heads of 4 heads of 128,
 // 262 MB of K and V) 62 us, 4.2 TB/s; one of 8 nodes over 700 f16 12.
 template <int DT, int NB, int CB>  // NB: blocks of 16 E dimensions
@@ -312,6 +426,7 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
   constexpr int ROW = 16 * E * NB + 4;    // floats of a column's answer in LDS (+ 4: off a bank's multiple)
   __shared__ __align__(16) float lds_o[4][16][ROW];
   __shared__ float lds_m[4][16], lds_l[4][16];
+  __shared__ uint32_t marks[2];
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t worker = blockIdx.x;
@@ -568,11 +683,10 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
         join_item<kThrough, DT, M>(p, d, all_parts, kv_head, tile, c, quad, quads);
       }
     };
-    // An infinity or a NaN in V leaves a NaN in every column that does not see it (0 times an infinity), and an infinity may in one that
-    // sees it with little weight, of which a 16-bit part is 0: such an item is done again.
-    bool alone = false;
+    bool bad[CB], any = false;  // (mark)
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb)
+    for (int cb = 0; cb < CB; ++cb) {
+      bad[cb] = false;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -580,23 +694,21 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float x = acc[cb][nb][e][i];
-            alone |= x != x;
+            bad[cb] |= x != x;
           }
-    if (__syncthreads_or(alone)) {
-      each_alone<DT, 256>(
-          p, d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),
-          p.scale, FACTOR, reinterpret_cast<uint32_t*>(&lds_o[0][0][0]),
-          [&](int c, int dim, float o, float sum) {
-            const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
-            if (whole) store_as<DT>(p.y, (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + of_all - n * p.group) * p.head_dim + dim, sum == 0.f ? 0.f : o * (1.f / sum));
-            else p.part[(static_cast<int64_t>(slot) * M + c) * p.head_dim + dim] = o;
-          },
-          [&](int c, float top, float sum) {
-            if (!whole) p.stats[static_cast<int64_t>(slot) * M + c] = make_float2(top, sum);
-          });
-      __threadfence();  // (these stores went by the XCD's L2)
-      join_here();
-      continue;
+      any |= bad[cb];
+    }
+    uint32_t alone = 0;  // columns to do again
+    if (__builtin_expect(__syncthreads_or(any), 0)) {
+      if (threadIdx.x < 2) marks[threadIdx.x] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        mark<16>(&marks[0], 16 * cb, bad[cb]);
+        mark<16>(&marks[1], 16 * cb, l[cb] != l[cb]);
+      }
+      __syncthreads();
+      alone = marks[0] & ~marks[1];
     }
     // The wavefronts' parts of the item meet in LDS, sixteen columns at a time.
 #pragma unroll
@@ -618,6 +730,7 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
       const int some = min(16, columns - 16 * cb);
       for (int i = threadIdx.x; i < some * quads; i += 256) {
         const int c = i / quads, dim = (i - c * quads) * 4;
+        if (alone >> (16 * cb + c) & 1u) continue;
         float top = lds_m[0][c], total = 0.f;
 #pragma unroll
         for (int w = 1; w < 4; ++w) top = fmaxf(top, lds_m[w][c]);
@@ -642,6 +755,22 @@ __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attent
         }
       }
       __syncthreads();
+    }
+    if (__builtin_expect(alone, 0)) {
+      if (threadIdx.x == 0) marks[0] = alone;
+      __syncthreads();
+      static_assert(kAloneRoom(256, 16 * E * NB) <= sizeof(lds_o), "");
+      each_alone<DT, 256>(
+          d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),
+          p.scale, FACTOR, marks, lds_o,
+          [&](int c, int dim, float o, float sum) {
+            const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
+            if (whole) store_as<DT>(p.y, (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + of_all - n * p.group) * p.head_dim + dim, sum == 0.f ? 0.f : o * (1.f / sum));
+            else put_value(p, (slot * M + c) * p.head_dim + dim, o);
+          },
+          [&](int c, float top, float sum) {
+            if (!whole) put_stats(p, slot * M + c, top, sum);
+          });
     }
     join_here();
   }
@@ -755,6 +884,7 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
   static_assert(TW % 32 == 0 && RW % 16 == 0, "");
   __shared__ __align__(16) uint8_t lds[2][STAGE];
   __shared__ float2 lds_ml[WT][M];
+  __shared__ uint32_t marks[2 * WC];
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wc = wave % WC, wt = wave / WC;
   const uint32_t worker = blockIdx.x;
@@ -1021,34 +1151,25 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
           if (32 * (i / DB) + col < columns) answer_column<DT>(p, d, kv_head, tile * M + 32 * (i / DB) + col, 32 * (i % DB) + 4 * h, o, total);
         }
     };
-    // An infinity or a NaN in V leaves a NaN in every column of its products, whether the column sees it or not (0 times an
-    // infinity): such an item is done again.
-    bool alone = false;
+    bool bad = false;  // (mark)
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float x = acc[db][i];
-        alone |= x != x;
+        bad |= x != x;
       }
-    if (__syncthreads_or(alone)) {
-      each_alone<DT, THREADS>(
-          p, d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),
-          p.scale == 0.f ? 0.f : copysignf(1.f, p.scale), __builtin_ldexpf(1.f, static_cast<int>(F)), reinterpret_cast<uint32_t*>(&lds[0][0]),
-          [&](int c, int dim, float o, float sum) {
-            const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
-            if (whole) store_as<DT>(p.y, (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + of_all - n * p.group) * p.head_dim + dim, sum == 0.f ? 0.f : o * (1.f / sum));
-            else p.part[static_cast<int64_t>(((slot * WC + c / 32) * (4 * DB) + dim / 8) * 64 + dim / 4 % 2 * 32 + c % 32) * 4 + dim % 4] = o;
-          },
-          [&](int c, float top, float sum) {
-            if (!whole) p.stats[slot * M + c] = make_float2(top, sum);
-          });
-      clear(2);
-      __threadfence();  // (these stores went by the XCD's L2)
-      join_here();
-      continue;
+    bool alone = false, mine = false;  // columns to do again, this lane's among them
+    if (__builtin_expect(__syncthreads_or(bad), 0)) {
+      if (threadIdx.x < 2 * WC) marks[threadIdx.x] = 0;
+      __syncthreads();
+      mark<32>(marks, 32 * wc, bad);
+      mark<32>(marks + WC, 32 * wc, l != l);
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WC; ++w) alone |= (marks[w] & ~marks[WC + w]) != 0;
+      mine = (marks[wc] & ~marks[WC + wc]) >> col & 1u;
     }
-
     // The wavefronts that share a tile's tokens meet in LDS, lane by lane; the first of them answers.
     {
       float low, high;
@@ -1090,14 +1211,32 @@ __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(T
         for (int db = 0; db < DB; ++db) {
           float4_t four[4];
           quads_of(acc[db], four);
-          if (32 * wc + col < columns) answer_column<DT>(p, d, kv_head, tile * M + 32 * wc + col, 32 * db + 4 * h, four, total);
+          if (32 * wc + col < columns && !mine) answer_column<DT>(p, d, kv_head, tile * M + 32 * wc + col, 32 * db + 4 * h, four, total);
         }
-      } else {
+      } else if (!mine) {
 #pragma unroll
         for (int i = 0; i < 4 * DB; ++i)
           put_part(p, ((slot * WC + wc) * (4 * DB) + i) * 64 + lane, float4_t{acc[i / 4][i % 4 * 4], acc[i / 4][i % 4 * 4 + 1], acc[i / 4][i % 4 * 4 + 2], acc[i / 4][i % 4 * 4 + 3]});
         if (h == 0) put_stats(p, slot * M + 32 * wc + col, top, total);
       }
+    }
+    if (__builtin_expect(alone, 0)) {
+      __syncthreads();  // the wavefronts' sums have been read
+      if (threadIdx.x < WC) marks[threadIdx.x] &= ~marks[WC + threadIdx.x];
+      __syncthreads();
+      static_assert(kAloneRoom(THREADS, 128 * NB) <= sizeof(lds), "");
+      each_alone<DT, THREADS>(
+          d, table, kv_head, tile * M, columns, (d.unit + static_cast<int>(from)) * UT, min(d.end, (d.unit + static_cast<int>(to)) * UT),
+          p.scale == 0.f ? 0.f : copysignf(1.f, p.scale), __builtin_ldexpf(1.f, static_cast<int>(F)), marks, lds,
+          [&](int c, int dim, float o, float sum) {
+            const int of_all = tile * M + c, n = static_cast<int>(p.by_group.div(static_cast<uint32_t>(of_all)));
+            if (whole) store_as<DT>(p.y, (d.row + n) * p.ldy + static_cast<int64_t>(kv_head * p.group + of_all - n * p.group) * p.head_dim + dim, sum == 0.f ? 0.f : o * (1.f / sum));
+            else put_value(p, (((slot * WC + c / 32) * (4 * DB) + dim / 8) * 64 + dim / 4 % 2 * 32 + c % 32) * 4 + dim % 4, o);
+          },
+          [&](int c, float top, float sum) {
+            if (!whole) put_stats(p, slot * M + c, top, sum);
+          });
+      clear(2);
     }
     join_here();
   }

@@ -512,7 +512,7 @@ int tmh_paged_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t B, i
  * tmh_paged_append for models that norm each query and key head: x * rsqrt(mean(x^2) + eps) * gamma over a head's
  * head_dim values, in f32, ahead of the rotation, which is rounded once. Values go to the cache as they are.
  *  d_q_gamma, d_k_gamma [head_dim] of gamma_dtype (F32, F16, BF16), at any address; either may be NULL, whose heads are
- *    then only turned (without both: tmh_paged_append)
+ *    then only turned (both is refused: that is tmh_paged_append)
  * The other arguments are tmh_paged_append's.
  */
 int tmh_paged_append_norm(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void* d_k, int64_t ldk, const void* d_v,
@@ -541,7 +541,9 @@ int tmh_paged_append_norm(tmh_ctx* ctx, const void* d_q, int64_t ldq, const void
  * It may have one on the time: rows that do not see an infinity or a NaN in V that others of their tile (up to 128 rows times query heads of a
  * kv head) see, and rows that see one, are computed a second time token by token, which takes 5 to 40 times as long as the call. One in a
  * query or a key costs nothing.
- * B at most 65535, T * heads / kv_heads below 2^31, max_pages * page_size up to 2^31 - 1024. The context's workspace keeps the parts of sequences that workgroups
+ * B at most 65535, T * heads / kv_heads below 2^31, max_pages * page_size up to 2^31 - 1024. Work is counted in 32 bits: a step is refused where
+ * its tiles, (T * heads / kv_heads / 16 + B) * kv_heads at most, times the table's units, max_pages * page_size / 32 + 5 at most, reach 2^31,
+ * whatever its lengths. The context's workspace keeps the parts of sequences that workgroups
  * share. How columns and tokens are shared out, and so the last bits, follows T / B, heads, max_pages and the window.
  */
 int tmh_paged_tree_attention(tmh_ctx* ctx, const void* d_q, int64_t ldq, int64_t T, int heads,

@@ -202,8 +202,8 @@ __device__ __forceinline__ float group_sum(float v) {
 
 // G lanes answer one head of one token, a lane eight of its dimensions, and with VEC of those that turn by halves their
 // partners too (of a value head: eight more, where G lanes do not hold it). Each row is read once: its squares are summed
-// among the group's lanes while its values stay in registers. Bound by memory: 4096 rows of 32 + 2 x 8 heads of 128 bf16 19.1 us, 4.5
-// TB/s; with all of a lane's loads on their way at once it took no less.
+// among the group's lanes while its values stay in registers. Bound by memory: 4096 rows of 32 + 2 x 4 heads of 128 bf16,
+// every sixteenth padded, 19.3 us, 4.4 TB/s; with all of a lane's loads on their way at once it took no less.
 template <int DT, bool VEC, int G>
 __global__ __launch_bounds__(256) void k_paged_append_norm(AppendNormArgs p, int64_t first, uint32_t count, bool table_vec, bool pairs_vec) {
   const AppendArgs& a = p.a;

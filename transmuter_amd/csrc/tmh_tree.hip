@@ -85,8 +85,10 @@ __device__ __forceinline__ Place place_in(const Draft& d, uint32_t before, uint3
 
 // Parts of items that several workers shared. Each worker leaves its part in memory (stores that pass the XCD's own L2), then counts
 // itself; the one that finds all others counted joins the parts, in their order, whoever it is. Items of more than MOST parts, which
-// would keep one workgroup too long, are left to a second kernel (join_most: half a MiB of parts). In us so, all by the second
-// kernel, and all in the kernel: 32 x 4 over 4000 bf16 62, 65, 62; 8 x 32 42, 51, 59; 2 x 100 over 20000 f16 68, 76, 96.
+// would keep one workgroup too long, are left to a second kernel (join_most: half a MiB of parts of 128 dimensions). In us so, all by the second
+// kernel, and all in the kernel: 32 x 4 over 4000 bf16 62, 65, 62; 8 x 32 42, 51, 59; 2 x 100 over 20000 f16 68, 76, 96. Narrow tiles of 256
+// dimensions keep that number of parts, of a MiB then: 1 x 2 over 6000, 8 heads of one kv head, f16 33.0, with half as many 36.5; 4 x 4 over 8000, 16 of
+// 4, bf16 52.9 and 56.2.
 constexpr int kThrough = 16;                // sc1 of a buffer access: past the XCD's L2, to where all XCDs meet
 constexpr uint32_t kNowhere = 0xFFFFFFF0u;  // an offset past every buffer's range here
 constexpr uint32_t join_most(int columns, int blocks) { return 1024u / (columns * blocks); }
@@ -413,7 +415,7 @@ __device__ __forceinline__ void join_item(const TreeArgs& p, const Draft& d, con
 // What a column sees of the step's own tokens is 32 bits a tile; what it does not see has a weight of 0, and where
 // an infinity or NaN is there (found by the NaN that it leaves) a column is done again (mark).
 // Bound by memory where tokens are many, else by the ways in and out: 32 x 4 nodes over 4000 bf16 (4 kv heads of 4 heads of 128,
-// 262 MB of K and V) 62 us, 4.2 TB/s; one of 8 nodes over 700 f16 12.
+// 262 MB of K and V) 62 us, 4.2 TB/s; one of 8 nodes over 700 f16 11.7.
 template <int DT, int NB, int CB>  // NB: blocks of 16 E dimensions
 __global__ __launch_bounds__(256, NB == 1 && CB <= 2 ? 2 : 1) void k_tree_attention(TreeArgs p) {
   constexpr bool F32 = DT == DT_F32;
@@ -867,12 +869,12 @@ __device__ const uint4_t kZeros[32] = {};
 // magnitude a (its sign goes to the queries), at most 2^(F + LAG) whatever size the scores have. It is computed as s a + (F - m a), one
 // instruction, up to maxima of FAR, where the roundings move weights by 2^-18 at most (from 2^27 on they would leave the 16-bit
 // parts' range); past that a branch subtracts the maximum from the scores first (always so, 4 x 512 over 4096 took 168 us for 164).
-// Probabilities go in two 16-bit parts, as in attention of one token (one part would make 4 x 512 over
+// Probabilities go in two 16-bit parts (cut2; one part would make 4 x 512 over
 // 4096 13% faster, and show in the answer). Maxima are followed where they grow by more than LAG only, as a rule never after a
 // column's first unit (0 instead, one of 64 over 131072 f16: 310 us with 32 heads and so, 297 with 4).
 // Bound by the products: 8192 more tokens of 4 x 512 bf16 rows cost 395 us, 1.04 PFLOP/s in all, where a large library product
 // comes to 1.20; without any exponentials it is 7% less, without reads of K from LDS no less. Beside that the ways in and out,
-// 35 us of the 148 of 4 x 512 over 4096.
+// 35 us of the 154 of 4 x 512 over 4096.
 template <int DT, int NB, int WC, int WT>
 __global__ __launch_bounds__(64 * WC * WT, NB == 1 ? 2 : 1) void k_tree_shared(TreeArgs p) {
   constexpr int THREADS = 64 * WC * WT, UT = 64 / NB, TW = UT / WT, M = 32 * WC;  // TW: a wavefront's tokens of a unit

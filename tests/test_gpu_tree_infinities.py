@@ -138,3 +138,31 @@ def test_values_that_some_rows_see(ctx, dtype, way):
         special = [2, 9] + [5, 11] * bool(node_seen[r])
         got[r][:, special] = want[:, special]
     check_draft(got.reshape(len(q), -1), q, k, clean, table, shapes, starts, mask, 16, h, g, d, dtype, 1 / math.sqrt(d), rows=rows)
+
+
+@pytest.mark.parametrize("dtype,way", TYPES)
+def test_values_that_some_windows_leave(ctx, dtype, way):
+    """A NaN in a value of a token that is in some rows' windows and before others', which answer as without it."""
+    say("values that some windows leave", dtype, way)
+    rng = np.random.default_rng(len(way) + 3)
+    shapes, h, g, d, wide = WAYS[way]
+    cache, k, v, table, q, starts, mask = draft_inputs(ctx, rng, shapes, h, g, d, 16, "token", dtype, "tree")
+    run = attend_tree_wide if wide else attend_tree
+    lengths, window, left = [n for n, _ in shapes], 12, {}
+    vals = v.copy()
+    for b, (n, m) in enumerate(shapes):
+        at = n - m - min(9, n - m)
+        vals[table[b, at // 16], at % 16, :, 3] = np.nan
+        left[b] = at
+    put(ctx, cache, k, vals, dtype)
+    y = run(ctx, cache, q, table, lengths, starts, mask, window=window).numpy()
+    got, clean = values(y).reshape(-1, h, d), []
+    for b, (n, m) in enumerate(shapes):
+        for i in range(m):
+            if drafts.sees(mask[starts[b] + i], i, m, n, window)[left[b]]:
+                assert np.isnan(got[starts[b] + i, :, 3]).all() and np.isfinite(got[starts[b] + i, :, 4:]).all()
+            else:
+                clean.append((b, i))
+                assert np.isfinite(got[starts[b] + i]).all()
+    assert len(clean) < len(q) and (clean or max(m for _, m in shapes) < 9)  # (few nodes are in all windows, and the token with them)
+    check_draft(y, q, k, v, table, shapes, starts, mask, 16, h, g, d, dtype, 1 / math.sqrt(d), window, rows=set(clean[:40]))

@@ -233,7 +233,7 @@ __device__ __forceinline__ void mark(uint32_t* words, int first, bool flag) {
 // at a time: a thread takes a token for their scores, then a dimension for their sums. put(column of these, dimension, sum,
 // weights' sum) and total(column of these, maximum, weights' sum) take the answers; the maxima are of products times `scale`, each worth
 // p.unit base-2 logarithms. Weights are multiplied by `factor`, as the other columns' are. It is slow (4 x 512 over 4096 bf16 with one NaN in
-// each kv head's V 9.6 ms, 0.16 without): for columns that need it only. `room`: kAloneRoom(THREADS, head_dim) bytes of LDS;
+// each kv head's V of one sequence 9.6 ms, 0.16 without): for columns that need it only. `room`: kAloneRoom(THREADS, head_dim) bytes of LDS;
 // `marked` lies in LDS too.
 constexpr int kAlone = 8;
 constexpr int kAloneRoom(int threads, int dim) { return threads * (12 + 4 * kAlone) + (dim + threads / 64 + 3) * 4 * kAlone; }
